@@ -198,6 +198,22 @@ MGP_API int mgp_gradient_matvec(void* handle, const float* V, int ncols, float* 
 MGP_API int mgp_gradient_trace(void* handle, const float* Lf, const float* Rf,
                                int ncols, double* out);
 
+/* out[i][q] = d/dx_iq sum_{a,b} K(x_a, x_b) sum_c Lf[c*n+a] Rf[c*n+b]: the
+ * gradient with respect to the training inputs, out [n][d], Lf and Rf
+ * [ncols][n].  With Lf = [-alpha/2 | U/(2T)] and Rf = [alpha | Z] (U = K^-1 Z)
+ * it is the marginal likelihood's gradient that goes back into the features
+ * of a deep kernel.  Single radial kernels, d <= 32.  Where the exponent is
+ * clamped (Matern kernels) the derivative keeps the clamped exponential, as
+ * the parameter gradients do; at coincident points it is 0.  No counterpart in
+ * the reference. */
+MGP_API int mgp_input_gradient(void* handle, const float* Lf, const float* Rf,
+                               int ncols, float* out);
+/* Same with device arrays: runs on the caller's HIP stream (NULL: the default
+ * stream), after the work queued there, and returns when it is done. */
+MGP_API int mgp_input_gradient_device(void* handle, const float* Lf_device,
+                                      const float* Rf_device, int ncols,
+                                      float* out_device, void* stream);
+
 /* Isolated timing of provider ops.  Replaces benchmark_provider_ops(info, rhs,
  * num_cols, op_code, repeats, warmup) (jit_engine_bindings.mojo:439-572);
  * op 0 forward matvec, 1 fused gradient products, 2 gradient products + the
@@ -714,6 +730,88 @@ MGP_API int mgp_rff_prior_values(const float* X, int64_t n, int d,
                                  const double* lengthscales, const double* W,
                                  const double* phase, int F, double outputscale,
                                  const double* weights, int K, float* out);
+
+/* ---- Learned features ---------------------------------------------------- */
+/* The layers of a deep kernel: device arrays the caller holds, in float32,
+ * bfloat16 or float16 (element types 0, 1, 2), row-major with unit column
+ * stride and any row stride (in elements).  Unlike the calls above these run
+ * asynchronously on the caller's HIP stream (NULL: the default stream), take
+ * their work buffers from the caller and allocate nothing, so that they can be
+ * recorded into a HIP graph; the device of the arrays must be current.  Sums
+ * and statistics are fp32.  Empty inputs (rows = 0) are valid: sums over them
+ * are 0.  No counterpart in the reference. */
+
+/* One layer norm over the rows of x [rows][width]: y = (x - mean) * rstd *
+ * weight + bias, rstd = 1 / sqrt(var + eps).  weight, bias [width] may be NULL
+ * (ones, zeros); param_type: their type, the element type or float32. */
+typedef struct mgp_layer_norm {
+  int type;
+  int param_type;
+  float eps;
+  int64_t rows;
+  int64_t width;
+  const void* x;
+  int64_t x_stride;
+  const void* weight;
+  const void* bias;
+} mgp_layer_norm_t;
+/* stats (may be NULL): [rows][2], mean and rstd, for the backward pass. */
+MGP_API int mgp_layer_norm_device(const mgp_layer_norm_t* args, void* y, int64_t y_stride,
+                                  float* stats, void* stream);
+/* dx [rows][width], dweight and dbias [width] (of param_type); any may be
+ * NULL.  The workspace (256-byte aligned, its size from the call above the
+ * backward pass) serves the weight's and bias' sums. */
+MGP_API int mgp_layer_norm_backward_workspace(const mgp_layer_norm_t* args, int64_t* bytes);
+MGP_API int mgp_layer_norm_backward_device(const mgp_layer_norm_t* args, const void* dy,
+                                           int64_t dy_stride, const float* stats, void* dx,
+                                           int64_t dx_stride, void* dweight, void* dbias,
+                                           void* workspace, int64_t workspace_bytes,
+                                           void* stream);
+
+/* y = residual + x * keep / (1 - rate) (residual may be NULL).  keep is a
+ * function of seed and the element's draw number offset + row * width + col:
+ * draw q is 16-bit half q % 2 of word (q % 8) / 2 of the Philox4x32-10 block
+ * with counter (q / 8, 0) and key seed, and keeps where it is at least
+ * round(65536 rate); the rate in effect is that multiple of 2^-16.  Dropped
+ * elements are 0 whatever x held.  The backward pass is the same call on dy
+ * with residual NULL.  A step that draws n elements moves the next offset on
+ * by n; multiples of 8 are fastest. */
+MGP_API int mgp_dropout_device(int type, const void* x, int64_t x_stride, int64_t rows,
+                               int64_t width, double rate, uint64_t seed, uint64_t offset,
+                               const void* residual, int64_t residual_stride, void* y,
+                               int64_t y_stride, void* stream);
+
+/* A gated layer: h = act(x w_gate^T + b_gate) * (x w_up^T + b_up), x
+ * [rows][width], weights [hidden][width], biases [hidden] (may be NULL), all of
+ * one element type.  activation: 0 x sigmoid(x), 1 x Phi(x) (exact GELU),
+ * 2 sigmoid, 3 relu. */
+typedef struct mgp_gated_layer {
+  int type;
+  int activation;
+  int64_t rows;
+  int64_t width;
+  int64_t hidden;
+  const void* x;
+  int64_t x_stride;
+  const void* w_gate;
+  int64_t w_gate_stride;
+  const void* w_up;
+  int64_t w_up_stride;
+  const void* b_gate;
+  const void* b_up;
+} mgp_gated_layer_t;
+/* Bytes of workspace (256-byte aligned) of the forward or backward pass. */
+MGP_API int mgp_gated_layer_workspace(const mgp_gated_layer_t* args, int backward,
+                                      int64_t* bytes);
+MGP_API int mgp_gated_layer_device(const mgp_gated_layer_t* args, void* h, int64_t h_stride,
+                                   void* workspace, int64_t workspace_bytes, void* stream);
+/* Gradients from dh [rows][hidden]; the projections are formed again, nothing
+ * is kept from the forward pass.  Contiguous outputs, any may be NULL. */
+MGP_API int mgp_gated_layer_backward_device(const mgp_gated_layer_t* args, const void* dh,
+                                            int64_t dh_stride, void* dx, void* dw_gate,
+                                            void* dw_up, void* db_gate, void* db_up,
+                                            void* workspace, int64_t workspace_bytes,
+                                            void* stream);
 
 /* Streaming device copy of `bytes` repeated `repeats` times; ms_avg gets the
  * mean duration of one copy.  Used only to calibrate HBM byte counters

@@ -50,6 +50,25 @@ class Progress(C.Structure):
     ]
 
 
+class LayerNorm(C.Structure):
+    """mgp_layer_norm_t"""
+    _fields_ = [
+        ("type", C.c_int), ("param_type", C.c_int), ("eps", C.c_float), ("rows", C.c_int64),
+        ("width", C.c_int64), ("x", C.c_void_p), ("x_stride", C.c_int64),
+        ("weight", C.c_void_p), ("bias", C.c_void_p),
+    ]
+
+
+class GatedLayer(C.Structure):
+    """mgp_gated_layer_t"""
+    _fields_ = [
+        ("type", C.c_int), ("activation", C.c_int), ("rows", C.c_int64), ("width", C.c_int64),
+        ("hidden", C.c_int64), ("x", C.c_void_p), ("x_stride", C.c_int64),
+        ("w_gate", C.c_void_p), ("w_gate_stride", C.c_int64), ("w_up", C.c_void_p),
+        ("w_up_stride", C.c_int64), ("b_gate", C.c_void_p), ("b_up", C.c_void_p),
+    ]
+
+
 PROGRESS_CB = C.CFUNCTYPE(None, C.POINTER(Progress), C.c_void_p)
 
 
@@ -262,6 +281,25 @@ _SIGNATURES = {
                                    C.c_int, C.c_int, c_float_p, C.c_int, c_float_p, C.c_int,
                                    C.c_uint64, c_float_p, c_float_p, c_int_p]),
     "mgp_icm_task_covariance_init": (C.c_int, [C.c_int, C.c_int, C.c_int, c_float_p]),
+    "mgp_input_gradient": (C.c_int, [C.c_void_p, c_float_p, c_float_p, C.c_int, c_float_p]),
+    "mgp_input_gradient_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
+                                            C.c_void_p, C.c_void_p]),
+    "mgp_layer_norm_device": (C.c_int, [C.POINTER(LayerNorm), C.c_void_p, C.c_int64, C.c_void_p,
+                                        C.c_void_p]),
+    "mgp_layer_norm_backward_workspace": (C.c_int, [C.POINTER(LayerNorm), c_int64_p]),
+    "mgp_layer_norm_backward_device": (C.c_int, [C.POINTER(LayerNorm), C.c_void_p, C.c_int64,
+                                                 C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p,
+                                                 C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
+    "mgp_dropout_device": (C.c_int, [C.c_int, C.c_void_p, C.c_int64, C.c_int64, C.c_int64,
+                                     C.c_double, C.c_uint64, C.c_uint64, C.c_void_p, C.c_int64,
+                                     C.c_void_p, C.c_int64, C.c_void_p]),
+    "mgp_gated_layer_workspace": (C.c_int, [C.POINTER(GatedLayer), C.c_int, c_int64_p]),
+    "mgp_gated_layer_device": (C.c_int, [C.POINTER(GatedLayer), C.c_void_p, C.c_int64,
+                                         C.c_void_p, C.c_int64, C.c_void_p]),
+    "mgp_gated_layer_backward_device": (C.c_int, [C.POINTER(GatedLayer), C.c_void_p, C.c_int64,
+                                                  C.c_void_p, C.c_void_p, C.c_void_p,
+                                                  C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
+                                                  C.c_void_p]),
     "mgp_rff_prior_values": (C.c_int, [c_float_p, C.c_int64, C.c_int, c_double_p, c_double_p,
                                        c_double_p, C.c_int, C.c_double, c_double_p, C.c_int,
                                        c_float_p]),

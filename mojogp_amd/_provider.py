@@ -199,6 +199,41 @@ class NativeProvider:
                   _lib.dptr(out))
         return out
 
+    def input_gradient(self, Lf, Rf) -> np.ndarray:
+        """out[i, q] = d/dx_iq sum_ab K(x_a, x_b) sum_c Lf[c, a] Rf[c, b] (float32,
+        [n, d]): the gradient with respect to the training inputs."""
+        L, _ = _cols(Lf, self.n)
+        R, _ = _cols(Rf, self.n)
+        if L.shape != R.shape:
+            raise ValueError("Lf and Rf must have the same shape")
+        out = np.empty((self.n, self.d), dtype=np.float32)
+        _lib.call("mgp_input_gradient", self.handle, _lib.fptr(L), _lib.fptr(R), L.shape[0],
+                  _lib.fptr(out))
+        return out
+
+    def input_gradient_device(self, Lf, Rf, out=None):
+        """input_gradient of device tensors ([ncols, n] or [n], float32, contiguous;
+        out [n, d]), on the calling program's current stream.  As every call of a
+        provider it returns when the work is done."""
+        from . import features
+        code, index, stream = features._first(Lf, "Lf")
+        shape = Lf.shape
+        if code != 0 or len(shape) not in (1, 2) or shape[-1] != self.n or 0 in shape:
+            raise ValueError(f"Lf must be float32 of shape (ncols, {self.n}), got "
+                             f"{Lf.dtype} {tuple(shape)}")
+        features._rows(Rf, "Rf", code, index, shape)
+        if not Lf.is_contiguous() or not Rf.is_contiguous():
+            raise ValueError("Lf and Rf must be contiguous")
+        if out is None:
+            out = Lf.new_empty((self.n, self.d))
+        else:
+            features._rows(out, "out", code, index, (self.n, self.d))
+            if not out.is_contiguous():
+                raise ValueError("out must be contiguous")
+        _lib.call("mgp_input_gradient_device", self.handle, Lf.data_ptr(), Rf.data_ptr(),
+                  shape[0] if len(shape) == 2 else 1, out.data_ptr(), stream)
+        return out
+
     def gradient_matvec(self, V) -> np.ndarray:
         """out[p, c, i] = sum_j dk_p(x_i, x_j) V[c, j] for the P engine parameters."""
         Vc, vec = _cols(V, self.n)

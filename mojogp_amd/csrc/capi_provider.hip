@@ -499,6 +499,35 @@ int mgp_gradient_trace(void* h, const float* Lf, const float* Rf, int ncols, dou
   });
 }
 
+int mgp_input_gradient(void* h, const float* Lf, const float* Rf, int ncols, float* out) {
+  return guarded([&] {
+    Provider* pv = as_provider(h);
+    MGP_REQUIRE(Lf && Rf && out && ncols >= 1, "bad arguments");
+    const size_t tot = (size_t)pv->n * ncols;
+    float* dl = pv->io_a.ensure(tot);
+    float* dr = pv->io_b.ensure(tot);
+    float* dg = pv->io_c.ensure((size_t)pv->n * pv->d);
+    MGP_HIP_CHECK(hipMemcpyAsync(dl, Lf, tot * sizeof(float), hipMemcpyHostToDevice, pv->st));
+    MGP_HIP_CHECK(hipMemcpyAsync(dr, Rf, tot * sizeof(float), hipMemcpyHostToDevice, pv->st));
+    point_gradient(*pv, dl, dr, ncols, dg, pv->st);
+    MGP_HIP_CHECK(hipMemcpyAsync(out, dg, (size_t)pv->n * pv->d * sizeof(float),
+                                 hipMemcpyDeviceToHost, pv->st));
+    MGP_HIP_CHECK(hipStreamSynchronize(pv->st));
+  });
+}
+
+int mgp_input_gradient_device(void* h, const float* Lf_dev, const float* Rf_dev, int ncols,
+                              float* out_dev, void* stream) {
+  return guarded([&] {
+    Provider* pv = as_provider(h);
+    MGP_REQUIRE(ncols >= 1, "ncols must be >= 1");
+    MGP_REQUIRE(Lf_dev && Rf_dev && out_dev, "null device array");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    point_gradient(*pv, Lf_dev, Rf_dev, ncols, out_dev, st);
+    MGP_HIP_CHECK(hipStreamSynchronize(st));
+  });
+}
+
 int mgp_benchmark_provider_ops(void* h, const float* rhs, int ncols, int op,
                                int repeats, int warmup, double* times_ms,
                                double* tile_ms_avg, float* out_or_null) {

@@ -24,32 +24,6 @@ constexpr int kGpCols = 16;              // factor columns per pass
 constexpr int kGpStride = kGpBlock + 16; // LDS stride of a factor column
 constexpr int kGpFlush = 2;              // 16-column tiles between fp64 flushes
 
-// k / os and the lengthscale factor h (dk/dl_q = os h dz_q^2 / (s^2 l_q)) from
-// the scaled squared distance.
-template <int KIND, bool ARD>
-__device__ __forceinline__ void value_and_h(float r2, float& kv, float& h) {
-  if constexpr (KIND == KIND_RBF) {
-    kv = __builtin_amdgcn_exp2f(-r2);  // not clamped
-    h = kv;
-  } else if constexpr (KIND == KIND_MATERN12) {
-    // h = log2(e) k / r with the reference's floored r = sqrt(r^2 + 1e-20);
-    // the exponent is clamped for ARD only (exp2_limit)
-    const float u = __builtin_amdgcn_sqrtf(r2);
-    kv = __builtin_amdgcn_exp2f(ARD ? -fminf(u, kExp2Clamp) : -u);
-    h = kLog2e * kv / __builtin_amdgcn_sqrtf(r2 + kM12RFloor);
-  } else if constexpr (KIND == KIND_MATERN32) {
-    const float u = __builtin_amdgcn_sqrtf(r2);
-    const float e = __builtin_amdgcn_exp2f(-fminf(u, kExp2Clamp));
-    kv = fmaf(u, kLn2, 1.0f) * e;
-    h = 3.0f * e;
-  } else {
-    const float u = __builtin_amdgcn_sqrtf(r2);
-    const float e = __builtin_amdgcn_exp2f(-fminf(u, kExp2Clamp));
-    kv = fmaf(u, fmaf(u, kM52B, kM52A), 1.0f) * e;
-    h = (5.0f / 3.0f) * fmaf(u, kLn2, 1.0f) * e;
-  }
-}
-
 // part[(y gx + x) nterms + q] = the workgroup's share of
 //   sum_ab W_ab h_ab dz_abq^2 (ARD: q < d; isotropic: the sum over q), then
 //   sum_ab W_ab k_ab / os,                W_ab = sum_c Lf[c][a] Rf[c][b].

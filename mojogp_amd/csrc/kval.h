@@ -43,4 +43,30 @@ __device__ __forceinline__ float kval(float s, float clampv = kExp2Clamp) {
   }
 }
 
+// k / os and the lengthscale factor h (dk/dl_q = os h dz_q^2 / (s^2 l_q)) from
+// the scaled squared distance.
+template <int KIND, bool ARD>
+__device__ __forceinline__ void value_and_h(float r2, float& kv, float& h) {
+  if constexpr (KIND == KIND_RBF) {
+    kv = __builtin_amdgcn_exp2f(-r2);  // not clamped
+    h = kv;
+  } else if constexpr (KIND == KIND_MATERN12) {
+    // h = log2(e) k / r with the reference's floored r = sqrt(r^2 + 1e-20);
+    // the exponent is clamped for ARD only (exp2_limit)
+    const float u = __builtin_amdgcn_sqrtf(r2);
+    kv = __builtin_amdgcn_exp2f(ARD ? -fminf(u, kExp2Clamp) : -u);
+    h = kLog2e * kv / __builtin_amdgcn_sqrtf(r2 + kM12RFloor);
+  } else if constexpr (KIND == KIND_MATERN32) {
+    const float u = __builtin_amdgcn_sqrtf(r2);
+    const float e = __builtin_amdgcn_exp2f(-fminf(u, kExp2Clamp));
+    kv = fmaf(u, kLn2, 1.0f) * e;
+    h = 3.0f * e;
+  } else {
+    const float u = __builtin_amdgcn_sqrtf(r2);
+    const float e = __builtin_amdgcn_exp2f(-fminf(u, kExp2Clamp));
+    kv = fmaf(u, fmaf(u, kM52B, kM52A), 1.0f) * e;
+    h = (5.0f / 3.0f) * fmaf(u, kLn2, 1.0f) * e;
+  }
+}
+
 }  // namespace mgp

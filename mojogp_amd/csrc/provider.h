@@ -135,10 +135,16 @@ struct Provider {
   // (pack_rhs over train), if the caller keeps one.
   void cross(const PackedPoints& rows, const float* V, int ncols, float* out,
              const RhsPack* packed = nullptr);
+  DevBuf<float> pg_ws;  // split sums of the input gradient
   DevBuf<float> love_v, love_var, love_diag;  // LOVE variance of a test set
   // out[c*n + i] = k(rows[r0 + c], x_i) for c < nrows (dense cross block).
   void fill_block(const PackedPoints& rows, int64_t r0, int64_t nrows, float* out);
 };
+
+// out[i][q] = d/dx_iq sum_ab K_ab sum_c Lf[c][a] Rf[c][b] over the training points
+// (device arrays, Lf and Rf [ncols][n], out [n][d]), on stream st.
+void point_gradient(Provider& pv, const float* Lf, const float* Rf, int ncols, float* out,
+                    hipStream_t st);
 
 // Live provider handles.  Every C entry point turns a handle into a Provider
 // through checked_provider(), which rejects null, unknown and destroyed handles
