@@ -33,19 +33,45 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 
 // ---------------------------------------------------------------- activation
 
+// 1 / (1 + exp(-g)).  FAST (the 16-bit types): one v_exp and one v_rcp, good to
+// a few fp32 roundings, where expf and a division cost ~40 instructions (the
+// epilogue of 65536 x 1024 -> 4096 took a quarter of the kernel's time).
+template <bool FAST>
+__device__ __forceinline__ float sigmoid(float g) {
+  if constexpr (FAST)
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * g));
+  else
+    return 1.0f / (1.0f + expf(-g));
+}
+
 // a = act(g) and its derivative
-template <int ACT>
+template <int ACT, bool FAST>
 __device__ __forceinline__ void activate(float g, float& a, float& slope) {
   if constexpr (ACT == ACT_SILU) {
-    const float s = 1.0f / (1.0f + expf(-g));
+    const float s = sigmoid<FAST>(g);
     a = g * s;
     slope = s * fmaf(g, 1.0f - s, 1.0f);
   } else if constexpr (ACT == ACT_SIGMOID) {
-    a = 1.0f / (1.0f + expf(-g));
+    a = sigmoid<FAST>(g);
     slope = a * (1.0f - a);
   } else if constexpr (ACT == ACT_RELU) {
-    a = g > 0.0f ? g : g * 0.0f;  // NaN stays NaN
+    a = g > 0.0f || g != g ? g : 0.0f;
     slope = g > 0.0f ? 1.0f : 0.0f;
+  } else if constexpr (FAST) {
+    // the normal integral by Abramowitz and Stegun 7.1.26 (absolute error
+    // 1.5e-7, a thousandth of the 16-bit types' rounding), whose exponential
+    // the derivative takes too
+    const float x = fabsf(g) * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.0f));
+    const float e = __builtin_amdgcn_exp2f(-0.5f * kLog2e * g * g);
+    const float q =
+        t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f),
+                         -0.284496736f),
+                 0.254829592f);
+    const float tail = 0.5f * q * e;  // 1 - Phi(|g|)
+    const float cdf = g > 0.0f ? 1.0f - tail : tail;
+    a = g * cdf;
+    slope = fmaf(g * 0.39894228040143268f, e, cdf);
   } else {
     const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
     a = g * cdf;
@@ -53,34 +79,31 @@ __device__ __forceinline__ void activate(float g, float& a, float& slope) {
   }
 }
 
-// Four consecutive elements of a row; vec: the row is aligned for them.
-template <class T>
-struct alignas(4 * sizeof(T)) Vec4 {
-  T v[4];
-};
-
-template <class T>
-__device__ __forceinline__ void load4(const T* p, int64_t left, bool vec, float* v) {
-  if (vec && left >= 4) {
-    const Vec4<T> a = *reinterpret_cast<const Vec4<T>*>(p);
+// N consecutive elements of a row, of which `left` exist; whole runs go as
+// vectors, which the memory path takes at any alignment.
+template <int N, class T>
+__device__ __forceinline__ void load_run(const T* p, int64_t left, float* v) {
+  if (left >= N) {
+    T a[N];
+    __builtin_memcpy(a, p, N * sizeof(T));
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = (float)a.v[k];
+    for (int k = 0; k < N; ++k) v[k] = (float)a[k];
   } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = k < left ? (float)p[k] : 0.0f;
+    for (int k = 0; k < N; ++k) v[k] = k < left ? (float)p[k] : 0.0f;
   }
 }
 
-template <class T>
-__device__ __forceinline__ void store4(T* p, int64_t left, bool vec, const float* v) {
-  if (vec && left >= 4) {
-    Vec4<T> a;
+template <int N, class T>
+__device__ __forceinline__ void store_run(T* p, int64_t left, const float* v) {
+  if (left >= N) {
+    T a[N];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) a.v[k] = (T)v[k];
-    *reinterpret_cast<Vec4<T>*>(p) = a;
+    for (int k = 0; k < N; ++k) a[k] = (T)v[k];
+    __builtin_memcpy(p, a, N * sizeof(T));
   } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < N; ++k)
       if (k < left) p[k] = (T)v[k];
   }
 }
@@ -125,19 +148,19 @@ struct Operand {
   const char* base;
   const char* base2;
   int64_t ld_bytes;
-  int64_t ld2_bytes;
   int64_t n;
 };
 
 struct GemmShape {
   Operand p, q;       // p: the side whose rows are the output's columns
   int64_t K;          // reduction length
-  int tiles_p, tiles_q;
+  int64_t tiles_p, tiles_q;
   int64_t k_split;    // reduction elements of one split (a multiple of a stage)
 };
 
 // Tile of 16 TN WN columns (p rows) by 16 TM WM rows (q rows), one wave 16 TN
-// by 16 TM of it.  Both operands go through LDS by direct loads, double
+// by 16 TM of it.  NT: the p rows are dealt to LDS so that a lane's results are
+// RUN = 4 TN (dual: 2 TN of each matrix) consecutive columns.  Both operands go through LDS by direct loads, double
 // buffered, 128 bytes of reduction a stage.  NT: 128-byte LDS rows, 16-byte
 // chunk c of row r at c ^ (r / 2 % 8).  TN: LDS rows of the tile's width, one
 // per reduction step, in the memory's order; 32-byte granules at g ^ (r % 8)
@@ -150,6 +173,8 @@ struct Tile {
   static constexpr bool TR = TR_, DUAL = DUAL_;
   static constexpr int W = WM * WN, THREADS = 64 * W;
   static constexpr int BQ = 16 * TM * WM, BP = 16 * TN * WN;
+  static constexpr int T1 = DUAL ? TN / 2 : TN;  // 16-row tiles of one matrix a wave
+  static constexpr int RUN = 4 * T1;
   static constexpr int E = sizeof(T);
   static constexpr int KS = kStageBytes / E;       // reduction elements a stage
   static constexpr int LDS = (BP + BQ) * kStageBytes;  // one buffer
@@ -157,54 +182,61 @@ struct Tile {
   static_assert(IP * W * 1024 == BP * kStageBytes && IQ * W * 1024 == BQ * kStageBytes, "");
 };
 
+// What a wave loads of a stage: I instructions a side, each 64 lanes x 16 bytes
+// = 1 KB of LDS.  The instructions of a side lie a multiple of 8 LDS rows (TN:
+// of 8, fp32 4, reduction rows) apart, so the lanes' offsets from each one's
+// uniform base are the same; only which rows exist differs.
 template <class TL>
 struct Loader {
-  int voff[TL::IP + TL::IQ];
-  int kcol[TL::IP + TL::IQ];  // NT: first reduction element; TN: reduction row
-  const char* base[TL::IP + TL::IQ];
+  static constexpr int I = TL::IP + TL::IQ;
+  int voff[2];        // byte offset of the lane from an instruction's base
+  int kpos[2];        // NT: its reduction element, TN: its reduction row within the stage
+  bool exists[I];     // NT: its row is one of the matrix
+  const char* base[I];
 
   template <bool P>
   __device__ __forceinline__ void init_side(const Operand& o, int64_t row0, int64_t k0) {
-    constexpr int I = P ? TL::IP : TL::IQ, S = P ? 0 : TL::IP;
+    constexpr int N = P ? TL::IP : TL::IQ, S = P ? 0 : TL::IP;
     constexpr int B = P ? TL::BP : TL::BQ;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if constexpr (!TL::TR) {
+      static_assert(TL::W % 2 == 0, "");  // the swizzle is that of wave * 8 + lane / 8
+      const int l8 = lane / 8;
+      const int c = (lane & 7) ^ ((wave * 4 + lane / 16) & 7);
+      // P: LDS row (wave w, matrix, tile t, row i) holds column
+      // 16 T1 w + (i / 4) RUN + 4 t + i % 4
+      const int lrow = P ? l8 / 4 * TL::RUN + l8 % 4 : l8;
+      kpos[!P] = c * (16 / TL::E);
+      voff[!P] = (int)(lrow * o.ld_bytes) + c * 16;
 #pragma unroll
-    for (int i = 0; i < I; ++i) {
-      const int id = i * TL::W + wave;
-      if constexpr (!TL::TR) {
-        const int r = id * 8 + lane / 8;  // tile row
-        const int c = (lane & 7) ^ ((r >> 1) & 7);
-        if constexpr (P && TL::DUAL) {
-          // the wave's rows: first half gate, second half up, of the same columns
-          constexpr int WR = 16 * TL::TN, H = WR / 2;
-          const int r8 = id * 8;
-          const bool up = (r8 % WR) >= H;  // wave uniform: H is a multiple of 8
-          const int64_t f0 = row0 + (r8 / WR) * H + r8 % H;
-          const int64_t f = min(f0 + lane / 8, o.n - 1);
-          const int64_t fb = min(f0, o.n - 1);
-          base[S + i] = (up ? o.base2 + fb * o.ld2_bytes : o.base + fb * o.ld_bytes) + k0 * TL::E;
-          voff[S + i] = (int)((f - fb) * (up ? o.ld2_bytes : o.ld_bytes)) + c * 16;
-        } else {
-          const int64_t rr = min(row0 + r, o.n - 1), rb = min(row0 + id * 8, o.n - 1);
-          base[S + i] = o.base + rb * o.ld_bytes + k0 * TL::E;
-          voff[S + i] = (int)((rr - rb) * o.ld_bytes) + c * 16;
+      for (int i = 0; i < N; ++i) {
+        const int r8 = (i * TL::W + wave) * 8;
+        int64_t r = row0 + r8;
+        const char* from = o.base;
+        if constexpr (P) {
+          const int t = r8 % (16 * TL::TN) / 16;
+          const bool up = t >= TL::T1;  // wave uniform
+          r = row0 + r8 / (16 * TL::TN) * 16 * TL::T1 + r8 % 16 / 4 * TL::RUN +
+              (up ? t - TL::T1 : t) * 4;
+          if (up) from = o.base2;
         }
-        kcol[S + i] = c * (16 / TL::E);
-      } else {
-        constexpr int RB = B * TL::E;  // bytes of an LDS row
-        const int byte = id * 1024 + lane * 16;
-        const int r = byte / RB;
-        int c = (byte % RB) / 16;
-        constexpr int M = RB / 16 - 1;
-        c ^= (TL::E == 2 ? ((r & 7) << 1) : ((r & 3) << 2)) & M;
-        const int64_t col = row0 + c * (16 / TL::E);
-        constexpr int R8 = 1024 / RB > 0 ? 1024 / RB : 1;  // rows an instruction covers
-        const int rb = id * 1024 / RB;
-        static_assert(R8 >= 1, "");
-        base[S + i] = o.base + (k0 + rb) * o.ld_bytes + row0 * TL::E;
-        voff[S + i] = col < o.n ? (int)((r - rb) * o.ld_bytes) + c * 16 : kOutOfRange;
-        kcol[S + i] = r;
+        exists[S + i] = r + lrow < o.n;
+        base[S + i] = from + r * o.ld_bytes + k0 * TL::E;
+      }
+    } else {
+      constexpr int RB = B * TL::E;  // bytes of an LDS row
+      static_assert(TL::W * 1024 / RB % 8 == 0, "");
+      const int byte = wave * 1024 + lane * 16, r = byte / RB, rb = wave * 1024 / RB;
+      const int c = (byte % RB / 16) ^
+                    ((TL::E == 2 ? ((r & 7) << 1) : ((r & 3) << 2)) & (RB / 16 - 1));
+      const bool in = row0 + c * (16 / TL::E) < o.n;
+      kpos[!P] = r;
+      voff[!P] = (int)((r - rb) * o.ld_bytes) + c * 16;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        exists[S + i] = in;
+        base[S + i] = o.base + (k0 + i * (TL::W * 1024 / RB) + rb) * o.ld_bytes + row0 * TL::E;
       }
     }
   }
@@ -213,12 +245,14 @@ struct Loader {
   __device__ __forceinline__ void load(char* __restrict__ buf, int64_t left, int64_t ldp,
                                        int64_t ldq) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l = (int)min(left, (int64_t)TL::KS);
 #pragma unroll
-    for (int i = 0; i < TL::IP + TL::IQ; ++i) {
+    for (int i = 0; i < I; ++i) {
       const bool p = i < TL::IP;
-      const int id = (p ? i : i - TL::IP) * TL::W + wave;
-      char* dst = buf + (p ? 0 : TL::BP * kStageBytes) + id * 1024;
-      load_lds(base[i], kcol[i] < left ? voff[i] : kOutOfRange, dst);
+      const int j = p ? i : i - TL::IP;
+      char* dst = buf + (p ? 0 : TL::BP * kStageBytes) + (j * TL::W + wave) * 1024;
+      const int step = TL::TR ? j * (TL::W * 1024 / ((p ? TL::BP : TL::BQ) * TL::E)) : 0;
+      load_lds(base[i], exists[i] && kpos[!p] < l - step ? voff[!p] : kOutOfRange, dst);
       base[i] += TL::TR ? (int64_t)TL::KS * (p ? ldp : ldq) : (int64_t)kStageBytes;
     }
   }
@@ -285,15 +319,30 @@ __device__ __forceinline__ void stage(Loader<TL>& ld, char* __restrict__ cur,
   __syncthreads();
 }
 
-// Element (m, n) of the tile: acc[tm][tn][e] of lane l holds output row
-// 16 (wm TM + tm) + l % 16, column 16 (wn TN + tn) + 4 (l / 16) + e.
+// Workgroups go round the 8 XCDs in turn: each XCD takes a stretch of tiles of
+// its own, ordered in groups of 8 tile rows, so that what its L2 holds serves
+// the tiles in flight on it.
+__device__ __forceinline__ void tile_of(int64_t id, int64_t tiles_p, int64_t tiles_q, int64_t& tp,
+                                        int64_t& tq) {
+  const int64_t total = tiles_p * tiles_q, xcd = id & 7, per = total >> 3, rest = total & 7;
+  id = xcd * per + min(xcd, rest) + (id >> 3);
+  const int64_t group = id / (8 * tiles_p), in = id - group * 8 * tiles_p;
+  const int64_t height = min((int64_t)8, tiles_q - group * 8);
+  tq = group * 8 + in % height;
+  tp = in / height;
+}
+
+// acc[tm][tn][e] of lane l holds output row 16 (wm TM + tm) + l % 16 and column
+// (NT, tn < T1) 16 T1 wn + RUN (l / 16) + 4 tn + e of either matrix, (TN)
+// 16 (wn TN + tn) + 4 (l / 16) + e.
 template <class TL, class EPI>
 __global__ __launch_bounds__(TL::THREADS) void k_gemm(GemmShape s, EPI epi) {
   __shared__ __align__(1024) char b0[TL::LDS];
   __shared__ __align__(1024) char b1[TL::LDS];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % TL::WM, wn = wave / TL::WM;
-  const int tp = blockIdx.x % s.tiles_p, tq = blockIdx.x / s.tiles_p;
+  int64_t tp, tq;
+  tile_of(blockIdx.x, s.tiles_p, s.tiles_q, tp, tq);
   constexpr int CP = TL::DUAL ? TL::BP / 2 : TL::BP;  // output columns a tile
   const int64_t n0 = (int64_t)tp * CP, m0 = (int64_t)tq * TL::BQ;
   const int64_t k0 = (int64_t)blockIdx.y * s.k_split;
@@ -309,12 +358,23 @@ __global__ __launch_bounds__(TL::THREADS) void k_gemm(GemmShape s, EPI epi) {
   ld.template init_side<true>(s.p, n0, k0);
   ld.template init_side<false>(s.q, m0, k0);
   const int64_t ldp = s.p.ld_bytes, ldq = s.q.ld_bytes;
-  ld.load(b0, K, ldp, ldq);
-  __syncthreads();
-  for (int64_t k = 0; k < K; k += 2 * TL::KS) {
-    stage<TL>(ld, b0, b1, K - k - TL::KS, ldp, ldq, wm, wn, acc);
-    if (k + TL::KS >= K) break;
-    stage<TL>(ld, b1, b0, K - k - 2 * TL::KS, ldp, ldq, wm, wn, acc);
+  // pairs of stages, so that each has its own buffers at compile time; an odd
+  // one goes first
+  int64_t left = K;
+  if ((K + TL::KS - 1) / TL::KS % 2 == 1) {
+    ld.load(b1, left, ldp, ldq);
+    __syncthreads();
+    left -= TL::KS;
+    stage<TL>(ld, b1, b0, left, ldp, ldq, wm, wn, acc);
+  } else {
+    ld.load(b0, left, ldp, ldq);
+    __syncthreads();
+  }
+  while (left > 0) {
+    left -= TL::KS;
+    stage<TL>(ld, b0, b1, left, ldp, ldq, wm, wn, acc);
+    left -= TL::KS;
+    stage<TL>(ld, b1, b0, left, ldp, ldq, wm, wn, acc);
   }
   epi.template run<TL>(acc, m0 + wm * TL::TM * 16, n0 + wn * (CP / TL::WN), tq * TL::WM + wm);
 }
@@ -326,32 +386,30 @@ struct ForwardEpi {
   const T *bg, *bu;
   T* h;
   int64_t ldh, rows, hidden;
-  int vec;
   template <class TL>
   __device__ __forceinline__ void run(f4 (&acc)[TL::TM][TL::TN], int64_t m0, int64_t n0,
                                       int64_t) const {
+    constexpr int N = TL::RUN;
     const int lane = threadIdx.x & 63;
+    const int64_t f = n0 + N * (lane >> 4), left = hidden - f;
+    if (left <= 0) return;
+    float g0[N], u0[N];
 #pragma unroll
-    for (int n = 0; n < TL::TN / 2; ++n) {
-      const int64_t f = n0 + n * 16 + 4 * (lane >> 4);
-      if (f >= hidden) continue;
-      const int64_t left = hidden - f;
-      float g0[4] = {0, 0, 0, 0}, u0[4] = {0, 0, 0, 0};
-      if (bg) load4(bg + f, left, false, g0);
-      if (bu) load4(bu + f, left, false, u0);
+    for (int k = 0; k < N; ++k) g0[k] = u0[k] = 0.0f;
+    if (bg) load_run<N>(bg + f, left, g0);
+    if (bu) load_run<N>(bu + f, left, u0);
 #pragma unroll
-      for (int m = 0; m < TL::TM; ++m) {
-        const int64_t r = m0 + m * 16 + (lane & 15);
-        if (r >= rows) continue;
-        float o[4];
+    for (int m = 0; m < TL::TM; ++m) {
+      const int64_t r = m0 + m * 16 + (lane & 15);
+      if (r >= rows) continue;
+      float o[N];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float a, slope;
-          activate<ACT>(acc[m][n][e] + g0[e], a, slope);
-          o[e] = a * (acc[m][n + TL::TN / 2][e] + u0[e]);
-        }
-        store4(h + r * ldh + f, left, vec, o);
+      for (int k = 0; k < N; ++k) {
+        float a, slope;
+        activate<ACT, sizeof(T) == 2>(acc[m][k / 4][k % 4] + g0[k], a, slope);
+        o[k] = a * (acc[m][TL::T1 + k / 4][k % 4] + u0[k]);
       }
+      store_run<N>(h + r * ldh + f, left, o);
     }
   }
 };
@@ -365,53 +423,50 @@ struct BackwardEpi {
   int64_t lddh, rows, hidden, pad;
   T* dgu;
   float* dbias;  // or null
-  int vec;
   template <class TL>
   __device__ __forceinline__ void run(f4 (&acc)[TL::TM][TL::TN], int64_t m0, int64_t n0,
                                       int64_t part) const {
+    constexpr int N = TL::RUN;
     const int lane = threadIdx.x & 63;
+    const int64_t f = n0 + N * (lane >> 4), left = hidden - f;
+    float g0[N], u0[N], sg[N], su[N];
 #pragma unroll
-    for (int n = 0; n < TL::TN / 2; ++n) {
-      const int64_t f = n0 + n * 16 + 4 * (lane >> 4);
-      const int64_t left = hidden - f;
-      float g0[4] = {0, 0, 0, 0}, u0[4] = {0, 0, 0, 0}, sg[4] = {0, 0, 0, 0}, su[4] = {0, 0, 0, 0};
-      if (f < hidden) {
-        if (bg) load4(bg + f, left, false, g0);
-        if (bu) load4(bu + f, left, false, u0);
+    for (int k = 0; k < N; ++k) g0[k] = u0[k] = sg[k] = su[k] = 0.0f;
+    if (left > 0) {
+      if (bg) load_run<N>(bg + f, left, g0);
+      if (bu) load_run<N>(bu + f, left, u0);
+    }
+#pragma unroll
+    for (int m = 0; m < TL::TM; ++m) {
+      const int64_t r = m0 + m * 16 + (lane & 15);
+      if (r >= rows || f >= pad) continue;
+      float d[N], dg[N], du[N];
+      load_run<N>(dh + r * lddh + f, left, d);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        float a, slope;
+        activate<ACT, sizeof(T) == 2>(acc[m][k / 4][k % 4] + g0[k], a, slope);
+        // columns past hidden are products of the last weights: cut off
+        const bool in = k < left;
+        dg[k] = in ? d[k] * (acc[m][TL::T1 + k / 4][k % 4] + u0[k]) * slope : 0.0f;
+        du[k] = in ? d[k] * a : 0.0f;
+        sg[k] += dg[k];
+        su[k] += du[k];
       }
+      store_run<N>(dgu + r * 2 * pad + f, pad - f, dg);
+      store_run<N>(dgu + r * 2 * pad + pad + f, pad - f, du);
+    }
+    if (dbias) {
 #pragma unroll
-      for (int m = 0; m < TL::TM; ++m) {
-        const int64_t r = m0 + m * 16 + (lane & 15);
-        if (r >= rows || f >= pad) continue;
-        float d[4] = {0, 0, 0, 0}, dg[4], du[4];
-        if (f < hidden) load4(dh + r * lddh + f, left, vec, d);
+      for (int k = 0; k < N; ++k) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float a, slope;
-          activate<ACT>(acc[m][n][e] + g0[e], a, slope);
-          // columns past hidden are products of the last weights: cut off
-          const bool in = e < left;
-          dg[e] = in ? d[e] * (acc[m][n + TL::TN / 2][e] + u0[e]) * slope : 0.0f;
-          du[e] = in ? d[e] * a : 0.0f;
-          sg[e] += dg[e];
-          su[e] += du[e];
+        for (int o = 8; o >= 1; o >>= 1) {
+          sg[k] += __shfl_xor(sg[k], o);
+          su[k] += __shfl_xor(su[k], o);
         }
-        // pad is a multiple of 4 and dgu aligned: whole vectors
-        store4(dgu + r * 2 * pad + f, 4, true, dg);
-        store4(dgu + r * 2 * pad + pad + f, 4, true, du);
-      }
-      if (dbias) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-#pragma unroll
-          for (int o = 8; o >= 1; o >>= 1) {
-            sg[e] += __shfl_xor(sg[e], o);
-            su[e] += __shfl_xor(su[e], o);
-          }
-          if ((lane & 15) == 0 && e < left) {
-            dbias[(part * 2) * hidden + f + e] = sg[e];
-            dbias[(part * 2 + 1) * hidden + f + e] = su[e];
-          }
+        if ((lane & 15) == 0 && k < left) {
+          dbias[(part * 2) * hidden + f + k] = sg[k];
+          dbias[(part * 2 + 1) * hidden + f + k] = su[k];
         }
       }
     }
@@ -422,22 +477,21 @@ template <class T>
 struct StoreEpi {
   T* out;
   int64_t ld, rows, cols;
-  int vec;
   template <class TL>
   __device__ __forceinline__ void run(f4 (&acc)[TL::TM][TL::TN], int64_t m0, int64_t n0,
                                       int64_t) const {
+    constexpr int N = TL::RUN;
     const int lane = threadIdx.x & 63;
+    const int64_t c = n0 + N * (lane >> 4);
+    if (c >= cols) return;
 #pragma unroll
-    for (int n = 0; n < TL::TN; ++n) {
-      const int64_t c = n0 + n * 16 + 4 * (lane >> 4);
-      if (c >= cols) continue;
+    for (int m = 0; m < TL::TM; ++m) {
+      const int64_t r = m0 + m * 16 + (lane & 15);
+      if (r >= rows) continue;
+      float o[N];
 #pragma unroll
-      for (int m = 0; m < TL::TM; ++m) {
-        const int64_t r = m0 + m * 16 + (lane & 15);
-        if (r >= rows) continue;
-        float o[4] = {acc[m][n][0], acc[m][n][1], acc[m][n][2], acc[m][n][3]};
-        store4(out + r * ld + c, cols - c, vec, o);
-      }
+      for (int k = 0; k < N; ++k) o[k] = acc[m][k / 4][k % 4];
+      store_run<N>(out + r * ld + c, cols - c, o);
     }
   }
 };
@@ -449,7 +503,6 @@ struct WeightEpi {
   T *dw_gate, *dw_up;
   float* part;
   int64_t hidden, pad, width;
-  int vec;
   template <class TL>
   __device__ __forceinline__ void run(f4 (&acc)[TL::TM][TL::TN], int64_t m0, int64_t n0,
                                       int64_t) const {
@@ -466,11 +519,11 @@ struct WeightEpi {
         if (c >= width) continue;
         float o[4] = {acc[m][n][0], acc[m][n][1], acc[m][n][2], acc[m][n][3]};
         if (part) {
-          store4(part + (((int64_t)blockIdx.y * 2 + up) * hidden + f) * width + c, width - c, vec,
-                 o);
+          store_run<4>(part + (((int64_t)blockIdx.y * 2 + up) * hidden + f) * width + c, width - c,
+                       o);
         } else {
           T* dst = up ? dw_up : dw_gate;
-          if (dst) store4(dst + f * width + c, width - c, vec, o);
+          if (dst) store_run<4>(dst + f * width + c, width - c, o);
         }
       }
     }
@@ -498,14 +551,13 @@ __global__ __launch_bounds__(256) void k_pack_rows(const T* __restrict__ src, in
 
 // dst[k][part pad + f] = W_part[f][k], zeros for f past hidden; 32 x 32 tiles
 template <class T>
-__global__ __launch_bounds__(256) void k_transpose_weights(const T* __restrict__ wg, int64_t ldg,
-                                                           const T* __restrict__ wu, int64_t ldu,
+__global__ __launch_bounds__(256) void k_transpose_weights(const T* __restrict__ wg,
+                                                           const T* __restrict__ wu, int64_t ld,
                                                            int64_t hidden, int64_t width,
                                                            int64_t pad, T* __restrict__ dst) {
   __shared__ T tile[32][33];
   const int64_t f0 = (int64_t)blockIdx.x * 32, k0 = (int64_t)blockIdx.y * 32;
   const T* w = blockIdx.z ? wu : wg;
-  const int64_t ld = blockIdx.z ? ldu : ldg;
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
 #pragma unroll
   for (int i = 0; i < 32; i += 8) {
@@ -562,17 +614,26 @@ __global__ __launch_bounds__(1024) void k_sum_bias(const float* __restrict__ par
 // ---------------------------------------------------------------- host side
 
 // Rows the product kernel can load directly: 16-byte aligned, whole 16-byte
-// chunks, and eight rows within 31-bit offsets.
+// chunks, and the rows of one load within 31-bit offsets.
 template <class T>
 bool direct(const void* p, int64_t stride, int64_t cols) {
   return aligned16(p) && stride % Vec16<T>::N == 0 && cols % Vec16<T>::N == 0 &&
-         stride * (int64_t)sizeof(T) < (int64_t)1 << 27;
+         stride * (int64_t)sizeof(T) < (int64_t)1 << 26;
 }
 
 constexpr size_t kAlign = 256;
 inline size_t align_up(size_t b) { return (b + kAlign - 1) / kAlign * kAlign; }
 
-constexpr int kBQ = 128, kBP = 128;
+// The two tile sizes: 256 x 256, one workgroup of 8 waves a CU, and 128 x 128,
+// two workgroups of 4 waves, for what would leave CUs idle otherwise.
+template <class T, bool TR, bool DUAL>
+using BigTile = Tile<T, 8, 4, 2, 4, TR, DUAL>;
+template <class T, bool TR, bool DUAL>
+using SmallTile = Tile<T, 4, 4, 2, 2, TR, DUAL>;
+constexpr int64_t kBigTiles = 512;  // 256 x 256 tiles from which on they are taken
+inline bool big_tiles(int64_t p_rows, int64_t q_rows) {
+  return ceil_div(p_rows, (int64_t)256) * ceil_div(q_rows, (int64_t)256) >= kBigTiles;
+}
 constexpr int64_t kSplitTarget = 512;  // workgroups the weight gradient aims at
 
 // What a call needs and where it lies in the workspace.
@@ -582,7 +643,8 @@ struct Plan {
   bool pack_x, pack_w;
   size_t x_off = 0, wg_off = 0, wu_off = 0, wt_off = 0, dgu_off = 0, dbias_off = 0, part_off = 0;
   size_t bytes = 0;
-  int64_t q_tiles = 0, splits = 1, k_split = 0;
+  bool big_dual = false, big_dx = false, big_dw = false;
+  int64_t bias_parts = 0, splits = 1, k_split = 0;
 
   Plan(const GatedArgs& a, bool backward) {
     constexpr int N = Vec16<T>::N;
@@ -590,7 +652,7 @@ struct Plan {
     hpad = round_up(a.hidden, N);
     pack_x = !direct<T>(a.x, a.x_stride, a.width);
     pack_w = !direct<T>(a.w_gate, a.w_gate_stride, a.width) ||
-             !direct<T>(a.w_up, a.w_up_stride, a.width);
+             !direct<T>(a.w_up, a.w_up_stride, a.width) || a.w_gate_stride != a.w_up_stride;
     auto take = [&](size_t n) {
       const size_t at = bytes;
       bytes += align_up(n);
@@ -601,17 +663,25 @@ struct Plan {
       wg_off = take((size_t)a.hidden * wpad * sizeof(T));
       wu_off = take((size_t)a.hidden * wpad * sizeof(T));
     }
-    q_tiles = ceil_div(std::max<int64_t>(a.rows, 1), (int64_t)kBQ);
+    const int64_t rows = std::max<int64_t>(a.rows, 1);
+    big_dual = big_tiles(2 * a.hidden, rows);
     if (!backward) return;
+    big_dx = big_tiles(a.width, rows);
     wt_off = take((size_t)a.width * 2 * hpad * sizeof(T));
     dgu_off = take((size_t)a.rows * 2 * hpad * sizeof(T));
-    dbias_off = take((size_t)q_tiles * 2 * 2 * a.hidden * sizeof(float));
+    bias_parts = 2 * ceil_div(rows, (int64_t)(big_dual ? 256 : 128));
+    dbias_off = take((size_t)bias_parts * 2 * a.hidden * sizeof(float));
     // split the reduction over the rows until the tiles fill the device; each
     // split's sums cost a write and a read of the gradients in fp32
     constexpr int64_t KS = kStageBytes / sizeof(T);
-    const int64_t tiles = ceil_div(2 * hpad, (int64_t)kBQ) * ceil_div(a.width, (int64_t)kBP);
-    const int64_t stages = ceil_div(std::max<int64_t>(a.rows, 1), KS);
-    splits = std::max<int64_t>(1, std::min(ceil_div(kSplitTarget, tiles), ceil_div(stages, (int64_t)8)));
+    const int64_t stages = ceil_div(rows, KS);
+    auto split_to = [&](int64_t side) {
+      const int64_t tiles = ceil_div(2 * hpad, side) * ceil_div(a.width, side);
+      return std::max<int64_t>(1, std::min(ceil_div(kSplitTarget, tiles),
+                                           ceil_div(stages, (int64_t)16)));
+    };
+    big_dw = 2 * hpad * a.width >= (int64_t)16 * 256 * 256 && stages >= 64;
+    splits = split_to(big_dw ? 256 : 128);
     const int64_t per = ceil_div(stages, splits);
     splits = ceil_div(stages, per);
     k_split = per * KS;
@@ -630,14 +700,14 @@ void pack_rows(const void* src, int64_t ld, int64_t rows, int64_t cols, int64_t 
 template <class T>
 struct Inputs {
   const T *x, *wg, *wu;
-  int64_t ldx, ldg, ldu;
+  int64_t ldx, ldw;
 };
 
 // x and the weights as the product kernel loads them.
 template <class T>
 Inputs<T> load_inputs(const GatedArgs& a, const Plan<T>& pl, char* ws, hipStream_t st) {
   Inputs<T> in{static_cast<const T*>(a.x), static_cast<const T*>(a.w_gate),
-               static_cast<const T*>(a.w_up), a.x_stride, a.w_gate_stride, a.w_up_stride};
+               static_cast<const T*>(a.w_up), a.x_stride, a.w_gate_stride};
   if (pl.pack_x) {
     T* x = reinterpret_cast<T*>(ws + pl.x_off);
     pack_rows<T>(a.x, a.x_stride, a.rows, a.width, pl.wpad, x, st);
@@ -650,7 +720,7 @@ Inputs<T> load_inputs(const GatedArgs& a, const Plan<T>& pl, char* ws, hipStream
     pack_rows<T>(a.w_up, a.w_up_stride, a.hidden, a.width, pl.wpad, u, st);
     in.wg = g;
     in.wu = u;
-    in.ldg = in.ldu = pl.wpad;
+    in.ldw = pl.wpad;
   }
   return in;
 }
@@ -662,23 +732,31 @@ void launch_gemm(const GemmShape& s, int64_t splits, const EPI& epi, hipStream_t
   MGP_HIP_CHECK(hipGetLastError());
 }
 
+template <class TL, class EPI>
+void launch_tiles(GemmShape s, int64_t splits, const EPI& epi, hipStream_t st) {
+  s.tiles_p = ceil_div(s.p.n, (int64_t)(TL::DUAL ? TL::BP / 2 : TL::BP));
+  s.tiles_q = ceil_div(s.q.n, (int64_t)TL::BQ);
+  launch_gemm<TL>(s, splits, epi, st);
+}
+
+template <class T, bool TR, bool DUAL, class EPI>
+void launch_product(bool big, const GemmShape& s, int64_t splits, const EPI& epi,
+                    hipStream_t st) {
+  if (big)
+    launch_tiles<BigTile<T, TR, DUAL>>(s, splits, epi, st);
+  else
+    launch_tiles<SmallTile<T, TR, DUAL>>(s, splits, epi, st);
+}
+
 template <class T, class EPI>
 void launch_dual(const GatedArgs& a, const Plan<T>& pl, const Inputs<T>& in, const EPI& epi,
                  hipStream_t st) {
-  using TL = Tile<T, 4, 4, 2, 2, false, true>;
-  GemmShape s;
+  GemmShape s{};
   s.p = {reinterpret_cast<const char*>(in.wg), reinterpret_cast<const char*>(in.wu),
-         in.ldg * (int64_t)sizeof(T), in.ldu * (int64_t)sizeof(T), a.hidden};
-  s.q = {reinterpret_cast<const char*>(in.x), nullptr, in.ldx * (int64_t)sizeof(T), 0, a.rows};
+         in.ldw * (int64_t)sizeof(T), a.hidden};
+  s.q = {reinterpret_cast<const char*>(in.x), nullptr, in.ldx * (int64_t)sizeof(T), a.rows};
   s.K = s.k_split = pl.wpad;
-  s.tiles_p = (int)ceil_div(a.hidden, (int64_t)(TL::BP / 2));
-  s.tiles_q = (int)ceil_div(a.rows, (int64_t)TL::BQ);
-  launch_gemm<TL>(s, 1, epi, st);
-}
-
-template <class T>
-bool vec4(const void* p, int64_t stride) {
-  return reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0 && stride % 4 == 0;
+  launch_product<T, false, true>(pl.big_dual, s, 1, epi, st);
 }
 
 template <class F>
@@ -707,9 +785,7 @@ void gated_forward(const GatedArgs& a, void* h, int64_t h_stride, void* ws, hipS
     const Inputs<T> in = load_inputs<T>(a, pl, static_cast<char*>(ws), st);
     dispatch_act(a.activation, [&](auto act) {
       ForwardEpi<T, act.value> epi{static_cast<const T*>(a.b_gate), static_cast<const T*>(a.b_up),
-                                   static_cast<T*>(h),              h_stride,
-                                   a.rows,                          a.hidden,
-                                   vec4<T>(h, h_stride)};
+                                   static_cast<T*>(h), h_stride, a.rows, a.hidden};
       launch_dual<T>(a, pl, in, epi, st);
     });
   });
@@ -737,48 +813,36 @@ void gated_backward(const GatedArgs& a, const void* dh, int64_t dh_stride, const
     float* dbias = dbg || dbu ? reinterpret_cast<float*>(ws + pl.dbias_off) : nullptr;
     dispatch_act(a.activation, [&](auto act) {
       BackwardEpi<T, act.value> epi{static_cast<const T*>(a.b_gate), static_cast<const T*>(a.b_up),
-                                    static_cast<const T*>(dh),       dh_stride,
-                                    a.rows,                          a.hidden,
-                                    pl.hpad,                         dgu,
-                                    dbias,                           vec4<T>(dh, dh_stride)};
+                                    static_cast<const T*>(dh), dh_stride, a.rows, a.hidden,
+                                    pl.hpad, dgu, dbias};
       launch_dual<T>(a, pl, in, epi, st);
     });
     if (dbias)
       k_sum_bias<T><<<(unsigned)ceil_div(2 * a.hidden, (int64_t)64), 1024, 0, st>>>(
-          dbias, pl.q_tiles * 2, a.hidden, dbg, dbu);
+          dbias, pl.bias_parts, a.hidden, dbg, dbu);
     const int64_t ldd = 2 * pl.hpad * (int64_t)sizeof(T);
     if (g.dx) {
-      using TL = Tile<T, 4, 4, 2, 2, false, false>;
       T* wt = reinterpret_cast<T*>(ws + pl.wt_off);
       k_transpose_weights<T><<<dim3((unsigned)ceil_div(pl.hpad, (int64_t)32),
                                     (unsigned)ceil_div(a.width, (int64_t)32), 2),
-                               256, 0, st>>>(in.wg, in.ldg, in.wu, in.ldu, a.hidden, a.width,
+                               256, 0, st>>>(in.wg, in.wu, in.ldw, a.hidden, a.width,
                                              pl.hpad, wt);
-      GemmShape s;
-      s.p = {reinterpret_cast<const char*>(wt), nullptr, ldd, 0, a.width};
-      s.q = {reinterpret_cast<const char*>(dgu), nullptr, ldd, 0, a.rows};
+      GemmShape s{};
+      s.p = {reinterpret_cast<const char*>(wt), nullptr, ldd, a.width};
+      s.q = {reinterpret_cast<const char*>(dgu), nullptr, ldd, a.rows};
       s.K = s.k_split = 2 * pl.hpad;
-      s.tiles_p = (int)ceil_div(a.width, (int64_t)TL::BP);
-      s.tiles_q = (int)ceil_div(a.rows, (int64_t)TL::BQ);
-      launch_gemm<TL>(s, 1,
-                      StoreEpi<T>{static_cast<T*>(g.dx), a.width, a.rows, a.width,
-                                  vec4<T>(g.dx, a.width)},
-                      st);
+      launch_product<T, false, false>(
+          pl.big_dx, s, 1, StoreEpi<T>{static_cast<T*>(g.dx), a.width, a.rows, a.width}, st);
     }
     if (dwg || dwu) {
-      using TL = Tile<T, 4, 4, 2, 2, true, false>;
       float* part = pl.splits > 1 ? reinterpret_cast<float*>(ws + pl.part_off) : nullptr;
-      GemmShape s;
-      s.p = {reinterpret_cast<const char*>(in.x), nullptr, in.ldx * (int64_t)sizeof(T), 0, pl.wpad};
-      s.q = {reinterpret_cast<const char*>(dgu), nullptr, ldd, 0, 2 * pl.hpad};
+      GemmShape s{};
+      s.p = {reinterpret_cast<const char*>(in.x), nullptr, in.ldx * (int64_t)sizeof(T), pl.wpad};
+      s.q = {reinterpret_cast<const char*>(dgu), nullptr, ldd, 2 * pl.hpad};
       s.K = a.rows;
       s.k_split = pl.k_split;
-      s.tiles_p = (int)ceil_div(a.width, (int64_t)TL::BP);
-      s.tiles_q = (int)ceil_div(2 * pl.hpad, (int64_t)TL::BQ);
-      const bool vec = part ? a.width % 4 == 0
-                            : (!dwg || vec4<T>(dwg, a.width)) && (!dwu || vec4<T>(dwu, a.width));
-      launch_gemm<TL>(s, pl.splits,
-                      WeightEpi<T>{dwg, dwu, part, a.hidden, pl.hpad, a.width, vec}, st);
+      launch_product<T, true, false>(pl.big_dw, s, pl.splits,
+                                     WeightEpi<T>{dwg, dwu, part, a.hidden, pl.hpad, a.width}, st);
       if (part)
         k_sum_parts<T><<<(unsigned)std::min<int64_t>(
                              ceil_div(2 * a.hidden * a.width, (int64_t)256), 8192),
