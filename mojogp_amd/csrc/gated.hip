@@ -33,49 +33,69 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 
 // ---------------------------------------------------------------- activation
 
-// 1 / (1 + exp(-g)).  FAST (the 16-bit types): one v_exp and one v_rcp, good to
-// a few fp32 roundings, where expf and a division cost ~40 instructions (the
-// epilogue of 65536 x 1024 -> 4096 took a quarter of the kernel's time).
+// exp(x + tail) by v_exp_f32.  FAST (the 16-bit types): the exponent's rounding
+// makes a relative error of 2^-24 |x|; fp32 takes it out to first order.  A
+// library expf and a division made ~40 instructions of each sigmoid, and the
+// epilogue of 65536 x 1024 -> 4096 a quarter of the kernel's time.
 template <bool FAST>
-__device__ __forceinline__ float sigmoid(float g) {
-  if constexpr (FAST)
-    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * g));
-  else
-    return 1.0f / (1.0f + expf(-g));
+__device__ __forceinline__ float exp_of(float x, float tail = 0.0f) {
+  if constexpr (FAST) return __builtin_amdgcn_exp2f(kLog2e * x);
+  constexpr float kLog2eLow = 1.92596299e-8f;  // log2(e) - kLog2e
+  x = x < -126.0f ? -126.0f : x;  // beyond, 0 and infinity all the same; NaN stays
+  x = x > 126.0f ? 126.0f : x;
+  const float t = x * kLog2e;
+  const float r = fmaf(x, kLog2e, -t) + fmaf(x, kLog2eLow, tail * kLog2e);
+  return __builtin_amdgcn_exp2f(t) * fmaf(r, kLn2, 1.0f);
+}
+
+// 1 - Phi(x) over exp(-x^2 / 2) for x = sqrt(2) v, v >= 0: a polynomial in
+// 1 / (1 + p v), p and the coefficients fitted by least squares reweighted
+// towards the smallest largest relative error over 0 <= v <= 9.5: 5.2e-6 (six
+// terms, the 16-bit types), 1.9e-8 (nine).
+template <bool FAST>
+__device__ __forceinline__ float normal_tail(float v) {
+  if constexpr (FAST) {
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.44f, v, 1.0f));
+    float q = -0.0730530247092247f;
+    q = fmaf(q, t, 0.17532674968242645f);
+    q = fmaf(q, t, 0.020365050062537193f);
+    q = fmaf(q, t, 0.13179342448711395f);
+    q = fmaf(q, t, 0.12128471583127975f);
+    return fmaf(q, t, 0.12428051233291626f) * t;
+  } else {
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3f, v, 1.0f));
+    float q = -0.06471703946590424f;
+    q = fmaf(q, t, 0.24254822731018066f);
+    q = fmaf(q, t, -0.2556132376194f);
+    q = fmaf(q, t, 0.2731975317001343f);
+    q = fmaf(q, t, -0.04681563004851341f);
+    q = fmaf(q, t, 0.10721813887357712f);
+    q = fmaf(q, t, 0.07424121350049973f);
+    q = fmaf(q, t, 0.08534596860408783f);
+    return fmaf(q, t, 0.08459480851888657f) * t;
+  }
 }
 
 // a = act(g) and its derivative
 template <int ACT, bool FAST>
 __device__ __forceinline__ void activate(float g, float& a, float& slope) {
   if constexpr (ACT == ACT_SILU) {
-    const float s = sigmoid<FAST>(g);
+    const float s = __builtin_amdgcn_rcpf(1.0f + exp_of<FAST>(-g));
     a = g * s;
     slope = s * fmaf(g, 1.0f - s, 1.0f);
   } else if constexpr (ACT == ACT_SIGMOID) {
-    a = sigmoid<FAST>(g);
+    a = __builtin_amdgcn_rcpf(1.0f + exp_of<FAST>(-g));
     slope = a * (1.0f - a);
   } else if constexpr (ACT == ACT_RELU) {
     a = g > 0.0f || g != g ? g : 0.0f;
     slope = g > 0.0f ? 1.0f : 0.0f;
-  } else if constexpr (FAST) {
-    // the normal integral by Abramowitz and Stegun 7.1.26 (absolute error
-    // 1.5e-7, a thousandth of the 16-bit types' rounding), whose exponential
-    // the derivative takes too
-    const float x = fabsf(g) * 0.70710678118654752f;
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.0f));
-    const float e = __builtin_amdgcn_exp2f(-0.5f * kLog2e * g * g);
-    const float q =
-        t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f),
-                         -0.284496736f),
-                 0.254829592f);
-    const float tail = 0.5f * q * e;  // 1 - Phi(|g|)
+  } else {
+    const float g2 = g * g;
+    const float e = exp_of<FAST>(-0.5f * g2, -0.5f * fmaf(g, g, -g2));
+    const float tail = normal_tail<FAST>(fabsf(g) * 0.70710678118654752f) * e;  // 1 - Phi(|g|)
     const float cdf = g > 0.0f ? 1.0f - tail : tail;
     a = g * cdf;
     slope = fmaf(g * 0.39894228040143268f, e, cdf);
-  } else {
-    const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
-    a = g * cdf;
-    slope = fmaf(g * 0.39894228040143268f, expf(-0.5f * g * g), cdf);
   }
 }
 
@@ -108,6 +128,22 @@ __device__ __forceinline__ void store_run(T* p, int64_t left, const float* v) {
   }
 }
 
+// The two fp16 parts of scaled values: v scale = hi + lo to 22 bits, hi at p and
+// lo `apart` elements on.
+template <int N>
+__device__ __forceinline__ void store_parts(_Float16* p, int64_t apart, int64_t left, float scale,
+                                            const float* v) {
+  float hi[N], lo[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const float x = v[k] * scale;
+    hi[k] = (float)(_Float16)x;
+    lo[k] = x - hi[k];
+  }
+  store_run<N>(p, left, hi);
+  store_run<N>(p + apart, left, lo);
+}
+
 // ---------------------------------------------------------------- product core
 
 // A 16-byte operand fragment: 8 narrow elements of 32 reduction steps spread
@@ -131,14 +167,16 @@ __device__ __forceinline__ f4 mma(const Frag& a, const Frag& b, f4 c) {
   }
 }
 
-constexpr int kStageBytes = 128;        // reduction bytes of a row a stage
 constexpr int kOutOfRange = (int)0x80000000u;  // past num_records: the load gives zeros
 constexpr int kNumRecords = 0x7fffffff;
 
-__device__ __forceinline__ void load_lds(const char* base, int voff, char* __restrict__ dst) {
+// base: wave uniform; soff (too): not part of the range check, so an offset out
+// of range stays it
+__device__ __forceinline__ void load_lds(const char* base, int voff, int soff,
+                                         char* __restrict__ dst) {
   const __amdgpu_buffer_rsrc_t r =
       __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, kNumRecords, 0x00020000);
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (MGP_LDS void*)dst, 16, voff, 0, 0, 0);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (MGP_LDS void*)dst, 16, voff, soff, 0, 0);
 }
 
 // One operand of a product: element (row, k) at base + row ld + k (NT) or
@@ -156,6 +194,7 @@ struct GemmShape {
   int64_t K;          // reduction length
   int64_t tiles_p, tiles_q;
   int64_t k_split;    // reduction elements of one split (a multiple of a stage)
+  int64_t p_lo, q_lo; // three-part products: byte distance of the low parts from the high ones
 };
 
 // Tile of 16 TN WN columns (p rows) by 16 TM WM rows (q rows), one wave 16 TN
@@ -166,33 +205,63 @@ struct GemmShape {
 // per reduction step, in the memory's order; 32-byte granules at g ^ (r % 8)
 // (narrow types, read by the transposing LDS load), 64-byte ones at g ^ (r % 4)
 // (fp32): both keep the fragment reads off each other's banks.
-template <class T, int TM_, int TN_, int WM_, int WN_, bool TR_, bool DUAL_>
+template <class T, int TM_, int TN_, int WM_, int WN_, bool TR_, bool DUAL_, int PARTS_>
 struct Tile {
   using Elem = T;
   static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_;
   static constexpr bool TR = TR_, DUAL = DUAL_;
+  static constexpr int PARTS = PARTS_;  // 3: fp32 operands as two fp16 parts
   static constexpr int W = WM * WN, THREADS = 64 * W;
   static constexpr int BQ = 16 * TM * WM, BP = 16 * TN * WN;
   static constexpr int T1 = DUAL ? TN / 2 : TN;  // 16-row tiles of one matrix a wave
   static constexpr int RUN = 4 * T1;
   static constexpr int E = sizeof(T);
-  static constexpr int KS = kStageBytes / E;       // reduction elements a stage
-  static constexpr int LDS = (BP + BQ) * kStageBytes;  // one buffer
-  static constexpr int IP = BP * kStageBytes / 1024 / W, IQ = BQ * kStageBytes / 1024 / W;
-  static_assert(IP * W * 1024 == BP * kStageBytes && IQ * W * 1024 == BQ * kStageBytes, "");
+  static constexpr int SB = 128;                   // reduction bytes of a row a stage
+  static constexpr int KS = SB / E;                // reduction elements a stage
+  static constexpr int LDS = (BP + BQ) * SB;  // one buffer
+  static constexpr int IP = BP * SB / 1024 / W, IQ = BQ * SB / 1024 / W;
+  static_assert(IP * W * 1024 == BP * SB && IQ * W * 1024 == BQ * SB, "");
 };
 
-// What a wave loads of a stage: I instructions a side, each 64 lanes x 16 bytes
-// = 1 KB of LDS.  The instructions of a side lie a multiple of 8 LDS rows (TN:
-// of 8, fp32 4, reduction rows) apart, so the lanes' offsets from each one's
-// uniform base are the same; only which rows exist differs.
+// What a wave loads of a stage: I instructions, each 64 lanes x 16 bytes = 1 KB
+// of LDS.  The instructions of a side lie a multiple of 8 LDS rows (TN: of 8,
+// fp32 4, reduction rows) apart, so the lanes' offsets from each one's uniform
+// start are the same; only which rows exist differs.
 template <class TL>
 struct Loader {
   static constexpr int I = TL::IP + TL::IQ;
-  int voff[2];        // byte offset of the lane from an instruction's base
-  int kpos[2];        // NT: its reduction element, TN: its reduction row within the stage
-  bool exists[I];     // NT: its row is one of the matrix
-  const char* base[I];
+  int voff[2];           // byte offset of the lane from an instruction's start
+  int kpos[2];           // NT: its reduction element, TN: its reduction row within the stage
+  bool exists[I];        // NT: its row is one of the matrix
+  int soff[I];           // bytes from the side's base to the instruction's start
+  const char* base[3];   // of p, of q, of p's second matrix
+  int64_t step[2];       // bytes of a stage
+  int64_t jump[2][2];    // three parts: bytes to the next product's start, after its stages
+  int64_t length, left;  // reduction elements of a part, and those still to load
+  int part;
+
+  // Whether instruction i of p loads the second matrix, for one wave: with 8
+  // waves that is the wave's (its base is then base[0]), with 4 it is i's.
+  static constexpr bool second(int i) { return TL::DUAL && TL::W == 4 && i % 2 == 1; }
+
+  __device__ __forceinline__ void init(const GemmShape& s, int64_t n0, int64_t m0, int64_t k0,
+                                       int64_t K) {
+    init_side<true>(s.p, n0, k0);
+    init_side<false>(s.q, m0, k0);
+    step[0] = TL::TR ? TL::KS * s.p.ld_bytes : TL::SB;
+    step[1] = TL::TR ? TL::KS * s.q.ld_bytes : TL::SB;
+    length = left = K;
+    if constexpr (TL::PARTS == 3) {
+      // p: high, low, high; q: high, high, low
+      const int64_t back_p = (K + TL::KS - 1) / TL::KS * step[0];
+      const int64_t back_q = (K + TL::KS - 1) / TL::KS * step[1];
+      jump[0][0] = s.p_lo - back_p;
+      jump[0][1] = -s.p_lo - back_p;
+      jump[1][0] = -back_q;
+      jump[1][1] = s.q_lo - back_q;
+      part = 0;
+    }
+  }
 
   template <bool P>
   __device__ __forceinline__ void init_side(const Operand& o, int64_t row0, int64_t k0) {
@@ -200,6 +269,7 @@ struct Loader {
     constexpr int B = P ? TL::BP : TL::BQ;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ld = (int)o.ld_bytes;
     if constexpr (!TL::TR) {
       static_assert(TL::W % 2 == 0, "");  // the swizzle is that of wave * 8 + lane / 8
       const int l8 = lane / 8;
@@ -208,52 +278,68 @@ struct Loader {
       // 16 T1 w + (i / 4) RUN + 4 t + i % 4
       const int lrow = P ? l8 / 4 * TL::RUN + l8 % 4 : l8;
       kpos[!P] = c * (16 / TL::E);
-      voff[!P] = (int)(lrow * o.ld_bytes) + c * 16;
+      voff[!P] = lrow * ld + c * 16;
+      const char* from = o.base;
+      if constexpr (P && TL::DUAL) {
+        static_assert(TL::TN == 4 && (TL::W == 8 || TL::W == 4), "");
+        base[2] = o.base2 + row0 * o.ld_bytes + k0 * TL::E;
+        if (TL::W == 8 && wave >= 4) from = o.base2;
+      }
+      base[!P] = from + row0 * o.ld_bytes + k0 * TL::E;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int r8 = (i * TL::W + wave) * 8;
-        int64_t r = row0 + r8;
-        const char* from = o.base;
+        int r = r8;
         if constexpr (P) {
           const int t = r8 % (16 * TL::TN) / 16;
-          const bool up = t >= TL::T1;  // wave uniform
-          r = row0 + r8 / (16 * TL::TN) * 16 * TL::T1 + r8 % 16 / 4 * TL::RUN +
-              (up ? t - TL::T1 : t) * 4;
-          if (up) from = o.base2;
+          r = r8 / (16 * TL::TN) * 16 * TL::T1 + r8 % 16 / 4 * TL::RUN + t % TL::T1 * 4;
         }
-        exists[S + i] = r + lrow < o.n;
-        base[S + i] = from + r * o.ld_bytes + k0 * TL::E;
+        exists[S + i] = row0 + r + lrow < o.n;
+        soff[S + i] = r * ld;
       }
     } else {
       constexpr int RB = B * TL::E;  // bytes of an LDS row
-      static_assert(TL::W * 1024 / RB % 8 == 0, "");
-      const int byte = wave * 1024 + lane * 16, r = byte / RB, rb = wave * 1024 / RB;
+      static_assert(TL::W * 1024 / RB % (TL::E == 2 ? 8 : 4) == 0, "");
+      const int byte = wave * 1024 + lane * 16, r = byte / RB;
       const int c = (byte % RB / 16) ^
                     ((TL::E == 2 ? ((r & 7) << 1) : ((r & 3) << 2)) & (RB / 16 - 1));
       const bool in = row0 + c * (16 / TL::E) < o.n;
       kpos[!P] = r;
-      voff[!P] = (int)((r - rb) * o.ld_bytes) + c * 16;
+      voff[!P] = r * ld + c * 16;
+      base[!P] = o.base + k0 * o.ld_bytes + row0 * TL::E;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         exists[S + i] = in;
-        base[S + i] = o.base + (k0 + i * (TL::W * 1024 / RB) + rb) * o.ld_bytes + row0 * TL::E;
+        soff[S + i] = i * (TL::W * 1024 / RB) * ld;
       }
     }
   }
 
-  // Loads the stage of `left` remaining reduction elements into buf and moves on.
-  __device__ __forceinline__ void load(char* __restrict__ buf, int64_t left, int64_t ldp,
-                                       int64_t ldq) {
+  // Loads the next stage into buf.
+  __device__ __forceinline__ void load(char* __restrict__ buf) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l = (int)min(left, (int64_t)TL::KS);
 #pragma unroll
     for (int i = 0; i < I; ++i) {
       const bool p = i < TL::IP;
       const int j = p ? i : i - TL::IP;
-      char* dst = buf + (p ? 0 : TL::BP * kStageBytes) + (j * TL::W + wave) * 1024;
-      const int step = TL::TR ? j * (TL::W * 1024 / ((p ? TL::BP : TL::BQ) * TL::E)) : 0;
-      load_lds(base[i], exists[i] && kpos[!p] < l - step ? voff[!p] : kOutOfRange, dst);
-      base[i] += TL::TR ? (int64_t)TL::KS * (p ? ldp : ldq) : (int64_t)kStageBytes;
+      char* dst = buf + (p ? 0 : TL::BP * TL::SB) + (j * TL::W + wave) * 1024;
+      const int at = TL::TR ? j * (TL::W * 1024 / ((p ? TL::BP : TL::BQ) * TL::E)) : 0;
+      load_lds(base[p ? (second(i) ? 2 : 0) : 1],
+               exists[i] && kpos[!p] < l - at ? voff[!p] : kOutOfRange, soff[i], dst);
+    }
+    left -= TL::KS;
+    const bool turn = TL::PARTS == 3 && left <= 0 && part < 2;
+#pragma unroll
+    for (int b = 0; b < (second(1) ? 3 : 2); ++b) {
+      base[b] += step[b & 1];
+      if constexpr (TL::PARTS == 3) {
+        if (turn) base[b] += part ? jump[b & 1][1] : jump[b & 1][0];
+      }
+    }
+    if (turn) {
+      left = length;
+      ++part;
     }
   }
 };
@@ -263,13 +349,17 @@ __device__ __forceinline__ Frag read_frag(const char* __restrict__ buf, int row,
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   if constexpr (!TL::TR) {
     const int c = (ks * 4 + g) ^ (i >> 1);
-    return {*reinterpret_cast<const f4*>(buf + (row + i) * kStageBytes + c * 16)};
+    return {*reinterpret_cast<const f4*>(buf + (row + i) * TL::SB + c * 16)};
   } else if constexpr (TL::E == 2) {
     // lane group g takes reduction rows 4 g .. 4 g + 3 and the same + 16; the
     // transposing load gives lane i the four rows' elements of column i
     constexpr int RB = B * TL::E, M = RB / 32 - 1;
     const int r = ks * 32 + 4 * g + (i >> 2);
-    const int a = r * RB + (((row >> 4) ^ ((r & 7) & M)) * 32) + (i & 3) * 8;
+    // tiles differ in the granule alone: one address, and an exclusive or a
+    // tile made where it is used (kept over the loop they would spill)
+    int a = r * RB + ((r & 7 & M) * 32) + (i & 3) * 8;
+    asm volatile("" : "+v"(a));
+    a ^= (row >> 4) * 32;
     const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MGP_LDS s4*)(buf + a));
     const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MGP_LDS s4*)(buf + a + 16 * RB));
     typedef short s8 __attribute__((ext_vector_type(8)));
@@ -288,9 +378,15 @@ __device__ __forceinline__ Frag read_frag(const char* __restrict__ buf, int row,
   }
 }
 
+// One stage: the loads of the next go out behind the first half's fragment
+// reads (before them, the reads wait in the queue: 4 % of the product's time).
+// The two buffers are distinct restrict arguments, so that the reads
+// need not wait for the loads in flight; the closing barrier waits for those
+// and for every wave's reads.
 template <class TL>
-__device__ __forceinline__ void compute(const char* __restrict__ cur, int wm, int wn,
-                                        f4 (&acc)[TL::TM][TL::TN]) {
+__device__ __forceinline__ void stage(Loader<TL>& ld, const char* __restrict__ cur,
+                                      char* __restrict__ nxt, bool more, int wm, int wn,
+                                      f4 (&acc)[TL::TM][TL::TN]) {
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks) {
     Frag p[TL::TN], q[TL::TM];
@@ -298,24 +394,17 @@ __device__ __forceinline__ void compute(const char* __restrict__ cur, int wm, in
     for (int t = 0; t < TL::TN; ++t) p[t] = read_frag<TL, TL::BP>(cur, (wn * TL::TN + t) * 16, ks);
 #pragma unroll
     for (int t = 0; t < TL::TM; ++t)
-      q[t] = read_frag<TL, TL::BQ>(cur + TL::BP * kStageBytes, (wm * TL::TM + t) * 16, ks);
+      q[t] = read_frag<TL, TL::BQ>(cur + TL::BP * TL::SB, (wm * TL::TM + t) * 16, ks);
+    if (ks == 0) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) ld.load(nxt);
+      __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
     for (int m = 0; m < TL::TM; ++m)
 #pragma unroll
       for (int n = 0; n < TL::TN; ++n) acc[m][n] = mma<typename TL::Elem>(p[n], q[m], acc[m][n]);
   }
-}
-
-// One stage: the loads of the next go out before this one's fragments are
-// read.  The two buffers are distinct restrict arguments, so that the reads
-// need not wait for the loads in flight; the closing barrier waits for those
-// and for every wave's reads.
-template <class TL>
-__device__ __forceinline__ void stage(Loader<TL>& ld, char* __restrict__ cur,
-                                      char* __restrict__ nxt, int64_t left_next, int64_t ldp,
-                                      int64_t ldq, int wm, int wn, f4 (&acc)[TL::TM][TL::TN]) {
-  if (left_next > 0) ld.load(nxt, left_next, ldp, ldq);
-  compute<TL>(cur, wm, wn, acc);
   __syncthreads();
 }
 
@@ -355,34 +444,39 @@ __global__ __launch_bounds__(TL::THREADS) void k_gemm(GemmShape s, EPI epi) {
     for (int n = 0; n < TL::TN; ++n) acc[m][n] = f4{0.f, 0.f, 0.f, 0.f};
 
   Loader<TL> ld;
-  ld.template init_side<true>(s.p, n0, k0);
-  ld.template init_side<false>(s.q, m0, k0);
-  const int64_t ldp = s.p.ld_bytes, ldq = s.q.ld_bytes;
+  ld.init(s, n0, m0, k0, K);
   // pairs of stages, so that each has its own buffers at compile time; an odd
   // one goes first
-  int64_t left = K;
-  if ((K + TL::KS - 1) / TL::KS % 2 == 1) {
-    ld.load(b1, left, ldp, ldq);
+  int64_t stages = (K + TL::KS - 1) / TL::KS * TL::PARTS;
+  if (stages % 2 == 1) {
+    ld.load(b1);
     __syncthreads();
-    left -= TL::KS;
-    stage<TL>(ld, b1, b0, left, ldp, ldq, wm, wn, acc);
+    --stages;
+    stage<TL>(ld, b1, b0, stages > 0, wm, wn, acc);
   } else {
-    ld.load(b0, left, ldp, ldq);
+    ld.load(b0);
     __syncthreads();
   }
-  while (left > 0) {
-    left -= TL::KS;
-    stage<TL>(ld, b0, b1, left, ldp, ldq, wm, wn, acc);
-    left -= TL::KS;
-    stage<TL>(ld, b1, b0, left, ldp, ldq, wm, wn, acc);
+  for (; stages > 0; stages -= 2) {
+    stage<TL>(ld, b0, b1, true, wm, wn, acc);
+    stage<TL>(ld, b1, b0, stages > 2, wm, wn, acc);
   }
   epi.template run<TL>(acc, m0 + wm * TL::TM * 16, n0 + wn * (CP / TL::WN), tq * TL::WM + wm);
 }
 
 // ---------------------------------------------------------------- epilogues
 
+// What the sums of a product are multiplied by: one, or (fp32 operands in scaled
+// fp16 parts) the power of two that undoes the parts' scales, which the packing
+// left on the device.
+struct Unscale {
+  const float* p;
+  __device__ __forceinline__ float get() const { return p ? *p : 1.0f; }
+};
+
 template <class T, int ACT>
 struct ForwardEpi {
+  Unscale scale;
   const T *bg, *bu;
   T* h;
   int64_t ldh, rows, hidden;
@@ -393,6 +487,7 @@ struct ForwardEpi {
     const int lane = threadIdx.x & 63;
     const int64_t f = n0 + N * (lane >> 4), left = hidden - f;
     if (left <= 0) return;
+    const float sc = scale.get();
     float g0[N], u0[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) g0[k] = u0[k] = 0.0f;
@@ -406,8 +501,8 @@ struct ForwardEpi {
 #pragma unroll
       for (int k = 0; k < N; ++k) {
         float a, slope;
-        activate<ACT, sizeof(T) == 2>(acc[m][k / 4][k % 4] + g0[k], a, slope);
-        o[k] = a * (acc[m][TL::T1 + k / 4][k % 4] + u0[k]);
+        activate<ACT, sizeof(T) == 2>(fmaf(acc[m][k / 4][k % 4], sc, g0[k]), a, slope);
+        o[k] = a * fmaf(acc[m][TL::T1 + k / 4][k % 4], sc, u0[k]);
       }
       store_run<N>(h + r * ldh + f, left, o);
     }
@@ -416,12 +511,15 @@ struct ForwardEpi {
 
 // dgu[row] = [dg | du], each `pad` columns (zeros past hidden);
 // dbias[part][2][hidden] the column sums over a wave's rows.
-template <class T, int ACT>
+// dgu of fp32 operands: two fp16 parts of the scaled values, the low ones after
+// the high ones of a row.
+template <class T, int ACT, bool SPLIT>
 struct BackwardEpi {
+  Unscale scale, dgu_scale;  // dgu_scale: what dg and du are multiplied by
   const T *bg, *bu;
   const T* dh;
   int64_t lddh, rows, hidden, pad;
-  T* dgu;
+  void* dgu;
   float* dbias;  // or null
   template <class TL>
   __device__ __forceinline__ void run(f4 (&acc)[TL::TM][TL::TN], int64_t m0, int64_t n0,
@@ -429,6 +527,7 @@ struct BackwardEpi {
     constexpr int N = TL::RUN;
     const int lane = threadIdx.x & 63;
     const int64_t f = n0 + N * (lane >> 4), left = hidden - f;
+    const float sc = scale.get(), ds = dgu_scale.get();
     float g0[N], u0[N], sg[N], su[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) g0[k] = u0[k] = sg[k] = su[k] = 0.0f;
@@ -445,16 +544,23 @@ struct BackwardEpi {
 #pragma unroll
       for (int k = 0; k < N; ++k) {
         float a, slope;
-        activate<ACT, sizeof(T) == 2>(acc[m][k / 4][k % 4] + g0[k], a, slope);
+        activate<ACT, sizeof(T) == 2>(fmaf(acc[m][k / 4][k % 4], sc, g0[k]), a, slope);
         // columns past hidden are products of the last weights: cut off
         const bool in = k < left;
-        dg[k] = in ? d[k] * (acc[m][TL::T1 + k / 4][k % 4] + u0[k]) * slope : 0.0f;
+        dg[k] = in ? d[k] * fmaf(acc[m][TL::T1 + k / 4][k % 4], sc, u0[k]) * slope : 0.0f;
         du[k] = in ? d[k] * a : 0.0f;
         sg[k] += dg[k];
         su[k] += du[k];
       }
-      store_run<N>(dgu + r * 2 * pad + f, pad - f, dg);
-      store_run<N>(dgu + r * 2 * pad + pad + f, pad - f, du);
+      if constexpr (SPLIT) {
+        _Float16* row = static_cast<_Float16*>(dgu) + r * 4 * pad + f;
+        store_parts<N>(row, 2 * pad, pad - f, ds, dg);
+        store_parts<N>(row + pad, 2 * pad, pad - f, ds, du);
+      } else {
+        T* row = static_cast<T*>(dgu) + r * 2 * pad + f;
+        store_run<N>(row, pad - f, dg);
+        store_run<N>(row + pad, pad - f, du);
+      }
     }
     if (dbias) {
 #pragma unroll
@@ -475,6 +581,7 @@ struct BackwardEpi {
 
 template <class T>
 struct StoreEpi {
+  Unscale scale;
   T* out;
   int64_t ld, rows, cols;
   template <class TL>
@@ -484,13 +591,14 @@ struct StoreEpi {
     const int lane = threadIdx.x & 63;
     const int64_t c = n0 + N * (lane >> 4);
     if (c >= cols) return;
+    const float sc = scale.get();
 #pragma unroll
     for (int m = 0; m < TL::TM; ++m) {
       const int64_t r = m0 + m * 16 + (lane & 15);
       if (r >= rows) continue;
       float o[N];
 #pragma unroll
-      for (int k = 0; k < N; ++k) o[k] = acc[m][k / 4][k % 4];
+      for (int k = 0; k < N; ++k) o[k] = acc[m][k / 4][k % 4] * sc;
       store_run<N>(out + r * ld + c, cols - c, o);
     }
   }
@@ -500,6 +608,7 @@ struct StoreEpi {
 // split: the gradients themselves; more: part[split][2][hidden][width] sums.
 template <class T>
 struct WeightEpi {
+  Unscale scale;
   T *dw_gate, *dw_up;
   float* part;
   int64_t hidden, pad, width;
@@ -507,6 +616,7 @@ struct WeightEpi {
   __device__ __forceinline__ void run(f4 (&acc)[TL::TM][TL::TN], int64_t m0, int64_t n0,
                                       int64_t) const {
     const int lane = threadIdx.x & 63;
+    const float sc = scale.get();
 #pragma unroll
     for (int m = 0; m < TL::TM; ++m) {
       const int64_t r = m0 + m * 16 + (lane & 15);
@@ -517,7 +627,7 @@ struct WeightEpi {
       for (int n = 0; n < TL::TN; ++n) {
         const int64_t c = n0 + n * 16 + 4 * (lane >> 4);
         if (c >= width) continue;
-        float o[4] = {acc[m][n][0], acc[m][n][1], acc[m][n][2], acc[m][n][3]};
+        float o[4] = {acc[m][n][0] * sc, acc[m][n][1] * sc, acc[m][n][2] * sc, acc[m][n][3] * sc};
         if (part) {
           store_run<4>(part + (((int64_t)blockIdx.y * 2 + up) * hidden + f) * width + c, width - c,
                        o);
@@ -611,14 +721,205 @@ __global__ __launch_bounds__(1024) void k_sum_bias(const float* __restrict__ par
   if (dst) dst[i < count ? i : i - count] = (T)s;
 }
 
+// ---------------------------------------------------------------- fp32 operands in fp16 parts
+
+// What the scales are made from, per tensor (x, both weights, dh): the largest
+// finite |value| and (a bound on) the largest 2-norm of a row.  Non-finite
+// values are left out, so that they spoil their own rows only.
+struct Stat {
+  float amax, norm;
+};
+enum : int { ST_X = 0, ST_W = 1, ST_DH = 2, kStats = 3 };
+constexpr int kStatBlocks = 256;  // partial results a tensor
+
+struct StatSource {
+  const float* p[2];
+  int64_t ld[2], rows, cols;  // rows of each of the matrices
+};
+struct StatSources {
+  StatSource s[kStats];
+};
+
+__device__ __forceinline__ Stat join(Stat a, Stat b) {
+  return {fmaxf(a.amax, b.amax), fmaxf(a.norm, b.norm)};
+}
+
+__device__ __forceinline__ Stat wave_join(Stat a) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1)
+    a = join(a, Stat{__shfl_xor(a.amax, o), __shfl_xor(a.norm, o)});
+  return a;
+}
+
+// part[tensor][block]: 16 lanes a row, so that few exchanges end a row and many
+// rows are in flight
+__global__ __launch_bounds__(256) void k_stats(StatSources src, Stat* __restrict__ part) {
+  __shared__ Stat red[4];
+  const StatSource& s = src.s[blockIdx.y];
+  const int lane = threadIdx.x & 15, group = threadIdx.x >> 4;
+  Stat all{0.0f, 0.0f};
+  const int64_t rows = s.p[1] ? 2 * s.rows : s.rows;
+  for (int64_t r = (int64_t)blockIdx.x * 16 + group; r < rows; r += kStatBlocks * 16) {
+    const bool second = r >= s.rows;
+    const float* p = second ? s.p[1] + (r - s.rows) * s.ld[1] : s.p[0] + r * s.ld[0];
+    float sum = 0.0f, big = 0.0f;
+#pragma unroll 4
+    for (int64_t c = 4 * lane; c < s.cols; c += 64) {
+      float v[4];
+      load_run<4>(p + c, s.cols - c, v);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float a = fabsf(v[k]);
+        big = a < INFINITY ? fmaxf(big, a) : big;
+        sum = fmaf(v[k], v[k], sum);
+      }
+    }
+#pragma unroll
+    for (int o = 8; o >= 1; o >>= 1) {
+      sum += __shfl_xor(sum, o);
+      big = fmaxf(big, __shfl_xor(big, o));
+    }
+    // squares that overflow, or a row with non-finite values
+    all = join(all, Stat{big, sum < INFINITY ? sqrtf(sum) : sqrtf((float)s.cols) * big});
+  }
+  all = wave_join(all);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = all;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int k = 1; k < 4; ++k) all = join(all, red[k]);
+  part[blockIdx.y * kStatBlocks + blockIdx.x] = all;
+}
+
+// The scales, powers of two, and the factors that undo them.
+struct Scales {
+  float x, w, d;          // of x, the weights, dg and du
+  float fwd, dx, dw;      // 1 / (x w), 1 / (d w), 1 / (d x)
+};
+
+__device__ __forceinline__ float pow2_below(float bound) {
+  // the largest 2^e with 2^e bound < 2^15
+  if (!(bound > 0.0f)) return 1.0f;
+  return ldexpf(1.0f, min(max(14 - ilogbf(fminf(bound, 3.0e38f)), -120), 120));
+}
+
+// Two fp16 parts hold 22 bits of a value down to 2^-17 of the largest; below,
+// the error stays 2^-40 of the largest.  dg and du are written by the kernel
+// that forms them, before their largest is known: their scale follows from
+// |u|, |g| <= |x| |w| + |b|, |dg| <= 1.13 |dh| |u| and |du| <= |dh| |act(g)|,
+// |act(g)| <= |g| (act_max 0) or 1 (the sigmoid), some five binades above what
+// occurs.
+__device__ __forceinline__ Scales make_scales(const Stat* part, int lane, float bmax,
+                                              float act_max) {
+  auto whole = [&](int tensor) {
+    Stat s{0.0f, 0.0f};
+#pragma unroll
+    for (int b = 0; b < kStatBlocks; b += 64) s = join(s, part[tensor * kStatBlocks + b + lane]);
+    return wave_join(s);
+  };
+  const Stat x = whole(ST_X), w = whole(ST_W), d = whole(ST_DH);
+  Scales s;
+  s.x = pow2_below(x.amax);
+  s.w = pow2_below(w.amax);
+  s.d = pow2_below(1.2f * d.amax * fmaxf(fmaf(x.norm, w.norm, bmax), act_max));
+  s.fwd = (1.0f / s.x) * (1.0f / s.w);
+  s.dx = (1.0f / s.d) * (1.0f / s.w);
+  s.dw = (1.0f / s.d) * (1.0f / s.x);
+  return s;
+}
+
+__device__ __forceinline__ float largest_bias(const float* bg, const float* bu, int64_t n,
+                                              int lane) {
+  float b = 0.0f;
+  for (int64_t i = lane; i < n; i += 64) {
+    const float g = bg ? fabsf(bg[i]) : 0.0f, u = bu ? fabsf(bu[i]) : 0.0f;
+    b = fmaxf(b, g < INFINITY ? g : 0.0f);
+    b = fmaxf(b, u < INFINITY ? u : 0.0f);
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) b = fmaxf(b, __shfl_xor(b, o));
+  return b;
+}
+
+struct SplitSource {
+  const float *x, *wg, *wu, *bg, *bu;
+  int64_t ldx, ldg, ldu, rows, hidden, width, wpad;
+  _Float16 *dx, *dwg, *dwu;  // [rows][2 wpad]: high parts, then low ones
+  const Stat* part;
+  float act_max;
+  Scales* scales;
+};
+
+// Every workgroup forms the scales from the partial statistics; the first one
+// leaves them for the kernels to come.
+__global__ __launch_bounds__(256) void k_split(SplitSource s) {
+  __shared__ Scales sc;
+  if (threadIdx.x < 64) {
+    const float b = blockIdx.x == 0 ? largest_bias(s.bg, s.bu, s.hidden, threadIdx.x) : 0.0f;
+    const Scales v = make_scales(s.part, threadIdx.x, b, s.act_max);
+    if (threadIdx.x == 0) {
+      sc = v;
+      if (blockIdx.x == 0) *s.scales = v;
+    }
+  }
+  __syncthreads();
+  const int64_t per = s.wpad / 8, total = (s.rows + 2 * s.hidden) * per;
+  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total;
+       q += (int64_t)gridDim.x * 256) {
+    int64_t r = q / per;
+    const int64_t c = (q - r * per) * 8;
+    const float* src;
+    _Float16* dst;
+    float scale = sc.w;
+    if (r < s.rows) {
+      src = s.x + r * s.ldx;
+      dst = s.dx + r * 2 * s.wpad;
+      scale = sc.x;
+    } else if ((r -= s.rows) < s.hidden) {
+      src = s.wg + r * s.ldg;
+      dst = s.dwg + r * 2 * s.wpad;
+    } else {
+      r -= s.hidden;
+      src = s.wu + r * s.ldu;
+      dst = s.dwu + r * 2 * s.wpad;
+    }
+    float v[8];
+    load_run<8>(src + c, s.width - c, v);
+    store_parts<8>(dst + c, s.wpad, 8, scale, v);
+  }
+}
+
+// dst[k][part pad + f] = the high part of W_part[f][k], 2 pad on the low one
+__global__ __launch_bounds__(256) void k_transpose_split(const _Float16* __restrict__ wg,
+                                                         const _Float16* __restrict__ wu,
+                                                         int64_t hidden, int64_t width,
+                                                         int64_t wpad, int64_t pad,
+                                                         _Float16* __restrict__ dst) {
+  __shared__ _Float16 tile[32][34];
+  const int64_t f0 = (int64_t)blockIdx.x * 32, k0 = (int64_t)blockIdx.y * 32;
+  const int up = blockIdx.z & 1, low = blockIdx.z >> 1;
+  const _Float16* w = (up ? wu : wg) + low * wpad;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    const int64_t f = f0 + ty + i, k = k0 + tx;
+    tile[ty + i][tx] = f < hidden && k < width ? w[f * 2 * wpad + k] : (_Float16)0.0f;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    const int64_t k = k0 + ty + i, f = f0 + tx;
+    if (k < width && f < pad) dst[k * 4 * pad + low * 2 * pad + up * pad + f] = tile[tx][ty + i];
+  }
+}
+
 // ---------------------------------------------------------------- host side
 
 // Rows the product kernel can load directly: 16-byte aligned, whole 16-byte
-// chunks, and the rows of one load within 31-bit offsets.
+// chunks, and a tile's rows within 31-bit offsets.
 template <class T>
 bool direct(const void* p, int64_t stride, int64_t cols) {
   return aligned16(p) && stride % Vec16<T>::N == 0 && cols % Vec16<T>::N == 0 &&
-         stride * (int64_t)sizeof(T) < (int64_t)1 << 26;
+         stride * (int64_t)sizeof(T) < (int64_t)1 << 23;
 }
 
 constexpr size_t kAlign = 256;
@@ -626,54 +927,71 @@ inline size_t align_up(size_t b) { return (b + kAlign - 1) / kAlign * kAlign; }
 
 // The two tile sizes: 256 x 256, one workgroup of 8 waves a CU, and 128 x 128,
 // two workgroups of 4 waves, for what would leave CUs idle otherwise.
-template <class T, bool TR, bool DUAL>
-using BigTile = Tile<T, 8, 4, 2, 4, TR, DUAL>;
-template <class T, bool TR, bool DUAL>
-using SmallTile = Tile<T, 4, 4, 2, 2, TR, DUAL>;
+template <class T, bool TR, bool DUAL, int PARTS>
+using BigTile = Tile<T, 8, 4, 2, 4, TR, DUAL, PARTS>;
+template <class T, bool TR, bool DUAL, int PARTS>
+using SmallTile = Tile<T, 4, 4, 2, 2, TR, DUAL, PARTS>;
 constexpr int64_t kBigTiles = 512;  // 256 x 256 tiles from which on they are taken
 inline bool big_tiles(int64_t p_rows, int64_t q_rows) {
   return ceil_div(p_rows, (int64_t)256) * ceil_div(q_rows, (int64_t)256) >= kBigTiles;
 }
 constexpr int64_t kSplitTarget = 512;  // workgroups the weight gradient aims at
 
-// What a call needs and where it lies in the workspace.
-template <class T>
+// fp32 layers go through the fp16 matrix cores in two parts of 11 bits a value
+// and three products (the low parts' own product is below 2^-22): three times
+// the work at nine times the rate.  Forming the parts takes two more kernels,
+// which pays from this many multiply-adds on.
+constexpr double kPartsWork = 1 << 28;
+inline bool takes_parts(const GatedArgs& a) {
+  return a.type == ELEM_F32 && (double)a.rows * (double)a.width * (double)a.hidden >= kPartsWork;
+}
+
+// What a call needs and where it lies in the workspace.  SPLIT: fp32 in parts.
+template <class T, bool SPLIT>
 struct Plan {
-  int64_t wpad, hpad;  // width and hidden rounded to whole 16-byte chunks
+  using E = typename std::conditional<SPLIT, _Float16, T>::type;  // what the products take
+  static constexpr int PARTS = SPLIT ? 3 : 1, COPIES = SPLIT ? 2 : 1;
+  // width and hidden rounded to whole 16-byte chunks, or to whole stages
+  static constexpr int WQ = SPLIT ? 64 : Vec16<T>::N, HQ = SPLIT ? 32 : Vec16<T>::N;
+  int64_t wpad, hpad;
   bool pack_x, pack_w;
   size_t x_off = 0, wg_off = 0, wu_off = 0, wt_off = 0, dgu_off = 0, dbias_off = 0, part_off = 0;
+  size_t stat_off = 0, scale_off = 0;
   size_t bytes = 0;
   bool big_dual = false, big_dx = false, big_dw = false;
   int64_t bias_parts = 0, splits = 1, k_split = 0;
 
   Plan(const GatedArgs& a, bool backward) {
-    constexpr int N = Vec16<T>::N;
-    wpad = round_up(a.width, N);
-    hpad = round_up(a.hidden, N);
-    pack_x = !direct<T>(a.x, a.x_stride, a.width);
-    pack_w = !direct<T>(a.w_gate, a.w_gate_stride, a.width) ||
+    wpad = round_up(a.width, WQ);
+    hpad = round_up(a.hidden, HQ);
+    pack_x = SPLIT || !direct<T>(a.x, a.x_stride, a.width);
+    pack_w = SPLIT || !direct<T>(a.w_gate, a.w_gate_stride, a.width) ||
              !direct<T>(a.w_up, a.w_up_stride, a.width) || a.w_gate_stride != a.w_up_stride;
     auto take = [&](size_t n) {
       const size_t at = bytes;
       bytes += align_up(n);
       return at;
     };
-    if (pack_x) x_off = take((size_t)a.rows * wpad * sizeof(T));
+    if (pack_x) x_off = take((size_t)a.rows * wpad * COPIES * sizeof(E));
     if (pack_w) {
-      wg_off = take((size_t)a.hidden * wpad * sizeof(T));
-      wu_off = take((size_t)a.hidden * wpad * sizeof(T));
+      wg_off = take((size_t)a.hidden * wpad * COPIES * sizeof(E));
+      wu_off = take((size_t)a.hidden * wpad * COPIES * sizeof(E));
+    }
+    if (SPLIT) {
+      stat_off = take(kStats * kStatBlocks * sizeof(Stat));
+      scale_off = take(sizeof(Scales));
     }
     const int64_t rows = std::max<int64_t>(a.rows, 1);
     big_dual = big_tiles(2 * a.hidden, rows);
     if (!backward) return;
     big_dx = big_tiles(a.width, rows);
-    wt_off = take((size_t)a.width * 2 * hpad * sizeof(T));
-    dgu_off = take((size_t)a.rows * 2 * hpad * sizeof(T));
+    wt_off = take((size_t)a.width * ldd() * sizeof(E));
+    dgu_off = take((size_t)a.rows * ldd() * sizeof(E));
     bias_parts = 2 * ceil_div(rows, (int64_t)(big_dual ? 256 : 128));
     dbias_off = take((size_t)bias_parts * 2 * a.hidden * sizeof(float));
     // split the reduction over the rows until the tiles fill the device; each
     // split's sums cost a write and a read of the gradients in fp32
-    constexpr int64_t KS = kStageBytes / sizeof(T);
+    constexpr int64_t KS = 128 / sizeof(E);
     const int64_t stages = ceil_div(rows, KS);
     auto split_to = [&](int64_t side) {
       const int64_t tiles = ceil_div(2 * hpad, side) * ceil_div(a.width, side);
@@ -687,6 +1005,7 @@ struct Plan {
     k_split = per * KS;
     if (splits > 1) part_off = take((size_t)splits * 2 * a.hidden * a.width * sizeof(float));
   }
+  int64_t ldd() const { return 2 * hpad * COPIES; }  // of [dg | du] and the transposed weights
 };
 
 template <class T>
@@ -697,66 +1016,90 @@ void pack_rows(const void* src, int64_t ld, int64_t rows, int64_t cols, int64_t 
       static_cast<const T*>(src), ld, rows, cols, pad, dst);
 }
 
-template <class T>
+template <class E>
 struct Inputs {
-  const T *x, *wg, *wu;
+  const E *x, *wg, *wu;
   int64_t ldx, ldw;
+  const Scales* scales;
 };
 
-// x and the weights as the product kernel loads them.
-template <class T>
-Inputs<T> load_inputs(const GatedArgs& a, const Plan<T>& pl, char* ws, hipStream_t st) {
-  Inputs<T> in{static_cast<const T*>(a.x), static_cast<const T*>(a.w_gate),
-               static_cast<const T*>(a.w_up), a.x_stride, a.w_gate_stride};
-  if (pl.pack_x) {
-    T* x = reinterpret_cast<T*>(ws + pl.x_off);
-    pack_rows<T>(a.x, a.x_stride, a.rows, a.width, pl.wpad, x, st);
-    in.x = x;
-    in.ldx = pl.wpad;
-  }
-  if (pl.pack_w) {
-    T *g = reinterpret_cast<T*>(ws + pl.wg_off), *u = reinterpret_cast<T*>(ws + pl.wu_off);
-    pack_rows<T>(a.w_gate, a.w_gate_stride, a.hidden, a.width, pl.wpad, g, st);
-    pack_rows<T>(a.w_up, a.w_up_stride, a.hidden, a.width, pl.wpad, u, st);
-    in.wg = g;
-    in.wu = u;
-    in.ldw = pl.wpad;
-  }
-  return in;
-}
+inline Unscale pick(const Scales* s, float Scales::*m) { return {s ? &(s->*m) : nullptr}; }
 
-template <class TL, class EPI>
-void launch_gemm(const GemmShape& s, int64_t splits, const EPI& epi, hipStream_t st) {
-  k_gemm<TL, EPI><<<dim3((unsigned)(s.tiles_p * s.tiles_q), (unsigned)splits), TL::THREADS, 0,
-                    st>>>(s, epi);
-  MGP_HIP_CHECK(hipGetLastError());
+// x and the weights as the product kernel loads them.
+template <class T, bool SPLIT>
+Inputs<typename Plan<T, SPLIT>::E> load_inputs(const GatedArgs& a, const Plan<T, SPLIT>& pl,
+                                               const void* dh, int64_t dh_stride, char* ws,
+                                               hipStream_t st) {
+  using E = typename Plan<T, SPLIT>::E;
+  E *x = reinterpret_cast<E*>(ws + pl.x_off), *wg = reinterpret_cast<E*>(ws + pl.wg_off),
+    *wu = reinterpret_cast<E*>(ws + pl.wu_off);
+  if constexpr (SPLIT) {
+    Stat* part = reinterpret_cast<Stat*>(ws + pl.stat_off);
+    Scales* scales = reinterpret_cast<Scales*>(ws + pl.scale_off);
+    auto f = [](const void* p) { return static_cast<const float*>(p); };
+    StatSources src;
+    src.s[ST_X] = {{f(a.x), nullptr}, {a.x_stride, 0}, a.rows, a.width};
+    src.s[ST_W] = {{f(a.w_gate), f(a.w_up)}, {a.w_gate_stride, a.w_up_stride}, a.hidden, a.width};
+    src.s[ST_DH] = {{f(dh), nullptr}, {dh_stride, 0}, dh ? a.rows : 0, a.hidden};
+    k_stats<<<dim3(kStatBlocks, kStats), 256, 0, st>>>(src, part);
+    const int64_t items = (a.rows + 2 * a.hidden) * (pl.wpad / 8);
+    k_split<<<(unsigned)std::min<int64_t>(ceil_div(items, (int64_t)256), 4096), 256, 0, st>>>(
+        {f(a.x), f(a.w_gate), f(a.w_up), f(a.b_gate), f(a.b_up), a.x_stride, a.w_gate_stride,
+         a.w_up_stride, a.rows, a.hidden, a.width, pl.wpad, x, wg, wu, part,
+         a.activation == ACT_SIGMOID ? 1.0f : 0.0f, scales});
+    return {x, wg, wu, 2 * pl.wpad, 2 * pl.wpad, scales};
+  } else {
+    Inputs<E> in{static_cast<const T*>(a.x), static_cast<const T*>(a.w_gate),
+                 static_cast<const T*>(a.w_up), a.x_stride, a.w_gate_stride, nullptr};
+    if (pl.pack_x) {
+      pack_rows<T>(a.x, a.x_stride, a.rows, a.width, pl.wpad, x, st);
+      in.x = x;
+      in.ldx = pl.wpad;
+    }
+    if (pl.pack_w) {
+      pack_rows<T>(a.w_gate, a.w_gate_stride, a.hidden, a.width, pl.wpad, wg, st);
+      pack_rows<T>(a.w_up, a.w_up_stride, a.hidden, a.width, pl.wpad, wu, st);
+      in.wg = wg;
+      in.wu = wu;
+      in.ldw = pl.wpad;
+    }
+    return in;
+  }
 }
 
 template <class TL, class EPI>
 void launch_tiles(GemmShape s, int64_t splits, const EPI& epi, hipStream_t st) {
   s.tiles_p = ceil_div(s.p.n, (int64_t)(TL::DUAL ? TL::BP / 2 : TL::BP));
   s.tiles_q = ceil_div(s.q.n, (int64_t)TL::BQ);
-  launch_gemm<TL>(s, splits, epi, st);
+  k_gemm<TL, EPI><<<dim3((unsigned)(s.tiles_p * s.tiles_q), (unsigned)splits), TL::THREADS, 0,
+                    st>>>(s, epi);
+  MGP_HIP_CHECK(hipGetLastError());
 }
 
-template <class T, bool TR, bool DUAL, class EPI>
+template <class PL, bool TR, bool DUAL, class EPI>
 void launch_product(bool big, const GemmShape& s, int64_t splits, const EPI& epi,
                     hipStream_t st) {
   if (big)
-    launch_tiles<BigTile<T, TR, DUAL>>(s, splits, epi, st);
+    launch_tiles<BigTile<typename PL::E, TR, DUAL, PL::PARTS>>(s, splits, epi, st);
   else
-    launch_tiles<SmallTile<T, TR, DUAL>>(s, splits, epi, st);
+    launch_tiles<SmallTile<typename PL::E, TR, DUAL, PL::PARTS>>(s, splits, epi, st);
 }
 
-template <class T, class EPI>
-void launch_dual(const GatedArgs& a, const Plan<T>& pl, const Inputs<T>& in, const EPI& epi,
-                 hipStream_t st) {
+template <class E>
+Operand operand(const E* p, int64_t ld, int64_t n, const E* p2 = nullptr) {
+  return {reinterpret_cast<const char*>(p), reinterpret_cast<const char*>(p2),
+          ld * (int64_t)sizeof(E), n};
+}
+
+template <class PL, class EPI>
+void launch_dual(const GatedArgs& a, const PL& pl, const Inputs<typename PL::E>& in,
+                 const EPI& epi, hipStream_t st) {
   GemmShape s{};
-  s.p = {reinterpret_cast<const char*>(in.wg), reinterpret_cast<const char*>(in.wu),
-         in.ldw * (int64_t)sizeof(T), a.hidden};
-  s.q = {reinterpret_cast<const char*>(in.x), nullptr, in.ldx * (int64_t)sizeof(T), a.rows};
+  s.p = operand(in.wg, in.ldw, a.hidden, in.wu);
+  s.q = operand(in.x, in.ldx, a.rows);
   s.K = s.k_split = pl.wpad;
-  launch_product<T, false, true>(pl.big_dual, s, 1, epi, st);
+  s.p_lo = s.q_lo = pl.wpad * (int64_t)sizeof(typename PL::E);
+  launch_product<PL, false, true>(pl.big_dual, s, 1, epi, st);
 }
 
 template <class F>
@@ -769,24 +1112,38 @@ void dispatch_act(int act, F&& f) {
   }
 }
 
+// Runs f with the element type and whether fp32 goes in parts.
+template <class F>
+void dispatch_layer(const GatedArgs& a, F&& f) {
+  if (takes_parts(a)) return f(float{}, std::true_type{});
+  dispatch_elem(a.type, [&](auto tag) { f(tag, std::false_type{}); });
+}
+
 }  // namespace
 
 size_t gated_bytes(const GatedArgs& a, bool backward) {
   size_t n = 0;
-  dispatch_elem(a.type, [&](auto tag) { n = Plan<decltype(tag)>(a, backward).bytes; });
+  dispatch_layer(a, [&](auto tag, auto split) {
+    n = Plan<decltype(tag), split.value>(a, backward).bytes;
+  });
   return n;
 }
 
 void gated_forward(const GatedArgs& a, void* h, int64_t h_stride, void* ws, hipStream_t st) {
   if (a.rows == 0) return;
-  dispatch_elem(a.type, [&](auto tag) {
+  dispatch_layer(a, [&](auto tag, auto split) {
     using T = decltype(tag);
-    const Plan<T> pl(a, false);
-    const Inputs<T> in = load_inputs<T>(a, pl, static_cast<char*>(ws), st);
+    const Plan<T, split.value> pl(a, false);
+    const auto in = load_inputs(a, pl, nullptr, 0, static_cast<char*>(ws), st);
     dispatch_act(a.activation, [&](auto act) {
-      ForwardEpi<T, act.value> epi{static_cast<const T*>(a.b_gate), static_cast<const T*>(a.b_up),
-                                   static_cast<T*>(h), h_stride, a.rows, a.hidden};
-      launch_dual<T>(a, pl, in, epi, st);
+      ForwardEpi<T, act.value> epi{pick(in.scales, &Scales::fwd),
+                                   static_cast<const T*>(a.b_gate),
+                                   static_cast<const T*>(a.b_up),
+                                   static_cast<T*>(h),
+                                   h_stride,
+                                   a.rows,
+                                   a.hidden};
+      launch_dual(a, pl, in, epi, st);
     });
   });
 }
@@ -794,8 +1151,10 @@ void gated_forward(const GatedArgs& a, void* h, int64_t h_stride, void* ws, hipS
 void gated_backward(const GatedArgs& a, const void* dh, int64_t dh_stride, const GatedGrads& g,
                     void* ws_v, hipStream_t st) {
   char* ws = static_cast<char*>(ws_v);
-  dispatch_elem(a.type, [&](auto tag) {
+  dispatch_layer(a, [&](auto tag, auto split) {
     using T = decltype(tag);
+    using PL = Plan<T, split.value>;
+    using E = typename PL::E;
     T *dwg = static_cast<T*>(g.dw_gate), *dwu = static_cast<T*>(g.dw_up);
     T *dbg = static_cast<T*>(g.db_gate), *dbu = static_cast<T*>(g.db_up);
     if (a.rows == 0) {  // sums over no rows (fills by a kernel: a caller may capture them)
@@ -807,42 +1166,62 @@ void gated_backward(const GatedArgs& a, const void* dh, int64_t dh_stride, const
       MGP_HIP_CHECK(hipGetLastError());
       return;
     }
-    const Plan<T> pl(a, true);
-    const Inputs<T> in = load_inputs<T>(a, pl, ws, st);
-    T* dgu = reinterpret_cast<T*>(ws + pl.dgu_off);
+    const PL pl(a, true);
+    const Inputs<E> in = load_inputs(a, pl, dh, dh_stride, ws, st);
+    E* dgu = reinterpret_cast<E*>(ws + pl.dgu_off);
     float* dbias = dbg || dbu ? reinterpret_cast<float*>(ws + pl.dbias_off) : nullptr;
     dispatch_act(a.activation, [&](auto act) {
-      BackwardEpi<T, act.value> epi{static_cast<const T*>(a.b_gate), static_cast<const T*>(a.b_up),
-                                    static_cast<const T*>(dh), dh_stride, a.rows, a.hidden,
-                                    pl.hpad, dgu, dbias};
-      launch_dual<T>(a, pl, in, epi, st);
+      BackwardEpi<T, act.value, split.value> epi{pick(in.scales, &Scales::fwd),
+                                                 pick(in.scales, &Scales::d),
+                                                 static_cast<const T*>(a.b_gate),
+                                                 static_cast<const T*>(a.b_up),
+                                                 static_cast<const T*>(dh),
+                                                 dh_stride,
+                                                 a.rows,
+                                                 a.hidden,
+                                                 pl.hpad,
+                                                 dgu,
+                                                 dbias};
+      launch_dual(a, pl, in, epi, st);
     });
     if (dbias)
       k_sum_bias<T><<<(unsigned)ceil_div(2 * a.hidden, (int64_t)64), 1024, 0, st>>>(
           dbias, pl.bias_parts, a.hidden, dbg, dbu);
-    const int64_t ldd = 2 * pl.hpad * (int64_t)sizeof(T);
+    const int64_t lo = 2 * pl.hpad * (int64_t)sizeof(E);
     if (g.dx) {
-      T* wt = reinterpret_cast<T*>(ws + pl.wt_off);
-      k_transpose_weights<T><<<dim3((unsigned)ceil_div(pl.hpad, (int64_t)32),
-                                    (unsigned)ceil_div(a.width, (int64_t)32), 2),
-                               256, 0, st>>>(in.wg, in.wu, in.ldw, a.hidden, a.width,
-                                             pl.hpad, wt);
+      E* wt = reinterpret_cast<E*>(ws + pl.wt_off);
+      const unsigned gx = (unsigned)ceil_div(pl.hpad, (int64_t)32);
+      const unsigned gy = (unsigned)ceil_div(a.width, (int64_t)32);
+      if constexpr (split.value)
+        k_transpose_split<<<dim3(gx, gy, 4), 256, 0, st>>>(in.wg, in.wu, a.hidden, a.width,
+                                                           pl.wpad, pl.hpad, wt);
+      else
+        k_transpose_weights<T><<<dim3(gx, gy, 2), 256, 0, st>>>(in.wg, in.wu, in.ldw, a.hidden,
+                                                                a.width, pl.hpad, wt);
       GemmShape s{};
-      s.p = {reinterpret_cast<const char*>(wt), nullptr, ldd, a.width};
-      s.q = {reinterpret_cast<const char*>(dgu), nullptr, ldd, a.rows};
+      s.p = operand(wt, pl.ldd(), a.width);
+      s.q = operand(dgu, pl.ldd(), a.rows);
       s.K = s.k_split = 2 * pl.hpad;
-      launch_product<T, false, false>(
-          pl.big_dx, s, 1, StoreEpi<T>{static_cast<T*>(g.dx), a.width, a.rows, a.width}, st);
+      s.p_lo = s.q_lo = lo;
+      launch_product<PL, false, false>(pl.big_dx, s, 1,
+                                       StoreEpi<T>{pick(in.scales, &Scales::dx),
+                                                   static_cast<T*>(g.dx), a.width, a.rows,
+                                                   a.width},
+                                       st);
     }
     if (dwg || dwu) {
       float* part = pl.splits > 1 ? reinterpret_cast<float*>(ws + pl.part_off) : nullptr;
       GemmShape s{};
-      s.p = {reinterpret_cast<const char*>(in.x), nullptr, in.ldx * (int64_t)sizeof(T), pl.wpad};
-      s.q = {reinterpret_cast<const char*>(dgu), nullptr, ldd, 2 * pl.hpad};
+      s.p = operand(in.x, in.ldx, pl.wpad);
+      s.q = operand(static_cast<const E*>(dgu), pl.ldd(), 2 * pl.hpad);
       s.K = a.rows;
       s.k_split = pl.k_split;
-      launch_product<T, true, false>(pl.big_dw, s, pl.splits,
-                                     WeightEpi<T>{dwg, dwu, part, a.hidden, pl.hpad, a.width}, st);
+      s.p_lo = pl.wpad * (int64_t)sizeof(E);
+      s.q_lo = lo;
+      launch_product<PL, true, false>(pl.big_dw, s, pl.splits,
+                                      WeightEpi<T>{pick(in.scales, &Scales::dw), dwg, dwu, part,
+                                                   a.hidden, pl.hpad, a.width},
+                                      st);
       if (part)
         k_sum_parts<T><<<(unsigned)std::min<int64_t>(
                              ceil_div(2 * a.hidden * a.width, (int64_t)256), 8192),
