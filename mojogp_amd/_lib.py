@@ -357,7 +357,7 @@ def last_error() -> str:
 
 def call(name: str, *args) -> None:
     """Call a status-returning entry point; raise NativeCallError on failure."""
-    lib = load()
+    lib = _lib or load()
     status = getattr(lib, name)(*args)
     if status != 0:
         raise NativeCallError(name, status, last_error())

@@ -216,18 +216,18 @@ class NativeProvider:
         out [n, d]), on the calling program's current stream.  As every call of a
         provider it returns when the work is done."""
         from . import features
-        code, index, stream = features._first(Lf, "Lf")
+        dtype, code, index, stream = features._first(Lf, "Lf")
         shape = Lf.shape
         if code != 0 or len(shape) not in (1, 2) or shape[-1] != self.n or 0 in shape:
             raise ValueError(f"Lf must be float32 of shape (ncols, {self.n}), got "
                              f"{Lf.dtype} {tuple(shape)}")
-        features._rows(Rf, "Rf", code, index, shape)
+        features._rows(Rf, "Rf", dtype, index, shape)
         if not Lf.is_contiguous() or not Rf.is_contiguous():
             raise ValueError("Lf and Rf must be contiguous")
         if out is None:
             out = Lf.new_empty((self.n, self.d))
         else:
-            features._rows(out, "out", code, index, (self.n, self.d))
+            features._rows(out, "out", dtype, index, (self.n, self.d))
             if not out.is_contiguous():
                 raise ValueError("out must be contiguous")
         _lib.call("mgp_input_gradient_device", self.handle, Lf.data_ptr(), Rf.data_ptr(),

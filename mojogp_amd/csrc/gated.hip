@@ -128,16 +128,16 @@ __device__ __forceinline__ void store_run(T* p, int64_t left, const float* v) {
   }
 }
 
-// The two fp16 parts of scaled values: v scale = hi + lo to 22 bits, hi at p and
-// lo `apart` elements on.
-template <int N>
-__device__ __forceinline__ void store_parts(_Float16* p, int64_t apart, int64_t left, float scale,
+// The two parts of scaled values: v scale = hi + lo to twice the type's bits, hi
+// at p and lo `apart` elements on.
+template <int N, class E>
+__device__ __forceinline__ void store_parts(E* p, int64_t apart, int64_t left, float scale,
                                             const float* v) {
   float hi[N], lo[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     const float x = v[k] * scale;
-    hi[k] = (float)(_Float16)x;
+    hi[k] = (float)(E)x;
     lo[k] = x - hi[k];
   }
   store_run<N>(p, left, hi);
@@ -147,7 +147,7 @@ __device__ __forceinline__ void store_parts(_Float16* p, int64_t apart, int64_t 
 // ---------------------------------------------------------------- product core
 
 // A 16-byte operand fragment: 8 narrow elements of 32 reduction steps spread
-// over the lane groups, or 4 floats of 16.
+// over the lane groups, or 4 floats of 16 (k_gated_few alone).
 struct Frag {
   f4 v;
 };
@@ -194,7 +194,7 @@ struct GemmShape {
   int64_t K;          // reduction length
   int64_t tiles_p, tiles_q;
   int64_t k_split;    // reduction elements of one split (a multiple of a stage)
-  int64_t p_lo, q_lo; // three-part products: byte distance of the low parts from the high ones
+  int64_t p_lo, q_lo; // operands in parts: byte distance of the low parts from the high ones
 };
 
 // Tile of 16 TN WN columns (p rows) by 16 TM WM rows (q rows), one wave 16 TN
@@ -202,20 +202,21 @@ struct GemmShape {
 // RUN = 4 TN (dual: 2 TN of each matrix) consecutive columns.  Both operands go through LDS by direct loads, double
 // buffered, 128 bytes of reduction a stage.  NT: 128-byte LDS rows, 16-byte
 // chunk c of row r at c ^ (r / 2 % 8).  TN: LDS rows of the tile's width, one
-// per reduction step, in the memory's order; 32-byte granules at g ^ (r % 8)
-// (narrow types, read by the transposing LDS load), 64-byte ones at g ^ (r % 4)
-// (fp32): both keep the fragment reads off each other's banks.
+// per reduction step, in the memory's order, their 32-byte granules at g ^ (r % 8)
+// and read by the transposing LDS load.  Both keep the fragment reads off each
+// other's banks.
 template <class T, int TM_, int TN_, int WM_, int WN_, bool TR_, bool DUAL_, int PARTS_>
 struct Tile {
   using Elem = T;
   static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_;
   static constexpr bool TR = TR_, DUAL = DUAL_;
-  static constexpr int PARTS = PARTS_;  // 3: fp32 operands as two fp16 parts
+  static constexpr int PARTS = PARTS_;  // products a sum is made of: 3 of two operands in two parts
+                                        // each, 2 of q in two parts, 1
   static constexpr int W = WM * WN, THREADS = 64 * W;
   static constexpr int BQ = 16 * TM * WM, BP = 16 * TN * WN;
   static constexpr int T1 = DUAL ? TN / 2 : TN;  // 16-row tiles of one matrix a wave
   static constexpr int RUN = 4 * T1;
-  static constexpr int E = sizeof(T);
+  static constexpr int E = sizeof(T);  // 2
   static constexpr int SB = 128;                   // reduction bytes of a row a stage
   static constexpr int KS = SB / E;                // reduction elements a stage
   static constexpr int LDS = (BP + BQ) * SB;  // one buffer
@@ -224,9 +225,9 @@ struct Tile {
 };
 
 // What a wave loads of a stage: I instructions, each 64 lanes x 16 bytes = 1 KB
-// of LDS.  The instructions of a side lie a multiple of 8 LDS rows (TN: of 8,
-// fp32 4, reduction rows) apart, so the lanes' offsets from each one's uniform
-// start are the same; only which rows exist differs.
+// of LDS.  The instructions of a side lie a multiple of 8 LDS rows apart, so the
+// lanes' offsets from each one's uniform start are the same; only which rows
+// exist differs.
 template <class TL>
 struct Loader {
   static constexpr int I = TL::IP + TL::IQ;
@@ -236,7 +237,7 @@ struct Loader {
   int soff[I];           // bytes from the side's base to the instruction's start
   const char* base[3];   // of p, of q, of p's second matrix
   int64_t step[2];       // bytes of a stage
-  int64_t jump[2][2];    // three parts: bytes to the next product's start, after its stages
+  int64_t jump[2][2];    // bytes to the next part product's start, after a part's stages
   int64_t length, left;  // reduction elements of a part, and those still to load
   int part;
 
@@ -251,14 +252,18 @@ struct Loader {
     step[0] = TL::TR ? TL::KS * s.p.ld_bytes : TL::SB;
     step[1] = TL::TR ? TL::KS * s.q.ld_bytes : TL::SB;
     length = left = K;
-    if constexpr (TL::PARTS == 3) {
-      // p: high, low, high; q: high, high, low
+    if constexpr (TL::PARTS > 1) {
       const int64_t back_p = (K + TL::KS - 1) / TL::KS * step[0];
       const int64_t back_q = (K + TL::KS - 1) / TL::KS * step[1];
-      jump[0][0] = s.p_lo - back_p;
-      jump[0][1] = -s.p_lo - back_p;
-      jump[1][0] = -back_q;
-      jump[1][1] = s.q_lo - back_q;
+      if constexpr (TL::PARTS == 3) {  // p: high, low, high; q: high, high, low
+        jump[0][0] = s.p_lo - back_p;
+        jump[0][1] = -s.p_lo - back_p;
+        jump[1][0] = -back_q;
+        jump[1][1] = s.q_lo - back_q;
+      } else {  // p twice; q: high, low
+        jump[0][0] = -back_p;
+        jump[1][0] = s.q_lo - back_q;
+      }
       part = 0;
     }
   }
@@ -299,10 +304,9 @@ struct Loader {
       }
     } else {
       constexpr int RB = B * TL::E;  // bytes of an LDS row
-      static_assert(TL::W * 1024 / RB % (TL::E == 2 ? 8 : 4) == 0, "");
+      static_assert(TL::W * 1024 / RB % 8 == 0, "");
       const int byte = wave * 1024 + lane * 16, r = byte / RB;
-      const int c = (byte % RB / 16) ^
-                    ((TL::E == 2 ? ((r & 7) << 1) : ((r & 3) << 2)) & (RB / 16 - 1));
+      const int c = (byte % RB / 16) ^ (((r & 7) << 1) & (RB / 16 - 1));
       const bool in = row0 + c * (16 / TL::E) < o.n;
       kpos[!P] = r;
       voff[!P] = r * ld + c * 16;
@@ -329,12 +333,12 @@ struct Loader {
                exists[i] && kpos[!p] < l - at ? voff[!p] : kOutOfRange, soff[i], dst);
     }
     left -= TL::KS;
-    const bool turn = TL::PARTS == 3 && left <= 0 && part < 2;
+    const bool turn = TL::PARTS > 1 && left <= 0 && part < TL::PARTS - 1;
 #pragma unroll
     for (int b = 0; b < (second(1) ? 3 : 2); ++b) {
       base[b] += step[b & 1];
-      if constexpr (TL::PARTS == 3) {
-        if (turn) base[b] += part ? jump[b & 1][1] : jump[b & 1][0];
+      if constexpr (TL::PARTS > 1) {
+        if (turn) base[b] += TL::PARTS == 3 && part ? jump[b & 1][1] : jump[b & 1][0];
       }
     }
     if (turn) {
@@ -350,7 +354,7 @@ __device__ __forceinline__ Frag read_frag(const char* __restrict__ buf, int row,
   if constexpr (!TL::TR) {
     const int c = (ks * 4 + g) ^ (i >> 1);
     return {*reinterpret_cast<const f4*>(buf + (row + i) * TL::SB + c * 16)};
-  } else if constexpr (TL::E == 2) {
+  } else {
     // lane group g takes reduction rows 4 g .. 4 g + 3 and the same + 16; the
     // transposing load gives lane i the four rows' elements of column i
     constexpr int RB = B * TL::E, M = RB / 32 - 1;
@@ -365,16 +369,6 @@ __device__ __forceinline__ Frag read_frag(const char* __restrict__ buf, int row,
     typedef short s8 __attribute__((ext_vector_type(8)));
     const s8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     return {__builtin_bit_cast(f4, v)};
-  } else {
-    constexpr int RB = B * TL::E;
-    Frag f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int r = ks * 16 + 4 * k + g, col = row + i;  // r % 4 = g
-      f.v[k] = *reinterpret_cast<const float*>(
-          buf + r * RB + (((col >> 2) ^ ((g << 2) & (RB / 16 - 1))) << 4) + (col & 3) * 4);
-    }
-    return f;
   }
 }
 
@@ -511,9 +505,8 @@ struct ForwardEpi {
 
 // dgu[row] = [dg | du], each `pad` columns (zeros past hidden);
 // dbias[part][2][hidden] the column sums over a wave's rows.
-// dgu of fp32 operands: two fp16 parts of the scaled values, the low ones after
-// the high ones of a row.
-template <class T, int ACT, bool SPLIT>
+// SPLIT: two parts of the scaled values, the low ones after the high ones of a row.
+template <class T, class E, int ACT, bool SPLIT>
 struct BackwardEpi {
   Unscale scale, dgu_scale;  // dgu_scale: what dg and du are multiplied by
   const T *bg, *bu;
@@ -553,11 +546,11 @@ struct BackwardEpi {
         su[k] += du[k];
       }
       if constexpr (SPLIT) {
-        _Float16* row = static_cast<_Float16*>(dgu) + r * 4 * pad + f;
+        E* row = static_cast<E*>(dgu) + r * 4 * pad + f;
         store_parts<N>(row, 2 * pad, pad - f, ds, dg);
         store_parts<N>(row + pad, 2 * pad, pad - f, ds, du);
       } else {
-        T* row = static_cast<T*>(dgu) + r * 2 * pad + f;
+        E* row = static_cast<E*>(dgu) + r * 2 * pad + f;
         store_run<N>(row, pad - f, dg);
         store_run<N>(row + pad, pad - f, du);
       }
@@ -579,11 +572,13 @@ struct BackwardEpi {
   }
 };
 
+// One split: the result; more: part[split][rows][cols] sums.
 template <class T>
 struct StoreEpi {
   Unscale scale;
   T* out;
-  int64_t ld, rows, cols;
+  float* part;
+  int64_t rows, cols;
   template <class TL>
   __device__ __forceinline__ void run(f4 (&acc)[TL::TM][TL::TN], int64_t m0, int64_t n0,
                                       int64_t) const {
@@ -599,7 +594,10 @@ struct StoreEpi {
       float o[N];
 #pragma unroll
       for (int k = 0; k < N; ++k) o[k] = acc[m][k / 4][k % 4] * sc;
-      store_run<N>(out + r * ld + c, cols - c, o);
+      if (part)
+        store_run<N>(part + ((int64_t)blockIdx.y * rows + r) * cols + c, cols - c, o);
+      else
+        store_run<N>(out + r * cols + c, cols - c, o);
     }
   }
 };
@@ -682,21 +680,30 @@ __global__ __launch_bounds__(256) void k_transpose_weights(const T* __restrict__
   }
 }
 
-// out_g / out_u [count] = sums over the parts of part[parts][2][count], in order
+// out0 / out1 [count] = sums over the parts of part[parts][outputs][count], in order
 template <class T>
 __global__ __launch_bounds__(256) void k_sum_parts(const float* __restrict__ part, int64_t parts,
-                                                   int64_t count, T* __restrict__ out_g,
-                                                   T* __restrict__ out_u) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < 2 * count;
+                                                   int64_t count, int outputs,
+                                                   T* __restrict__ out0, T* __restrict__ out1) {
+  const int64_t total = outputs * count;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
        i += (int64_t)gridDim.x * 256) {
-    const bool up = i >= count;
-    T* dst = up ? out_u : out_g;
+    const bool second = i >= count;
+    T* dst = second ? out1 : out0;
     if (dst == nullptr) continue;
     float s = 0.0f;
 #pragma unroll 8
-    for (int64_t p = 0; p < parts; ++p) s += part[p * 2 * count + i];
-    dst[i - (up ? count : 0)] = (T)s;
+    for (int64_t p = 0; p < parts; ++p) s += part[p * total + i];
+    dst[i - (second ? count : 0)] = (T)s;
   }
+}
+
+template <class T>
+void sum_parts(const float* part, int64_t parts, int64_t count, int outputs, T* out0, T* out1,
+               hipStream_t st) {
+  const int64_t blocks = ceil_div(outputs * count, (int64_t)256);
+  k_sum_parts<T><<<(unsigned)std::min<int64_t>(blocks, 8192), 256, 0, st>>>(part, parts, count,
+                                                                           outputs, out0, out1);
 }
 
 // The bias gradients: few columns, many parts; 64 columns a block, 16 waves
@@ -719,6 +726,89 @@ __global__ __launch_bounds__(1024) void k_sum_bias(const float* __restrict__ par
   for (int k = 1; k < 16; ++k) s += red[k][lane];
   T* dst = i < count ? out_g : out_u;
   if (dst) dst[i < count ? i : i - count] = (T)s;
+}
+
+// ---------------------------------------------------------------- little work
+
+struct FewArgs {
+  const void *x, *wg, *wu, *bg, *bu;
+  int64_t ldx, ldg, ldu, ldh, rows, width, hidden;
+  void* h;
+};
+
+// The forward pass where the product kernel's tiles would leave most of the
+// device idle (a single point, a batch of a few hundred): a workgroup takes 16
+// columns of both projections for 16 MT rows, its 8 waves share the reduction
+// and read their fragments from global memory, at any alignment.  Bound by
+// latency: one round of loads for a width of 512, one exchange through LDS.
+template <class T, int ACT, int MT>
+__global__ __launch_bounds__(512) void k_gated_few(FewArgs s) {
+  constexpr int N = Vec16<T>::N, W = 8;
+  __shared__ f4 red[W][2 * MT][64];
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t f0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * 16 * MT;
+  // rows past the last are read as the last and not stored
+  const int64_t f = min(f0 + i, s.hidden - 1);
+  const T* wg = static_cast<const T*>(s.wg) + f * s.ldg;
+  const T* wu = static_cast<const T*>(s.wu) + f * s.ldu;
+  const T* x[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+    x[t] = static_cast<const T*>(s.x) + min(m0 + 16 * t + i, s.rows - 1) * s.ldx;
+  f4 ag[MT], au[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) ag[t] = au[t] = f4{0.f, 0.f, 0.f, 0.f};
+  auto frag = [&](const T* p, int64_t k) __attribute__((always_inline)) {
+    T a[N];
+    if (k + N <= s.width) {
+      __builtin_memcpy(a, p + k, 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) a[e] = k + e < s.width ? p[k + e] : (T)0.0f;
+    }
+    Frag r;
+    __builtin_memcpy(&r, a, 16);
+    return r;
+  };
+#pragma unroll 2
+  for (int64_t k0 = wave * 4 * N; k0 < s.width; k0 += W * 4 * N) {
+    const int64_t k = k0 + g * N;
+    const Frag pg = frag(wg, k), pu = frag(wu, k);
+    Frag q[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) q[t] = frag(x[t], k);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      ag[t] = mma<T>(pg, q[t], ag[t]);
+      au[t] = mma<T>(pu, q[t], au[t]);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    red[wave][2 * t][lane] = ag[t];
+    red[wave][2 * t + 1][lane] = au[t];
+  }
+  __syncthreads();
+  if (wave >= MT) return;
+  f4 sg = red[0][2 * wave][lane], su = red[0][2 * wave + 1][lane];
+#pragma unroll
+  for (int w = 1; w < W; ++w) {
+    sg += red[w][2 * wave][lane];
+    su += red[w][2 * wave + 1][lane];
+  }
+  const int64_t r = m0 + 16 * wave + i, c = f0 + 4 * g, left = s.hidden - c;
+  if (r >= s.rows || left <= 0) return;
+  float b0[4] = {0, 0, 0, 0}, b1[4] = {0, 0, 0, 0}, o[4];
+  if (s.bg) load_run<4>(static_cast<const T*>(s.bg) + c, left, b0);
+  if (s.bu) load_run<4>(static_cast<const T*>(s.bu) + c, left, b1);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float a, slope;
+    activate<ACT, sizeof(T) == 2>(sg[e] + b0[e], a, slope);
+    o[e] = a * (su[e] + b1[e]);
+  }
+  store_run<4>(static_cast<T*>(s.h) + r * s.ldh + c, left, o);
 }
 
 // ---------------------------------------------------------------- fp32 operands in fp16 parts
@@ -935,31 +1025,42 @@ constexpr int64_t kBigTiles = 512;  // 256 x 256 tiles from which on they are ta
 inline bool big_tiles(int64_t p_rows, int64_t q_rows) {
   return ceil_div(p_rows, (int64_t)256) * ceil_div(q_rows, (int64_t)256) >= kBigTiles;
 }
-constexpr int64_t kSplitTarget = 512;  // workgroups the weight gradient aims at
+constexpr int64_t kSplitTarget = 512;  // workgroups that a split reduction aims at
 
 // fp32 layers go through the fp16 matrix cores in two parts of 11 bits a value
 // and three products (the low parts' own product is below 2^-22): three times
-// the work at nine times the rate.  Forming the parts takes two more kernels,
-// which pays from this many multiply-adds on.
-constexpr double kPartsWork = 1 << 28;
-inline bool takes_parts(const GatedArgs& a) {
-  return a.type == ELEM_F32 && (double)a.rows * (double)a.width * (double)a.hidden >= kPartsWork;
-}
+// the work at nine times the rate of the fp32 instructions, 24 against 128
+// cycles a reduction element of a tile.  Forming the parts takes two more
+// kernels.  20000 x 256 -> 512, both passes: 495 -> 343 us.
 
-// What a call needs and where it lies in the workspace.  SPLIT: fp32 in parts.
-template <class T, bool SPLIT>
+// The 16-bit types' dg and du are rounded to the type for the last two products;
+// with few rows the roundings do not average out, and dx's and the weight
+// gradients' error reaches 1.5 times that of their own rounding (1.41 with
+// many).  Up to one tile of rows dg and du go in two parts instead, which costs
+// the last two products twice: 3 of ~60 us there, 2 of 4.4 ms at 65536 rows.
+constexpr int64_t kFewRows = 128;
+
+enum Mode : int { PLAIN = 0, FP32_PARTS = 1, FEW_ROWS = 2 };
+
+// What a call needs and where it lies in the workspace.
+template <class T, int MODE_>
 struct Plan {
+  static constexpr int MODE = MODE_;
+  static constexpr bool SPLIT = MODE == FP32_PARTS;
   using E = typename std::conditional<SPLIT, _Float16, T>::type;  // what the products take
-  static constexpr int PARTS = SPLIT ? 3 : 1, COPIES = SPLIT ? 2 : 1;
+  // products of the projections and of the gradients; copies of x and the
+  // weights, and of dg and du
+  static constexpr int PARTS = SPLIT ? 3 : 1, GRAD_PARTS = SPLIT ? 3 : MODE == FEW_ROWS ? 2 : 1;
+  static constexpr int COPIES = SPLIT ? 2 : 1, D_COPIES = MODE == PLAIN ? 1 : 2;
   // width and hidden rounded to whole 16-byte chunks, or to whole stages
   static constexpr int WQ = SPLIT ? 64 : Vec16<T>::N, HQ = SPLIT ? 32 : Vec16<T>::N;
   int64_t wpad, hpad;
   bool pack_x, pack_w;
   size_t x_off = 0, wg_off = 0, wu_off = 0, wt_off = 0, dgu_off = 0, dbias_off = 0, part_off = 0;
-  size_t stat_off = 0, scale_off = 0;
+  size_t stat_off = 0, scale_off = 0, dxp_off = 0;
   size_t bytes = 0;
   bool big_dual = false, big_dx = false, big_dw = false;
-  int64_t bias_parts = 0, splits = 1, k_split = 0;
+  int64_t bias_parts = 0, splits = 1, k_split = 0, dx_splits = 1, dx_split = 0;
 
   Plan(const GatedArgs& a, bool backward) {
     wpad = round_up(a.width, WQ);
@@ -982,30 +1083,39 @@ struct Plan {
       scale_off = take(sizeof(Scales));
     }
     const int64_t rows = std::max<int64_t>(a.rows, 1);
-    big_dual = big_tiles(2 * a.hidden, rows);
+    big_dual = MODE != FEW_ROWS && big_tiles(2 * a.hidden, rows);
     if (!backward) return;
     big_dx = big_tiles(a.width, rows);
-    wt_off = take((size_t)a.width * ldd() * sizeof(E));
+    wt_off = take((size_t)a.width * ldt() * sizeof(E));
     dgu_off = take((size_t)a.rows * ldd() * sizeof(E));
     bias_parts = 2 * ceil_div(rows, (int64_t)(big_dual ? 256 : 128));
     dbias_off = take((size_t)bias_parts * 2 * a.hidden * sizeof(float));
-    // split the reduction over the rows until the tiles fill the device; each
-    // split's sums cost a write and a read of the gradients in fp32
+    // Where the tiles do not fill the device the reductions are split: of the
+    // weight gradients over the rows, of dx (few rows) over hidden.  Each
+    // split's sums cost a write and a read of the result in fp32.
     constexpr int64_t KS = 128 / sizeof(E);
     const int64_t stages = ceil_div(rows, KS);
-    auto split_to = [&](int64_t side) {
-      const int64_t tiles = ceil_div(2 * hpad, side) * ceil_div(a.width, side);
-      return std::max<int64_t>(1, std::min(ceil_div(kSplitTarget, tiles),
-                                           ceil_div(stages, (int64_t)16)));
-    };
     big_dw = 2 * hpad * a.width >= (int64_t)16 * 256 * 256 && stages >= 64;
-    splits = split_to(big_dw ? 256 : 128);
+    const int64_t side = big_dw ? 256 : 128;
+    split(stages, ceil_div(2 * hpad, side) * ceil_div(a.width, side), 16, splits, k_split);
+    if (splits > 1) part_off = take((size_t)splits * 2 * a.hidden * a.width * sizeof(float));
+    const int64_t dx_side = big_dx ? 256 : 128;
+    split(ceil_div(2 * hpad, KS), ceil_div(rows, dx_side) * ceil_div(a.width, dx_side), 8,
+          dx_splits, dx_split);
+    if (dx_splits > 1) dxp_off = take((size_t)dx_splits * a.rows * a.width * sizeof(float));
+  }
+  // Splits of `least` stages or more until there are kSplitTarget workgroups.
+  static void split(int64_t stages, int64_t tiles, int64_t least, int64_t& splits,
+                    int64_t& length) {
+    splits = std::max<int64_t>(
+        1, std::min(ceil_div(kSplitTarget, tiles), ceil_div(stages, least)));
+    if (tiles * 2 > kSplitTarget) splits = 1;
     const int64_t per = ceil_div(stages, splits);
     splits = ceil_div(stages, per);
-    k_split = per * KS;
-    if (splits > 1) part_off = take((size_t)splits * 2 * a.hidden * a.width * sizeof(float));
+    length = per * (128 / (int64_t)sizeof(E));
   }
-  int64_t ldd() const { return 2 * hpad * COPIES; }  // of [dg | du] and the transposed weights
+  int64_t ldd() const { return 2 * hpad * D_COPIES; }  // of [dg | du]
+  int64_t ldt() const { return 2 * hpad * COPIES; }    // of the transposed weights
 };
 
 template <class T>
@@ -1026,14 +1136,14 @@ struct Inputs {
 inline Unscale pick(const Scales* s, float Scales::*m) { return {s ? &(s->*m) : nullptr}; }
 
 // x and the weights as the product kernel loads them.
-template <class T, bool SPLIT>
-Inputs<typename Plan<T, SPLIT>::E> load_inputs(const GatedArgs& a, const Plan<T, SPLIT>& pl,
-                                               const void* dh, int64_t dh_stride, char* ws,
-                                               hipStream_t st) {
-  using E = typename Plan<T, SPLIT>::E;
+template <class T, int MODE>
+Inputs<typename Plan<T, MODE>::E> load_inputs(const GatedArgs& a, const Plan<T, MODE>& pl,
+                                              const void* dh, int64_t dh_stride, char* ws,
+                                              hipStream_t st) {
+  using E = typename Plan<T, MODE>::E;
   E *x = reinterpret_cast<E*>(ws + pl.x_off), *wg = reinterpret_cast<E*>(ws + pl.wg_off),
     *wu = reinterpret_cast<E*>(ws + pl.wu_off);
-  if constexpr (SPLIT) {
+  if constexpr (MODE == FP32_PARTS) {
     Stat* part = reinterpret_cast<Stat*>(ws + pl.stat_off);
     Scales* scales = reinterpret_cast<Scales*>(ws + pl.scale_off);
     auto f = [](const void* p) { return static_cast<const float*>(p); };
@@ -1079,10 +1189,12 @@ void launch_tiles(GemmShape s, int64_t splits, const EPI& epi, hipStream_t st) {
 template <class PL, bool TR, bool DUAL, class EPI>
 void launch_product(bool big, const GemmShape& s, int64_t splits, const EPI& epi,
                     hipStream_t st) {
-  if (big)
-    launch_tiles<BigTile<typename PL::E, TR, DUAL, PL::PARTS>>(s, splits, epi, st);
-  else
-    launch_tiles<SmallTile<typename PL::E, TR, DUAL, PL::PARTS>>(s, splits, epi, st);
+  constexpr int PARTS = DUAL ? PL::PARTS : PL::GRAD_PARTS;
+  if constexpr (PL::MODE != FEW_ROWS) {  // (which has too few for the large tiles)
+    if (big)
+      return launch_tiles<BigTile<typename PL::E, TR, DUAL, PARTS>>(s, splits, epi, st);
+  }
+  launch_tiles<SmallTile<typename PL::E, TR, DUAL, PARTS>>(s, splits, epi, st);
 }
 
 template <class E>
@@ -1112,28 +1224,69 @@ void dispatch_act(int act, F&& f) {
   }
 }
 
-// Runs f with the element type and whether fp32 goes in parts.
+// Forward passes by k_gated_few: up to this many of its workgroups it is the
+// faster one.  16 bits: 512 rows x 256 -> 1024 (512 workgroups) 5.6 against 6.1 us,
+// 1024 rows 9.1 against 6.3; fp32, against the three-part product and its two
+// kernels before it: 512 x 256 -> 1024 9.9 against ~20, 1024 rows 19 against 22.
+inline bool takes_few(const GatedArgs& a) {
+  return ceil_div(a.rows, (int64_t)64) * ceil_div(a.hidden, (int64_t)16) <=
+         (a.type == ELEM_F32 ? 768 : 512);
+}
+
+template <class T, int ACT>
+void launch_few(const FewArgs& s, hipStream_t st) {
+  auto go = [&](auto mt) {
+    constexpr int MT = decltype(mt)::value;
+    k_gated_few<T, ACT, MT><<<dim3((unsigned)ceil_div(s.hidden, (int64_t)16),
+                                   (unsigned)ceil_div(s.rows, (int64_t)(16 * MT))),
+                              512, 0, st>>>(s);
+  };
+  if (s.rows <= 16)
+    go(std::integral_constant<int, 1>{});
+  else if (s.rows <= 32)
+    go(std::integral_constant<int, 2>{});
+  else
+    go(std::integral_constant<int, 4>{});
+  MGP_HIP_CHECK(hipGetLastError());
+}
+
+// Runs f with the element type and the mode of a pass.
 template <class F>
-void dispatch_layer(const GatedArgs& a, F&& f) {
-  if (takes_parts(a)) return f(float{}, std::true_type{});
-  dispatch_elem(a.type, [&](auto tag) { f(tag, std::false_type{}); });
+void dispatch_layer(const GatedArgs& a, bool backward, F&& f) {
+  dispatch_elem(a.type, [&](auto tag) {
+    if constexpr (sizeof(tag) == 4)
+      f(tag, std::integral_constant<int, FP32_PARTS>{});
+    else if (backward && a.rows <= kFewRows)
+      f(tag, std::integral_constant<int, FEW_ROWS>{});
+    else
+      f(tag, std::integral_constant<int, PLAIN>{});
+  });
 }
 
 }  // namespace
 
 size_t gated_bytes(const GatedArgs& a, bool backward) {
+  if (!backward && takes_few(a)) return 0;
   size_t n = 0;
-  dispatch_layer(a, [&](auto tag, auto split) {
-    n = Plan<decltype(tag), split.value>(a, backward).bytes;
+  dispatch_layer(a, backward, [&](auto tag, auto mode) {
+    n = Plan<decltype(tag), mode.value>(a, backward).bytes;
   });
   return n;
 }
 
 void gated_forward(const GatedArgs& a, void* h, int64_t h_stride, void* ws, hipStream_t st) {
   if (a.rows == 0) return;
-  dispatch_layer(a, [&](auto tag, auto split) {
+  if (takes_few(a)) {
+    const FewArgs s{a.x,        a.w_gate, a.w_up, a.b_gate, a.b_up, a.x_stride, a.w_gate_stride,
+                    a.w_up_stride, h_stride, a.rows, a.width, a.hidden, h};
+    dispatch_elem(a.type, [&](auto tag) {
+      dispatch_act(a.activation, [&](auto act) { launch_few<decltype(tag), act.value>(s, st); });
+    });
+    return;
+  }
+  dispatch_layer(a, false, [&](auto tag, auto mode) {
     using T = decltype(tag);
-    const Plan<T, split.value> pl(a, false);
+    const Plan<T, mode.value> pl(a, false);
     const auto in = load_inputs(a, pl, nullptr, 0, static_cast<char*>(ws), st);
     dispatch_act(a.activation, [&](auto act) {
       ForwardEpi<T, act.value> epi{pick(in.scales, &Scales::fwd),
@@ -1151,18 +1304,15 @@ void gated_forward(const GatedArgs& a, void* h, int64_t h_stride, void* ws, hipS
 void gated_backward(const GatedArgs& a, const void* dh, int64_t dh_stride, const GatedGrads& g,
                     void* ws_v, hipStream_t st) {
   char* ws = static_cast<char*>(ws_v);
-  dispatch_layer(a, [&](auto tag, auto split) {
+  dispatch_layer(a, true, [&](auto tag, auto mode) {
     using T = decltype(tag);
-    using PL = Plan<T, split.value>;
+    using PL = Plan<T, mode.value>;
     using E = typename PL::E;
     T *dwg = static_cast<T*>(g.dw_gate), *dwu = static_cast<T*>(g.dw_up);
     T *dbg = static_cast<T*>(g.db_gate), *dbu = static_cast<T*>(g.db_up);
     if (a.rows == 0) {  // sums over no rows (fills by a kernel: a caller may capture them)
-      const unsigned grid =
-          (unsigned)std::min<int64_t>(ceil_div(2 * a.hidden * a.width, (int64_t)256), 4096);
-      if (dwg || dwu)
-        k_sum_parts<T><<<grid, 256, 0, st>>>(nullptr, 0, a.hidden * a.width, dwg, dwu);
-      if (dbg || dbu) k_sum_parts<T><<<grid, 256, 0, st>>>(nullptr, 0, a.hidden, dbg, dbu);
+      if (dwg || dwu) sum_parts<T>(nullptr, 0, a.hidden * a.width, 2, dwg, dwu, st);
+      if (dbg || dbu) sum_parts<T>(nullptr, 0, a.hidden, 2, dbg, dbu, st);
       MGP_HIP_CHECK(hipGetLastError());
       return;
     }
@@ -1171,17 +1321,17 @@ void gated_backward(const GatedArgs& a, const void* dh, int64_t dh_stride, const
     E* dgu = reinterpret_cast<E*>(ws + pl.dgu_off);
     float* dbias = dbg || dbu ? reinterpret_cast<float*>(ws + pl.dbias_off) : nullptr;
     dispatch_act(a.activation, [&](auto act) {
-      BackwardEpi<T, act.value, split.value> epi{pick(in.scales, &Scales::fwd),
-                                                 pick(in.scales, &Scales::d),
-                                                 static_cast<const T*>(a.b_gate),
-                                                 static_cast<const T*>(a.b_up),
-                                                 static_cast<const T*>(dh),
-                                                 dh_stride,
-                                                 a.rows,
-                                                 a.hidden,
-                                                 pl.hpad,
-                                                 dgu,
-                                                 dbias};
+      BackwardEpi<T, E, act.value, PL::D_COPIES == 2> epi{pick(in.scales, &Scales::fwd),
+                                                          pick(in.scales, &Scales::d),
+                                                          static_cast<const T*>(a.b_gate),
+                                                          static_cast<const T*>(a.b_up),
+                                                          static_cast<const T*>(dh),
+                                                          dh_stride,
+                                                          a.rows,
+                                                          a.hidden,
+                                                          pl.hpad,
+                                                          dgu,
+                                                          dbias};
       launch_dual(a, pl, in, epi, st);
     });
     if (dbias)
@@ -1192,22 +1342,24 @@ void gated_backward(const GatedArgs& a, const void* dh, int64_t dh_stride, const
       E* wt = reinterpret_cast<E*>(ws + pl.wt_off);
       const unsigned gx = (unsigned)ceil_div(pl.hpad, (int64_t)32);
       const unsigned gy = (unsigned)ceil_div(a.width, (int64_t)32);
-      if constexpr (split.value)
+      if constexpr (PL::SPLIT)
         k_transpose_split<<<dim3(gx, gy, 4), 256, 0, st>>>(in.wg, in.wu, a.hidden, a.width,
                                                            pl.wpad, pl.hpad, wt);
       else
         k_transpose_weights<T><<<dim3(gx, gy, 2), 256, 0, st>>>(in.wg, in.wu, in.ldw, a.hidden,
                                                                 a.width, pl.hpad, wt);
       GemmShape s{};
-      s.p = operand(wt, pl.ldd(), a.width);
+      s.p = operand(wt, pl.ldt(), a.width);
       s.q = operand(dgu, pl.ldd(), a.rows);
-      s.K = s.k_split = 2 * pl.hpad;
+      s.K = 2 * pl.hpad;
+      s.k_split = pl.dx_split;
       s.p_lo = s.q_lo = lo;
-      launch_product<PL, false, false>(pl.big_dx, s, 1,
-                                       StoreEpi<T>{pick(in.scales, &Scales::dx),
-                                                   static_cast<T*>(g.dx), a.width, a.rows,
-                                                   a.width},
-                                       st);
+      T* dx = static_cast<T*>(g.dx);
+      float* part = pl.dx_splits > 1 ? reinterpret_cast<float*>(ws + pl.dxp_off) : nullptr;
+      launch_product<PL, false, false>(
+          pl.big_dx, s, pl.dx_splits,
+          StoreEpi<T>{pick(in.scales, &Scales::dx), dx, part, a.rows, a.width}, st);
+      if (part) sum_parts<T>(part, pl.dx_splits, a.rows * a.width, 1, dx, nullptr, st);
     }
     if (dwg || dwu) {
       float* part = pl.splits > 1 ? reinterpret_cast<float*>(ws + pl.part_off) : nullptr;
@@ -1222,10 +1374,7 @@ void gated_backward(const GatedArgs& a, const void* dh, int64_t dh_stride, const
                                       WeightEpi<T>{pick(in.scales, &Scales::dw), dwg, dwu, part,
                                                    a.hidden, pl.hpad, a.width},
                                       st);
-      if (part)
-        k_sum_parts<T><<<(unsigned)std::min<int64_t>(
-                             ceil_div(2 * a.hidden * a.width, (int64_t)256), 8192),
-                         256, 0, st>>>(part, pl.splits, a.hidden * a.width, dwg, dwu);
+      if (part) sum_parts<T>(part, pl.splits, a.hidden * a.width, 2, dwg, dwu, st);
     }
     MGP_HIP_CHECK(hipGetLastError());
   });

@@ -39,58 +39,71 @@ class GatedGradients(NamedTuple):
     db_up: object
 
 
-_types: dict = {}
+_types: dict = {}  # torch's element types and this library's codes
 
 
-def _elem(a, name):
-    """Element type code of a tensor; torch is loaded if there is one."""
+def _torch():
+    """torch, which a program that holds device tensors has loaded."""
+    torch = sys.modules.get("torch")
+    if torch is None:
+        raise TypeError("the arrays must be device tensors of torch")
     if not _types:
-        torch = sys.modules.get("torch")
-        if torch is not None:
-            _types.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
-    code = _types.get(getattr(a, "dtype", None))
-    if code is None:
-        raise TypeError(f"{name} must be a float32, bfloat16 or float16 device tensor, got "
-                        f"{getattr(a, 'dtype', type(a).__name__)}")
-    return code
+        _types.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
+    return torch
+
+
+def _stream(torch, index):
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # without making an object of it
+    return raw(index) if raw else torch.cuda.current_stream(index).cuda_stream
 
 
 def _first(a, name):
-    """(element type, device index, stream) of a call from its first array."""
-    code = _elem(a, name)
-    if not a.is_cuda:
+    """(element type, its code, device index, stream) of a call from its first array."""
+    torch = _torch()
+    dtype = getattr(a, "dtype", None)
+    code = _types.get(dtype)
+    if code is None:
+        raise TypeError(f"{name} must be a float32, bfloat16 or float16 device tensor, got "
+                        f"{dtype or type(a).__name__}")
+    index = a.get_device()
+    if index < 0:
         raise ValueError(f"{name} must be a device tensor, got one on {a.device}")
-    cuda = sys.modules["torch"].cuda
-    index = a.device.index
-    if index != cuda.current_device():
+    if index != torch.cuda.current_device():
         raise ValueError(f"{name} is on device {index}, the current device is "
-                         f"{cuda.current_device()}")
-    return code, index, cuda.current_stream(index).cuda_stream
+                         f"{torch.cuda.current_device()}")
+    return dtype, code, index, _stream(torch, index)
 
 
-def _rows(a, name, code, index, shape=None):
-    """(address, rows, width, row stride) of an array as a matrix of rows."""
-    if _elem(a, name) != code:
-        raise TypeError(f"{name} must have the element type of the first array, got {a.dtype}")
-    if not a.is_cuda or a.device.index != index:
+def _check(a, name, dtype, index):
+    if getattr(a, "dtype", None) is not dtype:
+        raise TypeError(f"{name} must have the element type of the first array ({dtype}), got "
+                        f"{getattr(a, 'dtype', type(a).__name__)}")
+    if a.get_device() != index:
         raise ValueError(f"{name} must be on device {index}, got {a.device}")
-    if shape is not None and a.shape != shape:
-        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(a.shape)}")
-    dims = a.dim()
-    if dims == 0:
+
+
+def _rows(a, name, dtype, index, shape=None):
+    """(address, rows, width, row stride) of an array as a matrix of rows."""
+    _check(a, name, dtype, index)
+    got, strides = a.shape, a.stride()
+    if shape is not None and got != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(got)}")
+    dims = len(got)
+    if dims == 2:
+        rows, width = got
+        stride = strides[0]
+    elif dims == 1:
+        rows, width, stride = 1, got[0], 0
+    elif dims == 0:
         raise ValueError(f"{name} must have at least one dimension")
-    width = a.shape[-1]
+    else:
+        width = got[-1]
+        rows, stride = _collapse(got, strides, name)
     if width == 0:
         raise ValueError(f"{name} must have at least one column")
-    if width > 1 and a.stride(-1) != 1:
+    if strides[-1] != 1 and width > 1:
         raise ValueError(f"{name} must have unit stride along its last dimension, got strides "
-                         f"{a.stride()}")
-    if dims == 1:
-        return a.data_ptr(), 1, width, width
-    if dims == 2:
-        rows, stride = a.shape[0], a.stride(0)
-    else:
-        rows, stride = _collapse(a, name)
+                         f"{strides}")
     if rows <= 1:
         stride = width
     elif stride < width:
@@ -98,47 +111,44 @@ def _rows(a, name, code, index, shape=None):
     return a.data_ptr(), rows, width, stride
 
 
-def _collapse(a, name):
+def _collapse(shape, strides, name):
     """Rows and row stride of more than two dimensions."""
-    rows, stride = 1, a.shape[-1]
-    for size, step in zip(reversed(a.shape[:-1]), reversed(a.stride()[:-1])):
+    rows, stride = 1, shape[-1]
+    for size, step in zip(reversed(shape[:-1]), reversed(strides[:-1])):
         if size == 1:
             continue
         if rows == 1:
             stride = step
         elif step != rows * stride:
             raise ValueError(f"the leading dimensions of {name} do not collapse to rows of one "
-                             f"stride (shape {tuple(a.shape)}, strides {a.stride()})")
+                             f"stride (shape {tuple(shape)}, strides {strides})")
         rows *= size
     return rows, stride
 
 
-def _vector(a, name, width, code, index, also=None):
+def _vector(a, name, width, dtype, index):
     """Address of a contiguous [width] vector, or None."""
     if a is None:
         return None
-    got = _elem(a, name)
-    if got != code and got != also:
-        raise TypeError(f"{name} has element type {a.dtype}, which does not fit the other arrays")
-    if not a.is_cuda or a.device.index != index:
-        raise ValueError(f"{name} must be on device {index}, got {a.device}")
-    if a.dim() != 1 or a.shape[0] != width:
+    _check(a, name, dtype, index)
+    if a.shape != (width,):
         raise ValueError(f"{name} must have shape ({width},), got {tuple(a.shape)}")
     if width > 1 and a.stride(0) != 1:
         raise ValueError(f"{name} must be contiguous")
     return a.data_ptr()
 
 
-def _result(a, name, like, code, index):
-    """A given result array (checked against `like`), or a new contiguous one."""
+def _result(a, name, like, shape, dtype, index):
+    """(array, address, row stride) of a given result, checked, or a new one."""
     if a is None:
-        return like.new_empty(like.shape)
-    _rows(a, name, code, index, like.shape)
-    return a
+        a = like.new_empty(shape)
+        return a, a.data_ptr(), shape[-1]
+    address, _, _, stride = _rows(a, name, dtype, index, shape)
+    return a, address, stride
 
 
 def _workspace(like, nbytes):
-    return like.new_empty((nbytes,), dtype=sys.modules["torch"].uint8) if nbytes else None
+    return like.new_empty((nbytes,), dtype=_torch().uint8) if nbytes else None
 
 
 def _address(a):
@@ -148,15 +158,19 @@ def _address(a):
 # ---------------------------------------------------------------- layer norm
 
 def _norm_args(x, weight, bias, eps):
-    code, index, stream = _first(x, "x")
-    px, rows, width, stride = _rows(x, "x", code, index)
-    pw = _vector(weight, "weight", width, code, index, also=0)
-    pb = _vector(bias, "bias", width, code, index, also=0)
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise TypeError("weight and bias must have one element type")
+    dtype, code, index, stream = _first(x, "x")
+    px, rows, width, stride = _rows(x, "x", dtype, index)
     given = weight if weight is not None else bias
-    ptype = code if given is None else _types[given.dtype]
-    return _lib.LayerNorm(code, ptype, eps, rows, width, px, stride, pw, pb), index, stream
+    ptype, pcode = dtype, code
+    if given is not None and given.dtype is not dtype:
+        ptype, pcode = given.dtype, _types.get(given.dtype)
+        if pcode != 0:
+            raise TypeError(f"weight and bias must have x's element type or be float32, got "
+                            f"{ptype}, which does not fit {dtype}")
+    pw = _vector(weight, "weight", width, ptype, index)
+    pb = _vector(bias, "bias", width, ptype, index)
+    return (_lib.LayerNorm(code, pcode, eps, rows, width, px, stride, pw, pb), dtype, index,
+            stream)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, *, save=False, out=None):
@@ -165,10 +179,9 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, save=False, out=None):
     weight and bias ([width], of x's type or float32) may be None.  With
     ``save=True`` returns ``(y, saved)``, ``saved`` being what the backward
     pass takes (mean and reciprocal deviation of every row, float32)."""
-    a, index, stream = _norm_args(x, weight, bias, eps)
-    y = _result(out, "out", x, a.type, index)
-    py, _, _, stride = _rows(y, "out", a.type, index)
-    stats = x.new_empty((a.rows, 2), dtype=sys.modules["torch"].float32) if save else None
+    a, dtype, index, stream = _norm_args(x, weight, bias, eps)
+    y, py, stride = _result(out, "out", x, x.shape, dtype, index)
+    stats = x.new_empty((a.rows, 2), dtype=_torch().float32) if save else None
     _lib.call("mgp_layer_norm_device", C.byref(a), py, stride, _address(stats), stream)
     return (y, stats) if save else y
 
@@ -178,10 +191,10 @@ def layer_norm_backward(dy, x, weight, saved, *, bias=True):
 
     dweight and dbias have weight's type (x's where weight is None; dweight is
     then None).  ``bias=False``: the layer has none, dbias is None."""
-    a, index, stream = _norm_args(x, weight, None, 0.0)
-    pdy, _, _, dy_stride = _rows(dy, "dy", a.type, index, x.shape)
-    if saved is None or tuple(saved.shape) != (a.rows, 2) or _elem(saved, "saved") != 0 \
-            or not saved.is_contiguous() or saved.device != x.device:
+    a, dtype, index, stream = _norm_args(x, weight, None, 0.0)
+    pdy, _, _, dy_stride = _rows(dy, "dy", dtype, index, x.shape)
+    if saved is None or saved.shape != (a.rows, 2) or _types.get(saved.dtype) != 0 \
+            or not saved.is_contiguous() or saved.get_device() != index:
         raise ValueError("saved must be what layer_norm(..., save=True) returned for this x")
     dx = x.new_empty(x.shape)
     params = x if weight is None else weight
@@ -200,15 +213,14 @@ def layer_norm_backward(dy, x, weight, saved, *, bias=True):
 # ---------------------------------------------------------------- dropout
 
 def _dropout(x, name, rate, seed, offset, residual, out):
-    code, index, stream = _first(x, name)
-    px, rows, width, stride = _rows(x, name, code, index)
+    dtype, code, index, stream = _first(x, name)
+    px, rows, width, stride = _rows(x, name, dtype, index)
     pr, r_stride = None, 0
     if residual is not None:
-        pr, _, _, r_stride = _rows(residual, "residual", code, index, x.shape)
+        pr, _, _, r_stride = _rows(residual, "residual", dtype, index, x.shape)
     if not 0 <= seed < _MAX_DRAWS or not 0 <= offset < _MAX_DRAWS:
         raise ValueError("seed and offset must be in [0, 2^64)")
-    y = _result(out, "out", x, code, index)
-    py, _, _, y_stride = _rows(y, "out", code, index)
+    y, py, y_stride = _result(out, "out", x, x.shape, dtype, index)
     _lib.call("mgp_dropout_device", code, px, stride, rows, width, rate, seed, offset, pr,
               r_stride, py, y_stride, stream)
     return y
@@ -233,23 +245,19 @@ def dropout_backward(dy, rate, seed, *, offset=0, out=None):
 # ---------------------------------------------------------------- gated layer
 
 def _gated_args(x, w_gate, w_up, b_gate, b_up, activation):
-    code, index, stream = _first(x, "x")
-    try:
-        act = ACTIVATIONS[activation]
-    except (KeyError, TypeError):
-        raise ValueError(f"unknown activation {activation!r}; one of {sorted(ACTIVATIONS)}") \
-            from None
-    px, rows, width, stride = _rows(x, "x", code, index)
-    if w_gate.dim() != 2 or w_gate.shape[1] != width:
+    dtype, code, index, stream = _first(x, "x")
+    act = ACTIVATIONS.get(activation) if isinstance(activation, str) else None
+    if act is None:
+        raise ValueError(f"unknown activation {activation!r}; one of {sorted(ACTIVATIONS)}")
+    px, rows, width, stride = _rows(x, "x", dtype, index)
+    pg, hidden, w_width, g_stride = _rows(w_gate, "w_gate", dtype, index)
+    if w_gate.dim() != 2 or w_width != width or hidden == 0:
         raise ValueError(f"w_gate must have shape (hidden, {width}), got {tuple(w_gate.shape)}")
-    pg, hidden, _, g_stride = _rows(w_gate, "w_gate", code, index)
-    if hidden == 0:
-        raise ValueError("w_gate must have at least one row")
-    pu, _, _, u_stride = _rows(w_up, "w_up", code, index, w_gate.shape)
-    bg = _vector(b_gate, "b_gate", hidden, code, index)
-    bu = _vector(b_up, "b_up", hidden, code, index)
-    return _lib.GatedLayer(code, act, rows, width, hidden, px, stride, pg, g_stride, pu, u_stride,
-                           bg, bu), index, stream
+    pu, _, _, u_stride = _rows(w_up, "w_up", dtype, index, w_gate.shape)
+    bg = _vector(b_gate, "b_gate", hidden, dtype, index)
+    bu = _vector(b_up, "b_up", hidden, dtype, index)
+    return (_lib.GatedLayer(code, act, rows, width, hidden, px, stride, pg, g_stride, pu,
+                            u_stride, bg, bu), (*x.shape[:-1], hidden), dtype, index, stream)
 
 
 def _gated_workspace(a, x, backward):
@@ -264,13 +272,8 @@ def gated_layer(x, w_gate, w_up, b_gate=None, b_up=None, *, activation="silu", o
     x [..., width], weights [hidden, width], biases [hidden] or None, all of one
     element type; result [..., hidden].  activation: "silu", "gelu" (with the
     normal distribution's exact integral), "sigmoid" or "relu"."""
-    a, index, stream = _gated_args(x, w_gate, w_up, b_gate, b_up, activation)
-    shape = (*x.shape[:-1], a.hidden)
-    if out is None:
-        out = x.new_empty(shape)
-    elif tuple(out.shape) != shape:
-        raise ValueError(f"out must have shape {shape}, got {tuple(out.shape)}")
-    ph, _, _, h_stride = _rows(out, "out", a.type, index)
+    a, shape, dtype, index, stream = _gated_args(x, w_gate, w_up, b_gate, b_up, activation)
+    out, ph, h_stride = _result(out, "out", x, shape, dtype, index)
     ws, nbytes = _gated_workspace(a, x, 0)
     _lib.call("mgp_gated_layer_device", C.byref(a), ph, h_stride, _address(ws), nbytes, stream)
     return out
@@ -283,10 +286,8 @@ def gated_layer_backward(dh, x, w_gate, w_up, b_gate=None, b_up=None, *, activat
     The projections are formed again from x: nothing is kept between the
     passes.  ``need_dx=False`` (the first layer, whose x is data) and
     ``need_dw=False`` leave those products out."""
-    a, index, stream = _gated_args(x, w_gate, w_up, b_gate, b_up, activation)
-    if tuple(dh.shape) != (*x.shape[:-1], a.hidden):
-        raise ValueError(f"dh must have shape {(*x.shape[:-1], a.hidden)}, got {tuple(dh.shape)}")
-    pdh, _, _, dh_stride = _rows(dh, "dh", a.type, index)
+    a, shape, dtype, index, stream = _gated_args(x, w_gate, w_up, b_gate, b_up, activation)
+    pdh, _, _, dh_stride = _rows(dh, "dh", dtype, index, shape)
     g = GatedGradients(
         x.new_empty(x.shape) if need_dx else None,
         x.new_empty((a.hidden, a.width)) if need_dw else None,
