@@ -10,6 +10,7 @@
 #include "layers.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace mgp {
 
@@ -44,65 +45,61 @@ __device__ __forceinline__ float kept(float x, uint32_t draw, uint32_t cut, floa
   return draw >= cut ? x * scale : 0.0f;
 }
 
-// Contiguous, 16-byte aligned arrays with offset % 8 == 0: a thread takes the
-// eight elements of a block.
-template <class T, bool RES>
-__global__ __launch_bounds__(256) void k_dropout(const T* __restrict__ x,
-                                                 const T* __restrict__ residual, int64_t total,
-                                                 uint32_t cut, float scale, uint64_t seed,
-                                                 uint64_t block0, T* __restrict__ y) {
-  constexpr int N = Vec16<T>::N, NV = 8 / N;
-  const int64_t blocks = (total + 7) / 8;
-  for (int64_t b = (int64_t)blockIdx.x * 256 + threadIdx.x; b < blocks;
-       b += (int64_t)gridDim.x * 256) {
-    const Draws dr = philox(block0 + (uint64_t)b, seed);
-    const int64_t e0 = b * 8;
-    if (e0 + 8 <= total) {
+// Eight elements at any alignment (the memory path takes it).
+template <class T>
+__device__ __forceinline__ void load8(const T* p, float* v) {
+  T a[8];
+  __builtin_memcpy(a, p, sizeof(a));
 #pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        Vec16<T> a = *reinterpret_cast<const Vec16<T>*>(x + e0 + v * N), r;
-        if constexpr (RES) r = *reinterpret_cast<const Vec16<T>*>(residual + e0 + v * N);
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-          float f = kept((float)a.v[k], dr.half(v * N + k), cut, scale);
-          if constexpr (RES) f += (float)r.v[k];
-          a.v[k] = (T)f;
-        }
-        *reinterpret_cast<Vec16<T>*>(y + e0 + v * N) = a;
-      }
-    } else {
-      for (int k = 0; e0 + k < total; ++k) {
-        float f = kept((float)x[e0 + k], dr.half(k), cut, scale);
-        if constexpr (RES) f += (float)residual[e0 + k];
-        y[e0 + k] = (T)f;
-      }
-    }
-  }
+  for (int k = 0; k < 8; ++k) v[k] = (float)a[k];
 }
 
-// Any strides, alignment and offset: a thread takes the elements of one block,
-// an element at a time.
-template <class T>
-__global__ __launch_bounds__(256) void k_dropout_any(const T* __restrict__ x, int64_t ldx,
-                                                     const T* __restrict__ residual, int64_t ldr,
-                                                     int64_t total, int64_t width, uint32_t cut,
-                                                     float scale, uint64_t seed, uint64_t offset,
-                                                     T* __restrict__ y, int64_t ldy) {
+// A thread takes the up to eight elements of one block of draws, loaded before
+// the rounds so that those run while the loads do.  FLAT: contiguous arrays;
+// otherwise rows of their own strides, eight elements of one row at a time
+// where the block lies in one.
+template <class T, bool FLAT, bool RES>
+__global__ __launch_bounds__(256) void k_dropout(const T* __restrict__ x, int64_t ldx,
+                                                 const T* __restrict__ residual, int64_t ldr,
+                                                 int64_t total, int64_t width, uint32_t cut,
+                                                 float scale, uint64_t seed, uint64_t offset,
+                                                 T* __restrict__ y, int64_t ldy) {
   const int head = (int)(offset & 7);  // draws of the first block before element 0
   const int64_t blocks = (total + head + 7) / 8;
   for (int64_t b = (int64_t)blockIdx.x * 256 + threadIdx.x; b < blocks;
        b += (int64_t)gridDim.x * 256) {
-    const Draws dr = philox((offset >> 3) + (uint64_t)b, seed);
     const int64_t first = b * 8 - head;
-    int64_t row = (first > 0 ? first : 0) / width, col = (first > 0 ? first : 0) - row * width;
+    int64_t row = 0, col = first > 0 ? first : 0;
+    if constexpr (!FLAT) {
+      row = col / width;
+      col -= row * width;
+    }
+    const bool whole = first >= 0 && first + 8 <= total && (FLAT || col + 8 <= width);
+    const T *px = x + row * ldx + col, *pr = RES ? residual + row * ldr + col : nullptr;
+    float v[8], r[8];
+    if (whole) {
+      load8(px, v);
+      if constexpr (RES) load8(pr, r);
+    }
+    const Draws dr = philox((offset >> 3) + (uint64_t)b, seed);
+    if (whole) {
+      T a[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        float f = kept(v[k], dr.half(k), cut, scale);
+        if constexpr (RES) f += r[k];
+        a[k] = (T)f;
+      }
+      __builtin_memcpy(y + row * ldy + col, a, sizeof(a));
+      continue;
+    }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const int64_t e = first + k;
-      if (e < 0 || e >= total) continue;
+      if (first + k < 0 || first + k >= total) continue;
       float f = kept((float)x[row * ldx + col], dr.half(k), cut, scale);
-      if (residual) f += (float)residual[row * ldr + col];
+      if constexpr (RES) f += (float)residual[row * ldr + col];
       y[row * ldy + col] = (T)f;
-      if (++col == width) {
+      if (++col == width && !FLAT) {
         col = 0;
         ++row;
       }
@@ -118,24 +115,19 @@ void dropout(const DropoutArgs& a, void* y, int64_t y_stride, hipStream_t st) {
   const float scale = 65536.0f / (float)(65536 - a.cut);
   dispatch_elem(a.type, [&](auto tag) {
     using T = decltype(tag);
-    auto flat = [&](const void* p, int64_t stride) {
-      return p == nullptr || (aligned16(p) && (stride == a.width || a.rows == 1));
-    };
+    auto flat = [&](int64_t stride) { return stride == a.width || a.rows == 1; };
     const T *x = static_cast<const T*>(a.x), *r = static_cast<const T*>(a.residual);
     const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(total / 8 + 2, (int64_t)256), 8192);
-    if (flat(a.x, a.x_stride) && flat(a.residual, a.residual_stride) && flat(y, y_stride) &&
-        a.offset % 8 == 0) {
-      if (r)
-        k_dropout<T, true><<<grid, 256, 0, st>>>(x, r, total, a.cut, scale, a.seed, a.offset / 8,
-                                                 static_cast<T*>(y));
-      else
-        k_dropout<T, false><<<grid, 256, 0, st>>>(x, r, total, a.cut, scale, a.seed, a.offset / 8,
-                                                  static_cast<T*>(y));
-    } else {
-      k_dropout_any<T><<<grid, 256, 0, st>>>(x, a.x_stride, r, a.residual_stride, total, a.width,
-                                             a.cut, scale, a.seed, a.offset, static_cast<T*>(y),
-                                             y_stride);
-    }
+    auto go = [&](auto fl, auto res) {
+      k_dropout<T, fl.value, res.value><<<grid, 256, 0, st>>>(
+          x, a.x_stride, r, a.residual_stride, total, a.width, a.cut, scale, a.seed, a.offset,
+          static_cast<T*>(y), y_stride);
+    };
+    const bool all = flat(a.x_stride) && flat(y_stride) && (!r || flat(a.residual_stride));
+    if (all && r) go(std::true_type{}, std::true_type{});
+    if (all && !r) go(std::true_type{}, std::false_type{});
+    if (!all && r) go(std::false_type{}, std::true_type{});
+    if (!all && !r) go(std::false_type{}, std::false_type{});
     MGP_HIP_CHECK(hipGetLastError());
   });
 }

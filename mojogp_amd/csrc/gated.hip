@@ -19,6 +19,7 @@
 #include "layers.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace mgp {
 

@@ -19,26 +19,40 @@ namespace {
 
 constexpr int kNormThreads = 256;
 
-template <class T, int VEC>
-__device__ __forceinline__ void load_vec(const T* p, float* v) {
-  if constexpr (VEC == 1) {
-    v[0] = (float)p[0];
-  } else {
-    const Vec16<T> a = *reinterpret_cast<const Vec16<T>*>(p);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = (float)a.v[i];
-  }
+template <class T>
+struct Raw {  // one vector as it lies in memory
+  T v[Vec16<T>::N];
+};
+
+// Vectors go at any alignment (rows of odd widths, of tables).
+template <class T>
+__device__ __forceinline__ Raw<T> load_raw(const T* p) {
+  Raw<T> a;
+  __builtin_memcpy(&a, p, sizeof(a));
+  return a;
 }
 
 template <class T, int VEC>
 __device__ __forceinline__ void store_vec(T* p, const float* v) {
-  if constexpr (VEC == 1) {
-    p[0] = (T)v[0];
-  } else {
-    Vec16<T> a;
+  T a[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) a.v[i] = (T)v[i];
-    *reinterpret_cast<Vec16<T>*>(p) = a;
+  for (int i = 0; i < VEC; ++i) a[i] = (T)v[i];
+  __builtin_memcpy(p, a, sizeof(a));
+}
+
+// VEC parameters from column c on, or the default
+template <class T, int VEC>
+__device__ __forceinline__ void load_params(const void* p, int64_t c, bool f32, float none,
+                                            float* v) {
+  if (p == nullptr) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[k] = none;
+  } else if (f32) {
+    __builtin_memcpy(v, static_cast<const float*>(p) + c, VEC * sizeof(float));
+  } else {
+    const Raw<T> a = load_raw(static_cast<const T*>(p) + c);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[k] = (float)a.v[k];
   }
 }
 
@@ -70,56 +84,83 @@ __device__ __forceinline__ void group_sum2(float& a, float& b, float (*red)[8], 
   }
 }
 
-// L threads a row, NV vectors of VEC elements a thread, NV VEC <= 32.
-template <class T, int L, int NV, int VEC>
+// Where a thread's vector i lies: column `at`, of which the first `skip` elements
+// are another thread's.  RAGGED (the width is no multiple of the vector): the
+// last vector of a row is moved back to end with it; what it then shares with
+// its neighbour counts there and is stored by both with the same value, so that
+// every access is a whole vector.
+template <int L, int VEC, bool RAGGED>
+struct Place {
+  int at, skip;
+  bool live;
+  __device__ __forceinline__ Place(int i, int t, int width) {
+    const int c = (i * L + t) * VEC;
+    live = c < width;
+    at = RAGGED ? min(c, width - VEC) : c;
+    skip = RAGGED ? c - at : 0;
+  }
+  __device__ __forceinline__ bool mine(int k) const { return live && (!RAGGED || k >= skip); }
+};
+
+// L threads a row, NV vectors of VEC elements a thread, NV VEC <= 32.  The next
+// row's loads are out while this one's sums are formed: a row takes two rounds
+// of lane exchanges, and without that the kernel waits for memory in between.
+template <class T, int L, int NV, bool RAGGED>
 __global__ __launch_bounds__(kNormThreads) void k_norm_fwd(
     const T* __restrict__ x, int64_t ldx, int64_t rows, int width,
     const void* __restrict__ weight, const void* __restrict__ bias, int f32_params, float eps,
     T* __restrict__ y, int64_t ldy, float* __restrict__ stats) {
   constexpr int G = kNormThreads / L;  // rows a block works on at a time
+  constexpr int VEC = Vec16<T>::N;
+  using Pl = Place<L, VEC, RAGGED>;
   __shared__ float red[2][8];
   int slot = 0;
   const int t = threadIdx.x % L, g = threadIdx.x / L;
+  const int64_t step = (int64_t)gridDim.x * G;
+  Raw<T> next[NV];
+  auto fetch = [&](int64_t r) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const Pl p(i, t, width);
+      if (r < rows && p.live) next[i] = load_raw(x + r * ldx + p.at);
+    }
+  };
+  int64_t r = (int64_t)blockIdx.x * G + g;
+  fetch(r);
   float w[NV * VEC], b[NV * VEC];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (i * L + t) * VEC;
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      w[i * VEC + k] = weight && c < width ? load_param<T>(weight, c + k, f32_params) : 1.0f;
-      b[i * VEC + k] = bias && c < width ? load_param<T>(bias, c + k, f32_params) : 0.0f;
-    }
+    const Pl p(i, t, width);
+    if (!p.live) continue;
+    load_params<T, VEC>(weight, p.at, f32_params, 1.0f, w + i * VEC);
+    load_params<T, VEC>(bias, p.at, f32_params, 0.0f, b + i * VEC);
   }
   const float inv = 1.0f / (float)width;
-  for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < rows; r0 += (int64_t)gridDim.x * G) {
-    const int64_t r = r0 + g;
+  for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < rows; r0 += step, r += step) {
     const bool live = r < rows;
     float v[NV * VEC], s = 0.0f, none = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * L + t) * VEC;
-      if (live && c < width) {
-        load_vec<T, VEC>(x + r * ldx + c, v + i * VEC);
-      } else {
+      const Pl p(i, t, width);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) v[i * VEC + k] = 0.0f;
+      for (int k = 0; k < VEC; ++k) {
+        v[i * VEC + k] = live && p.live ? (float)next[i].v[k] : 0.0f;
+        s += p.mine(k) ? v[i * VEC + k] : 0.0f;
       }
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) s += v[i * VEC + k];
     }
+    fetch(r + step);
     group_sum2<L>(s, none, red, slot);
     const float mean = s * inv;
     float q = 0.0f, off = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const bool in = (i * L + t) * VEC < width;
+      const Pl p(i, t, width);
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
         v[i * VEC + k] -= mean;
-        if (in) {
-          q = fmaf(v[i * VEC + k], v[i * VEC + k], q);
-          off += v[i * VEC + k];
-        }
+        const float d = p.mine(k) ? v[i * VEC + k] : 0.0f;
+        q = fmaf(d, d, q);
+        off += d;
       }
     }
     // off: what the mean's rounding left, taken out of both moments (a
@@ -134,66 +175,78 @@ __global__ __launch_bounds__(kNormThreads) void k_norm_fwd(
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * L + t) * VEC;
+      const Pl p(i, t, width);
 #pragma unroll
       for (int k = 0; k < VEC; ++k)
         v[i * VEC + k] = fmaf((v[i * VEC + k] - off) * rstd, w[i * VEC + k], b[i * VEC + k]);
-      if (c < width) store_vec<T, VEC>(y + r * ldy + c, v + i * VEC);
+      if (p.live) store_vec<T, VEC>(y + r * ldy + p.at, v + i * VEC);
     }
   }
 }
 
 // part[block][2][width]: the block's sums of dy xhat and dy (null: not wanted).
-template <class T, int L, int NV, int VEC>
+template <class T, int L, int NV, bool RAGGED>
 __global__ __launch_bounds__(kNormThreads) void k_norm_bwd(
     const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx, int64_t rows,
     int width, const void* __restrict__ weight, int f32_params, const float* __restrict__ stats,
     T* __restrict__ dx, int64_t lddx, float* __restrict__ part) {
-  constexpr int G = kNormThreads / L;
+  constexpr int G = kNormThreads / L, VEC = Vec16<T>::N;
+  using Pl = Place<L, VEC, RAGGED>;
   __shared__ float red[2][8];
   __shared__ float comb[G > 1 ? 2 * kNormThreads * NV * VEC : 1];
   int slot = 0;
   const int t = threadIdx.x % L, g = threadIdx.x / L;
+  const int64_t step = (int64_t)gridDim.x * G;
+  Raw<T> next_x[NV], next_d[NV];
+  float next_mean = 0.0f, next_rstd = 0.0f;
+  auto fetch = [&](int64_t r) __attribute__((always_inline)) {
+    if (r >= rows) return;
+    next_mean = stats[2 * r];
+    next_rstd = stats[2 * r + 1];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const Pl p(i, t, width);
+      if (!p.live) continue;
+      next_x[i] = load_raw(x + r * ldx + p.at);
+      next_d[i] = load_raw(dy + r * lddy + p.at);
+    }
+  };
+  int64_t r = (int64_t)blockIdx.x * G + g;
+  fetch(r);
   float w[NV * VEC], dw[NV * VEC], db[NV * VEC];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (i * L + t) * VEC;
+    const Pl p(i, t, width);
+    if (p.live) load_params<T, VEC>(weight, p.at, f32_params, 1.0f, w + i * VEC);
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
-      w[i * VEC + k] = weight && c < width ? load_param<T>(weight, c + k, f32_params) : 1.0f;
       dw[i * VEC + k] = 0.0f;
       db[i * VEC + k] = 0.0f;
     }
   }
   const float inv = 1.0f / (float)width;
-  for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < rows; r0 += (int64_t)gridDim.x * G) {
-    const int64_t r = r0 + g;
+  for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < rows; r0 += step, r += step) {
     const bool live = r < rows;
-    const float mean = live ? stats[2 * r] : 0.0f, rstd = live ? stats[2 * r + 1] : 0.0f;
+    const float mean = next_mean, rstd = next_rstd;
     float xh[NV * VEC], d[NV * VEC], s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * L + t) * VEC;
-      if (live && c < width) {
-        load_vec<T, VEC>(x + r * ldx + c, xh + i * VEC);
-        load_vec<T, VEC>(dy + r * lddy + c, d + i * VEC);
-      } else {
+      const Pl p(i, t, width);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          xh[i * VEC + k] = mean;
-          d[i * VEC + k] = 0.0f;
-        }
+      for (int k = 0; k < VEC; ++k) {
+        const int e = i * VEC + k;
+        const bool in = live && p.live;
+        xh[e] = in ? ((float)next_x[i].v[k] - mean) * rstd : 0.0f;
+        d[e] = in ? (float)next_d[i].v[k] : 0.0f;
+        dw[e] = fmaf(d[e], xh[e], dw[e]);
+        db[e] += d[e];
+        d[e] = in ? d[e] * w[e] : 0.0f;
+        const float m = p.mine(k) ? d[e] : 0.0f;
+        s1 += m;
+        s2 = fmaf(m, xh[e], s2);
       }
     }
-#pragma unroll
-    for (int e = 0; e < NV * VEC; ++e) {
-      xh[e] = (xh[e] - mean) * rstd;
-      dw[e] = fmaf(d[e], xh[e], dw[e]);
-      db[e] += d[e];
-      d[e] *= w[e];
-      s1 += d[e];
-      s2 = fmaf(d[e], xh[e], s2);
-    }
+    fetch(r + step);
     if (dx == nullptr) continue;
     group_sum2<L>(s1, s2, red, slot);
     if (!live) continue;
@@ -201,13 +254,13 @@ __global__ __launch_bounds__(kNormThreads) void k_norm_bwd(
     s2 *= inv;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * L + t) * VEC;
+      const Pl p(i, t, width);
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
         const int e = i * VEC + k;
         d[e] = rstd * (d[e] - s1 - xh[e] * s2);
       }
-      if (c < width) store_vec<T, VEC>(dx + r * lddx + c, d + i * VEC);
+      if (p.live) store_vec<T, VEC>(dx + r * lddx + p.at, d + i * VEC);
     }
   }
   if (part == nullptr) return;
@@ -222,24 +275,25 @@ __global__ __launch_bounds__(kNormThreads) void k_norm_bwd(
     __syncthreads();
     for (int q = threadIdx.x; q < 2 * NV * VEC * L; q += kNormThreads) {
       const int tt = q % L, e2 = q / L, e = e2 >> 1;
-      const int c = (e / VEC * L + tt) * VEC + e % VEC;
+      const Pl p(e / VEC, tt, width);
       float s = 0.0f;
       for (int k = 0; k < G; ++k) s += comb[e2 * kNormThreads + k * L + tt];
-      if (c < width) pw[(e2 & 1) * width + c] = s;
+      if (p.mine(e % VEC)) pw[(e2 & 1) * width + p.at + e % VEC] = s;
     }
   } else {
 #pragma unroll
     for (int e = 0; e < NV * VEC; ++e) {
-      const int c = (e / VEC * L + t) * VEC + e % VEC;
-      if (c < width) {
-        pw[c] = dw[e];
-        pw[width + c] = db[e];
+      const Pl p(e / VEC, t, width);
+      if (p.mine(e % VEC)) {
+        pw[p.at + e % VEC] = dw[e];
+        pw[width + p.at + e % VEC] = db[e];
       }
     }
   }
 }
 
-// Rows too wide for registers: three passes over the row, which the caches hold.
+// Rows too wide for registers, or narrower than a vector: three passes over the
+// row, which the caches hold.
 template <class T>
 __global__ __launch_bounds__(kNormThreads) void k_norm_fwd_wide(
     const T* __restrict__ x, int64_t ldx, int64_t rows, int64_t width,
@@ -294,6 +348,8 @@ __global__ __launch_bounds__(kNormThreads) void k_norm_bwd_wide(
     s1 /= (float)width;
     s2 /= (float)width;
     for (int64_t c = threadIdx.x; c < width; c += kNormThreads) {
+      // g rounded as in its sum: the gradient of a single column is 0
+#pragma clang fp contract(off)
       const float g = (float)dr[c] * (weight ? load_param<T>(weight, c, f32_params) : 1.0f);
       dx[r * lddx + c] = (T)(rstd * (g - s1 - ((float)xr[c] - mean) * rstd * s2));
     }
@@ -329,7 +385,7 @@ __global__ __launch_bounds__(1024) void k_norm_sum(const float* __restrict__ par
   const int64_t c = (int64_t)blockIdx.x * 64 + lane;  // column of [2][width]
   float s = 0.0f;
   if (c < 2 * width) {
-#pragma unroll 4
+#pragma unroll 16
     for (int b = wave; b < nblk; b += 16) s += part[(int64_t)b * 2 * width + c];
   }
   red[wave][lane] = s;
@@ -347,77 +403,63 @@ __global__ __launch_bounds__(1024) void k_norm_sum(const float* __restrict__ par
 }
 
 struct NormShape {
-  int L;    // threads a row: 8 .. 64, or 256; 0: the wide kernels
-  int NV;   // vectors a thread
-  int VEC;  // elements a vector
+  int L;   // threads a row: 8 .. 64, or 256; 0: the wide kernels
+  int NV;  // vectors a thread
 };
 
-// The vector kernels need every row of every array 16-byte aligned; others
-// take one element a load.  A row takes the fewest lanes that hold it with one
-// vector each, up to a wave; beyond 16 elements a lane of a wave, or with too
-// few rows to fill the device with waves, the block shares it.
+// A row takes the fewest lanes that hold it with one vector each, up to a wave;
+// beyond 16 elements a lane of a wave, or with too few rows to fill the device
+// with waves, the block shares it.
 template <class T>
-NormShape norm_shape(bool vec, int64_t rows, int64_t width) {
-  constexpr int VF = Vec16<T>::N;
-  const int VEC = vec ? VF : 1;
+NormShape norm_shape(int64_t rows, int64_t width) {
+  constexpr int VEC = Vec16<T>::N;
   const int64_t vecs = ceil_div(width, VEC);
-  const int max_nv = 32 / VEC;
   auto pow2 = [](int64_t v) {
     int p = 1;
     while (p < v) p *= 2;
     return p;
   };
-  if (vecs <= 64) return {std::max(8, pow2(vecs)), 1, VEC};
+  if (width < VEC) return {0, 0};
+  if (vecs <= 64) return {std::max(8, pow2(vecs)), 1};
   const int nv_wave = pow2(ceil_div(vecs, 64));
-  if (nv_wave * VEC <= 16 && (rows > 1024 || nv_wave == 1)) return {64, nv_wave, VEC};
+  if (nv_wave * VEC <= 16 && rows > 1024) return {64, nv_wave};
   const int nv = pow2(ceil_div(vecs, 256));
-  if (nv > max_nv) return {0, 0, 1};
-  return {256, nv, VEC};
+  if (nv * VEC > 32) return {0, 0};
+  return {256, nv};
 }
 
 template <int V>
 using Int = std::integral_constant<int, V>;
 
 template <class T, class F>
-void pick_shape(const NormShape& s, F&& f) {
-  constexpr int VF = Vec16<T>::N;
-#define MGP_NORM_CASE(LL, NN, VV) \
-  if (s.L == LL && s.NV == NN && s.VEC == VV) return f(Int<LL>{}, Int<NN>{}, Int<VV>{});
-  MGP_NORM_CASE(8, 1, VF)
-  MGP_NORM_CASE(16, 1, VF)
-  MGP_NORM_CASE(32, 1, VF)
-  MGP_NORM_CASE(64, 1, VF)
-  MGP_NORM_CASE(64, 2, VF)
-  if constexpr (VF == 4) { MGP_NORM_CASE(64, 4, VF) }
-  MGP_NORM_CASE(256, 1, VF)
-  MGP_NORM_CASE(256, 2, VF)
-  MGP_NORM_CASE(256, 4, VF)
-  if constexpr (VF == 4) { MGP_NORM_CASE(256, 8, VF) }
-  MGP_NORM_CASE(8, 1, 1)
-  MGP_NORM_CASE(16, 1, 1)
-  MGP_NORM_CASE(32, 1, 1)
-  MGP_NORM_CASE(64, 1, 1)
-  MGP_NORM_CASE(64, 2, 1)
-  MGP_NORM_CASE(64, 4, 1)
-  MGP_NORM_CASE(64, 8, 1)
-  MGP_NORM_CASE(64, 16, 1)
-  MGP_NORM_CASE(256, 1, 1)
-  MGP_NORM_CASE(256, 2, 1)
-  MGP_NORM_CASE(256, 4, 1)
-  MGP_NORM_CASE(256, 8, 1)
-  MGP_NORM_CASE(256, 16, 1)
-  MGP_NORM_CASE(256, 32, 1)
+void pick_shape(const NormShape& s, bool ragged, F&& f) {
+  constexpr int VEC = Vec16<T>::N;
+#define MGP_NORM_CASE(LL, NN)                                     \
+  if (s.L == LL && s.NV == NN) {                                  \
+    if (ragged) return f(Int<LL>{}, Int<NN>{}, std::true_type{}); \
+    return f(Int<LL>{}, Int<NN>{}, std::false_type{});            \
+  }
+  MGP_NORM_CASE(8, 1)
+  MGP_NORM_CASE(16, 1)
+  MGP_NORM_CASE(32, 1)
+  MGP_NORM_CASE(64, 1)
+  MGP_NORM_CASE(64, 2)
+  if constexpr (VEC == 4) { MGP_NORM_CASE(64, 4) }
+  MGP_NORM_CASE(256, 1)
+  MGP_NORM_CASE(256, 2)
+  MGP_NORM_CASE(256, 4)
+  if constexpr (VEC == 4) { MGP_NORM_CASE(256, 8) }
 #undef MGP_NORM_CASE
   throw Error(ST_INTERNAL, "no layer norm kernel for this shape");
 }
 
-template <class T>
-bool vec_rows(const void* p, int64_t stride) {
-  return p == nullptr || (aligned16(p) && stride % Vec16<T>::N == 0);
+// Blocks of the backward pass.  Each writes one set of column sums, which the
+// sum over them reads: few blocks, but enough waves to keep the memory busy
+// (bf16, 12007 x 771: 1024 blocks 24 us, 512 18.7; 1000 x 4096: 512 26.5, 256 19.6).
+constexpr int64_t kNormBlocks = 512, kNormBlocksLeast = 256;
+inline int64_t norm_blocks(int64_t groups) {
+  return std::min(groups, std::max(kNormBlocksLeast, std::min(groups / 4, kNormBlocks)));
 }
-
-// blocks of the backward pass: each keeps one set of column sums
-constexpr int kNormBlocks = 1024;
 constexpr int64_t kNormWideRows = 64;  // row stretches of the wide column sums
 
 }  // namespace
@@ -426,9 +468,8 @@ void layer_norm(const NormArgs& a, void* y, int64_t y_stride, float* stats, hipS
   if (a.rows == 0) return;
   dispatch_elem(a.type, [&](auto tag) {
     using T = decltype(tag);
-    const bool vec = a.width % Vec16<T>::N == 0 && vec_rows<T>(a.x, a.x_stride) &&
-                     vec_rows<T>(y, y_stride);
-    const NormShape s = norm_shape<T>(vec, a.rows, a.width);
+    const NormShape s = norm_shape<T>(a.rows, a.width);
+    const bool ragged = a.width % Vec16<T>::N != 0;
     const T* x = static_cast<const T*>(a.x);
     if (s.L == 0) {
       k_norm_fwd_wide<T><<<(unsigned)std::min<int64_t>(a.rows, 2048), kNormThreads, 0, st>>>(
@@ -436,8 +477,8 @@ void layer_norm(const NormArgs& a, void* y, int64_t y_stride, float* stats, hipS
           static_cast<T*>(y), y_stride, stats);
     } else {
       const int64_t groups = ceil_div(a.rows, (int64_t)(kNormThreads / s.L));
-      pick_shape<T>(s, [&](auto L, auto NV, auto VEC) {
-        k_norm_fwd<T, L.value, NV.value, VEC.value>
+      pick_shape<T>(s, ragged, [&](auto L, auto NV, auto R) {
+        k_norm_fwd<T, L.value, NV.value, R.value>
             <<<(unsigned)std::min<int64_t>(groups, 2048), kNormThreads, 0, st>>>(
                 x, a.x_stride, a.rows, (int)a.width, a.weight, a.bias, a.f32_params, a.eps,
                 static_cast<T*>(y), y_stride, stats);
@@ -460,9 +501,8 @@ void layer_norm_backward(const NormArgs& a, const void* dy, int64_t dy_stride, c
   float* part = cols ? static_cast<float*>(ws) : nullptr;
   dispatch_elem(a.type, [&](auto tag) {
     using T = decltype(tag);
-    const bool vec = a.width % Vec16<T>::N == 0 && vec_rows<T>(a.x, a.x_stride) &&
-                     vec_rows<T>(dy, dy_stride) && vec_rows<T>(dx, dx_stride);
-    const NormShape s = norm_shape<T>(vec, a.rows, a.width);
+    const NormShape s = norm_shape<T>(a.rows, a.width);
+    const bool ragged = a.width % Vec16<T>::N != 0;
     const T *x = static_cast<const T*>(a.x), *d = static_cast<const T*>(dy);
     int nblk = 0;
     if (a.rows > 0 && s.L == 0) {
@@ -479,9 +519,9 @@ void layer_norm_backward(const NormArgs& a, const void* dy, int64_t dy_stride, c
       }
     } else if (a.rows > 0) {
       const int64_t groups = ceil_div(a.rows, (int64_t)(kNormThreads / s.L));
-      nblk = (int)std::min<int64_t>(groups, kNormBlocks);
-      pick_shape<T>(s, [&](auto L, auto NV, auto VEC) {
-        k_norm_bwd<T, L.value, NV.value, VEC.value><<<(unsigned)nblk, kNormThreads, 0, st>>>(
+      nblk = (int)norm_blocks(groups);
+      pick_shape<T>(s, ragged, [&](auto L, auto NV, auto R) {
+        k_norm_bwd<T, L.value, NV.value, R.value><<<(unsigned)nblk, kNormThreads, 0, st>>>(
             d, dy_stride, x, a.x_stride, a.rows, (int)a.width, a.weight, a.f32_params, stats,
             static_cast<T*>(dx), dx_stride, part);
       });
