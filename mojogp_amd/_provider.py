@@ -213,8 +213,7 @@ class NativeProvider:
 
     def input_gradient_device(self, Lf, Rf, out=None):
         """input_gradient of device tensors ([ncols, n] or [n], float32, contiguous;
-        out [n, d]), on the calling program's current stream.  As every call of a
-        provider it returns when the work is done."""
+        out [n, d]), asynchronously on the calling program's current stream."""
         from . import features
         dtype, code, index, stream = features._first(Lf, "Lf")
         shape = Lf.shape

@@ -196,6 +196,7 @@ int mgp_destroy_provider(void* h) {
     Provider* pv = as_provider(h);
     unregister_provider(pv);
     if (pv->st) (void)hipStreamSynchronize(pv->st);
+    pv->points_use.wait();
     if (pv->ws.ev0) (void)hipEventDestroy(pv->ws.ev0);
     if (pv->ws.ev1) (void)hipEventDestroy(pv->ws.ev1);
     hipStream_t st = pv->st;
@@ -522,9 +523,10 @@ int mgp_input_gradient_device(void* h, const float* Lf_dev, const float* Rf_dev,
     Provider* pv = as_provider(h);
     MGP_REQUIRE(ncols >= 1, "ncols must be >= 1");
     MGP_REQUIRE(Lf_dev && Rf_dev && out_dev, "null device array");
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    point_gradient(*pv, Lf_dev, Rf_dev, ncols, out_dev, st);
-    MGP_HIP_CHECK(hipStreamSynchronize(st));
+    int device = -1;
+    MGP_HIP_CHECK(hipGetDevice(&device));
+    MGP_REQUIRE(device == pv->device, "the provider's device is not the current one");
+    point_gradient(*pv, Lf_dev, Rf_dev, ncols, out_dev, static_cast<hipStream_t>(stream));
   });
 }
 

@@ -13,6 +13,33 @@
 
 namespace mgp {
 
+// The last use of a provider's arrays that a call left running on a caller's
+// stream: later work on other streams, changes of the arrays and their release
+// wait for it.
+struct PendingUse {
+  hipEvent_t ev = nullptr;
+  bool pending = false;
+  PendingUse() = default;
+  PendingUse(const PendingUse&) = delete;
+  PendingUse& operator=(const PendingUse&) = delete;
+  ~PendingUse() {
+    wait();
+    if (ev) (void)hipEventDestroy(ev);
+  }
+  void record(hipStream_t st) {
+    if (!ev) MGP_HIP_CHECK(hipEventCreateWithFlags(&ev, hipEventDisableTiming));
+    MGP_HIP_CHECK(hipEventRecord(ev, st));
+    pending = true;
+  }
+  void order(hipStream_t st) const {
+    if (pending) MGP_HIP_CHECK(hipStreamWaitEvent(st, ev, 0));
+  }
+  void wait() noexcept {
+    if (pending) (void)hipEventSynchronize(ev);
+    pending = false;
+  }
+};
+
 struct Provider {
   int kind = KIND_RBF;
   bool ard = false;
@@ -135,7 +162,12 @@ struct Provider {
   // (pack_rhs over train), if the caller keeps one.
   void cross(const PackedPoints& rows, const float* V, int ncols, float* out,
              const RhsPack* packed = nullptr);
-  DevBuf<float> pg_ws;  // split sums of the input gradient
+  DevBuf<float> pg_ws;  // operands and split sums of the input gradient
+  PendingUse points_use;  // of train and pg_ws, by mgp_input_gradient_device
+  float* pg_buffer(size_t count) {
+    if (count > pg_ws.count) points_use.wait();
+    return pg_ws.ensure(count);
+  }
   DevBuf<float> love_v, love_var, love_diag;  // LOVE variance of a test set
   // out[c*n + i] = k(rows[r0 + c], x_i) for c < nrows (dense cross block).
   void fill_block(const PackedPoints& rows, int64_t r0, int64_t nrows, float* out);

@@ -11,6 +11,7 @@
 namespace mgp {
 
 void Provider::refresh_coords() {
+  points_use.wait();
   if (is_tree) {
     for (int q = 0; q < nparams; ++q)
       MGP_REQUIRE(std::isfinite(params[q]) && params[q] > 0.f,

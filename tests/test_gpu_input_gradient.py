@@ -163,3 +163,82 @@ def test_refusals():
             tree.input_gradient(L, R)
     finally:
         tree.close()
+
+
+def _reference(kind, X, params, L, R):
+    """ol.input_gradient a block of rows at a time, for thousands of points."""
+    X, L, R = (a.astype(np.float64) for a in (X, L, R))
+    ls = np.broadcast_to(params[:-1].astype(np.float64), (X.shape[1],))
+    z, out = X / ls, np.empty_like(X)
+    for i in range(0, X.shape[0], 500):
+        df = z[i:i + 500, None, :] - z[None, :, :]
+        r2 = np.einsum("abq,abq->ab", df, df)
+        u = np.sqrt({"rbf": 1.0, "matern32": 3.0, "matern52": 5.0}[kind] * r2)
+        h = {"rbf": lambda: np.exp(-0.5 * r2), "matern32": lambda: 3.0 * np.exp(-u),
+             "matern52": lambda: 5.0 / 3.0 * (1.0 + u) * np.exp(-u)}[kind]()
+        h *= L[:, i:i + 500].T @ R + R[:, i:i + 500].T @ L
+        out[i:i + 500] = -params[-1] / ls * np.einsum("ab,abq->aq", h, df)
+    return out
+
+
+@pytest.mark.parametrize("kind", ["rbf", "matern32", "matern52"])
+@pytest.mark.parametrize("n, d, t", [(4000, 8, 11), (4001, 1, 1), (4111, 9, 16), (4500, 16, 20),
+                                     (4015, 19, 5), (4100, 24, 3), (4097, 30, 6)])
+def test_matrix_core_route(kind, n, d, t):
+    """Sets large enough for the matrix cores, over operand counts and ragged
+    ends; two levels of fp32 sums: the tolerance of the smaller sets holds."""
+    X, params, L, R = _inputs(n, d, t, True, seed=3)
+    params[:-1] *= np.float32(1.5)  # norms below the route's bounds
+    want = _reference(kind, X, params, L, R)
+    p = NativeProvider(kind, True, X, params, 0.1)
+    try:
+        got = p.input_gradient(L, R)
+        assert np.array_equal(got, p.input_gradient(L, R))
+    finally:
+        p.close()
+    assert np.linalg.norm(got - want) <= TOL * np.linalg.norm(want)
+
+
+def test_routes_agree_across_the_norm_bound():
+    """The same points and lengthscales, once beside an outlier whose norm sends
+    them to the differences: its own weight is zero, so nothing else changes."""
+    X, params, L, R = _inputs(4200, 5, 7, True, seed=4)
+    far = np.vstack([X, np.full((1, 5), 60.0, np.float32)])
+    zero = np.zeros((7, 1), np.float32)
+    a, b = NativeProvider("matern52", True, X, params, 0.1), \
+        NativeProvider("matern52", True, far, params, 0.1)
+    try:
+        ga = a.input_gradient(L, R)
+        gb = b.input_gradient(np.hstack([L, zero]), np.hstack([R, zero]))
+    finally:
+        a.close()
+        b.close()
+    assert not np.array_equal(ga, gb[:-1]) and not gb[-1].any()
+    assert np.linalg.norm(ga - gb[:-1]) <= TOL * np.linalg.norm(ga)
+
+
+def test_calls_in_flight_are_waited_for():
+    """Calls of one handle on two streams share its work buffers, parameters
+    change and the handle goes while a call may still run: every result is
+    that of the parameters at its call."""
+    X, params, L, R = _inputs(6000, 4, 11, True, seed=5)
+    p = NativeProvider("rbf", True, X, params, 0.1)
+    l, r = torch.from_numpy(L).cuda(), torch.from_numpy(R).cuda()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    first = p.input_gradient(L, R)
+    got = []
+    for k in range(6):
+        with torch.cuda.stream(streams[k % 2]):
+            got.append(p.input_gradient_device(l, r))
+    p.update_params(params * np.float32(1.3))
+    with torch.cuda.stream(streams[0]):
+        late = p.input_gradient_device(l[:3], r[:3])
+    p.close()
+    torch.cuda.synchronize()
+    assert all(np.array_equal(g.cpu().numpy(), first) for g in got)
+    q = NativeProvider("rbf", True, X, params * np.float32(1.3), 0.1)
+    try:
+        assert np.array_equal(late.cpu().numpy(), q.input_gradient(L[:3], R[:3]))
+    finally:
+        q.close()
