@@ -641,20 +641,43 @@ struct WeightEpi {
 
 // ---------------------------------------------------------------- helpers
 
-// dst[row][cols_pad] = src[row][cols], zeros past cols
+// Up to three matrices of one width in one launch: dst[row][pad] = src[row][cols],
+// zeros past cols.
 template <class T>
-__global__ __launch_bounds__(256) void k_pack_rows(const T* __restrict__ src, int64_t ld,
-                                                   int64_t rows, int64_t cols, int64_t cols_pad,
-                                                   T* __restrict__ dst) {
+struct PackSource {
+  const T* src[3];
+  int64_t ld[3], rows[3], cols, pad;
+  T* dst[3];
+};
+
+template <class T>
+__global__ __launch_bounds__(256) void k_pack_rows(PackSource<T> s) {
   constexpr int N = Vec16<T>::N;
-  const int64_t per = cols_pad / N, total = rows * per;
+  const int64_t per = s.pad / N, total = (s.rows[0] + s.rows[1] + s.rows[2]) * per;
   for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total;
        q += (int64_t)gridDim.x * 256) {
-    const int64_t r = q / per, c = (q - r * per) * N;
-    Vec16<T> v;
+    int64_t r = q / per;
+    const int64_t c = (q - r * per) * N;
+    int m = 0;
+    if (r >= s.rows[0]) {
+      r -= s.rows[0];
+      m = 1;
+      if (r >= s.rows[1]) {
+        r -= s.rows[1];
+        m = 2;
+      }
+    }
+    const T* src = (m == 0 ? s.src[0] : m == 1 ? s.src[1] : s.src[2]) +
+                   r * (m == 0 ? s.ld[0] : m == 1 ? s.ld[1] : s.ld[2]) + c;
+    T* dst = (m == 0 ? s.dst[0] : m == 1 ? s.dst[1] : s.dst[2]) + r * s.pad + c;
+    T v[N];
+    if (c + N <= s.cols) {
+      __builtin_memcpy(v, src, sizeof(v));
+    } else {
 #pragma unroll
-    for (int k = 0; k < N; ++k) v.v[k] = c + k < cols ? src[r * ld + c + k] : (T)0.0f;
-    *reinterpret_cast<Vec16<T>*>(dst + r * cols_pad + c) = v;
+      for (int k = 0; k < N; ++k) v[k] = c + k < s.cols ? src[k] : (T)0.0f;
+    }
+    __builtin_memcpy(dst, v, sizeof(v));
   }
 }
 
@@ -821,7 +844,7 @@ struct Stat {
   float amax, norm;
 };
 enum : int { ST_X = 0, ST_W = 1, ST_DH = 2, kStats = 3 };
-constexpr int kStatBlocks = 256;  // partial results a tensor
+constexpr int kStatBlocks = 512;  // partial results a tensor
 
 struct StatSource {
   const float* p[2];
@@ -1119,14 +1142,6 @@ struct Plan {
   int64_t ldt() const { return 2 * hpad * COPIES; }    // of the transposed weights
 };
 
-template <class T>
-void pack_rows(const void* src, int64_t ld, int64_t rows, int64_t cols, int64_t pad, T* dst,
-               hipStream_t st) {
-  const int64_t items = rows * (pad / Vec16<T>::N);
-  k_pack_rows<T><<<(unsigned)std::min<int64_t>(ceil_div(items, (int64_t)256), 8192), 256, 0, st>>>(
-      static_cast<const T*>(src), ld, rows, cols, pad, dst);
-}
-
 template <class E>
 struct Inputs {
   const E *x, *wg, *wu;
@@ -1162,18 +1177,33 @@ Inputs<typename Plan<T, MODE>::E> load_inputs(const GatedArgs& a, const Plan<T, 
   } else {
     Inputs<E> in{static_cast<const T*>(a.x), static_cast<const T*>(a.w_gate),
                  static_cast<const T*>(a.w_up), a.x_stride, a.w_gate_stride, nullptr};
+    PackSource<T> p{};
+    p.cols = a.width;
+    p.pad = pl.wpad;
     if (pl.pack_x) {
-      pack_rows<T>(a.x, a.x_stride, a.rows, a.width, pl.wpad, x, st);
+      p.src[0] = in.x;
+      p.ld[0] = a.x_stride;
+      p.rows[0] = a.rows;
+      p.dst[0] = x;
       in.x = x;
       in.ldx = pl.wpad;
     }
     if (pl.pack_w) {
-      pack_rows<T>(a.w_gate, a.w_gate_stride, a.hidden, a.width, pl.wpad, wg, st);
-      pack_rows<T>(a.w_up, a.w_up_stride, a.hidden, a.width, pl.wpad, wu, st);
+      p.src[1] = in.wg;
+      p.src[2] = in.wu;
+      p.ld[1] = a.w_gate_stride;
+      p.ld[2] = a.w_up_stride;
+      p.rows[1] = p.rows[2] = a.hidden;
+      p.dst[1] = wg;
+      p.dst[2] = wu;
       in.wg = wg;
       in.wu = wu;
       in.ldw = pl.wpad;
     }
+    const int64_t items = (p.rows[0] + p.rows[1] + p.rows[2]) * (pl.wpad / Vec16<T>::N);
+    if (items > 0)
+      k_pack_rows<T><<<(unsigned)std::min<int64_t>(ceil_div(items, (int64_t)256), 8192), 256, 0,
+                       st>>>(p);
     return in;
   }
 }

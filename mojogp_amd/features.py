@@ -68,9 +68,9 @@ def _first(a, name):
     index = a.get_device()
     if index < 0:
         raise ValueError(f"{name} must be a device tensor, got one on {a.device}")
-    if index != torch.cuda.current_device():
-        raise ValueError(f"{name} is on device {index}, the current device is "
-                         f"{torch.cuda.current_device()}")
+    current = torch.cuda.current_device()
+    if index != current:
+        raise ValueError(f"{name} is on device {index}, the current device is {current}")
     return dtype, code, index, _stream(torch, index)
 
 
