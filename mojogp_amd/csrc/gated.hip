@@ -1045,11 +1045,43 @@ template <class T, bool TR, bool DUAL, int PARTS>
 using BigTile = Tile<T, 8, 4, 2, 4, TR, DUAL, PARTS>;
 template <class T, bool TR, bool DUAL, int PARTS>
 using SmallTile = Tile<T, 4, 4, 2, 2, TR, DUAL, PARTS>;
-constexpr int64_t kBigTiles = 512;  // 256 x 256 tiles from which on they are taken
-inline bool big_tiles(int64_t p_rows, int64_t q_rows) {
-  return ceil_div(p_rows, (int64_t)256) * ceil_div(q_rows, (int64_t)256) >= kBigTiles;
+// How a product is cut: the tile, and into how many parts its reduction, whose
+// sums are then written and read once each in fp32.  By the time as measured:
+// whole rounds of the device (512 small tiles or 256 big ones at a time), each
+// that of a tile's prologue and epilogue and of its stages (small, 4 / 7 / 16
+// stages: 7.1 / 11 / 19 us a round; big: 13.8 / 19 / 34), and the parts' sums at
+// 4.5 TB/s.  So 8192 rows x 1024 -> 1024 bf16 go by big tiles (33.9 us forward, 38.1
+// by small ones), 12007 x 392 -> 1024 by small ones (33.1, 38.7); the weight
+// gradient of 4096 x 1024 -> 4096 by small ones in one part (70 us; big ones in two
+// 102, in four 143), that of 65536 rows by big ones in two.
+struct Cut {
+  bool big = false;
+  int64_t splits = 1, per = 0;  // parts, and stages of each
+};
+inline Cut cut_product(int64_t p_rows, int64_t q_rows, int64_t stages, int64_t parts_a_stage,
+                       bool may_big, int64_t max_splits, double outputs) {
+  Cut best;
+  double least = 0.0;
+  for (int big = 0; big <= (may_big ? 1 : 0); ++big) {
+    const int64_t side = big ? 256 : 128;
+    const int64_t tiles = ceil_div(p_rows, side) * ceil_div(q_rows, side);
+    for (int64_t want = 1; want <= std::min(max_splits, std::max<int64_t>(1, stages / 4)); ++want) {
+      const int64_t per = ceil_div(stages, want), splits = ceil_div(stages, per);
+      const double rounds = (double)ceil_div(tiles * splits, (int64_t)(big ? 256 : 512));
+      const double work = (double)(per * parts_a_stage);
+      const double us = rounds * (big ? 7.1 + 1.7 * work : 3.3 + 1.0 * work) +
+                        (splits > 1 ? 5.0 + (double)splits * outputs * 8.0 / 4.5e6 : 0.0);
+      if ((big == 0 && want == 1) || us < least) {
+        least = us;
+        best.big = big != 0;
+        best.splits = splits;
+        best.per = per;
+      }
+    }
+  }
+  return best;
 }
-constexpr int64_t kSplitTarget = 512;  // workgroups that a split reduction aims at
+constexpr int64_t kMaxSplits = 64;
 
 // fp32 layers go through the fp16 matrix cores in two parts of 11 bits a value
 // and three products (the low parts' own product is below 2^-22): three times
@@ -1083,8 +1115,9 @@ struct Plan {
   size_t x_off = 0, wg_off = 0, wu_off = 0, wt_off = 0, dgu_off = 0, dbias_off = 0, part_off = 0;
   size_t stat_off = 0, scale_off = 0, dxp_off = 0;
   size_t bytes = 0;
-  bool big_dual = false, big_dx = false, big_dw = false;
-  int64_t bias_parts = 0, splits = 1, k_split = 0, dx_splits = 1, dx_split = 0;
+  bool big_dual = false;
+  Cut dx, dw;
+  int64_t bias_parts = 0;
 
   Plan(const GatedArgs& a, bool backward) {
     wpad = round_up(a.width, WQ);
@@ -1107,37 +1140,24 @@ struct Plan {
       scale_off = take(sizeof(Scales));
     }
     const int64_t rows = std::max<int64_t>(a.rows, 1);
-    big_dual = MODE != FEW_ROWS && big_tiles(2 * a.hidden, rows);
+    constexpr int64_t KS = 128 / sizeof(E);
+    constexpr bool may_big = MODE != FEW_ROWS;  // (which has too few rows for them)
+    big_dual = cut_product(2 * a.hidden, rows, ceil_div(wpad, KS), PARTS, may_big, 1, 0.0).big;
     if (!backward) return;
-    big_dx = big_tiles(a.width, rows);
     wt_off = take((size_t)a.width * ldt() * sizeof(E));
     dgu_off = take((size_t)a.rows * ldd() * sizeof(E));
     bias_parts = 2 * ceil_div(rows, (int64_t)(big_dual ? 256 : 128));
     dbias_off = take((size_t)bias_parts * 2 * a.hidden * sizeof(float));
-    // Where the tiles do not fill the device the reductions are split: of the
-    // weight gradients over the rows, of dx (few rows) over hidden.  Each
-    // split's sums cost a write and a read of the result in fp32.
-    constexpr int64_t KS = 128 / sizeof(E);
-    const int64_t stages = ceil_div(rows, KS);
-    big_dw = 2 * hpad * a.width >= (int64_t)16 * 256 * 256 && stages >= 64;
-    const int64_t side = big_dw ? 256 : 128;
-    split(stages, ceil_div(2 * hpad, side) * ceil_div(a.width, side), 16, splits, k_split);
-    if (splits > 1) part_off = take((size_t)splits * 2 * a.hidden * a.width * sizeof(float));
-    const int64_t dx_side = big_dx ? 256 : 128;
-    split(ceil_div(2 * hpad, KS), ceil_div(rows, dx_side) * ceil_div(a.width, dx_side), 8,
-          dx_splits, dx_split);
-    if (dx_splits > 1) dxp_off = take((size_t)dx_splits * a.rows * a.width * sizeof(float));
+    // the weight gradients' reduction is over the rows, dx's over hidden
+    const int64_t weights = 2 * a.hidden * a.width;
+    dw = cut_product(a.width, 2 * hpad, ceil_div(rows, KS), GRAD_PARTS, may_big, kMaxSplits,
+                     (double)weights);
+    if (dw.splits > 1) part_off = take((size_t)dw.splits * weights * sizeof(float));
+    dx = cut_product(a.width, rows, ceil_div(2 * hpad, KS), GRAD_PARTS, may_big, kMaxSplits,
+                     (double)a.rows * (double)a.width);
+    if (dx.splits > 1) dxp_off = take((size_t)dx.splits * a.rows * a.width * sizeof(float));
   }
-  // Splits of `least` stages or more until there are kSplitTarget workgroups.
-  static void split(int64_t stages, int64_t tiles, int64_t least, int64_t& splits,
-                    int64_t& length) {
-    splits = std::max<int64_t>(
-        1, std::min(ceil_div(kSplitTarget, tiles), ceil_div(stages, least)));
-    if (tiles * 2 > kSplitTarget) splits = 1;
-    const int64_t per = ceil_div(stages, splits);
-    splits = ceil_div(stages, per);
-    length = per * (128 / (int64_t)sizeof(E));
-  }
+  static int64_t reduction(const Cut& c) { return c.per * (128 / (int64_t)sizeof(E)); }
   int64_t ldd() const { return 2 * hpad * D_COPIES; }  // of [dg | du]
   int64_t ldt() const { return 2 * hpad * COPIES; }    // of the transposed weights
 };
@@ -1383,29 +1403,29 @@ void gated_backward(const GatedArgs& a, const void* dh, int64_t dh_stride, const
       s.p = operand(wt, pl.ldt(), a.width);
       s.q = operand(dgu, pl.ldd(), a.rows);
       s.K = 2 * pl.hpad;
-      s.k_split = pl.dx_split;
+      s.k_split = PL::reduction(pl.dx);
       s.p_lo = s.q_lo = lo;
       T* dx = static_cast<T*>(g.dx);
-      float* part = pl.dx_splits > 1 ? reinterpret_cast<float*>(ws + pl.dxp_off) : nullptr;
+      float* part = pl.dx.splits > 1 ? reinterpret_cast<float*>(ws + pl.dxp_off) : nullptr;
       launch_product<PL, false, false>(
-          pl.big_dx, s, pl.dx_splits,
+          pl.dx.big, s, pl.dx.splits,
           StoreEpi<T>{pick(in.scales, &Scales::dx), dx, part, a.rows, a.width}, st);
-      if (part) sum_parts<T>(part, pl.dx_splits, a.rows * a.width, 1, dx, nullptr, st);
+      if (part) sum_parts<T>(part, pl.dx.splits, a.rows * a.width, 1, dx, nullptr, st);
     }
     if (dwg || dwu) {
-      float* part = pl.splits > 1 ? reinterpret_cast<float*>(ws + pl.part_off) : nullptr;
+      float* part = pl.dw.splits > 1 ? reinterpret_cast<float*>(ws + pl.part_off) : nullptr;
       GemmShape s{};
       s.p = operand(in.x, in.ldx, pl.wpad);
       s.q = operand(static_cast<const E*>(dgu), pl.ldd(), 2 * pl.hpad);
       s.K = a.rows;
-      s.k_split = pl.k_split;
+      s.k_split = PL::reduction(pl.dw);
       s.p_lo = pl.wpad * (int64_t)sizeof(E);
       s.q_lo = lo;
-      launch_product<PL, true, false>(pl.big_dw, s, pl.splits,
+      launch_product<PL, true, false>(pl.dw.big, s, pl.dw.splits,
                                       WeightEpi<T>{pick(in.scales, &Scales::dw), dwg, dwu, part,
                                                    a.hidden, pl.hpad, a.width},
                                       st);
-      if (part) sum_parts<T>(part, pl.splits, a.hidden * a.width, 2, dwg, dwu, st);
+      if (part) sum_parts<T>(part, pl.dw.splits, a.hidden * a.width, 2, dwg, dwu, st);
     }
     MGP_HIP_CHECK(hipGetLastError());
   });
