@@ -113,7 +113,7 @@ def likelihood_gradients(provider, y, probes, tol=1e-3):
     right = torch.cat([u[:1], probes])
     points = provider.input_gradient_device(left, right)
     kernel = provider.gradient_trace(left.cpu().numpy(), right.cpu().numpy())
-    return float(y @ u[0]), points, np.append(kernel, float((left * right).sum()))
+    return float((y * u[0]).sum()), points, np.append(kernel, float((left * right).sum()))
 
 
 class Adam:

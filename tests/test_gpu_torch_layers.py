@@ -5,7 +5,12 @@ rounded once to a type of unit roundoff u is at most u off; the fp32 sums of
 up to n terms of either sign add about 2^-24 sqrt(n) (n up to 2000 rows or
 columns here), taken as F32 = 4e-6.  The gated layer's gradients also carry
 the rounding of dg and du, which the matrix cores take in the element type:
-another u, and 2 u where both meet in dx."""
+another u, and 2 u where both meet in dx.
+
+(The test_gpu_torch_* modules run torch on the device; their names put them
+after test_gpu_scratch_limit, which needs the free memory that the runtime
+reports to be all it has: the runtime also has what it holds as scratch for
+earlier kernels.)"""
 
 import numpy as np
 import pytest
