@@ -200,9 +200,9 @@ struct GemmShape {
 
 // Tile of 16 TN WN columns (p rows) by 16 TM WM rows (q rows), one wave 16 TN
 // by 16 TM of it.  NT: the p rows are dealt to LDS so that a lane's results are
-// RUN = 4 TN (dual: 2 TN of each matrix) consecutive columns.  Both operands go through LDS by direct loads, double
-// buffered, 128 bytes of reduction a stage.  NT: 128-byte LDS rows, 16-byte
-// chunk c of row r at c ^ (r / 2 % 8).  TN: LDS rows of the tile's width, one
+// RUN = 4 TN (dual: 2 TN of each matrix) consecutive columns.  Both operands go
+// through LDS by direct loads, double buffered, 128 bytes of reduction a stage.
+// NT: 128-byte LDS rows, 16-byte chunk c of row r at c ^ (r / 2 % 8).  TN: LDS rows of the tile's width, one
 // per reduction step, in the memory's order, their 32-byte granules at g ^ (r % 8)
 // and read by the transposing LDS load.  Both keep the fragment reads off each
 // other's banks.
@@ -406,57 +406,90 @@ __device__ __forceinline__ void stage(Loader<TL>& ld, const char* __restrict__ c
 // Workgroups go round the 8 XCDs in turn: each XCD takes a stretch of tiles of
 // its own, ordered in groups of 8 tile rows, so that what its L2 holds serves
 // the tiles in flight on it.
-__device__ __forceinline__ void tile_of(int64_t id, int64_t tiles_p, int64_t tiles_q, int64_t& tp,
-                                        int64_t& tq) {
-  const int64_t total = tiles_p * tiles_q, xcd = id & 7, per = total >> 3, rest = total & 7;
+__device__ __forceinline__ void tile_of(uint32_t id, uint32_t tiles_p, uint32_t tiles_q,
+                                        uint32_t& tp, uint32_t& tq) {
+  const uint32_t total = tiles_p * tiles_q, xcd = id & 7, per = total >> 3, rest = total & 7;
   id = xcd * per + min(xcd, rest) + (id >> 3);
-  const int64_t group = id / (8 * tiles_p), in = id - group * 8 * tiles_p;
-  const int64_t height = min((int64_t)8, tiles_q - group * 8);
+  const uint32_t group = id / (8 * tiles_p), in = id - group * 8 * tiles_p;
+  const uint32_t height = min(8u, tiles_q - group * 8);
   tq = group * 8 + in % height;
   tp = in / height;
 }
 
+// Whether a workgroup goes on to further tiles (of its XCD: the grid is a
+// multiple of 8 then), the first stage of which it loads before the epilogue of
+// the one before. For the big tile, alone on its CU, in the forward pass: bf16,
+// 65536 x 1024 -> 4096 1005 -> 988 us, 30000 x 768 -> 2304 224 -> 216, 32768 x 256 ->
+// 1024 55.4 -> 52.4, a single round of tiles (8192 x 1024 -> 1024) 33.5 -> 34.4; the
+// backward pass' longer epilogue has no registers to spare (65536 rows: 1328 ->
+// 1347), the gradients' products have many stages or one round (dx 916 -> 909).
+template <class TL, class EPI>
+constexpr bool stays = TL::W == 8 && EPI::FORWARD;
+
 // acc[tm][tn][e] of lane l holds output row 16 (wm TM + tm) + l % 16 and column
 // (NT, tn < T1) 16 T1 wn + RUN (l / 16) + 4 tn + e of either matrix, (TN)
 // 16 (wn TN + tn) + 4 (l / 16) + e.
+//
+// Bound by the matrix cores' feeding: 65536 x 1024 -> 4096 in bf16 takes 990 us
+// forward (1110 TFLOP/s), 1325 for g, u, dg and du, 930 for dx (1180) and 960 for
+// the weight gradients (1145), where a plain large product reaches 1420.  The big
+// tile leaves room for one workgroup a CU, whose epilogue nothing covers; two of the
+// small one cover each other, but read twice the operands from LDS and the L1 cache.
 template <class TL, class EPI>
 __global__ __launch_bounds__(TL::THREADS) void k_gemm(GemmShape s, EPI epi) {
   __shared__ __align__(1024) char b0[TL::LDS];
   __shared__ __align__(1024) char b1[TL::LDS];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % TL::WM, wn = wave / TL::WM;
-  int64_t tp, tq;
-  tile_of(blockIdx.x, s.tiles_p, s.tiles_q, tp, tq);
   constexpr int CP = TL::DUAL ? TL::BP / 2 : TL::BP;  // output columns a tile
-  const int64_t n0 = (int64_t)tp * CP, m0 = (int64_t)tq * TL::BQ;
+  constexpr bool STAYS = stays<TL, EPI>;
+  const uint32_t tiles = (uint32_t)(s.tiles_p * s.tiles_q);
   const int64_t k0 = (int64_t)blockIdx.y * s.k_split;
   const int64_t K = min(s.k_split, s.K - k0);
+  const int64_t all = (K + TL::KS - 1) / TL::KS * TL::PARTS;
 
-  f4 acc[TL::TM][TL::TN];
-#pragma unroll
-  for (int m = 0; m < TL::TM; ++m)
-#pragma unroll
-    for (int n = 0; n < TL::TN; ++n) acc[m][n] = f4{0.f, 0.f, 0.f, 0.f};
-
+  uint32_t tp, tq;
+  tile_of(blockIdx.x, (uint32_t)s.tiles_p, (uint32_t)s.tiles_q, tp, tq);
   Loader<TL> ld;
-  ld.init(s, n0, m0, k0, K);
+  ld.init(s, (int64_t)tp * CP, (int64_t)tq * TL::BQ, k0, K);
   // pairs of stages, so that each has its own buffers at compile time; an odd
   // one goes first
-  int64_t stages = (K + TL::KS - 1) / TL::KS * TL::PARTS;
-  if (stages % 2 == 1) {
-    ld.load(b1);
-    __syncthreads();
-    --stages;
-    stage<TL>(ld, b1, b0, stages > 0, wm, wn, acc);
-  } else {
-    ld.load(b0);
-    __syncthreads();
+  const bool odd = all % 2 == 1;
+  ld.load(odd ? b1 : b0);
+  __syncthreads();
+  for (uint32_t id = blockIdx.x;;) {
+    const int64_t n0 = (int64_t)tp * CP + wn * (CP / TL::WN);
+    const int64_t m0 = (int64_t)tq * TL::BQ + wm * TL::TM * 16, part = (int64_t)tq * TL::WM + wm;
+    const bool next = STAYS && id + gridDim.x < tiles;
+    id += gridDim.x;
+    f4 acc[TL::TM][TL::TN];
+#pragma unroll
+    for (int m = 0; m < TL::TM; ++m)
+#pragma unroll
+      for (int n = 0; n < TL::TN; ++n) acc[m][n] = f4{0.f, 0.f, 0.f, 0.f};
+    const auto to_next = [&] {
+      tile_of(id, (uint32_t)s.tiles_p, (uint32_t)s.tiles_q, tp, tq);
+      ld.init(s, (int64_t)tp * CP, (int64_t)tq * TL::BQ, k0, K);
+    };
+    int64_t stages = all;
+    if (odd) stage<TL>(ld, b1, b0, --stages > 0, wm, wn, acc);
+    for (; stages > 0; stages -= 2) {
+      stage<TL>(ld, b0, b1, true, wm, wn, acc);
+      bool more = stages > 2;
+      if (STAYS && !more && next && !odd) {
+        to_next();
+        more = true;
+      }
+      stage<TL>(ld, b1, b0, more, wm, wn, acc);
+    }
+    if (STAYS && next && odd) {
+      to_next();
+      ld.load(b1);
+    }
+    epi.template run<TL>(acc, m0, n0, part);
+    if (!STAYS || !next) return;
+    if (odd) __syncthreads();
   }
-  for (; stages > 0; stages -= 2) {
-    stage<TL>(ld, b0, b1, true, wm, wn, acc);
-    stage<TL>(ld, b1, b0, stages > 2, wm, wn, acc);
-  }
-  epi.template run<TL>(acc, m0 + wm * TL::TM * 16, n0 + wn * (CP / TL::WN), tq * TL::WM + wm);
 }
 
 // ---------------------------------------------------------------- epilogues
@@ -471,6 +504,7 @@ struct Unscale {
 
 template <class T, int ACT>
 struct ForwardEpi {
+  static constexpr bool FORWARD = true;
   Unscale scale;
   const T *bg, *bu;
   T* h;
@@ -509,6 +543,7 @@ struct ForwardEpi {
 // SPLIT: two parts of the scaled values, the low ones after the high ones of a row.
 template <class T, class E, int ACT, bool SPLIT>
 struct BackwardEpi {
+  static constexpr bool FORWARD = false;
   Unscale scale, dgu_scale;  // dgu_scale: what dg and du are multiplied by
   const T *bg, *bu;
   const T* dh;
@@ -576,6 +611,7 @@ struct BackwardEpi {
 // One split: the result; more: part[split][rows][cols] sums.
 template <class T>
 struct StoreEpi {
+  static constexpr bool FORWARD = false;
   Unscale scale;
   T* out;
   float* part;
@@ -607,6 +643,7 @@ struct StoreEpi {
 // split: the gradients themselves; more: part[split][2][hidden][width] sums.
 template <class T>
 struct WeightEpi {
+  static constexpr bool FORWARD = false;
   Unscale scale;
   T *dw_gate, *dw_up;
   float* part;
@@ -764,7 +801,8 @@ struct FewArgs {
 // device idle (a single point, a batch of a few hundred): a workgroup takes 16
 // columns of both projections for 16 MT rows, its 8 waves share the reduction
 // and read their fragments from global memory, at any alignment.  Bound by
-// latency: one round of loads for a width of 512, one exchange through LDS.
+// latency: one round of loads for a width of 512, one exchange through LDS
+// (bf16, one row x 512 -> 2048: 3.3 us for 4.2 MB of weights).
 template <class T, int ACT, int MT>
 __global__ __launch_bounds__(512) void k_gated_few(FewArgs s) {
   constexpr int N = Vec16<T>::N, W = 8;
@@ -1087,13 +1125,14 @@ constexpr int64_t kMaxSplits = 64;
 // and three products (the low parts' own product is below 2^-22): three times
 // the work at nine times the rate of the fp32 instructions, 24 against 128
 // cycles a reduction element of a tile.  Forming the parts takes two more
-// kernels.  20000 x 256 -> 512, both passes: 495 -> 343 us.
+// kernels.  20000 x 256 -> 512, both passes: 494 -> 330 us.
 
 // The 16-bit types' dg and du are rounded to the type for the last two products;
 // with few rows the roundings do not average out, and dx's and the weight
 // gradients' error reaches 1.5 times that of their own rounding (1.41 with
-// many).  Up to one tile of rows dg and du go in two parts instead, which costs
-// the last two products twice: 3 of ~60 us there, 2 of 4.4 ms at 65536 rows.
+// many).  Up to one tile of rows dg and du go in two parts instead, and the last
+// two products run twice: bf16, 128 x 256 -> 1024, backward 31 -> 41 us, 100 x 1024 ->
+// 4096 59 -> 70; at 65536 rows it would cost 1.9 of 3.2 ms.
 constexpr int64_t kFewRows = 128;
 
 enum Mode : int { PLAIN = 0, FP32_PARTS = 1, FEW_ROWS = 2 };
@@ -1232,8 +1271,9 @@ template <class TL, class EPI>
 void launch_tiles(GemmShape s, int64_t splits, const EPI& epi, hipStream_t st) {
   s.tiles_p = ceil_div(s.p.n, (int64_t)(TL::DUAL ? TL::BP / 2 : TL::BP));
   s.tiles_q = ceil_div(s.q.n, (int64_t)TL::BQ);
-  k_gemm<TL, EPI><<<dim3((unsigned)(s.tiles_p * s.tiles_q), (unsigned)splits), TL::THREADS, 0,
-                    st>>>(s, epi);
+  int64_t blocks = s.tiles_p * s.tiles_q;
+  if (stays<TL, EPI>) blocks = std::min(blocks, (int64_t)256);  // (never split)
+  k_gemm<TL, EPI><<<dim3((unsigned)blocks, (unsigned)splits), TL::THREADS, 0, st>>>(s, epi);
   MGP_HIP_CHECK(hipGetLastError());
 }
 
