@@ -6,7 +6,8 @@
 // (q / 8, 0) and key seed (Salmon, Moraes, Dror, Shaw, "Parallel random
 // numbers: as easy as 1, 2, 3", 2011).  Sixteen bits a draw make one block
 // serve eight elements: with 32 bits the ten rounds (two 32 x 32 -> 64 bit
-// products each) would take longer than the array's transfer.
+// products each) would take longer than the array's transfer.  HBM bound: bf16,
+// 250000 x 1024 with a residual 300 us (5.1 TB/s), without 193 (5.3).
 #include "layers.h"
 
 #include <algorithm>

@@ -6,7 +6,8 @@
 //
 // HBM bound: a row stays in registers between the reduction and the result,
 // so the forward pass reads x and writes y once, the backward pass reads x and
-// dy and writes dx once.  Statistics and sums are fp32; the variance is that
+// dy and writes dx once (fp32, 250000 x 256: 91 us, 5.6 TB/s, and 153 us, 5.0 TB/s).
+// Statistics and sums are fp32; the variance is that
 // of the centred row.
 #include "layers.h"
 
@@ -409,7 +410,8 @@ struct NormShape {
 
 // A row takes the fewest lanes that hold it with one vector each, up to a wave;
 // beyond 16 elements a lane of a wave, or with too few rows to fill the device
-// with waves, the block shares it.
+// with waves, the block shares it (bf16 x 771, backward: 1000 rows 10.3 us by blocks,
+// 12.1 by waves; 1500 rows 13.4, 9.3; 12007 rows 32.5, 19.7).
 template <class T>
 NormShape norm_shape(int64_t rows, int64_t width) {
   constexpr int VEC = Vec16<T>::N;

@@ -37,7 +37,7 @@ constexpr int kPgStride = kPgBlock + 16; // LDS stride of a weight column
 // (four weight columns an instruction); result e belongs to the pair (column
 // 4 (lane/16) + e, row lane%16), so a lane keeps its rows and their sums in
 // registers and reads columns from LDS.  VALU bound: 3 d + ~12 instructions a
-// pair.
+// pair (Matern-5/2, 8 dimensions, 50000 points: 3130 us, 0.8e12 pairs a second).
 template <int KIND, int D, bool ARD, int R>
 __global__ __launch_bounds__(256) void k_point_grad(
     const float* __restrict__ Z, int64_t n, int d, const float* __restrict__ Lf,
@@ -178,7 +178,8 @@ __global__ __launch_bounds__(256) void k_point_grad_sum(const float* __restrict_
 using PgFn = void (*)(const float*, int64_t, int, const float*, const float*, int, int64_t,
                       int64_t, float*);
 
-constexpr int64_t kPgFewPoints = 3000;  // below, 64-row blocks (300 points: 25.7 -> 23.4 us a call)
+// below, 64-row blocks (300 points 12.7 -> 10.1 us, 2000 18.2 -> 16.4, 3000 31.0 -> 31.2)
+constexpr int64_t kPgFewPoints = 3000;
 
 // the dimension steps of the difference products (direct.hip)
 template <int KIND, bool ARD, int R>
@@ -401,7 +402,8 @@ __device__ __forceinline__ void mm_stage(const char* next, int fragments, int kw
 // 4 (lane/16) + e, row lane%16): W h is then the A operand of the sum over the
 // columns as it stands, no lane exchanges it.  Bound by the VALU (Matern-5/2:
 // 5 instructions, a square root and an exponential a pair, 208 cycles a 16 x 16
-// tile) beside 192 cycles of matrix instructions of d <= 8.
+// tile) beside 192 cycles of matrix instructions of d <= 8; the two add up more than
+// they overlap: 50000 points, 11 columns, 1640 us, 1.5e12 pairs a second.
 template <int KIND, int KB, int DZ, int R>
 __global__ __launch_bounds__(256, 3) void k_point_grad_mm(
     const char* __restrict__ col, const uint4* __restrict__ B, const uint4* __restrict__ wrow,
@@ -500,11 +502,14 @@ struct MmKernel {
   int dz, row_tiles;  // 16-row tiles of a workgroup
 };
 
-// Rows a wave: 50000 points of 8 dimensions 1754 us with four 16-row tiles, 1804
-// with two; with two distance operands the registers make it 402 against 364
-// (20000 points of 16).
+// Rows a wave: four 16-row tiles for many points (8 dimensions, 30000 points 594
+// us, 620 with two; 50000 1640, 1676), two below, for more workgroups (10000 points
+// 95 us, 102 with four; 20000 276, 298), and with two distance operands, where four
+// leave too few registers (20000 points of 16 dimensions 298, 335).
+constexpr int64_t kMmFourTiles = 25000;
 template <int KIND>
-MmKernel pick_mm(int kb, int d) {
+MmKernel pick_mm(int kb, int d, int64_t n) {
+  if (kb == 1 && n <= kMmFourTiles) return {k_point_grad_mm<KIND, 1, 1, 2>, 1, 8};
   if (kb == 1) return {k_point_grad_mm<KIND, 1, 1, 4>, 1, 16};
   if (kb == 2 && d <= 16) return {k_point_grad_mm<KIND, 2, 1, 2>, 1, 8};
   if (kb == 2) return {k_point_grad_mm<KIND, 2, 2, 2>, 2, 8};
@@ -512,11 +517,11 @@ MmKernel pick_mm(int kb, int d) {
   return {nullptr, 0, 0};
 }
 
-MmKernel pick_mm(int kind, int kb, int d) {
+MmKernel pick_mm(int kind, int kb, int d, int64_t n) {
   switch (kind) {
-    case KIND_RBF: return pick_mm<KIND_RBF>(kb, d);
-    case KIND_MATERN32: return pick_mm<KIND_MATERN32>(kb, d);
-    case KIND_MATERN52: return pick_mm<KIND_MATERN52>(kb, d);
+    case KIND_RBF: return pick_mm<KIND_RBF>(kb, d, n);
+    case KIND_MATERN32: return pick_mm<KIND_MATERN32>(kb, d, n);
+    case KIND_MATERN52: return pick_mm<KIND_MATERN52>(kb, d, n);
     default: return {nullptr, 0, 0};
   }
 }
@@ -528,8 +533,9 @@ MmKernel pick_mm(int kind, int kb, int d) {
 inline float mm_norm_bound(int kind) {
   return kind == KIND_RBF ? 32.0f : kind == KIND_MATERN32 ? 256.0f : 512.0f;
 }
-// and the points from which its two more kernels pay (4000 points of 8
-// dimensions 53.8 -> 52.7 us, 10000 162 -> 126, 50000 3460 -> 1754).
+// and the points from which its two more kernels pay (8
+// dimensions, 3000 points 31 -> 35 us, 4000 40 -> 34, 10000 140 -> 95, 50000 3130 ->
+// 1640).
 constexpr int64_t kMmPoints = 4000;
 
 struct PgWork {
@@ -605,7 +611,7 @@ void point_gradient(Provider& pv, const float* Lf, const float* Rf, int ncols, f
                                     ((double)kernel_scale(pv.kind) * (double)pv.lengthscale(k)))
                           : 0.0f;
   const MmKernel mm = pv.n >= kMmPoints && pv.train.max_norm <= mm_norm_bound(pv.kind)
-                          ? pick_mm(pv.kind, pv.train.kb, pv.d)
+                          ? pick_mm(pv.kind, pv.train.kb, pv.d, pv.n)
                           : MmKernel{nullptr, 0, 0};
   pv.points_use.order(st);
   for (int c0 = 0; c0 < ncols; c0 += kPgCols) {
