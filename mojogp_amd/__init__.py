@@ -1,7 +1,9 @@
 """mojogp_amd — exact Gaussian-process engine for AMD Instinct MI355X (gfx950).
 
 Python + NumPy host surface over hand-written HIP kernels reached through the
-C-ABI library libmojogp_amd.so (ctypes).  No torch in the product path.
+C-ABI library libmojogp_amd.so (ctypes).  Nothing here imports torch;
+mojogp_amd.features (layers that learn a GP's inputs) works on the torch device
+tensors that its caller brings.
 
     from mojogp_amd import SingleOutputGP, MultiOutputGP, MultiOutputLMCGP, RBF, Matern52
 """

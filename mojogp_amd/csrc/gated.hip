@@ -802,7 +802,7 @@ struct FewArgs {
 // columns of both projections for 16 MT rows, its 8 waves share the reduction
 // and read their fragments from global memory, at any alignment.  Bound by
 // latency: one round of loads for a width of 512, one exchange through LDS
-// (bf16, one row x 512 -> 2048: 3.3 us for 4.2 MB of weights).
+// (bf16, one row x 512 -> 2048: 4.2 us for 4.2 MB of weights).
 template <class T, int ACT, int MT>
 __global__ __launch_bounds__(512) void k_gated_few(FewArgs s) {
   constexpr int N = Vec16<T>::N, W = 8;
