@@ -1088,7 +1088,7 @@ using SmallTile = Tile<T, 4, 4, 2, 2, TR, DUAL, PARTS>;
 // whole rounds of the device (512 small tiles or 256 big ones at a time), each
 // that of a tile's prologue and epilogue and of its stages (small, 4 / 7 / 16
 // stages: 7.1 / 11 / 19 us a round; big: 13.8 / 19 / 34), and the parts' sums at
-// 4.5 TB/s.  So 8192 rows x 1024 -> 1024 bf16 go by big tiles (33.9 us forward, 38.1
+// 4.5 TB/s.  So 8192 rows x 1024 -> 1024 bf16 go by big tiles (34.4 us forward, 38.1
 // by small ones), 12007 x 392 -> 1024 by small ones (33.1, 38.7); the weight
 // gradient of 4096 x 1024 -> 4096 by small ones in one part (70 us; big ones in two
 // 102, in four 143), that of 65536 rows by big ones in two.

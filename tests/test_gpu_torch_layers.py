@@ -186,6 +186,18 @@ def test_gated_layer_strides(kind, act, pad):
     _gated_check(args, dh, act, kind, biased=pad == 8)
 
 
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("width", [40, 128, 129])
+def test_gated_layer_many_tiles(kind, width):
+    """More large tiles than the device takes at a time, one, two and three steps
+    of the reduction each: rows from every tile."""
+    rng = np.random.default_rng(width)
+    x, *weights = _gated(rng, 32760, width, 1279, kind)
+    h = features.gated_layer(x, *weights)
+    _check(h[::37], ol.gated_layer(_host(x[::37]), *[_host(w) for w in weights]),
+           UNIT[kind] + F32, TYPES[kind])
+
+
 def test_gated_layer_directional_differences():
     """The gradients against differences of the forward pass itself."""
     rng = np.random.default_rng(3)
