@@ -129,20 +129,26 @@ __device__ __forceinline__ void store_run(T* p, int64_t left, const float* v) {
   }
 }
 
-// The two parts of scaled values: v scale = hi + lo to twice the type's bits, hi
-// at p and lo `apart` elements on.
-template <int N, class E>
-__device__ __forceinline__ void store_parts(E* p, int64_t apart, int64_t left, float scale,
-                                            const float* v) {
-  float hi[N], lo[N];
+// The P parts of values, each what the ones before leave, rounded to the type:
+// the first at p, the others `apart` elements on each.  Only the last takes
+// infinities and NaN (and what bfloat16 would round to infinity), so that no
+// difference of infinities is formed and a product meets them once.
+template <int P, int N, class E>
+__device__ __forceinline__ void store_parts(E* p, int64_t apart, int64_t left, const float* v) {
+  constexpr float kMost = std::is_same<E, __bf16>::value ? 3.3895313892515355e38f : 65504.0f;
+  float rest[N], part[N];
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    const float x = v[k] * scale;
-    hi[k] = (float)(E)x;
-    lo[k] = x - hi[k];
+  for (int k = 0; k < N; ++k) rest[k] = v[k];
+#pragma unroll
+  for (int i = 0; i < P - 1; ++i) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      part[k] = (float)(E)fminf(fmaxf(rest[k], -kMost), kMost);
+      rest[k] -= part[k];
+    }
+    store_run<N>(p + i * apart, left, part);
   }
-  store_run<N>(p, left, hi);
-  store_run<N>(p + apart, left, lo);
+  store_run<N>(p + (P - 1) * apart, left, rest);
 }
 
 // ---------------------------------------------------------------- product core
@@ -195,8 +201,34 @@ struct GemmShape {
   int64_t K;          // reduction length
   int64_t tiles_p, tiles_q;
   int64_t k_split;    // reduction elements of one split (a multiple of a stage)
-  int64_t p_lo, q_lo; // operands in parts: byte distance of the low parts from the high ones
+  int64_t p_apart, q_apart; // operands in parts: byte distance of one part from the next
 };
+
+// The products a sum is made of where operands come in parts: the parts of p and
+// q of each, in order.  6: both in three parts; the smallest products first, so that
+// the larger ones alone meet the rounding of the whole sum, and without those
+// below 2^-25 of the largest.  2: q in two.
+template <int PARTS>
+struct PartOrder {
+  static constexpr int p[1] = {0}, q[1] = {0};
+};
+template <>
+struct PartOrder<2> {
+  static constexpr int p[2] = {0, 0}, q[2] = {0, 1};
+};
+template <>
+struct PartOrder<6> {
+  static constexpr int p[6] = {2, 0, 1, 1, 0, 0}, q[6] = {0, 2, 1, 0, 1, 0};
+};
+// how many parts on the next product's operand lies, 4 bits a step, 2 for none
+template <int PARTS>
+constexpr uint32_t part_steps(bool of_p) {
+  using O = PartOrder<PARTS>;
+  uint32_t v = 0;
+  for (int i = 0; i + 1 < PARTS; ++i)
+    v |= (uint32_t)((of_p ? O::p[i + 1] - O::p[i] : O::q[i + 1] - O::q[i]) + 2) << (4 * i);
+  return v;
+}
 
 // Tile of 16 TN WN columns (p rows) by 16 TM WM rows (q rows), one wave 16 TN
 // by 16 TM of it.  NT: the p rows are dealt to LDS so that a lane's results are
@@ -211,8 +243,7 @@ struct Tile {
   using Elem = T;
   static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_;
   static constexpr bool TR = TR_, DUAL = DUAL_;
-  static constexpr int PARTS = PARTS_;  // products a sum is made of: 3 of two operands in two parts
-                                        // each, 2 of q in two parts, 1
+  static constexpr int PARTS = PARTS_;  // products a sum is made of (PartOrder)
   static constexpr int W = WM * WN, THREADS = 64 * W;
   static constexpr int BQ = 16 * TM * WM, BP = 16 * TN * WN;
   static constexpr int T1 = DUAL ? TN / 2 : TN;  // 16-row tiles of one matrix a wave
@@ -238,7 +269,7 @@ struct Loader {
   int soff[I];           // bytes from the side's base to the instruction's start
   const char* base[3];   // of p, of q, of p's second matrix
   int64_t step[2];       // bytes of a stage
-  int64_t jump[2][2];    // bytes to the next part product's start, after a part's stages
+  int64_t apart[2], back[2];  // bytes from one part to the next, and of a part's stages
   int64_t length, left;  // reduction elements of a part, and those still to load
   int part;
 
@@ -254,17 +285,14 @@ struct Loader {
     step[1] = TL::TR ? TL::KS * s.q.ld_bytes : TL::SB;
     length = left = K;
     if constexpr (TL::PARTS > 1) {
-      const int64_t back_p = (K + TL::KS - 1) / TL::KS * step[0];
-      const int64_t back_q = (K + TL::KS - 1) / TL::KS * step[1];
-      if constexpr (TL::PARTS == 3) {  // p: high, low, high; q: high, high, low
-        jump[0][0] = s.p_lo - back_p;
-        jump[0][1] = -s.p_lo - back_p;
-        jump[1][0] = -back_q;
-        jump[1][1] = s.q_lo - back_q;
-      } else {  // p twice; q: high, low
-        jump[0][0] = -back_p;
-        jump[1][0] = s.q_lo - back_q;
-      }
+      apart[0] = s.p_apart;
+      apart[1] = s.q_apart;
+      back[0] = (K + TL::KS - 1) / TL::KS * step[0];
+      back[1] = (K + TL::KS - 1) / TL::KS * step[1];
+      using O = PartOrder<TL::PARTS>;
+      base[0] += O::p[0] * apart[0];
+      base[1] += O::q[0] * apart[1];
+      if constexpr (second(1)) base[2] += O::p[0] * apart[0];
       part = 0;
     }
   }
@@ -339,7 +367,11 @@ struct Loader {
     for (int b = 0; b < (second(1) ? 3 : 2); ++b) {
       base[b] += step[b & 1];
       if constexpr (TL::PARTS > 1) {
-        if (turn) base[b] += TL::PARTS == 3 && part ? jump[b & 1][1] : jump[b & 1][0];
+        if (turn) {
+          const uint32_t steps = b & 1 ? part_steps<TL::PARTS>(false) : part_steps<TL::PARTS>(true);
+          const int64_t on = (int)(steps >> (4 * part) & 15) - 2;
+          base[b] += on * apart[b & 1] - back[b & 1];
+        }
       }
     }
     if (turn) {
@@ -494,18 +526,9 @@ __global__ __launch_bounds__(TL::THREADS) void k_gemm(GemmShape s, EPI epi) {
 
 // ---------------------------------------------------------------- epilogues
 
-// What the sums of a product are multiplied by: one, or (fp32 operands in scaled
-// fp16 parts) the power of two that undoes the parts' scales, which the packing
-// left on the device.
-struct Unscale {
-  const float* p;
-  __device__ __forceinline__ float get() const { return p ? *p : 1.0f; }
-};
-
 template <class T, int ACT>
 struct ForwardEpi {
   static constexpr bool FORWARD = true;
-  Unscale scale;
   const T *bg, *bu;
   T* h;
   int64_t ldh, rows, hidden;
@@ -516,7 +539,6 @@ struct ForwardEpi {
     const int lane = threadIdx.x & 63;
     const int64_t f = n0 + N * (lane >> 4), left = hidden - f;
     if (left <= 0) return;
-    const float sc = scale.get();
     float g0[N], u0[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) g0[k] = u0[k] = 0.0f;
@@ -530,8 +552,8 @@ struct ForwardEpi {
 #pragma unroll
       for (int k = 0; k < N; ++k) {
         float a, slope;
-        activate<ACT, sizeof(T) == 2>(fmaf(acc[m][k / 4][k % 4], sc, g0[k]), a, slope);
-        o[k] = a * fmaf(acc[m][TL::T1 + k / 4][k % 4], sc, u0[k]);
+        activate<ACT, sizeof(T) == 2>(acc[m][k / 4][k % 4] + g0[k], a, slope);
+        o[k] = a * (acc[m][TL::T1 + k / 4][k % 4] + u0[k]);
       }
       store_run<N>(h + r * ldh + f, left, o);
     }
@@ -540,11 +562,10 @@ struct ForwardEpi {
 
 // dgu[row] = [dg | du], each `pad` columns (zeros past hidden);
 // dbias[part][2][hidden] the column sums over a wave's rows.
-// SPLIT: two parts of the scaled values, the low ones after the high ones of a row.
-template <class T, class E, int ACT, bool SPLIT>
+// In COPIES parts: [dg | du] of the first, then of the others.
+template <class T, class E, int ACT, int COPIES>
 struct BackwardEpi {
   static constexpr bool FORWARD = false;
-  Unscale scale, dgu_scale;  // dgu_scale: what dg and du are multiplied by
   const T *bg, *bu;
   const T* dh;
   int64_t lddh, rows, hidden, pad;
@@ -556,7 +577,6 @@ struct BackwardEpi {
     constexpr int N = TL::RUN;
     const int lane = threadIdx.x & 63;
     const int64_t f = n0 + N * (lane >> 4), left = hidden - f;
-    const float sc = scale.get(), ds = dgu_scale.get();
     float g0[N], u0[N], sg[N], su[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) g0[k] = u0[k] = sg[k] = su[k] = 0.0f;
@@ -573,23 +593,17 @@ struct BackwardEpi {
 #pragma unroll
       for (int k = 0; k < N; ++k) {
         float a, slope;
-        activate<ACT, sizeof(T) == 2>(fmaf(acc[m][k / 4][k % 4], sc, g0[k]), a, slope);
+        activate<ACT, sizeof(T) == 2>(acc[m][k / 4][k % 4] + g0[k], a, slope);
         // columns past hidden are products of the last weights: cut off
         const bool in = k < left;
-        dg[k] = in ? d[k] * fmaf(acc[m][TL::T1 + k / 4][k % 4], sc, u0[k]) * slope : 0.0f;
+        dg[k] = in ? d[k] * (acc[m][TL::T1 + k / 4][k % 4] + u0[k]) * slope : 0.0f;
         du[k] = in ? d[k] * a : 0.0f;
         sg[k] += dg[k];
         su[k] += du[k];
       }
-      if constexpr (SPLIT) {
-        E* row = static_cast<E*>(dgu) + r * 4 * pad + f;
-        store_parts<N>(row, 2 * pad, pad - f, ds, dg);
-        store_parts<N>(row + pad, 2 * pad, pad - f, ds, du);
-      } else {
-        E* row = static_cast<E*>(dgu) + r * 2 * pad + f;
-        store_run<N>(row, pad - f, dg);
-        store_run<N>(row + pad, pad - f, du);
-      }
+      E* row = static_cast<E*>(dgu) + r * 2 * COPIES * pad + f;
+      store_parts<COPIES, N>(row, 2 * pad, pad - f, dg);
+      store_parts<COPIES, N>(row + pad, 2 * pad, pad - f, du);
     }
     if (dbias) {
 #pragma unroll
@@ -612,7 +626,6 @@ struct BackwardEpi {
 template <class T>
 struct StoreEpi {
   static constexpr bool FORWARD = false;
-  Unscale scale;
   T* out;
   float* part;
   int64_t rows, cols;
@@ -623,14 +636,13 @@ struct StoreEpi {
     const int lane = threadIdx.x & 63;
     const int64_t c = n0 + N * (lane >> 4);
     if (c >= cols) return;
-    const float sc = scale.get();
 #pragma unroll
     for (int m = 0; m < TL::TM; ++m) {
       const int64_t r = m0 + m * 16 + (lane & 15);
       if (r >= rows) continue;
       float o[N];
 #pragma unroll
-      for (int k = 0; k < N; ++k) o[k] = acc[m][k / 4][k % 4] * sc;
+      for (int k = 0; k < N; ++k) o[k] = acc[m][k / 4][k % 4];
       if (part)
         store_run<N>(part + ((int64_t)blockIdx.y * rows + r) * cols + c, cols - c, o);
       else
@@ -644,7 +656,6 @@ struct StoreEpi {
 template <class T>
 struct WeightEpi {
   static constexpr bool FORWARD = false;
-  Unscale scale;
   T *dw_gate, *dw_up;
   float* part;
   int64_t hidden, pad, width;
@@ -652,7 +663,6 @@ struct WeightEpi {
   __device__ __forceinline__ void run(f4 (&acc)[TL::TM][TL::TN], int64_t m0, int64_t n0,
                                       int64_t) const {
     const int lane = threadIdx.x & 63;
-    const float sc = scale.get();
 #pragma unroll
     for (int m = 0; m < TL::TM; ++m) {
       const int64_t r = m0 + m * 16 + (lane & 15);
@@ -663,7 +673,7 @@ struct WeightEpi {
       for (int n = 0; n < TL::TN; ++n) {
         const int64_t c = n0 + n * 16 + 4 * (lane >> 4);
         if (c >= width) continue;
-        float o[4] = {acc[m][n][0] * sc, acc[m][n][1] * sc, acc[m][n][2] * sc, acc[m][n][3] * sc};
+        const float o[4] = {acc[m][n][0], acc[m][n][1], acc[m][n][2], acc[m][n][3]};
         if (part) {
           store_run<4>(part + (((int64_t)blockIdx.y * 2 + up) * hidden + f) * width + c, width - c,
                        o);
@@ -873,194 +883,62 @@ __global__ __launch_bounds__(512) void k_gated_few(FewArgs s) {
   store_run<4>(static_cast<T*>(s.h) + r * s.ldh + c, left, o);
 }
 
-// ---------------------------------------------------------------- fp32 operands in fp16 parts
-
-// What the scales are made from, per tensor (x, both weights, dh): the largest
-// finite |value| and (a bound on) the largest 2-norm of a row.  Non-finite
-// values are left out, so that they spoil their own rows only.
-struct Stat {
-  float amax, norm;
-};
-enum : int { ST_X = 0, ST_W = 1, ST_DH = 2, kStats = 3 };
-constexpr int kStatBlocks = 512;  // partial results a tensor
-
-struct StatSource {
-  const float* p[2];
-  int64_t ld[2], rows, cols;  // rows of each of the matrices
-};
-struct StatSources {
-  StatSource s[kStats];
-};
-
-__device__ __forceinline__ Stat join(Stat a, Stat b) {
-  return {fmaxf(a.amax, b.amax), fmaxf(a.norm, b.norm)};
-}
-
-__device__ __forceinline__ Stat wave_join(Stat a) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1)
-    a = join(a, Stat{__shfl_xor(a.amax, o), __shfl_xor(a.norm, o)});
-  return a;
-}
-
-// part[tensor][block]: 16 lanes a row, so that few exchanges end a row and many
-// rows are in flight
-__global__ __launch_bounds__(256) void k_stats(StatSources src, Stat* __restrict__ part) {
-  __shared__ Stat red[4];
-  const StatSource& s = src.s[blockIdx.y];
-  const int lane = threadIdx.x & 15, group = threadIdx.x >> 4;
-  Stat all{0.0f, 0.0f};
-  const int64_t rows = s.p[1] ? 2 * s.rows : s.rows;
-  for (int64_t r = (int64_t)blockIdx.x * 16 + group; r < rows; r += kStatBlocks * 16) {
-    const bool second = r >= s.rows;
-    const float* p = second ? s.p[1] + (r - s.rows) * s.ld[1] : s.p[0] + r * s.ld[0];
-    float sum = 0.0f, big = 0.0f;
-#pragma unroll 4
-    for (int64_t c = 4 * lane; c < s.cols; c += 64) {
-      float v[4];
-      load_run<4>(p + c, s.cols - c, v);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float a = fabsf(v[k]);
-        big = a < INFINITY ? fmaxf(big, a) : big;
-        sum = fmaf(v[k], v[k], sum);
-      }
-    }
-#pragma unroll
-    for (int o = 8; o >= 1; o >>= 1) {
-      sum += __shfl_xor(sum, o);
-      big = fmaxf(big, __shfl_xor(big, o));
-    }
-    // squares that overflow, or a row with non-finite values
-    all = join(all, Stat{big, sum < INFINITY ? sqrtf(sum) : sqrtf((float)s.cols) * big});
-  }
-  all = wave_join(all);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = all;
-  __syncthreads();
-  if (threadIdx.x != 0) return;
-  for (int k = 1; k < 4; ++k) all = join(all, red[k]);
-  part[blockIdx.y * kStatBlocks + blockIdx.x] = all;
-}
-
-// The scales, powers of two, and the factors that undo them.
-struct Scales {
-  float x, w, d;          // of x, the weights, dg and du
-  float fwd, dx, dw;      // 1 / (x w), 1 / (d w), 1 / (d x)
-};
-
-__device__ __forceinline__ float pow2_below(float bound) {
-  // the largest 2^e with 2^e bound < 2^15
-  if (!(bound > 0.0f)) return 1.0f;
-  return ldexpf(1.0f, min(max(14 - ilogbf(fminf(bound, 3.0e38f)), -120), 120));
-}
-
-// Two fp16 parts hold 22 bits of a value down to 2^-17 of the largest; below,
-// the error stays 2^-40 of the largest.  dg and du are written by the kernel
-// that forms them, before their largest is known: their scale follows from
-// |u|, |g| <= |x| |w| + |b|, |dg| <= 1.13 |dh| |u| and |du| <= |dh| |act(g)|,
-// |act(g)| <= |g| (act_max 0) or 1 (the sigmoid), some five binades above what
-// occurs.
-__device__ __forceinline__ Scales make_scales(const Stat* part, int lane, float bmax,
-                                              float act_max) {
-  auto whole = [&](int tensor) {
-    Stat s{0.0f, 0.0f};
-#pragma unroll
-    for (int b = 0; b < kStatBlocks; b += 64) s = join(s, part[tensor * kStatBlocks + b + lane]);
-    return wave_join(s);
-  };
-  const Stat x = whole(ST_X), w = whole(ST_W), d = whole(ST_DH);
-  Scales s;
-  s.x = pow2_below(x.amax);
-  s.w = pow2_below(w.amax);
-  s.d = pow2_below(1.2f * d.amax * fmaxf(fmaf(x.norm, w.norm, bmax), act_max));
-  s.fwd = (1.0f / s.x) * (1.0f / s.w);
-  s.dx = (1.0f / s.d) * (1.0f / s.w);
-  s.dw = (1.0f / s.d) * (1.0f / s.x);
-  return s;
-}
-
-__device__ __forceinline__ float largest_bias(const float* bg, const float* bu, int64_t n,
-                                              int lane) {
-  float b = 0.0f;
-  for (int64_t i = lane; i < n; i += 64) {
-    const float g = bg ? fabsf(bg[i]) : 0.0f, u = bu ? fabsf(bu[i]) : 0.0f;
-    b = fmaxf(b, g < INFINITY ? g : 0.0f);
-    b = fmaxf(b, u < INFINITY ? u : 0.0f);
-  }
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) b = fmaxf(b, __shfl_xor(b, o));
-  return b;
-}
+// ---------------------------------------------------------------- fp32 operands in bf16 parts
 
 struct SplitSource {
-  const float *x, *wg, *wu, *bg, *bu;
+  const float *x, *wg, *wu;
   int64_t ldx, ldg, ldu, rows, hidden, width, wpad;
-  _Float16 *dx, *dwg, *dwu;  // [rows][2 wpad]: high parts, then low ones
-  const Stat* part;
-  float act_max;
-  Scales* scales;
+  __bf16 *dx, *dwg, *dwu;  // [rows][kSplit][wpad]
 };
+constexpr int kSplit = 3;
 
-// Every workgroup forms the scales from the partial statistics; the first one
-// leaves them for the kernels to come.
 __global__ __launch_bounds__(256) void k_split(SplitSource s) {
-  __shared__ Scales sc;
-  if (threadIdx.x < 64) {
-    const float b = blockIdx.x == 0 ? largest_bias(s.bg, s.bu, s.hidden, threadIdx.x) : 0.0f;
-    const Scales v = make_scales(s.part, threadIdx.x, b, s.act_max);
-    if (threadIdx.x == 0) {
-      sc = v;
-      if (blockIdx.x == 0) *s.scales = v;
-    }
-  }
-  __syncthreads();
   const int64_t per = s.wpad / 8, total = (s.rows + 2 * s.hidden) * per;
   for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total;
        q += (int64_t)gridDim.x * 256) {
     int64_t r = q / per;
     const int64_t c = (q - r * per) * 8;
     const float* src;
-    _Float16* dst;
-    float scale = sc.w;
+    __bf16* dst;
     if (r < s.rows) {
       src = s.x + r * s.ldx;
-      dst = s.dx + r * 2 * s.wpad;
-      scale = sc.x;
+      dst = s.dx;
     } else if ((r -= s.rows) < s.hidden) {
       src = s.wg + r * s.ldg;
-      dst = s.dwg + r * 2 * s.wpad;
+      dst = s.dwg;
     } else {
       r -= s.hidden;
       src = s.wu + r * s.ldu;
-      dst = s.dwu + r * 2 * s.wpad;
+      dst = s.dwu;
     }
     float v[8];
     load_run<8>(src + c, s.width - c, v);
-    store_parts<8>(dst + c, s.wpad, 8, scale, v);
+    store_parts<kSplit, 8>(dst + r * kSplit * s.wpad + c, s.wpad, 8, v);
   }
 }
 
-// dst[k][part pad + f] = the high part of W_part[f][k], 2 pad on the low one
-__global__ __launch_bounds__(256) void k_transpose_split(const _Float16* __restrict__ wg,
-                                                         const _Float16* __restrict__ wu,
+// dst[k][part][pad of the gate, pad of up] = parts of W[f][k]
+__global__ __launch_bounds__(256) void k_transpose_split(const __bf16* __restrict__ wg,
+                                                         const __bf16* __restrict__ wu,
                                                          int64_t hidden, int64_t width,
                                                          int64_t wpad, int64_t pad,
-                                                         _Float16* __restrict__ dst) {
-  __shared__ _Float16 tile[32][34];
+                                                         __bf16* __restrict__ dst) {
+  __shared__ __bf16 tile[32][34];
   const int64_t f0 = (int64_t)blockIdx.x * 32, k0 = (int64_t)blockIdx.y * 32;
-  const int up = blockIdx.z & 1, low = blockIdx.z >> 1;
-  const _Float16* w = (up ? wu : wg) + low * wpad;
+  const int up = blockIdx.z & 1, part = blockIdx.z >> 1;
+  const __bf16* w = (up ? wu : wg) + part * wpad;
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
 #pragma unroll
   for (int i = 0; i < 32; i += 8) {
     const int64_t f = f0 + ty + i, k = k0 + tx;
-    tile[ty + i][tx] = f < hidden && k < width ? w[f * 2 * wpad + k] : (_Float16)0.0f;
+    tile[ty + i][tx] = f < hidden && k < width ? w[f * kSplit * wpad + k] : (__bf16)0.0f;
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 32; i += 8) {
     const int64_t k = k0 + ty + i, f = f0 + tx;
-    if (k < width && f < pad) dst[k * 4 * pad + low * 2 * pad + up * pad + f] = tile[tx][ty + i];
+    if (k < width && f < pad)
+      dst[k * kSplit * 2 * pad + part * 2 * pad + up * pad + f] = tile[tx][ty + i];
   }
 }
 
@@ -1121,11 +999,14 @@ inline Cut cut_product(int64_t p_rows, int64_t q_rows, int64_t stages, int64_t p
 }
 constexpr int64_t kMaxSplits = 64;
 
-// fp32 layers go through the fp16 matrix cores in two parts of 11 bits a value
-// and three products (the low parts' own product is below 2^-22): three times
-// the work at nine times the rate of the fp32 instructions, 24 against 128
-// cycles a reduction element of a tile.  Forming the parts takes two more
-// kernels.  20000 x 256 -> 512, both passes: 494 -> 330 us.
+// fp32 layers go through the bf16 matrix cores: three parts of 8 bits hold a
+// value's 24 whatever its size beside the others', as bf16 has the range of fp32
+// (below 2^-100 the last part is lost), and six products make the sum, those left
+// out being below 2^-25 of it.  Six times the work at 16 times the rate of the fp32
+// instructions.  20000 x 256 -> 512, both passes: 494 us by fp32 instructions, 465
+// so, 2.4e-7 off; two fp16 parts and three products take 320, but a common scale
+// then ties every row to the largest value of all, and a scale a row still ties
+// the columns of a row to its largest.
 
 // The 16-bit types' dg and du are rounded to the type for the last two products;
 // with few rows the roundings do not average out, and dx's and the weight
@@ -1142,17 +1023,18 @@ template <class T, int MODE_>
 struct Plan {
   static constexpr int MODE = MODE_;
   static constexpr bool SPLIT = MODE == FP32_PARTS;
-  using E = typename std::conditional<SPLIT, _Float16, T>::type;  // what the products take
+  using E = typename std::conditional<SPLIT, __bf16, T>::type;  // what the products take
   // products of the projections and of the gradients; copies of x and the
   // weights, and of dg and du
-  static constexpr int PARTS = SPLIT ? 3 : 1, GRAD_PARTS = SPLIT ? 3 : MODE == FEW_ROWS ? 2 : 1;
-  static constexpr int COPIES = SPLIT ? 2 : 1, D_COPIES = MODE == PLAIN ? 1 : 2;
+  static constexpr int PARTS = SPLIT ? 6 : 1, GRAD_PARTS = SPLIT ? 6 : MODE == FEW_ROWS ? 2 : 1;
+  static constexpr int COPIES = SPLIT ? kSplit : 1;
+  static constexpr int D_COPIES = SPLIT ? kSplit : MODE == FEW_ROWS ? 2 : 1;
   // width and hidden rounded to whole 16-byte chunks, or to whole stages
   static constexpr int WQ = SPLIT ? 64 : Vec16<T>::N, HQ = SPLIT ? 32 : Vec16<T>::N;
   int64_t wpad, hpad;
   bool pack_x, pack_w;
   size_t x_off = 0, wg_off = 0, wu_off = 0, wt_off = 0, dgu_off = 0, dbias_off = 0, part_off = 0;
-  size_t stat_off = 0, scale_off = 0, dxp_off = 0;
+  size_t dxp_off = 0;
   size_t bytes = 0;
   bool big_dual = false;
   Cut dx, dw;
@@ -1173,10 +1055,6 @@ struct Plan {
     if (pack_w) {
       wg_off = take((size_t)a.hidden * wpad * COPIES * sizeof(E));
       wu_off = take((size_t)a.hidden * wpad * COPIES * sizeof(E));
-    }
-    if (SPLIT) {
-      stat_off = take(kStats * kStatBlocks * sizeof(Stat));
-      scale_off = take(sizeof(Scales));
     }
     const int64_t rows = std::max<int64_t>(a.rows, 1);
     constexpr int64_t KS = 128 / sizeof(E);
@@ -1205,37 +1083,25 @@ template <class E>
 struct Inputs {
   const E *x, *wg, *wu;
   int64_t ldx, ldw;
-  const Scales* scales;
 };
-
-inline Unscale pick(const Scales* s, float Scales::*m) { return {s ? &(s->*m) : nullptr}; }
 
 // x and the weights as the product kernel loads them.
 template <class T, int MODE>
 Inputs<typename Plan<T, MODE>::E> load_inputs(const GatedArgs& a, const Plan<T, MODE>& pl,
-                                              const void* dh, int64_t dh_stride, char* ws,
-                                              hipStream_t st) {
+                                              char* ws, hipStream_t st) {
   using E = typename Plan<T, MODE>::E;
   E *x = reinterpret_cast<E*>(ws + pl.x_off), *wg = reinterpret_cast<E*>(ws + pl.wg_off),
     *wu = reinterpret_cast<E*>(ws + pl.wu_off);
   if constexpr (MODE == FP32_PARTS) {
-    Stat* part = reinterpret_cast<Stat*>(ws + pl.stat_off);
-    Scales* scales = reinterpret_cast<Scales*>(ws + pl.scale_off);
     auto f = [](const void* p) { return static_cast<const float*>(p); };
-    StatSources src;
-    src.s[ST_X] = {{f(a.x), nullptr}, {a.x_stride, 0}, a.rows, a.width};
-    src.s[ST_W] = {{f(a.w_gate), f(a.w_up)}, {a.w_gate_stride, a.w_up_stride}, a.hidden, a.width};
-    src.s[ST_DH] = {{f(dh), nullptr}, {dh_stride, 0}, dh ? a.rows : 0, a.hidden};
-    k_stats<<<dim3(kStatBlocks, kStats), 256, 0, st>>>(src, part);
     const int64_t items = (a.rows + 2 * a.hidden) * (pl.wpad / 8);
-    k_split<<<(unsigned)std::min<int64_t>(ceil_div(items, (int64_t)256), 4096), 256, 0, st>>>(
-        {f(a.x), f(a.w_gate), f(a.w_up), f(a.b_gate), f(a.b_up), a.x_stride, a.w_gate_stride,
-         a.w_up_stride, a.rows, a.hidden, a.width, pl.wpad, x, wg, wu, part,
-         a.activation == ACT_SIGMOID ? 1.0f : 0.0f, scales});
-    return {x, wg, wu, 2 * pl.wpad, 2 * pl.wpad, scales};
+    k_split<<<(unsigned)std::min<int64_t>(ceil_div(items, (int64_t)256), 8192), 256, 0, st>>>(
+        {f(a.x), f(a.w_gate), f(a.w_up), a.x_stride, a.w_gate_stride, a.w_up_stride, a.rows,
+         a.hidden, a.width, pl.wpad, x, wg, wu});
+    return {x, wg, wu, kSplit * pl.wpad, kSplit * pl.wpad};
   } else {
     Inputs<E> in{static_cast<const T*>(a.x), static_cast<const T*>(a.w_gate),
-                 static_cast<const T*>(a.w_up), a.x_stride, a.w_gate_stride, nullptr};
+                 static_cast<const T*>(a.w_up), a.x_stride, a.w_gate_stride};
     PackSource<T> p{};
     p.cols = a.width;
     p.pad = pl.wpad;
@@ -1301,7 +1167,7 @@ void launch_dual(const GatedArgs& a, const PL& pl, const Inputs<typename PL::E>&
   s.p = operand(in.wg, in.ldw, a.hidden, in.wu);
   s.q = operand(in.x, in.ldx, a.rows);
   s.K = s.k_split = pl.wpad;
-  s.p_lo = s.q_lo = pl.wpad * (int64_t)sizeof(typename PL::E);
+  s.p_apart = s.q_apart = pl.wpad * (int64_t)sizeof(typename PL::E);
   launch_product<PL, false, true>(pl.big_dual, s, 1, epi, st);
 }
 
@@ -1317,8 +1183,8 @@ void dispatch_act(int act, F&& f) {
 
 // Forward passes by k_gated_few: up to this many of its workgroups it is the
 // faster one.  16 bits: 512 rows x 256 -> 1024 (512 workgroups) 5.6 against 6.1 us,
-// 1024 rows 9.1 against 6.3; fp32, against the three-part product and its two
-// kernels before it: 512 x 256 -> 1024 9.9 against ~20, 1024 rows 19 against 22.
+// 1024 rows 9.1 against 6.3; fp32, by fp32 instructions against the six products
+// and the kernel before them: 512 x 256 -> 1024 9.9 us, 1024 rows 19.
 inline bool takes_few(const GatedArgs& a) {
   return ceil_div(a.rows, (int64_t)64) * ceil_div(a.hidden, (int64_t)16) <=
          (a.type == ELEM_F32 ? 768 : 512);
@@ -1378,10 +1244,9 @@ void gated_forward(const GatedArgs& a, void* h, int64_t h_stride, void* ws, hipS
   dispatch_layer(a, false, [&](auto tag, auto mode) {
     using T = decltype(tag);
     const Plan<T, mode.value> pl(a, false);
-    const auto in = load_inputs(a, pl, nullptr, 0, static_cast<char*>(ws), st);
+    const auto in = load_inputs(a, pl, static_cast<char*>(ws), st);
     dispatch_act(a.activation, [&](auto act) {
-      ForwardEpi<T, act.value> epi{pick(in.scales, &Scales::fwd),
-                                   static_cast<const T*>(a.b_gate),
+      ForwardEpi<T, act.value> epi{static_cast<const T*>(a.b_gate),
                                    static_cast<const T*>(a.b_up),
                                    static_cast<T*>(h),
                                    h_stride,
@@ -1408,33 +1273,31 @@ void gated_backward(const GatedArgs& a, const void* dh, int64_t dh_stride, const
       return;
     }
     const PL pl(a, true);
-    const Inputs<E> in = load_inputs(a, pl, dh, dh_stride, ws, st);
+    const Inputs<E> in = load_inputs(a, pl, ws, st);
     E* dgu = reinterpret_cast<E*>(ws + pl.dgu_off);
     float* dbias = dbg || dbu ? reinterpret_cast<float*>(ws + pl.dbias_off) : nullptr;
     dispatch_act(a.activation, [&](auto act) {
-      BackwardEpi<T, E, act.value, PL::D_COPIES == 2> epi{pick(in.scales, &Scales::fwd),
-                                                          pick(in.scales, &Scales::d),
-                                                          static_cast<const T*>(a.b_gate),
-                                                          static_cast<const T*>(a.b_up),
-                                                          static_cast<const T*>(dh),
-                                                          dh_stride,
-                                                          a.rows,
-                                                          a.hidden,
-                                                          pl.hpad,
-                                                          dgu,
-                                                          dbias};
+      BackwardEpi<T, E, act.value, PL::D_COPIES> epi{static_cast<const T*>(a.b_gate),
+                                                     static_cast<const T*>(a.b_up),
+                                                     static_cast<const T*>(dh),
+                                                     dh_stride,
+                                                     a.rows,
+                                                     a.hidden,
+                                                     pl.hpad,
+                                                     dgu,
+                                                     dbias};
       launch_dual(a, pl, in, epi, st);
     });
     if (dbias)
       k_sum_bias<T><<<(unsigned)ceil_div(2 * a.hidden, (int64_t)64), 1024, 0, st>>>(
           dbias, pl.bias_parts, a.hidden, dbg, dbu);
-    const int64_t lo = 2 * pl.hpad * (int64_t)sizeof(E);
+    const int64_t apart = 2 * pl.hpad * (int64_t)sizeof(E);
     if (g.dx) {
       E* wt = reinterpret_cast<E*>(ws + pl.wt_off);
       const unsigned gx = (unsigned)ceil_div(pl.hpad, (int64_t)32);
       const unsigned gy = (unsigned)ceil_div(a.width, (int64_t)32);
       if constexpr (PL::SPLIT)
-        k_transpose_split<<<dim3(gx, gy, 4), 256, 0, st>>>(in.wg, in.wu, a.hidden, a.width,
+        k_transpose_split<<<dim3(gx, gy, 2 * kSplit), 256, 0, st>>>(in.wg, in.wu, a.hidden, a.width,
                                                            pl.wpad, pl.hpad, wt);
       else
         k_transpose_weights<T><<<dim3(gx, gy, 2), 256, 0, st>>>(in.wg, in.wu, in.ldw, a.hidden,
@@ -1444,12 +1307,12 @@ void gated_backward(const GatedArgs& a, const void* dh, int64_t dh_stride, const
       s.q = operand(dgu, pl.ldd(), a.rows);
       s.K = 2 * pl.hpad;
       s.k_split = PL::reduction(pl.dx);
-      s.p_lo = s.q_lo = lo;
+      s.p_apart = s.q_apart = apart;
       T* dx = static_cast<T*>(g.dx);
       float* part = pl.dx.splits > 1 ? reinterpret_cast<float*>(ws + pl.dxp_off) : nullptr;
       launch_product<PL, false, false>(
           pl.dx.big, s, pl.dx.splits,
-          StoreEpi<T>{pick(in.scales, &Scales::dx), dx, part, a.rows, a.width}, st);
+          StoreEpi<T>{dx, part, a.rows, a.width}, st);
       if (part) sum_parts<T>(part, pl.dx.splits, a.rows * a.width, 1, dx, nullptr, st);
     }
     if (dwg || dwu) {
@@ -1459,11 +1322,10 @@ void gated_backward(const GatedArgs& a, const void* dh, int64_t dh_stride, const
       s.q = operand(static_cast<const E*>(dgu), pl.ldd(), 2 * pl.hpad);
       s.K = a.rows;
       s.k_split = PL::reduction(pl.dw);
-      s.p_lo = pl.wpad * (int64_t)sizeof(E);
-      s.q_lo = lo;
+      s.p_apart = pl.wpad * (int64_t)sizeof(E);
+      s.q_apart = apart;
       launch_product<PL, true, false>(pl.dw.big, s, pl.dw.splits,
-                                      WeightEpi<T>{pick(in.scales, &Scales::dw), dwg, dwu, part,
-                                                   a.hidden, pl.hpad, a.width},
+                                      WeightEpi<T>{dwg, dwu, part, a.hidden, pl.hpad, a.width},
                                       st);
       if (part) sum_parts<T>(part, pl.dw.splits, a.hidden * a.width, 2, dwg, dwu, st);
     }
