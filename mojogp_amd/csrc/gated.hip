@@ -562,10 +562,13 @@ struct ForwardEpi {
 
 // dgu[row] = [dg | du], each `pad` columns (zeros past hidden);
 // dbias[part][2][hidden] the column sums over a wave's rows.
-// In COPIES parts: [dg | du] of the first, then of the others.
+// In COPIES parts: [dg | du] of the first, then of the others.  float16: times the
+// row's scale.
 template <class T, class E, int ACT, int COPIES>
 struct BackwardEpi {
   static constexpr bool FORWARD = false;
+  static constexpr bool SCALED = std::is_same<E, _Float16>::value;
+  const float* scale;  // of each row
   const T *bg, *bu;
   const T* dh;
   int64_t lddh, rows, hidden, pad;
@@ -601,6 +604,14 @@ struct BackwardEpi {
         sg[k] += dg[k];
         su[k] += du[k];
       }
+      if constexpr (SCALED) {
+        const float sc = scale[r];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          dg[k] *= sc;
+          du[k] *= sc;
+        }
+      }
       E* row = static_cast<E*>(dgu) + r * 2 * COPIES * pad + f;
       store_parts<COPIES, N>(row, 2 * pad, pad - f, dg);
       store_parts<COPIES, N>(row + pad, 2 * pad, pad - f, du);
@@ -622,10 +633,12 @@ struct BackwardEpi {
   }
 };
 
-// One split: the result; more: part[split][rows][cols] sums.
+// One split: the result; more: part[split][rows][cols] sums.  scale: that of each
+// row, to be undone, or null.
 template <class T>
 struct StoreEpi {
   static constexpr bool FORWARD = false;
+  const float* scale;
   T* out;
   float* part;
   int64_t rows, cols;
@@ -643,6 +656,11 @@ struct StoreEpi {
       float o[N];
 #pragma unroll
       for (int k = 0; k < N; ++k) o[k] = acc[m][k / 4][k % 4];
+      if constexpr (std::is_same<T, _Float16>::value) {
+        const float sc = 1.0f / scale[r];
+#pragma unroll
+        for (int k = 0; k < N; ++k) o[k] *= sc;
+      }
       if (part)
         store_run<N>(part + ((int64_t)blockIdx.y * rows + r) * cols + c, cols - c, o);
       else
@@ -653,9 +671,11 @@ struct StoreEpi {
 
 // Rows of [dg | du]^T x: row m < pad of dw_gate, row m - pad of dw_up.  One
 // split: the gradients themselves; more: part[split][2][hidden][width] sums.
+// float16: unscale undoes the scale of the sum.
 template <class T>
 struct WeightEpi {
   static constexpr bool FORWARD = false;
+  const float* unscale;
   T *dw_gate, *dw_up;
   float* part;
   int64_t hidden, pad, width;
@@ -663,6 +683,8 @@ struct WeightEpi {
   __device__ __forceinline__ void run(f4 (&acc)[TL::TM][TL::TN], int64_t m0, int64_t n0,
                                       int64_t) const {
     const int lane = threadIdx.x & 63;
+    float sc = 1.0f;
+    if constexpr (std::is_same<T, _Float16>::value) sc = *unscale;
 #pragma unroll
     for (int m = 0; m < TL::TM; ++m) {
       const int64_t r = m0 + m * 16 + (lane & 15);
@@ -673,7 +695,8 @@ struct WeightEpi {
       for (int n = 0; n < TL::TN; ++n) {
         const int64_t c = n0 + n * 16 + 4 * (lane >> 4);
         if (c >= width) continue;
-        const float o[4] = {acc[m][n][0], acc[m][n][1], acc[m][n][2], acc[m][n][3]};
+        const float o[4] = {acc[m][n][0] * sc, acc[m][n][1] * sc, acc[m][n][2] * sc,
+                            acc[m][n][3] * sc};
         if (part) {
           store_run<4>(part + (((int64_t)blockIdx.y * 2 + up) * hidden + f) * width + c, width - c,
                        o);
@@ -942,6 +965,147 @@ __global__ __launch_bounds__(256) void k_transpose_split(const __bf16* __restric
   }
 }
 
+// ---------------------------------------------------------------- float16 dg and du
+
+// float16 ends at 65504 and loses bits below 2^-14, which dg and du of usual
+// gradients pass at either end.  Each row of [dg | du] is stored times a power of
+// two of its own, from a bound on the row that is known before its values are:
+// |u|, |g| <= |x| |w| + |b|, |dg| <= 1.13 |dh| |u| and |du| <= |dh| |act(g)|,
+// |act(g)| <= |g| or 1 (the sigmoid), some five of float16's 29 binades above what
+// occurs.  dx takes a row's scale out again; the weight gradients, which sum over
+// rows, take x over the row's scale instead of x, times the power of two that
+// fits the largest.  bfloat16 and float32 have the range as they are.  Three kernels
+// that read dh and x once, HBM and latency bound: backward, 128 x 256 -> 1024 42 -> 52
+// us, 20000 x 256 -> 512 95 -> 129, 65536 x 1024 -> 4096 3310 -> 3810 (255 of it here, the
+// rest the epilogue's).
+struct ScaleSource {
+  const _Float16 *x, *dh, *wg, *wu, *bg, *bu;
+  int64_t ldx, lddh, ldg, ldu, rows, hidden, width, wpad;
+  float act_max;
+  int wblocks, blocks;  // workgroups of k_weight_sizes, of the kernels of the rows
+  float* wpart;    // [2][kWeightBlocks]: largest norm of a weight row, largest bias
+  float* scale;    // [rows]
+  float* xpart;    // [kScaleBlocks]: largest |x| over its row's scale
+  _Float16* xs;    // [rows][wpad]
+  float* unscale;  // of the weight gradients
+};
+constexpr int kWeightBlocks = 512, kScaleBlocks = 2048;  // four rows at a time each, at most
+
+__device__ __forceinline__ float pow2_below(float bound) {
+  // the largest 2^e with 2^e bound < 2^15
+  if (!(bound > 0.0f)) return 1.0f;
+  return ldexpf(1.0f, min(max(14 - ilogbf(bound), -120), 120));
+}
+
+__device__ __forceinline__ float wave_max(float a) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) a = fmaxf(a, __shfl_xor(a, o));
+  return a;
+}
+
+// The largest finite |value| of a row and the sum of the finite squares, over a
+// wave.  Values that are not finite spoil their own row only.
+__device__ __forceinline__ void row_sizes(const _Float16* p, int64_t cols, float& big,
+                                          float& sum) {
+  big = sum = 0.0f;
+#pragma unroll 4
+  for (int64_t c = 8 * (threadIdx.x & 63); c < cols; c += 512) {
+    float v[8];
+    load_run<8>(p + c, cols - c, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      float a = fabsf(v[k]);
+      a = a < INFINITY ? a : 0.0f;
+      big = fmaxf(big, a);
+      sum = fmaf(a, a, sum);
+    }
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    sum += __shfl_xor(sum, o);
+    big = fmaxf(big, __shfl_xor(big, o));
+  }
+}
+
+__device__ __forceinline__ float block_max(float a, float* red) {
+  a = wave_max(a);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
+  __syncthreads();
+  return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+// the largest of count <= N partial results, every load out at once
+template <int N>
+__device__ __forceinline__ float largest_of(const float* part, int count) {
+  const int lane = threadIdx.x & 63;
+  float v[N / 64], a = 0.0f;
+#pragma unroll
+  for (int b = 0; b < N / 64; ++b) v[b] = b * 64 + lane < count ? part[b * 64 + lane] : 0.0f;
+#pragma unroll
+  for (int b = 0; b < N / 64; ++b) a = fmaxf(a, v[b]);
+  return wave_max(a);
+}
+
+__global__ __launch_bounds__(256) void k_weight_sizes(ScaleSource s) {
+  __shared__ float red[4];
+  float norm = 0.0f, bias = 0.0f;
+  for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < 2 * s.hidden;
+       r += (int64_t)gridDim.x * 4) {
+    const bool up = r >= s.hidden;
+    const int64_t f = up ? r - s.hidden : r;
+    float big, sum;
+    row_sizes(up ? s.wu + f * s.ldu : s.wg + f * s.ldg, s.width, big, sum);
+    norm = fmaxf(norm, sqrtf(sum));
+    const _Float16* b = up ? s.bu : s.bg;
+    const float v = b ? fabsf((float)b[f]) : 0.0f;
+    bias = fmaxf(bias, v < INFINITY ? v : 0.0f);
+  }
+  norm = block_max(norm, red);
+  bias = block_max(bias, red);
+  if (threadIdx.x == 0) {
+    s.wpart[blockIdx.x] = norm;
+    s.wpart[kWeightBlocks + blockIdx.x] = bias;
+  }
+}
+
+__global__ __launch_bounds__(256) void k_row_scales(ScaleSource s) {
+  __shared__ float red[4];
+  const float norm = largest_of<kWeightBlocks>(s.wpart, s.wblocks);
+  const float bias = largest_of<kWeightBlocks>(s.wpart + kWeightBlocks, s.wblocks);
+  float most = 0.0f;
+  for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < s.rows;
+       r += (int64_t)gridDim.x * 4) {
+    float d, x, sum, unused;
+    row_sizes(s.dh + r * s.lddh, s.hidden, d, unused);
+    row_sizes(s.x + r * s.ldx, s.width, x, sum);
+    const float sc = pow2_below(1.2f * d * fmaxf(fmaf(sqrtf(sum), norm, bias), s.act_max));
+    if ((threadIdx.x & 63) == 0) s.scale[r] = d > 0.0f ? sc : 0.0f;
+    if (d > 0.0f) most = fmaxf(most, x / sc);
+  }
+  most = block_max(most, red);
+  if (threadIdx.x == 0) s.xpart[blockIdx.x] = most;
+}
+
+// A row with no gradient has scale 0 so far, which makes its part of xs 0; from
+// here on 1.
+__global__ __launch_bounds__(256) void k_scale_rows(ScaleSource s) {
+  const float all = pow2_below(largest_of<kScaleBlocks>(s.xpart, s.blocks));
+  if (blockIdx.x == 0 && threadIdx.x == 0) *s.unscale = 1.0f / all;
+  for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < s.rows;
+       r += (int64_t)gridDim.x * 4) {
+    const float sc = s.scale[r], by = sc > 0.0f ? all / sc : 0.0f;
+    for (int64_t c = 8 * (threadIdx.x & 63); c < s.wpad; c += 512) {
+      float v[8];
+      load_run<8>(s.x + r * s.ldx + c, s.width - c, v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] *= by;
+      store_run<8>(s.xs + r * s.wpad + c, 8, v);
+    }
+    if ((threadIdx.x & 63) == 0 && !(sc > 0.0f)) s.scale[r] = 1.0f;
+  }
+}
+
 // ---------------------------------------------------------------- host side
 
 // Rows the product kernel can load directly: 16-byte aligned, whole 16-byte
@@ -1023,6 +1187,7 @@ template <class T, int MODE_>
 struct Plan {
   static constexpr int MODE = MODE_;
   static constexpr bool SPLIT = MODE == FP32_PARTS;
+  static constexpr bool SCALED = std::is_same<T, _Float16>::value;  // dg and du, by rows
   using E = typename std::conditional<SPLIT, __bf16, T>::type;  // what the products take
   // products of the projections and of the gradients; copies of x and the
   // weights, and of dg and du
@@ -1034,7 +1199,7 @@ struct Plan {
   int64_t wpad, hpad;
   bool pack_x, pack_w;
   size_t x_off = 0, wg_off = 0, wu_off = 0, wt_off = 0, dgu_off = 0, dbias_off = 0, part_off = 0;
-  size_t dxp_off = 0;
+  size_t dxp_off = 0, scale_off = 0, xs_off = 0;
   size_t bytes = 0;
   bool big_dual = false;
   Cut dx, dw;
@@ -1073,6 +1238,10 @@ struct Plan {
     dx = cut_product(a.width, rows, ceil_div(2 * hpad, KS), GRAD_PARTS, may_big, kMaxSplits,
                      (double)a.rows * (double)a.width);
     if (dx.splits > 1) dxp_off = take((size_t)dx.splits * a.rows * a.width * sizeof(float));
+    if (SCALED) {
+      scale_off = take((2 * kWeightBlocks + kScaleBlocks + 1 + (size_t)a.rows) * sizeof(float));
+      xs_off = take((size_t)a.rows * wpad * sizeof(E));
+    }
   }
   static int64_t reduction(const Cut& c) { return c.per * (128 / (int64_t)sizeof(E)); }
   int64_t ldd() const { return 2 * hpad * D_COPIES; }  // of [dg | du]
@@ -1131,6 +1300,27 @@ Inputs<typename Plan<T, MODE>::E> load_inputs(const GatedArgs& a, const Plan<T, 
                        st>>>(p);
     return in;
   }
+}
+
+// Scales of the rows of [dg | du], and x for the weight gradients.
+template <class PL>
+ScaleSource scale_rows(const GatedArgs& a, const PL& pl, const void* dh, int64_t dh_stride,
+                       char* ws, hipStream_t st) {
+  auto f = [](const void* p) { return static_cast<const _Float16*>(p); };
+  auto blocks = [](int64_t rows, int most) {
+    return (int)std::min<int64_t>(ceil_div(rows, (int64_t)4), most);
+  };
+  float *w = reinterpret_cast<float*>(ws + pl.scale_off), *xpart = w + 2 * kWeightBlocks;
+  const ScaleSource s{f(a.x), f(dh), f(a.w_gate), f(a.w_up), f(a.b_gate), f(a.b_up), a.x_stride,
+                      dh_stride, a.w_gate_stride, a.w_up_stride, a.rows, a.hidden, a.width,
+                      pl.wpad, a.activation == ACT_SIGMOID ? 1.0f : 0.0f,
+                      blocks(2 * a.hidden, kWeightBlocks), blocks(a.rows, kScaleBlocks), w,
+                      xpart + kScaleBlocks + 1, xpart,
+                      reinterpret_cast<_Float16*>(ws + pl.xs_off), xpart + kScaleBlocks};
+  k_weight_sizes<<<s.wblocks, 256, 0, st>>>(s);
+  k_row_scales<<<s.blocks, 256, 0, st>>>(s);
+  k_scale_rows<<<s.blocks, 256, 0, st>>>(s);
+  return s;
 }
 
 template <class TL, class EPI>
@@ -1276,8 +1466,11 @@ void gated_backward(const GatedArgs& a, const void* dh, int64_t dh_stride, const
     const Inputs<E> in = load_inputs(a, pl, ws, st);
     E* dgu = reinterpret_cast<E*>(ws + pl.dgu_off);
     float* dbias = dbg || dbu ? reinterpret_cast<float*>(ws + pl.dbias_off) : nullptr;
+    ScaleSource sc{};
+    if constexpr (PL::SCALED) sc = scale_rows(a, pl, dh, dh_stride, ws, st);
     dispatch_act(a.activation, [&](auto act) {
-      BackwardEpi<T, E, act.value, PL::D_COPIES> epi{static_cast<const T*>(a.b_gate),
+      BackwardEpi<T, E, act.value, PL::D_COPIES> epi{sc.scale,
+                                                     static_cast<const T*>(a.b_gate),
                                                      static_cast<const T*>(a.b_up),
                                                      static_cast<const T*>(dh),
                                                      dh_stride,
@@ -1312,20 +1505,22 @@ void gated_backward(const GatedArgs& a, const void* dh, int64_t dh_stride, const
       float* part = pl.dx.splits > 1 ? reinterpret_cast<float*>(ws + pl.dxp_off) : nullptr;
       launch_product<PL, false, false>(
           pl.dx.big, s, pl.dx.splits,
-          StoreEpi<T>{dx, part, a.rows, a.width}, st);
+          StoreEpi<T>{sc.scale, dx, part, a.rows, a.width}, st);
       if (part) sum_parts<T>(part, pl.dx.splits, a.rows * a.width, 1, dx, nullptr, st);
     }
     if (dwg || dwu) {
       float* part = pl.dw.splits > 1 ? reinterpret_cast<float*>(ws + pl.part_off) : nullptr;
       GemmShape s{};
       s.p = operand(in.x, in.ldx, pl.wpad);
+      if constexpr (PL::SCALED) s.p = operand(static_cast<const E*>(sc.xs), pl.wpad, pl.wpad);
       s.q = operand(static_cast<const E*>(dgu), pl.ldd(), 2 * pl.hpad);
       s.K = a.rows;
       s.k_split = PL::reduction(pl.dw);
       s.p_apart = pl.wpad * (int64_t)sizeof(E);
       s.q_apart = apart;
       launch_product<PL, true, false>(pl.dw.big, s, pl.dw.splits,
-                                      WeightEpi<T>{dwg, dwu, part, a.hidden, pl.hpad, a.width},
+                                      WeightEpi<T>{sc.unscale, dwg, dwu, part, a.hidden, pl.hpad,
+                                                   a.width},
                                       st);
       if (part) sum_parts<T>(part, pl.dw.splits, a.hidden * a.width, 2, dwg, dwu, st);
     }

@@ -109,3 +109,72 @@ def test_float32_non_finite_rows_stay_their_own():
         want = np.where(g > 0, g * u, 0.0).astype(np.float32)  # silu of +-1e37
     assert np.array_equal(np.isinf(want), np.isinf(got[700].cpu().numpy()))
     assert np.array_equal(np.sign(want), np.sign(got[700].cpu().numpy()))
+
+
+# ---------------------------------------------------------------- float16
+
+U16 = 2.0 ** -11
+
+
+def _half(a):
+    return torch.from_numpy(np.asarray(a)).to("cuda", torch.float16)
+
+
+def _half_layer(rng, rows, width=64, hidden=128):
+    return [_half(a) for a in (rng.normal(size=(rows, width)),
+                               rng.normal(size=(hidden, width)) / np.sqrt(width),
+                               rng.normal(size=(hidden, width)) / np.sqrt(width),
+                               0.3 * rng.normal(size=hidden), 0.3 * rng.normal(size=hidden))]
+
+
+def _half_check(got, want, tol, axis=None):
+    """On the 2-norm of the whole result or of each row, entries that pass 65504
+    (infinite in float16) among it: the roundings of dg and du that meet in an entry
+    are those of terms as large as in any other.  A result's own rounding is absolute
+    below 2^-14."""
+    got = got.double().cpu().numpy()
+    inside = abs(want) < 65504 * (1 - 2 * tol)
+    assert np.all(np.isfinite(got[inside])) and np.all(abs(got[abs(want) > 65536]) > 65000)
+    count = want.size if axis is None else want.shape[axis]
+    err = np.linalg.norm(np.where(inside, got, 0.0) - np.where(inside, want, 0.0), axis=axis)
+    assert np.all(err <= tol * np.linalg.norm(want, axis=axis) + 2.0 ** -25 * np.sqrt(count))
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid", "relu"])
+@pytest.mark.parametrize("rows", [100, 3000])
+@pytest.mark.parametrize("size", [1e4, 1.0, 1e-5, 4e-6])
+def test_float16_gradients_of_any_size(size, rows, act):
+    """dg and du pass float16's largest and smallest values long before the
+    gradients formed from them do.  Units of rounding as in test_gpu_torch_layers."""
+    rng = np.random.default_rng(rows)
+    args = _half_layer(rng, rows)
+    dh = _half(size * rng.normal(size=(rows, 128)))
+    got = features.gated_layer_backward(dh, *args, activation=act)
+    host = [a.double().cpu().numpy() for a in (dh, *args)]
+    for g, want, units in zip(got, ol.gated_layer_backward(*host, act=act), (3, 2, 2, 1, 1)):
+        _half_check(g, want, units * U16 + 4e-6)
+
+
+@pytest.mark.parametrize("rows", [100, 3000])
+def test_float16_rows_of_different_sizes(rows):
+    """dx, row by row, with rows of dh and of x 2^27 and 2^16 apart, some of dh zero."""
+    rng = np.random.default_rng(5)
+    args = _half_layer(rng, rows)
+    args[0] *= _half(2.0 ** rng.integers(-8, 9, size=(rows, 1)))
+    dh = 2.0 ** rng.integers(-14, 14, size=(rows, 1)) * rng.normal(size=(rows, 128))
+    dh[::17] = 0.0
+    dh = _half(dh)
+    args[0][17, 3] = float("inf")  # of a row that has no gradient
+    got = features.gated_layer_backward(dh, *args, need_dw=False)
+    host = [a.double().cpu().numpy() for a in (dh, *args)]
+    host[1][17, 3] = 0.0
+    want = ol.gated_layer_backward(*host)[0]
+    keep = np.arange(rows) != 17
+    _half_check(got.dx[torch.from_numpy(keep).cuda()], want[keep], 3 * U16 + 4e-6, axis=1)
+
+
+def test_float16_without_gradient():
+    rng = np.random.default_rng(6)
+    args = _half_layer(rng, 300)
+    for g in features.gated_layer_backward(torch.zeros(300, 128, device="cuda").half(), *args):
+        assert not g.any()
