@@ -802,7 +802,11 @@ typedef struct mgp_gated_layer {
   const void* b_gate;
   const void* b_up;
 } mgp_gated_layer_t;
-/* Bytes of workspace (256-byte aligned) of the forward or backward pass. */
+/* Bytes of workspace (256-byte aligned) of the forward or backward pass.  The
+ * products hold up to 12 bytes of work buffers a column and refuse rows of them of
+ * 8 MB and more: in float32 width from 1398081 and, in the backward pass, hidden
+ * from 699041 on; in the 16-bit types width from 4194297 and hidden from 2097145 on
+ * (1048569 up to 128 rows). */
 MGP_API int mgp_gated_layer_workspace(const mgp_gated_layer_t* args, int backward,
                                       int64_t* bytes);
 MGP_API int mgp_gated_layer_device(const mgp_gated_layer_t* args, void* h, int64_t h_stride,

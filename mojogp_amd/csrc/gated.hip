@@ -1110,10 +1110,11 @@ __global__ __launch_bounds__(256) void k_scale_rows(ScaleSource s) {
 
 // Rows the product kernel can load directly: 16-byte aligned, whole 16-byte
 // chunks, and a tile's rows within 31-bit offsets.
+constexpr int64_t kRowBytes = (int64_t)1 << 23;  // 256 rows, the most of a tile, in 2^31 bytes
 template <class T>
 bool direct(const void* p, int64_t stride, int64_t cols) {
   return aligned16(p) && stride % Vec16<T>::N == 0 && cols % Vec16<T>::N == 0 &&
-         stride * (int64_t)sizeof(T) < (int64_t)1 << 23;
+         stride * (int64_t)sizeof(T) < kRowBytes;
 }
 
 constexpr size_t kAlign = 256;
@@ -1211,6 +1212,13 @@ struct Plan {
     pack_x = SPLIT || !direct<T>(a.x, a.x_stride, a.width);
     pack_w = SPLIT || !direct<T>(a.w_gate, a.w_gate_stride, a.width) ||
              !direct<T>(a.w_up, a.w_up_stride, a.width) || a.w_gate_stride != a.w_up_stride;
+    auto require = [](int64_t row, const char* what) {
+      MGP_REQUIRE(row * (int64_t)sizeof(E) < kRowBytes,
+                  std::string("the ") + what + " of a gated layer is too large (the products "
+                  "take rows of less than 8 MB)");
+    };
+    require(wpad * COPIES, "width");
+    if (backward) require(std::max(ldd(), ldt()), "hidden width");
     auto take = [&](size_t n) {
       const size_t at = bytes;
       bytes += align_up(n);
