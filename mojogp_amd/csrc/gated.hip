@@ -91,8 +91,10 @@ __device__ __forceinline__ void activate(float g, float& a, float& slope) {
     a = g > 0.0f || g != g ? g : 0.0f;
     slope = g > 0.0f ? 1.0f : 0.0f;
   } else {
-    const float g2 = g * g;
-    const float e = exp_of<FAST>(-0.5f * g2, -0.5f * fmaf(g, g, -g2));
+    // fp32: from |g| = 40 on e is 0, and a square that passes fp32 has no remainder
+    const float c = FAST ? g : fminf(fabsf(g), 40.0f);
+    const float g2 = c * c;
+    const float e = exp_of<FAST>(-0.5f * g2, -0.5f * fmaf(c, c, -g2));
     const float tail = normal_tail<FAST>(fabsf(g) * 0.70710678118654752f) * e;  // 1 - Phi(|g|)
     const float cdf = g > 0.0f ? 1.0f - tail : tail;
     a = g * cdf;

@@ -111,6 +111,27 @@ def test_float32_non_finite_rows_stay_their_own():
     assert np.array_equal(np.sign(want), np.sign(got[700].cpu().numpy()))
 
 
+@pytest.mark.parametrize("rows, hidden", [(3, 20), (1500, 600)])  # by either kernel
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+def test_gelu_far_from_zero(kind, rows, hidden):
+    """Up to the largest values it is g or 0, and its derivative 1 or 0."""
+    far = np.array([30.0, 39.0, 41.0, 1e10, 1.8e19, 1.9e19, 1e25, 3e38])
+    gate = np.resize(np.concatenate([far, -far, [np.inf]]), hidden)
+    bg = torch.from_numpy(gate).to("cuda", kind)
+    x, w = torch.zeros(rows, 8, device="cuda", dtype=kind), \
+        torch.zeros(hidden, 8, device="cuda", dtype=kind)
+    ones = torch.ones(hidden, device="cuda", dtype=kind)
+    h = features.gated_layer(x, w, w, bg, ones, activation="gelu")
+    want = torch.where(bg > 0, bg, torch.zeros_like(bg))
+    assert torch.equal(h, want.expand(rows, hidden))
+    g = features.gated_layer_backward(ones.expand(rows, hidden).contiguous(), x, w, w, bg, ones,
+                                      activation="gelu")
+    finite = torch.isfinite(bg)
+    slopes = rows * (bg > 0).double()
+    # bfloat16 rounds the sum over the rows
+    assert torch.equal(g.db_gate[finite], slopes.to(kind)[finite])
+
+
 # ---------------------------------------------------------------- float16
 
 U16 = 2.0 ** -11
