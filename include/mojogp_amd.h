@@ -211,7 +211,8 @@ MGP_API int mgp_input_gradient(void* handle, const float* Lf, const float* Rf,
 /* Same with device arrays, asynchronously on the caller's HIP stream (NULL:
  * the default stream).  Calls of one handle from several streams run one after
  * another, and a change of the parameters or the handle's destruction waits for
- * them; the arrays must stay until the stream has passed the call. */
+ * them; the arrays must stay until the stream has passed the call.  A stream that
+ * is being recorded into a graph is refused. */
 MGP_API int mgp_input_gradient_device(void* handle, const float* Lf_device,
                                       const float* Rf_device, int ncols,
                                       float* out_device, void* stream);

@@ -213,7 +213,8 @@ class NativeProvider:
 
     def input_gradient_device(self, Lf, Rf, out=None):
         """input_gradient of device tensors ([ncols, n] or [n], float32, contiguous;
-        out [n, d]), asynchronously on the calling program's current stream."""
+        out [n, d]), asynchronously on the calling program's current stream, which
+        must not be one that is being captured into a graph."""
         from . import features
         dtype, code, index, stream = features._first(Lf, "Lf")
         shape = Lf.shape

@@ -526,6 +526,13 @@ int mgp_input_gradient_device(void* h, const float* Lf_dev, const float* Rf_dev,
     int device = -1;
     MGP_HIP_CHECK(hipGetDevice(&device));
     MGP_REQUIRE(device == pv->device, "the provider's device is not the current one");
+    // a graph would keep the addresses of buffers that the handle may replace, and
+    // its replays would run past what a change of the handle waits for
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    MGP_HIP_CHECK(hipStreamIsCapturing(static_cast<hipStream_t>(stream), &capture));
+    MGP_REQUIRE(capture == hipStreamCaptureStatusNone,
+                "the input gradient cannot be recorded into a graph: its work buffers are the "
+                "handle's");
     point_gradient(*pv, Lf_dev, Rf_dev, ncols, out_dev, static_cast<hipStream_t>(stream));
   });
 }
