@@ -209,10 +209,10 @@ MGP_API int mgp_gradient_trace(void* handle, const float* Lf, const float* Rf,
 MGP_API int mgp_input_gradient(void* handle, const float* Lf, const float* Rf,
                                int ncols, float* out);
 /* Same with device arrays, asynchronously on the caller's HIP stream (NULL:
- * the default stream).  Calls of one handle from several streams run one after
- * another, and a change of the parameters or the handle's destruction waits for
- * them; the arrays must stay until the stream has passed the call.  A stream that
- * is being recorded into a graph is refused. */
+ * the default stream).  Calls of one handle from several streams and threads
+ * run one after another, and a change of the parameters or the handle's
+ * destruction waits for them; the arrays must stay until the stream has passed
+ * the call.  A stream that is being recorded into a graph is refused. */
 MGP_API int mgp_input_gradient_device(void* handle, const float* Lf_device,
                                       const float* Rf_device, int ncols,
                                       float* out_device, void* stream);

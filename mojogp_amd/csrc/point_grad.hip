@@ -605,6 +605,7 @@ void point_gradient(Provider& pv, const float* Lf, const float* Rf, int ncols, f
                     hipStream_t st) {
   MGP_REQUIRE(!pv.is_tree, "the input gradient does not serve kernel trees");
   MGP_REQUIRE(pv.d >= 1 && pv.d <= 32, "the input gradient supports d <= 32");
+  const std::lock_guard<std::mutex> hold(pv.points_lock);
   PgScale scale;
   for (int k = 0; k < 32; ++k)
     scale.v[k] = k < pv.d ? (float)(-(double)pv.outputscale() /

@@ -5,6 +5,7 @@
 // points (mojogp/codegen_engine/emit/fn_ptr_module.py:159-211, 651-703).
 #pragma once
 
+#include <mutex>
 #include <vector>
 
 #include "dense.h"
@@ -164,6 +165,9 @@ struct Provider {
              const RhsPack* packed = nullptr);
   DevBuf<float> pg_ws;  // operands and split sums of the input gradient
   PendingUse points_use;  // of train and pg_ws, by mgp_input_gradient_device
+  // Held from the wait for the last use to the record of the next, and while the
+  // points change: one use after another, whichever threads make the calls.
+  std::mutex points_lock;
   float* pg_buffer(size_t count) {
     if (count > pg_ws.count) points_use.wait();
     return pg_ws.ensure(count);

@@ -11,6 +11,7 @@
 namespace mgp {
 
 void Provider::refresh_coords() {
+  const std::lock_guard<std::mutex> hold(points_lock);
   points_use.wait();
   if (is_tree) {
     for (int q = 0; q < nparams; ++q)

@@ -1,5 +1,7 @@
 """How calls of the input gradient share a handle: graphs, threads, errors."""
 
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -41,3 +43,37 @@ def test_a_stream_in_capture_is_refused():
         assert np.array_equal(p.input_gradient_device(l, r).cpu().numpy(), p.input_gradient(L, R))
     finally:
         p.close()
+
+
+def test_threads_of_one_handle():
+    """Calls from several threads, each on a stream of its own and of another size,
+    share the work buffers one after another."""
+    X, params, L, R = _inputs(6000, 4, 20)
+    p = NativeProvider("matern52", True, X, params, 0.1)
+    l, r = torch.from_numpy(L).cuda(), torch.from_numpy(R).cuda()
+    columns = (1, 5, 16, 20)
+    want = [p.input_gradient(L[:t], R[:t]) for t in columns]
+    torch.cuda.synchronize()
+    got, errors = [[] for _ in columns], []
+    start = threading.Barrier(len(columns))
+
+    def work(k):
+        try:
+            stream = torch.cuda.Stream()
+            start.wait()
+            with torch.cuda.stream(stream):
+                for _ in range(25):
+                    got[k].append(p.input_gradient_device(l[:columns[k]], r[:columns[k]]))
+            stream.synchronize()
+        except Exception as e:  # noqa: BLE001 - reported below
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(len(columns))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    p.close()
+    assert not errors
+    for k in range(len(columns)):
+        assert all(np.array_equal(g.cpu().numpy(), want[k]) for g in got[k])
