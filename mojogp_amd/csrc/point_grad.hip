@@ -614,7 +614,7 @@ void point_gradient(Provider& pv, const float* Lf, const float* Rf, int ncols, f
   const MmKernel mm = pv.n >= kMmPoints && pv.train.max_norm <= mm_norm_bound(pv.kind)
                           ? pick_mm(pv.kind, pv.train.kb, pv.d, pv.n)
                           : MmKernel{nullptr, 0, 0};
-  pv.points_use.order(st);
+  const UseScope use(pv.points_use, st);
   for (int c0 = 0; c0 < ncols; c0 += kPgCols) {
     const PgWork w{pv, Lf + (int64_t)c0 * pv.n, Rf + (int64_t)c0 * pv.n,
                    std::min(kPgCols, ncols - c0), c0 > 0, out, st};
@@ -624,7 +624,6 @@ void point_gradient(Provider& pv, const float* Lf, const float* Rf, int ncols, f
       gradient_differences(w, scale);
     MGP_HIP_CHECK(hipGetLastError());
   }
-  pv.points_use.record(st);
 }
 
 }  // namespace mgp

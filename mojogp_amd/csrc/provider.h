@@ -27,18 +27,29 @@ struct PendingUse {
     wait();
     if (ev) (void)hipEventDestroy(ev);
   }
-  void record(hipStream_t st) {
-    if (!ev) MGP_HIP_CHECK(hipEventCreateWithFlags(&ev, hipEventDisableTiming));
-    MGP_HIP_CHECK(hipEventRecord(ev, st));
-    pending = true;
+  // Records the use; where that fails, waits for it instead.
+  void record(hipStream_t st) noexcept {
+    pending = (ev || hipEventCreateWithFlags(&ev, hipEventDisableTiming) == hipSuccess) &&
+              hipEventRecord(ev, st) == hipSuccess;
+    if (!pending) (void)hipStreamSynchronize(st);
   }
   void order(hipStream_t st) const {
     if (pending) MGP_HIP_CHECK(hipStreamWaitEvent(st, ev, 0));
   }
   void wait() noexcept {
-    if (pending) (void)hipEventSynchronize(ev);
+    if (pending && hipEventSynchronize(ev) != hipSuccess) (void)hipDeviceSynchronize();
     pending = false;
   }
+};
+// Records a use at the end of its scope, by an exception too: what was launched
+// before it runs on.
+struct UseScope {
+  PendingUse& use;
+  hipStream_t st;
+  UseScope(PendingUse& u, hipStream_t s) : use(u), st(s) { use.order(st); }
+  UseScope(const UseScope&) = delete;
+  UseScope& operator=(const UseScope&) = delete;
+  ~UseScope() { use.record(st); }
 };
 
 struct Provider {

@@ -8,6 +8,7 @@ import torch
 
 from mojogp_amd import _lib
 from mojogp_amd._provider import NativeProvider
+from test_zz_no_alloc import _hip
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +78,25 @@ def test_threads_of_one_handle():
     assert not errors
     for k in range(len(columns)):
         assert all(np.array_equal(g.cpu().numpy(), want[k]) for g in got[k])
+
+
+def test_a_call_that_fails_after_its_launches_is_waited_for():
+    """An error that the runtime still held from elsewhere ends the call once its
+    kernels run: a change of the parameters waits for them all the same, and the
+    next calls are right."""
+    X, params, L, R = _inputs(20000, 8, 16)
+    p = NativeProvider("matern52", True, X, params, 0.1)
+    l, r = torch.from_numpy(L).cuda(), torch.from_numpy(R).cuda()
+    out = torch.zeros(20000, 8, device="cuda")
+    try:
+        want = p.input_gradient(L, R)
+        torch.cuda.synchronize()
+        assert _hip().hipSetDevice(10 ** 6) != 0  # no such device
+        with pytest.raises(_lib.NativeCallError):
+            p.input_gradient_device(l, r, out=out)
+        p.update_params(params * np.float32(2.0))
+        torch.cuda.synchronize()
+        assert np.array_equal(out.cpu().numpy(), want)
+        assert np.array_equal(p.input_gradient_device(l, r).cpu().numpy(), p.input_gradient(L, R))
+    finally:
+        p.close()
