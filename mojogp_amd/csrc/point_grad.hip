@@ -13,7 +13,11 @@
 // with large norms and for small sets.  k_point_grad_mm has the matrix cores
 // form the distances (Gram form, as the tile products), the weights and the
 // sums sum_b W h and sum_b W h z_b, which leaves the VALU the value alone;
-// out is then z_i times the first minus the second.
+// out is then z_i times the first minus the second.  Where that difference
+// cancels (points in clusters, weights on near pairs) or weights are far below the
+// largest, it has lost the digits that differences keep: every block of rows is
+// weighed against the error of its sums, and one that falls short is formed again
+// by k_point_grad.
 #include "kval.h"
 #include "provider.h"
 
@@ -30,6 +34,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 constexpr int kPgBlock = 128;            // columns staged at a time
 constexpr int kPgCols = 16;              // weight columns per pass
 constexpr int kPgStride = kPgBlock + 16; // LDS stride of a weight column
+constexpr int kPgRows = 128;             // rows of a workgroup (R = 2)
 
 // part[split][i][q] = sum over the split's columns b of
 // (W_ib + W_bi) h_ib (z_i - z_b)_q, ordered pairs.
@@ -38,10 +43,13 @@ constexpr int kPgStride = kPgBlock + 16; // LDS stride of a weight column
 // 4 (lane/16) + e, row lane%16), so a lane keeps its rows and their sums in
 // registers and reads columns from LDS.  VALU bound: 3 d + ~12 instructions a
 // pair (Matern-5/2, 8 dimensions, 50000 points: 3130 us, 0.8e12 pairs a second).
+// wanted: for each block of rows whether it is formed (null: all are).
 template <int KIND, int D, bool ARD, int R>
 __global__ __launch_bounds__(256) void k_point_grad(
     const float* __restrict__ Z, int64_t n, int d, const float* __restrict__ Lf,
-    const float* __restrict__ Rf, int cn, int64_t nb, int64_t bps, float* __restrict__ part) {
+    const float* __restrict__ Rf, int cn, int64_t nb, int64_t bps,
+    const int* __restrict__ wanted, float* __restrict__ part) {
+  if (wanted && !wanted[blockIdx.x]) return;
   constexpr int B = kPgBlock, CS = kPgStride;
   constexpr int DS = D <= 2 ? D : (D + 3) / 4 * 4;  // LDS stride of a point
   __shared__ __align__(16) float sx[B * DS];
@@ -160,13 +168,16 @@ struct PgScale {
   float v[32];  // -os / (s l_q)
 };
 
-// out[i][q] (+)= scale_q sum over the splits of part[split][i][q], in order
+// out[i][q] (+)= scale_q sum over the splits of part[split][i][q], in order, of the
+// blocks of kPgRows rows that are wanted (null: all)
 __global__ __launch_bounds__(256) void k_point_grad_sum(const float* __restrict__ part,
                                                         int64_t splits, int64_t n, int d,
                                                         PgScale scale, int accumulate,
+                                                        const int* __restrict__ wanted,
                                                         float* __restrict__ out) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n * d;
        i += (int64_t)gridDim.x * 256) {
+    if (wanted && !wanted[i / d / kPgRows]) continue;
     float s = 0.0f;
 #pragma unroll 4
     for (int64_t p = 0; p < splits; ++p) s += part[p * n * d + i];
@@ -176,7 +187,7 @@ __global__ __launch_bounds__(256) void k_point_grad_sum(const float* __restrict_
 }
 
 using PgFn = void (*)(const float*, int64_t, int, const float*, const float*, int, int64_t,
-                      int64_t, float*);
+                      int64_t, const int*, float*);
 
 // below, 64-row blocks (300 points 12.7 -> 10.1 us, 2000 18.2 -> 16.4, 3000 31.0 -> 31.2)
 constexpr int64_t kPgFewPoints = 3000;
@@ -336,14 +347,15 @@ template <int KIND, int KB, int DZ, int R>
 __device__ __forceinline__ void mm_stage(const char* next, int fragments, int kw, bool more,
                                          const char* __restrict__ cur, char* __restrict__ nxt,
                                          int64_t tile0, int64_t row_tile0, const h8 (&bi)[R][KB],
-                                         const h8 (&wb)[R][3], float (&sum)[R], f4 (&hz)[R][DZ]) {
+                                         const h8 (&wb)[R][3], float (&sum)[R], float (&sq)[R],
+                                         f4 (&hz)[R][DZ]) {
   if (more) mm_load(next, fragments, nxt);
   const int lane = threadIdx.x & 63, lm = lane & 15, lq = lane >> 4;
-  float s1[R];
+  float s1[R], s2[R];
   f4 acc[R][DZ];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    s1[r] = 0.0f;
+    s1[r] = s2[r] = 0.0f;
 #pragma unroll
     for (int q = 0; q < DZ; ++q) acc[r][q] = f4{0.f, 0.f, 0.f, 0.f};
   }
@@ -381,6 +393,7 @@ __device__ __forceinline__ void mm_stage(const char* next, int fragments, int kw
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         s1[r] += hw[e];
+        s2[r] = fmaf(hw[e], hw[e], s2[r]);
 #pragma unroll
         for (int q = 0; q < DZ; ++q)
           acc[r][q] = __builtin_amdgcn_mfma_f32_16x16x4f32(hw[e], z[q][e], acc[r][q], 0, 0, 0);
@@ -391,19 +404,21 @@ __device__ __forceinline__ void mm_stage(const char* next, int fragments, int kw
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     sum[r] += s1[r];
+    sq[r] += s2[r];
 #pragma unroll
     for (int q = 0; q < DZ; ++q) hz[r][q] += acc[r][q];
   }
   __syncthreads();
 }
 
-// part[split][i][q] = sum_b W h z_bq and, from sums on, sums[split][i] = sum_b W h
-// over the split's columns b.  Result e of a lane belongs to the pair (column
+// part[split][i][q] = sum_b W h z_bq and, from sums on, sums[split][0][i] = sum_b W h
+// and sums[split][1][i] = sum_b (W h)^2 over the split's columns b.  Result e of a lane belongs to the pair (column
 // 4 (lane/16) + e, row lane%16): W h is then the A operand of the sum over the
 // columns as it stands, no lane exchanges it.  Bound by the VALU (Matern-5/2:
-// 5 instructions, a square root and an exponential a pair, 208 cycles a 16 x 16
+// 6 instructions, a square root and an exponential a pair, 224 cycles a 16 x 16
 // tile) beside 192 cycles of matrix instructions of d <= 8; the two add up more than
-// they overlap: 50000 points, 11 columns, 1640 us, 1.5e12 pairs a second.
+// they overlap: 50000 points, 16 columns, the whole call 1710 us, 1.5e12 pairs a
+// second; 1635 without the sum of squares and what follows from it.
 template <int KIND, int KB, int DZ, int R>
 __global__ __launch_bounds__(256, 3) void k_point_grad_mm(
     const char* __restrict__ col, const uint4* __restrict__ B, const uint4* __restrict__ wrow,
@@ -415,7 +430,7 @@ __global__ __launch_bounds__(256, 3) void k_point_grad_mm(
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t rt0 = ((int64_t)blockIdx.x * 4 + wave) * R;
   h8 bi[R][KB], wb[R][3];
-  float sum[R];
+  float sum[R], sq[R];
   f4 hz[R][DZ];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
@@ -425,7 +440,7 @@ __global__ __launch_bounds__(256, 3) void k_point_grad_mm(
 #pragma unroll
     for (int m = 0; m < 3; ++m)
       if (m < kw) wb[r][m] = __builtin_bit_cast(h8, wrow[((rt0 + r) * kw + m) * 64 + lane]);
-    sum[r] = 0.0f;
+    sum[r] = sq[r] = 0.0f;
 #pragma unroll
     for (int q = 0; q < DZ; ++q) hz[r][q] = f4{0.f, 0.f, 0.f, 0.f};
   }
@@ -442,7 +457,7 @@ __global__ __launch_bounds__(256, 3) void k_point_grad_mm(
     __syncthreads();
     --left;
     mm_stage<KIND, KB, DZ, R>(at + bytes, fragments, kw, left > 0, b1, b0, tile, rt0, bi, wb, sum,
-                              hz);
+                              sq, hz);
     at += bytes;
     tile += kMmTiles;
   } else {
@@ -450,19 +465,25 @@ __global__ __launch_bounds__(256, 3) void k_point_grad_mm(
     __syncthreads();
   }
   for (; left > 0; left -= 2) {
-    mm_stage<KIND, KB, DZ, R>(at + bytes, fragments, kw, true, b0, b1, tile, rt0, bi, wb, sum, hz);
+    mm_stage<KIND, KB, DZ, R>(at + bytes, fragments, kw, true, b0, b1, tile, rt0, bi, wb, sum, sq,
+                              hz);
     mm_stage<KIND, KB, DZ, R>(at + 2 * bytes, fragments, kw, left > 2, b1, b0, tile + kMmTiles,
-                              rt0, bi, wb, sum, hz);
+                              rt0, bi, wb, sum, sq, hz);
     at += 2 * bytes;
     tile += 2 * kMmTiles;
   }
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    float s = sum[r];
+    float s = sum[r], s2 = sq[r];
     s += __shfl_xor(s, 16);
     s += __shfl_xor(s, 32);
+    s2 += __shfl_xor(s2, 16);
+    s2 += __shfl_xor(s2, 32);
     const int64_t i0 = (rt0 + r) * 16;
-    if (lq == 0 && i0 + lm < n) sums[(int64_t)blockIdx.y * n + i0 + lm] = s;
+    if (lq == 0 && i0 + lm < n) {
+      sums[(int64_t)blockIdx.y * 2 * n + i0 + lm] = s;
+      sums[((int64_t)blockIdx.y * 2 + 1) * n + i0 + lm] = s2;
+    }
 #pragma unroll
     for (int q = 0; q < DZ; ++q)
 #pragma unroll
@@ -474,23 +495,72 @@ __global__ __launch_bounds__(256, 3) void k_point_grad_mm(
   }
 }
 
-// out[i][q] (+)= scale_q unscale (z_iq sum of sums - sum of part)
-__global__ __launch_bounds__(256) void k_point_grad_mm_sum(
+// out[i][q] (+)= scale_q unscale v_iq, v_iq = z_iq S_i - sum of part, S_i = sum of
+// sums, for a block of kPgRows rows, if its v stands out from the error that its sums
+// left.  That error's norm over a row, measured on 4096 points of 1 to 24
+// dimensions, Gaussian and in clusters of radius 1 to 0.001, all three kernels, is
+// 1.8e-7 to 6e-7 of |z_i| sqrt(Q_i), Q_i = sum_b (W h)^2 (the roundings of distances,
+// weights and sums); long sums of one sign round off up to 1.2e-7 of |z_i| |S_i|.
+// With 4.8e-7 for the first a block passes where both are below 1.5e-6 of |v|:
+// |v|^2 >= sum_i |z_i|^2 (Q_i + S_i^2 / 16) / 10; Gaussian points have 0.2 to 0.9 of
+// |z|^2 Q.  And where every row's weights stand out from the end of their two parts,
+// 2^-25 beside factors of up to 2^15: Q_i >= floor = (2^-10 / 1.5e-6)^2 2 ncols n.
+// failed[block]: to be formed by differences.
+__global__ __launch_bounds__(1024) void k_point_grad_mm_sum(
     const float* __restrict__ part, const float* __restrict__ sums, const float* __restrict__ Z,
     int64_t splits, int64_t n, int d, PgScale scale, const float* __restrict__ unscale,
-    int accumulate, float* __restrict__ out) {
-  const double un = *unscale;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n * d;
-       i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / d;
-    double s = 0.0, hz = 0.0;
-#pragma unroll 4
+    float floor, int accumulate, int* __restrict__ failed, float* __restrict__ out) {
+  __shared__ double total[kPgRows];
+  __shared__ float value[kPgRows * 32], red[2][16];
+  const int64_t row0 = (int64_t)blockIdx.x * kPgRows;
+  const int rows = (int)min((int64_t)kPgRows, n - row0);
+  float need = 0.0f, have = 0.0f;
+  if ((int)threadIdx.x < rows) {
+    const int64_t row = row0 + threadIdx.x;
+    double s = 0.0, q = 0.0;
+#pragma unroll 8
     for (int64_t p = 0; p < splits; ++p) {
-      s += (double)sums[p * n + row];
-      hz += (double)part[p * n * d + i];
+      s += (double)sums[2 * p * n + row];
+      q += (double)sums[(2 * p + 1) * n + row];
     }
-    const float v = (float)((double)scale.v[i - row * d] * un * ((double)Z[i] * s - hz));
-    out[i] = accumulate ? out[i] + v : v;
+    total[threadIdx.x] = s;
+    float zz = 0.0f;
+    for (int k = 0; k < d; ++k) zz = fmaf(Z[row * d + k], Z[row * d + k], zz);
+    need = q >= (double)floor ? 0.1f * zz * (float)(q + 0.0625 * s * s) : INFINITY;
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < rows * d; e += 1024) {
+    double hz = 0.0;
+#pragma unroll 8
+    for (int64_t p = 0; p < splits; ++p) hz += (double)part[(p * n + row0) * d + e];
+    const float v = (float)((double)Z[row0 * d + e] * total[e / d] - hz);
+    value[e] = v;
+    have = fmaf(v, v, have);
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    need += __shfl_xor(need, o);
+    have += __shfl_xor(have, o);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    red[0][threadIdx.x >> 6] = need;
+    red[1][threadIdx.x >> 6] = have;
+  }
+  __syncthreads();
+  need = have = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    need += red[0][w];
+    have += red[1][w];
+  }
+  const bool passes = have >= need;  // (not where either is NaN)
+  if (threadIdx.x == 0) failed[blockIdx.x] = !passes;
+  if (!passes) return;
+  const double un = *unscale;
+  for (int e = threadIdx.x; e < rows * d; e += 1024) {
+    const float v = (float)((double)scale.v[e % d] * un * (double)value[e]);
+    float* o = out + row0 * d + e;
+    *o = accumulate ? *o + v : v;
   }
 }
 
@@ -526,10 +596,8 @@ MmKernel pick_mm(int kind, int kb, int d, int64_t n) {
   }
 }
 
-// Largest norm |z|^2 of the points for the matrix-core route.  Its errors grow
-// with the norms, of the distances and of the closing difference: measured in
-// float32 against 64 bits over 1 to 16 dimensions they stay below 7e-7 of the
-// result up to these (1.5e-7 to 4e-7 on differences).
+// Largest norm |z|^2 of the points for the matrix-core route: beyond it the rounding
+// of the Gram form's distances alone comes near the bound of k_point_grad_mm_sum.
 inline float mm_norm_bound(int kind) {
   return kind == KIND_RBF ? 32.0f : kind == KIND_MATERN32 ? 256.0f : 512.0f;
 }
@@ -547,32 +615,48 @@ struct PgWork {
   hipStream_t st;
 };
 
-void gradient_differences(const PgWork& w, const PgScale& scale) {
-  const int64_t n = w.pv.n;
-  const int d = w.pv.d;
-  // few points: 64-row blocks, for more workgroups
-  const bool few = n < kPgFewPoints;
-  const int64_t nb = ceil_div(n, (int64_t)kPgBlock), rb = ceil_div(n, (int64_t)(few ? 64 : 128));
+struct PgSplit {
+  int64_t nb, rb, bps, splits;  // column blocks, row blocks, column blocks a split, splits
+};
+
+PgSplit split_differences(int64_t n, bool few) {
+  const int64_t nb = ceil_div(n, (int64_t)kPgBlock);
+  const int64_t rb = ceil_div(n, (int64_t)(few ? kPgRows / 2 : kPgRows));
   // column splits until there are 2048 workgroups, one column block at least
   const int64_t bps = ceil_div(nb, std::min(nb, ceil_div(2048, rb)));
-  const int64_t splits = ceil_div(nb, bps);
-  float* part = w.pv.pg_buffer((size_t)splits * n * d);
-  const PgFn fn = few ? pick_pg<1>(w.pv.kind, w.pv.ard, d) : pick_pg<2>(w.pv.kind, w.pv.ard, d);
-  MGP_REQUIRE(fn != nullptr, "no input gradient kernel for this dimension");
-  hipLaunchKernelGGL(fn, dim3((unsigned)rb, (unsigned)splits), dim3(256), 0, w.st,
-                     w.pv.train.z.ptr, n, d, w.Lf, w.Rf, w.ncols, nb, bps, part);
-  k_point_grad_sum<<<(unsigned)std::min<int64_t>(ceil_div(n * d, (int64_t)256), 4096), 256, 0,
-                     w.st>>>(part, splits, n, d, scale, w.accumulate, w.out);
+  return {nb, rb, bps, ceil_div(nb, bps)};
 }
 
-void gradient_matrix_cores(const PgWork& w, const MmKernel& kernel, PgScale scale) {
+// part: splits n d floats.  wanted: of which blocks of kPgRows rows (null: all)
+void gradient_differences(const PgWork& w, const PgScale& scale, const PgSplit& s, bool few,
+                          float* part, const int* wanted) {
+  const int64_t n = w.pv.n;
+  const int d = w.pv.d;
+  const PgFn fn = few ? pick_pg<1>(w.pv.kind, w.pv.ard, d) : pick_pg<2>(w.pv.kind, w.pv.ard, d);
+  MGP_REQUIRE(fn != nullptr, "no input gradient kernel for this dimension");
+  hipLaunchKernelGGL(fn, dim3((unsigned)s.rb, (unsigned)s.splits), dim3(256), 0, w.st,
+                     w.pv.train.z.ptr, n, d, w.Lf, w.Rf, w.ncols, s.nb, s.bps, wanted, part);
+  k_point_grad_sum<<<(unsigned)std::min<int64_t>(ceil_div(n * d, (int64_t)256), 4096), 256, 0,
+                     w.st>>>(part, s.splits, n, d, scale, w.accumulate, wanted, w.out);
+}
+
+void gradient_differences(const PgWork& w, const PgScale& scale) {
+  // few points: 64-row blocks, for more workgroups
+  const bool few = w.pv.n < kPgFewPoints;
+  const PgSplit s = split_differences(w.pv.n, few);
+  float* part = w.pv.pg_buffer((size_t)s.splits * w.pv.n * w.pv.d);
+  gradient_differences(w, scale, s, few, part, nullptr);
+}
+
+void gradient_matrix_cores(const PgWork& w, const MmKernel& kernel, const PgScale& scale) {
   Provider& pv = w.pv;
   const PackedPoints& pts = pv.train;
   const int64_t n = pv.n;
   const int d = pv.d, kw = (6 * w.ncols + 31) / 32, dz = kernel.dz;
   const double factor =
       pv.kind == KIND_MATERN32 ? 3.0 : pv.kind == KIND_MATERN52 ? 5.0 / 3.0 : 1.0;
-  for (int k = 0; k < d; ++k) scale.v[k] = (float)(factor * (double)scale.v[k]);
+  PgScale scaled = scale;
+  for (int k = 0; k < d; ++k) scaled.v[k] = (float)(factor * (double)scale.v[k]);
   const int64_t stages = ceil_div(pts.ntiles, (int64_t)kMmTiles);
   const int64_t rb = ceil_div(pts.ntiles, (int64_t)kernel.row_tiles);
   const int64_t sps = ceil_div(stages, std::min(ceil_div(stages, 4), ceil_div(2048, rb)));
@@ -580,23 +664,37 @@ void gradient_matrix_cores(const PgWork& w, const MmKernel& kernel, PgScale scal
   // workgroups read whole blocks of tiles: the packing covers them
   const int64_t tiles = pts.ntiles_alloc;
   MGP_REQUIRE(rb * kernel.row_tiles <= tiles && stages * kMmTiles <= tiles, "packing too small");
+  const PgSplit again = split_differences(n, false);
+  size_t count = 0;  // of the buffer, in floats
+  auto take = [&](size_t floats) {
+    const size_t at = count;
+    count += (size_t)round_up((int64_t)floats, 64);
+    return at;
+  };
   const size_t frag = 256;  // floats of a fragment
-  const size_t col = (size_t)tiles * (pts.kb + kw + dz) * frag, wrow = (size_t)tiles * kw * frag;
-  const size_t sums = round_up(splits * n, 64), tail = 2 * kMmMaxBlocks + 64;
-  float* ws = pv.pg_buffer(col + wrow + sums + tail + (size_t)splits * n * d);
-  float *pw = ws + col, *ps = pw + wrow, *pm = ps + sums, *un = pm + 2 * kMmMaxBlocks;
-  float* part = pm + tail;
-  k_pg_max<<<dim3(kMmMaxBlocks, 2), 256, 0, w.st>>>(w.Lf, w.Rf, n * w.ncols, pm);
+  const size_t col = take((size_t)tiles * (pts.kb + kw + dz) * frag);
+  const size_t wrow = take((size_t)tiles * kw * frag), sums = take((size_t)splits * 2 * n);
+  const size_t maxima = take(2 * kMmMaxBlocks), unscale = take(1);
+  const size_t failed = take((size_t)again.rb);
+  // the sums of either route: the first's are done with when the second's come
+  const size_t part = take((size_t)std::max(splits, again.splits) * n * d);
+  float* ws = pv.pg_buffer(count);
+  int* fail = reinterpret_cast<int*>(ws + failed);
+  k_pg_max<<<dim3(kMmMaxBlocks, 2), 256, 0, w.st>>>(w.Lf, w.Rf, n * w.ncols, ws + maxima);
   k_pg_pack<<<(unsigned)ceil_div(tiles, (int64_t)4), 256, 0, w.st>>>(
       reinterpret_cast<const uint4*>(pts.A.ptr), pts.z.ptr, w.Lf, w.Rf, n, d, w.ncols, pts.kb, kw,
-      dz, tiles, pm, reinterpret_cast<uint4*>(ws), reinterpret_cast<uint4*>(pw), un);
+      dz, tiles, ws + maxima, reinterpret_cast<uint4*>(ws + col),
+      reinterpret_cast<uint4*>(ws + wrow), ws + unscale);
   hipLaunchKernelGGL(kernel.fn, dim3((unsigned)rb, (unsigned)splits), dim3(256), 0, w.st,
-                     reinterpret_cast<const char*>(ws),
-                     reinterpret_cast<const uint4*>(pts.B.ptr), reinterpret_cast<const uint4*>(pw),
-                     kw, n, d, stages, sps, part, ps);
-  k_point_grad_mm_sum<<<(unsigned)std::min<int64_t>(ceil_div(n * d, (int64_t)256), 4096), 256, 0,
-                        w.st>>>(part, ps, pts.z.ptr, splits, n, d, scale, un, w.accumulate,
-                                w.out);
+                     reinterpret_cast<const char*>(ws + col),
+                     reinterpret_cast<const uint4*>(pts.B.ptr),
+                     reinterpret_cast<const uint4*>(ws + wrow), kw, n, d, stages, sps, ws + part,
+                     ws + sums);
+  const float floor = 4.24e5f * 2.0f * (float)w.ncols * (float)n;  // (see the kernel)
+  k_point_grad_mm_sum<<<(unsigned)again.rb, 1024, 0, w.st>>>(
+      ws + part, ws + sums, pts.z.ptr, splits, n, d, scaled, ws + unscale, floor, w.accumulate,
+      fail, w.out);
+  gradient_differences(w, scale, again, false, ws + part, fail);
 }
 
 }  // namespace
