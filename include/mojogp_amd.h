@@ -740,8 +740,9 @@ MGP_API int mgp_rff_prior_values(const float* X, int64_t n, int d,
  * stride and any row stride (in elements).  Unlike the calls above these run
  * asynchronously on the caller's HIP stream (NULL: the default stream), take
  * their work buffers from the caller and allocate nothing, so that they can be
- * recorded into a HIP graph; the device of the arrays must be current.  Sums
- * and statistics are fp32.  Empty inputs (rows = 0) are valid: sums over them
+ * recorded into a HIP graph; the device of the arrays must be current.  Results
+ * share no memory with what a call reads, except that a layer norm's y may be x, its
+ * dx dy or x, and a dropout's y x or residual.  Sums and statistics are fp32.  Empty inputs (rows = 0) are valid: sums over them
  * are 0.  No counterpart in the reference. */
 
 /* One layer norm over the rows of x [rows][width]: y = (x - mean) * rstd *

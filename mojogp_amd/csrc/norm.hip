@@ -507,10 +507,6 @@ void layer_norm_backward(const NormArgs& a, const void* dy, int64_t dy_stride, c
     const T *x = static_cast<const T*>(a.x), *d = static_cast<const T*>(dy);
     int nblk = 0;
     if (a.rows > 0 && s.L == 0) {
-      if (dx)
-        k_norm_bwd_wide<T><<<(unsigned)std::min<int64_t>(a.rows, 2048), kNormThreads, 0, st>>>(
-            d, dy_stride, x, a.x_stride, a.rows, a.width, a.weight, a.f32_params, stats,
-            static_cast<T*>(dx), dx_stride);
       if (cols) {
         nblk = (int)std::min(a.rows, kNormWideRows);
         k_norm_cols_wide<T><<<dim3((unsigned)ceil_div(a.width, (int64_t)kNormThreads),
@@ -518,6 +514,10 @@ void layer_norm_backward(const NormArgs& a, const void* dy, int64_t dy_stride, c
                               kNormThreads, 0, st>>>(d, dy_stride, x, a.x_stride, a.rows, a.width,
                                                      stats, part);
       }
+      if (dx)  // (last: dx may be dy or x)
+        k_norm_bwd_wide<T><<<(unsigned)std::min<int64_t>(a.rows, 2048), kNormThreads, 0, st>>>(
+            d, dy_stride, x, a.x_stride, a.rows, a.width, a.weight, a.f32_params, stats,
+            static_cast<T*>(dx), dx_stride);
     } else if (a.rows > 0) {
       const int64_t groups = ceil_div(a.rows, (int64_t)(kNormThreads / s.L));
       nblk = (int)norm_blocks(groups);

@@ -176,7 +176,8 @@ def _norm_args(x, weight, bias, eps):
 def layer_norm(x, weight=None, bias=None, eps=1e-5, *, save=False, out=None):
     """Layer norm over the last dimension: ``(x - mean) / sqrt(var + eps) * weight + bias``.
 
-    weight and bias ([width], of x's type or float32) may be None.  With
+    weight and bias ([width], of x's type or float32) may be None.  ``out`` may be
+    x, but share no memory with it otherwise.  With
     ``save=True`` returns ``(y, saved)``, ``saved`` being what the backward
     pass takes (mean and reciprocal deviation of every row, float32)."""
     a, dtype, index, stream = _norm_args(x, weight, bias, eps)
@@ -233,7 +234,8 @@ def dropout(x, rate, seed, *, offset=0, residual=None, out=None):
     draw number ``offset + i`` alone, so that ``dropout_backward`` with the same
     seed and offset draws the same mask; the next call's offset is this one's
     plus ``x.numel()`` (multiples of 8 are fastest).  The rate in effect is
-    ``rate`` rounded to a multiple of 2^-16.  ``out`` may be x or residual."""
+    ``rate`` rounded to a multiple of 2^-16.  ``out`` may be x or residual, but share
+    no memory with them otherwise."""
     return _dropout(x, "x", rate, seed, offset, residual, out)
 
 
@@ -271,7 +273,8 @@ def gated_layer(x, w_gate, w_up, b_gate=None, b_up=None, *, activation="silu", o
 
     x [..., width], weights [hidden, width], biases [hidden] or None, all of one
     element type; result [..., hidden].  activation: "silu", "gelu" (with the
-    normal distribution's exact integral), "sigmoid" or "relu"."""
+    normal distribution's exact integral), "sigmoid" or "relu".  ``out`` shares no
+    memory with the inputs."""
     a, shape, dtype, index, stream = _gated_args(x, w_gate, w_up, b_gate, b_up, activation)
     out, ph, h_stride = _result(out, "out", x, shape, dtype, index)
     ws, nbytes = _gated_workspace(a, x, 0)
