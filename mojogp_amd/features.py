@@ -113,6 +113,8 @@ def _rows(a, name, dtype, index, shape=None):
 
 def _collapse(shape, strides, name):
     """Rows and row stride of more than two dimensions."""
+    if 0 in shape[:-1]:
+        return 0, shape[-1]
     rows, stride = 1, shape[-1]
     for size, step in zip(reversed(shape[:-1]), reversed(strides[:-1])):
         if size == 1:
