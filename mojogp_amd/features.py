@@ -14,7 +14,9 @@ float16, unit stride along the last dimension, leading dimensions that collapse
 to one row stride).  Their addresses go to the library's kernels; torch is not
 imported here and computes nothing, it provides the arrays, the memory of the
 results and the current stream, on which every call runs asynchronously.  The
-calls are explicit forward and backward passes and take no part in autograd.
+calls are explicit forward and backward passes and take no part in autograd: an
+array that requires a gradient is refused unless torch.no_grad() says that none is
+recorded.
 """
 
 from __future__ import annotations
@@ -65,6 +67,7 @@ def _first(a, name):
     if code is None:
         raise TypeError(f"{name} must be a float32, bfloat16 or float16 device tensor, got "
                         f"{dtype or type(a).__name__}")
+    _no_graph(torch, a, name)
     index = a.get_device()
     if index < 0:
         raise ValueError(f"{name} must be a device tensor, got one on {a.device}")
@@ -74,7 +77,16 @@ def _first(a, name):
     return dtype, code, index, _stream(torch, index)
 
 
+def _no_graph(torch, a, name):
+    """These calls record nothing: where a graph is being recorded, it would end here
+    without a word."""
+    if getattr(a, "requires_grad", False) and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, which these calls do not record: use "
+                         "detach() or torch.no_grad() and the explicit backward passes")
+
+
 def _check(a, name, dtype, index):
+    _no_graph(sys.modules.get("torch"), a, name)
     if getattr(a, "dtype", None) is not dtype:
         raise TypeError(f"{name} must have the element type of the first array ({dtype}), got "
                         f"{getattr(a, 'dtype', type(a).__name__)}")

@@ -38,3 +38,17 @@ def test_rows_of_more_dimensions():
     assert _rows(t[:, :1, :, :24][:1]) == (5, 24, 40)
     with pytest.raises(ValueError, match="collapse"):
         _rows(t[:, :, :4])
+
+
+def test_arrays_that_require_a_gradient_are_refused():
+    """No graph is recorded through these calls, so none may end in them unnoticed."""
+    x, w = torch.zeros(4, 8), torch.zeros(8, requires_grad=True)
+    with pytest.raises(ValueError, match="x requires a gradient"):
+        features.layer_norm(x.clone().requires_grad_())
+    with pytest.raises(ValueError, match="weight requires a gradient"):
+        features._vector(w, "weight", 8, torch.float32, -1)
+    with torch.no_grad():
+        assert features._vector(w, "weight", 8, torch.float32, -1) == w.data_ptr()
+        with pytest.raises(ValueError, match="device tensor"):  # the next check
+            features.layer_norm(x.clone().requires_grad_())
+    assert features._vector(w.detach(), "weight", 8, torch.float32, -1) == w.data_ptr()
