@@ -1382,12 +1382,14 @@ void dispatch_act(int act, F&& f) {
 }
 
 // Forward passes by k_gated_few: up to this many of its workgroups it is the
-// faster one.  16 bits: 512 rows x 256 -> 1024 (512 workgroups) 5.6 against 6.1 us,
-// 1024 rows 9.1 against 6.3; fp32, by fp32 instructions against the six products
-// and the kernel before them: 512 x 256 -> 1024 9.9 us, 1024 rows 19.
+// faster one, at any width, as either kernel's time grows with it.  Device time,
+// few against tiles, by workgroups, at widths 64 / 256 / 1024: 16 bits, 256 3.4 - 4.2 /
+// 4.3 - 5.9 / 8.1 - 12.2 us, 512 4.0 - 4.5 / 5.9 - 6.3 / 13.7 - 12.9, 768 5.5 - 4.7 / 8.0 - 6.6 /
+// 19 - 13; fp32, against six products and the kernel before them, 512 5.2 - 12 / 10.5 -
+// 26 / 30 - 78, 1024 8.4 - 13 / 18 - 27 / 56 - 83, 2048 15 - 14.5 / 32 - 31 / 106 - 87.
 inline bool takes_few(const GatedArgs& a) {
   return ceil_div(a.rows, (int64_t)64) * ceil_div(a.hidden, (int64_t)16) <=
-         (a.type == ELEM_F32 ? 768 : 512);
+         (a.type == ELEM_F32 ? 1536 : 512);
 }
 
 template <class T, int ACT>

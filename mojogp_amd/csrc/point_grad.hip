@@ -601,10 +601,12 @@ MmKernel pick_mm(int kind, int kb, int d, int64_t n) {
 inline float mm_norm_bound(int kind) {
   return kind == KIND_RBF ? 32.0f : kind == KIND_MATERN32 ? 256.0f : 512.0f;
 }
-// and the points from which its two more kernels pay (8
-// dimensions, 3000 points 31 -> 35 us, 4000 40 -> 34, 10000 140 -> 95, 50000 3130 ->
-// 1640).
-constexpr int64_t kMmPoints = 4000;
+// The points from which the matrix cores' five kernels pay: the differences' time
+// grows with the dimensions, theirs hardly.  Matern-5/2, 11 columns, differences
+// against matrix cores: 2 dimensions, 8000 points 67 - 79 us, 12000 131 - 133, 20000 336 -
+// 293; 4, 8000 77 - 80, 12000 150 - 133; 6, 4000 33 - 42, 6000 61 - 63, 8000 87 - 80; 8, 4000 43 -
+// 43, 6000 72 - 64; 16, 4000 63 - 46.
+inline int64_t mm_points(int d) { return d <= 4 ? 10000 : 4000; }
 
 struct PgWork {
   Provider& pv;
@@ -709,7 +711,7 @@ void point_gradient(Provider& pv, const float* Lf, const float* Rf, int ncols, f
     scale.v[k] = k < pv.d ? (float)(-(double)pv.outputscale() /
                                     ((double)kernel_scale(pv.kind) * (double)pv.lengthscale(k)))
                           : 0.0f;
-  const MmKernel mm = pv.n >= kMmPoints && pv.train.max_norm <= mm_norm_bound(pv.kind)
+  const MmKernel mm = pv.n >= mm_points(pv.d) && pv.train.max_norm <= mm_norm_bound(pv.kind)
                           ? pick_mm(pv.kind, pv.train.kb, pv.d, pv.n)
                           : MmKernel{nullptr, 0, 0};
   const UseScope use(pv.points_use, st);

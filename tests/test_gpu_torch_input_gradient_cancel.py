@@ -100,7 +100,7 @@ def test_clusters_in_some_rows_only(kind):
 def test_weights_on_near_pairs(kind):
     """Columns that weigh single pairs of neighbours."""
     rng = np.random.default_rng(9)
-    X = (rng.normal(size=(4200, 2)) * 2.0 / SCALE[kind]).astype(np.float32)
+    X = (rng.normal(size=(4200, 5)) * 1.5 / SCALE[kind]).astype(np.float32)
     L, R = (np.zeros((8, 4200), np.float32) for _ in range(2))
     for c, i in enumerate(rng.integers(0, 4200, 8)):
         near = np.argsort(((X - X[i]) ** 2).sum(axis=1))[1]

@@ -83,7 +83,7 @@ def _check_layer(args, act, kind, biased=True):
 def test_tiled_products(kind, act, width, pad):
     """More workgroups than the few-row kernel takes; rows direct loads can and
     cannot take, with and without biases."""
-    _check_layer(_layer(1501, width, 603, kind, pad), act, kind, biased=pad != 8)
+    _check_layer(_layer(1501, width, 1103, kind, pad), act, kind, biased=pad != 8)
 
 
 @pytest.mark.parametrize("kind", sorted(TYPES))
@@ -102,7 +102,7 @@ def test_large_tiles_of_every_product(kind, rows, width, hidden, pad):
 
 
 @pytest.mark.parametrize("kind", sorted(TYPES))
-@pytest.mark.parametrize("rows, width, hidden", [(1501, 250, 603), (32760, 96, 1279)])
+@pytest.mark.parametrize("rows, width, hidden", [(1501, 250, 1103), (32760, 96, 1279)])
 def test_tiled_products_keep_non_finite_rows_apart(kind, rows, width, hidden):
     x, *weights, dh = _layer(rows, width, hidden, kind)
     clean = features.gated_layer(x, *weights)
