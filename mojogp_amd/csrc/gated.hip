@@ -52,7 +52,7 @@ __device__ __forceinline__ float exp_of(float x, float tail = 0.0f) {
 // 1 - Phi(x) over exp(-x^2 / 2) for x = sqrt(2) v, v >= 0: a polynomial in
 // 1 / (1 + p v), p and the coefficients fitted by least squares reweighted
 // towards the smallest largest relative error over 0 <= v <= 9.5: 5.2e-6 (six
-// terms, the 16-bit types), 1.9e-8 (nine).
+// terms, the 16-bit types), 3.8e-8 (nine; 3.5e-7 as fp32 evaluates it).
 template <bool FAST>
 __device__ __forceinline__ float normal_tail(float v) {
   if constexpr (FAST) {
@@ -1175,11 +1175,11 @@ constexpr int64_t kMaxSplits = 64;
 // then ties every row to the largest value of all, and a scale a row still ties
 // the columns of a row to its largest.
 
-// The 16-bit types' dg and du are rounded to the type for the last two products;
-// with few rows the roundings do not average out, and dx's and the weight
-// gradients' error reaches 1.5 times that of their own rounding (1.41 with
-// many).  Up to one tile of rows dg and du go in two parts instead, and the last
-// two products run twice: bf16, 128 x 256 -> 1024, backward 31 -> 41 us, 100 x 1024 ->
+// The 16-bit types' dg and du are rounded to the type for the last two products:
+// with the result's own rounding that makes dx and the weight gradients 1.41 times
+// as far off as rounding alone, at any number of rows.  A second part takes that back
+// and runs the two products twice.  Up to one tile of rows, where a call is its
+// launches, it is worth it: bf16, 128 x 256 -> 1024, backward 31 -> 41 us, 100 x 1024 ->
 // 4096 59 -> 70; at 65536 rows it would cost 1.9 of 3.2 ms.
 constexpr int64_t kFewRows = 128;
 

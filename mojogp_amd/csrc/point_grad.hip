@@ -351,11 +351,11 @@ __device__ __forceinline__ void mm_stage(const char* next, int fragments, int kw
                                          f4 (&hz)[R][DZ]) {
   if (more) mm_load(next, fragments, nxt);
   const int lane = threadIdx.x & 63, lm = lane & 15, lq = lane >> 4;
-  float s1[R], s2[R];
+  float s1[R];
   f4 acc[R][DZ];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    s1[r] = s2[r] = 0.0f;
+    s1[r] = 0.0f;
 #pragma unroll
     for (int q = 0; q < DZ; ++q) acc[r][q] = f4{0.f, 0.f, 0.f, 0.f};
   }
@@ -393,18 +393,17 @@ __device__ __forceinline__ void mm_stage(const char* next, int fragments, int kw
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         s1[r] += hw[e];
-        s2[r] = fmaf(hw[e], hw[e], s2[r]);
+        sq[r] = fmaf(hw[e], hw[e], sq[r]);
 #pragma unroll
         for (int q = 0; q < DZ; ++q)
           acc[r][q] = __builtin_amdgcn_mfma_f32_16x16x4f32(hw[e], z[q][e], acc[r][q], 0, 0, 0);
       }
     }
   }
-  // two levels keep the rounding of long sums down
+  // two levels keep the rounding of long sums down (sq is for an estimate)
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     sum[r] += s1[r];
-    sq[r] += s2[r];
 #pragma unroll
     for (int q = 0; q < DZ; ++q) hz[r][q] += acc[r][q];
   }
@@ -417,8 +416,8 @@ __device__ __forceinline__ void mm_stage(const char* next, int fragments, int kw
 // columns as it stands, no lane exchanges it.  Bound by the VALU (Matern-5/2:
 // 6 instructions, a square root and an exponential a pair, 224 cycles a 16 x 16
 // tile) beside 192 cycles of matrix instructions of d <= 8; the two add up more than
-// they overlap: 50000 points, 16 columns, the whole call 1710 us, 1.5e12 pairs a
-// second; 1635 without the sum of squares and what follows from it.
+// they overlap: 50000 points, 16 columns, the whole call 1700 us, 1.5e12 pairs a
+// second; 1630 without the sum of squares and what follows from it.
 template <int KIND, int KB, int DZ, int R>
 __global__ __launch_bounds__(256, 3) void k_point_grad_mm(
     const char* __restrict__ col, const uint4* __restrict__ B, const uint4* __restrict__ wrow,
@@ -572,10 +571,11 @@ struct MmKernel {
   int dz, row_tiles;  // 16-row tiles of a workgroup
 };
 
-// Rows a wave: four 16-row tiles for many points (8 dimensions, 30000 points 594
-// us, 620 with two; 50000 1640, 1676), two below, for more workgroups (10000 points
-// 95 us, 102 with four; 20000 276, 298), and with two distance operands, where four
-// leave too few registers (20000 points of 16 dimensions 298, 335).
+// Rows a wave: four 16-row tiles for many points (8 dimensions, 30000 points 619
+// us, 647 with two; 50000 1701, 1750), two below, for more workgroups (10000 points
+// 112 us, 120 with four; 20000 294, 315), and with two distance operands, where four
+// leave too few registers (20000 points of 16 dimensions, without the sum of
+// squares, 298, 335).
 constexpr int64_t kMmFourTiles = 25000;
 template <int KIND>
 MmKernel pick_mm(int kb, int d, int64_t n) {

@@ -301,7 +301,9 @@ def gated_layer_backward(dh, x, w_gate, w_up, b_gate=None, b_up=None, *, activat
     """Gradients of ``gated_layer`` as ``GatedGradients(dx, dw_gate, dw_up, db_gate, db_up)``.
 
     The projections are formed again from x: nothing is kept between the
-    passes.  ``need_dx=False`` (the first layer, whose x is data) and
+    passes.  In the 16-bit types the gradients of g and u are rounded to the type
+    (float16: times a power of two for each row) before the last products; up to 128
+    rows they go in two parts.  ``need_dx=False`` (the first layer, whose x is data) and
     ``need_dw=False`` leave those products out."""
     a, shape, dtype, index, stream = _gated_args(x, w_gate, w_up, b_gate, b_up, activation)
     pdh, _, _, dh_stride = _rows(dh, "dh", dtype, index, shape)
