@@ -137,6 +137,9 @@ __device__ __forceinline__ void store_run(T* p, int64_t left, const float* v) {
 // difference of infinities is formed and a product meets them once.
 template <int P, int N, class E>
 __device__ __forceinline__ void store_parts(E* p, int64_t apart, int64_t left, const float* v) {
+  // (without the copies below: the backward epilogue of bf16 12007 x 391 -> 1027 is
+  // scheduled 12 % faster)
+  if constexpr (P == 1) return store_run<N>(p, left, v);
   constexpr float kMost = std::is_same<E, __bf16>::value ? 3.3895313892515355e38f : 65504.0f;
   float rest[N], part[N];
 #pragma unroll
@@ -464,9 +467,10 @@ constexpr bool stays = TL::W == 8 && EPI::FORWARD;
 // (NT, tn < T1) 16 T1 wn + RUN (l / 16) + 4 tn + e of either matrix, (TN)
 // 16 (wn TN + tn) + 4 (l / 16) + e.
 //
-// Bound by the matrix cores' feeding: 65536 x 1024 -> 4096 in bf16 takes 990 us
-// forward (1110 TFLOP/s), 1325 for g, u, dg and du, 930 for dx (1180) and 960 for
-// the weight gradients (1145), where a plain large product reaches 1420.  The big
+// Bound by the matrix cores' feeding: of 65536 x 1024 -> 4096 in bf16 the forward
+// pass takes 1070 us (1030 TFLOP/s), g, u, dg and du 1480 (740: the epilogue reads and
+// writes 1.6 GB), dx 920 (1195) and the weight gradients 975 (1130), all in turn, where
+// a plain large product reaches 1420; the forward pass alone 990.  The big
 // tile leaves room for one workgroup a CU, whose epilogue nothing covers; two of the
 // small one cover each other, but read twice the operands from LDS and the L1 cache.
 template <class TL, class EPI>
@@ -978,7 +982,7 @@ __global__ __launch_bounds__(256) void k_transpose_split(const __bf16* __restric
 // rows, take x over the row's scale instead of x, times the power of two that
 // fits the largest.  bfloat16 and float32 have the range as they are.  Three kernels
 // that read dh and x once, HBM and latency bound: backward, 128 x 256 -> 1024 42 -> 52
-// us, 20000 x 256 -> 512 95 -> 129, 65536 x 1024 -> 4096 3310 -> 3810 (255 of it here, the
+// us, 20000 x 256 -> 512 96 -> 126, 65536 x 1024 -> 4096 3340 -> 3660 (255 of it here, the
 // rest the epilogue's).
 struct ScaleSource {
   const _Float16 *x, *dh, *wg, *wu, *bg, *bu;
