@@ -67,7 +67,8 @@ def _first(a, name):
     if code is None:
         raise TypeError(f"{name} must be a float32, bfloat16 or float16 device tensor, got "
                         f"{dtype or type(a).__name__}")
-    _no_graph(torch, a, name)
+    if a.requires_grad:
+        _no_graph(name)
     index = a.get_device()
     if index < 0:
         raise ValueError(f"{name} must be a device tensor, got one on {a.device}")
@@ -77,19 +78,20 @@ def _first(a, name):
     return dtype, code, index, _stream(torch, index)
 
 
-def _no_graph(torch, a, name):
+def _no_graph(name):
     """These calls record nothing: where a graph is being recorded, it would end here
     without a word."""
-    if getattr(a, "requires_grad", False) and torch.is_grad_enabled():
+    if _torch().is_grad_enabled():
         raise ValueError(f"{name} requires a gradient, which these calls do not record: use "
                          "detach() or torch.no_grad() and the explicit backward passes")
 
 
 def _check(a, name, dtype, index):
-    _no_graph(sys.modules.get("torch"), a, name)
     if getattr(a, "dtype", None) is not dtype:
         raise TypeError(f"{name} must have the element type of the first array ({dtype}), got "
                         f"{getattr(a, 'dtype', type(a).__name__)}")
+    if a.requires_grad:
+        _no_graph(name)
     if a.get_device() != index:
         raise ValueError(f"{name} must be on device {index}, got {a.device}")
 

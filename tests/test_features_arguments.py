@@ -9,7 +9,7 @@ from mojogp_amd import features
 
 def _rows(t):
     class Device:  # the tensor, but for its device
-        dtype, shape = t.dtype, t.shape
+        dtype, shape, requires_grad = t.dtype, t.shape, t.requires_grad
 
         def stride(self):
             return t.stride()
