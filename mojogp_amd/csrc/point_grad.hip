@@ -496,21 +496,24 @@ __global__ __launch_bounds__(256, 3) void k_point_grad_mm(
 
 // out[i][q] (+)= scale_q unscale v_iq, v_iq = z_iq S_i - sum of part, S_i = sum of
 // sums, for a block of kPgRows rows, if its v stands out from the error that its sums
-// left.  That error's norm over a row, measured on 4096 points of 1 to 24
-// dimensions, Gaussian and in clusters of radius 1 to 0.001, all three kernels, is
-// 1.8e-7 to 6e-7 of |z_i| sqrt(Q_i), Q_i = sum_b (W h)^2 (the roundings of distances,
-// weights and sums); long sums of one sign round off up to 1.2e-7 of |z_i| |S_i|.
-// With 4.8e-7 for the first a block passes where both are below 1.5e-6 of |v|:
-// |v|^2 >= sum_i |z_i|^2 (Q_i + S_i^2 / 16) / 10; Gaussian points have 0.2 to 0.9 of
-// |z|^2 Q.  And where every row's weights stand out from the end of their two parts,
-// 2^-25 beside factors of up to 2^15: Q_i >= floor = (2^-10 / 1.5e-6)^2 2 ncols n.
+// left.  Over a row that is taken as
+//   5e-7 |z_i| sqrt(Q_i) and 1e-6 |z_i| |S_i| of the closing difference, Q_i = sum_b (W h)^2,
+//   share |z_i|^2 of v_i itself, as the distances' roundings grow with the norms,
+// measured on 561 sets of 4100 to 26000 points of 2 to 31 dimensions: Gaussian,
+// uniform, in clusters, in pairs, in order on a line and on a shell at the norm's
+// bound, weights random, constant, smooth and those of a marginal likelihood.  A block
+// passes below 3e-6 of its v; those that did were up to 2.9e-6 off (Matern) and, RBF,
+// 4.1e-6 in 99 of 100, at most 8.2e-6 (points in order far out, smooth weights).
+// And every row's weights have to stand out from the end of their two parts, 2^-25
+// beside factors of up to 2^15: Q_i >= floor = (2^-10 / 1.5e-6)^2 2 ncols n.
 // failed[block]: to be formed by differences.
 __global__ __launch_bounds__(1024) void k_point_grad_mm_sum(
     const float* __restrict__ part, const float* __restrict__ sums, const float* __restrict__ Z,
     int64_t splits, int64_t n, int d, PgScale scale, const float* __restrict__ unscale,
-    float floor, int accumulate, int* __restrict__ failed, float* __restrict__ out) {
+    float floor, float share, int accumulate, int* __restrict__ failed,
+    float* __restrict__ out) {
   __shared__ double total[kPgRows];
-  __shared__ float value[kPgRows * 32], red[2][16];
+  __shared__ float value[kPgRows * 32], own[kPgRows], red[2][16];
   const int64_t row0 = (int64_t)blockIdx.x * kPgRows;
   const int rows = (int)min((int64_t)kPgRows, n - row0);
   float need = 0.0f, have = 0.0f;
@@ -525,7 +528,9 @@ __global__ __launch_bounds__(1024) void k_point_grad_mm_sum(
     total[threadIdx.x] = s;
     float zz = 0.0f;
     for (int k = 0; k < d; ++k) zz = fmaf(Z[row * d + k], Z[row * d + k], zz);
-    need = q >= (double)floor ? 0.1f * zz * (float)(q + 0.0625 * s * s) : INFINITY;
+    need = q >= (double)floor ? zz * (float)(q / 36.0 + s * s / 9.0) : INFINITY;
+    const float lost = share / 3e-6f * zz;
+    own[threadIdx.x] = fmaf(-lost, lost, 1.0f);
   }
   __syncthreads();
   for (int e = threadIdx.x; e < rows * d; e += 1024) {
@@ -534,7 +539,7 @@ __global__ __launch_bounds__(1024) void k_point_grad_mm_sum(
     for (int64_t p = 0; p < splits; ++p) hz += (double)part[(p * n + row0) * d + e];
     const float v = (float)((double)Z[row0 * d + e] * total[e / d] - hz);
     value[e] = v;
-    have = fmaf(v, v, have);
+    have = fmaf(v * own[e / d], v, have);
   }
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) {
@@ -600,6 +605,10 @@ MmKernel pick_mm(int kind, int kb, int d, int64_t n) {
 // of the Gram form's distances alone comes near the bound of k_point_grad_mm_sum.
 inline float mm_norm_bound(int kind) {
   return kind == KIND_RBF ? 32.0f : kind == KIND_MATERN32 ? 256.0f : 512.0f;
+}
+// and what their rounding takes of a row, over |z|^2 (k_point_grad_mm_sum)
+inline float mm_error_share(int kind) {
+  return kind == KIND_RBF ? 1.3e-7f : kind == KIND_MATERN32 ? 3.8e-8f : 1.7e-8f;
 }
 // The points from which the matrix cores' five kernels pay: the differences' time
 // grows with the dimensions, theirs hardly.  Matern-5/2, 11 columns, differences
@@ -694,8 +703,8 @@ void gradient_matrix_cores(const PgWork& w, const MmKernel& kernel, const PgScal
                      ws + sums);
   const float floor = 4.24e5f * 2.0f * (float)w.ncols * (float)n;  // (see the kernel)
   k_point_grad_mm_sum<<<(unsigned)again.rb, 1024, 0, w.st>>>(
-      ws + part, ws + sums, pts.z.ptr, splits, n, d, scaled, ws + unscale, floor, w.accumulate,
-      fail, w.out);
+      ws + part, ws + sums, pts.z.ptr, splits, n, d, scaled, ws + unscale, floor,
+      mm_error_share(pv.kind), w.accumulate, fail, w.out);
   gradient_differences(w, scale, again, false, ws + part, fail);
 }
 

@@ -131,3 +131,37 @@ def test_weights_of_different_sizes(kind, case):
     got, (want, coords, own, terms) = _gradient(kind, X, L, R), _formula(kind, X, L, R)
     err = np.linalg.norm(got - want, axis=1)
     assert np.all(err <= 3 * 6e-7 * coords + 4 * TOL * own + 2.0 ** -21 * terms + 1e-37)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_points_in_order(kind):
+    """Points in order on a line out to the route's bound, weights as those of a
+    marginal likelihood: the roundings of neighbours are alike and do not average out.
+    Block by block of 128 rows, twice what the route lets pass (RBF, whose values fall
+    fastest with the distance: three times), beside the coordinates' rounding, here of
+    sums S of one sign as well."""
+    rng = np.random.default_rng(21)
+    n = 10240
+    X = np.zeros((n, 5))
+    X[:, 0] = np.linspace(-0.9, 0.9, n) * np.sqrt(REACH[kind]) / SCALE[kind]
+    X[:, 1] = 0.01 * np.sin(np.arange(n))
+    X = X.astype(np.float32)
+    alpha, probes = 10.0 * (np.sin(3.0 * X[:, 0]) + 0.1 * rng.normal(size=n)), \
+        rng.normal(size=(10, n))
+    L = np.vstack([-0.5 * alpha, probes / 20.0]).astype(np.float32)
+    R = np.vstack([alpha, probes]).astype(np.float32)
+    got, (want, coords, _, _) = _gradient(kind, X, L, R), _formula(kind, X, L, R)
+    sums = np.empty(n)
+    for i in range(0, n, 512):  # |z| sum_b W h
+        df = (X[i:i + 512, None, :2] - X[None, :, :2]).astype(np.float64)
+        u = np.sqrt((df ** 2).sum(axis=2) * {"rbf": 1.0, "matern32": 3.0, "matern52": 5.0}[kind])
+        h = np.exp(-0.5 * u ** 2) if kind == "rbf" else np.exp(-u) * \
+            (3.0 if kind == "matern32" else 5.0 / 3.0 * (1.0 + u))
+        w = L[:, i:i + 512].astype(np.float64).T @ R + R[:, i:i + 512].astype(np.float64).T @ L
+        sums[i:i + 512] = (h * w).sum(axis=1)
+    sums *= np.linalg.norm(X - X.mean(axis=0), axis=1)
+    blocks = [np.sqrt((a ** 2).reshape(n // 128, -1).sum(axis=1))
+              for a in (got - want, want, coords, sums)]
+    err, size, coords, sums = blocks
+    times = 3 if kind == "rbf" else 2
+    assert np.all(err <= times * 3e-6 * size + 2.0 ** -24 * (coords + sums))
