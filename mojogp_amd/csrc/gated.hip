@@ -14,8 +14,9 @@
 // epilogue, dx against the transposed weights, and the weight gradients with
 // the reduction over the rows split over the device.
 //
-// dg and du are rounded to the element type before the last two products, as
-// the matrix cores take them; g, u, all sums and the bias gradients stay fp32.
+// dg and du go into the last two products as the matrix cores take them: rounded to
+// bfloat16, to float16 times a power of two of their row, in float32 in three parts
+// (24 bits); g, u, all sums and the bias gradients stay fp32.
 #include "layers.h"
 
 #include <algorithm>
