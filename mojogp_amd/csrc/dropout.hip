@@ -8,38 +8,15 @@
 // serve eight elements: with 32 bits the ten rounds (two 32 x 32 -> 64 bit
 // products each) would take longer than the array's transfer.  HBM bound: bf16,
 // 250000 x 1024 with a residual 300 us (5.1 TB/s), without 193 (5.3).
-#include "layers.h"
-
 #include <algorithm>
 #include <type_traits>
+
+#include "layers.h"
+#include "philox.h"
 
 namespace mgp {
 
 namespace {
-
-struct Draws {
-  uint32_t w[4];
-  __device__ __forceinline__ uint32_t half(int i) const {
-    return (w[i >> 1] >> (16 * (i & 1))) & 0xffffu;
-  }
-};
-
-__device__ __forceinline__ Draws philox(uint64_t block, uint64_t seed) {
-  uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32), c2 = 0, c3 = 0;
-  uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
-#pragma unroll
-  for (int i = 0; i < 10; ++i) {
-    const uint64_t p0 = (uint64_t)c0 * 0xD2511F53u, p1 = (uint64_t)c2 * 0xCD9E8D57u;
-    const uint32_t n0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0, n2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1;
-    c1 = (uint32_t)p1;
-    c3 = (uint32_t)p0;
-    c0 = n0;
-    c2 = n2;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
-  }
-  return {{c0, c1, c2, c3}};
-}
 
 __device__ __forceinline__ float kept(float x, uint32_t draw, uint32_t cut, float scale) {
   // a dropped element is 0 whatever it held, infinities and NaN included
