@@ -821,6 +821,77 @@ MGP_API int mgp_gated_layer_backward_device(const mgp_gated_layer_t* args, const
                                             void* workspace, int64_t workspace_bytes,
                                             void* stream);
 
+/* AdamW over many tensors at once (decoupled weight decay):
+ *   g = grad * grad_scale * min(1, max_norm / norm), norm = |all grads * grad_scale|
+ *   m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - rate decay) - rate (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps)
+ * Parameters: contiguous arrays of one element type that share no memory.  The
+ * states and the fp32 master copies (of 16-bit parameters; they are then what is
+ * updated, the parameters being rounded from them) lie in arrays of `values` values,
+ * each tensor's from a multiple of 256 on; what lies behind a tensor's last value
+ * stays unread.
+ * 32-bit states: exp_avg, exp_avg_sq are float.  8-bit states: bytes, with one float
+ * scale for 256 values.  exp_avg: an OCP e4m3 value times its scale (largest |m| *
+ * (1/448)).  exp_avg_sq: exponent e (5 bits) and mantissa f (3 bits), (1 + f/8)
+ * 2^(e-31) or, for e = 0, f/8 2^-30, times its scale (largest v * (1/1.875)).  Value i
+ * is rounded by word i % 4 of the Philox4x32-10 block of counter (i / 4, t) and key
+ * seed, its low half for m, its high half for v: in units of a code's step, the value
+ * plus (half + 1/2) / 2^16 is cut off.  A v above 0 has code 1 at least.  Blocks
+ * whose largest value is below 2^-120 become 0; an infinity or NaN makes NaN of its
+ * block's state. */
+typedef struct mgp_adamw_tensor {
+  void* param;
+  int64_t size;
+  float weight_decay;
+} mgp_adamw_tensor_t;
+typedef struct mgp_adamw {
+  int type;
+  int bits;          /* of the states: 32 or 8 */
+  int master_copies;
+  int64_t count;
+  const mgp_adamw_tensor_t* tensors; /* host array */
+  double beta1;
+  double beta2;
+  double eps;
+  uint64_t seed;     /* of the 8-bit states' rounding */
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;
+  float* exp_avg_sq_scale;
+  float* master;
+  const void* table; /* device array of table_bytes */
+} mgp_adamw_t;
+/* Values of a state array and bytes of the table. */
+MGP_API int mgp_adamw_layout(const mgp_adamw_t* args, int64_t* values, int64_t* table_bytes);
+/* A plan (host memory only) and the table's content, which the caller copies to
+ * args->table before the first step. */
+MGP_API int mgp_adamw_create(const mgp_adamw_t* args, void* host_table, int64_t bytes,
+                             void** plan);
+MGP_API int mgp_adamw_destroy(void* plan);
+/* One step: t is step (from 1 on), or what step_device holds; the rate likewise
+ * (float).  grads: a host array of device arrays, of the parameters' type or of
+ * float32 (grad_type); tensors whose entry is NULL are left as they are.  form_norm:
+ * the norm is formed and written to norm (may be NULL), gradients are scaled down to
+ * max_norm (infinity: they are not), and nothing is changed where it is not finite. */
+typedef struct mgp_adamw_step {
+  const void* const* grads;
+  int grad_type;
+  int form_norm;
+  double grad_scale;
+  double max_norm;
+  float* norm;
+  int64_t step;
+  const int64_t* step_device;
+  const float* rate_device;
+  float rate;
+} mgp_adamw_step_t;
+MGP_API int mgp_adamw_workspace(void* plan, const mgp_adamw_step_t* args, int64_t* bytes);
+MGP_API int mgp_adamw_step_device(void* plan, const mgp_adamw_step_t* args, void* workspace,
+                                  int64_t workspace_bytes, void* stream);
+/* What 8-bit states stand for, [values] each. */
+MGP_API int mgp_adamw_values_device(void* plan, float* exp_avg, float* exp_avg_sq,
+                                    void* stream);
+
 /* Streaming device copy of `bytes` repeated `repeats` times; ms_avg gets the
  * mean duration of one copy.  Used only to calibrate HBM byte counters
  * (FETCH_SIZE / WRITE_SIZE) against a kernel of known traffic.  No reference

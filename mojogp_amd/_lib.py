@@ -69,6 +69,32 @@ class GatedLayer(C.Structure):
     ]
 
 
+class AdamWTensor(C.Structure):
+    """mgp_adamw_tensor_t"""
+    _fields_ = [("param", C.c_void_p), ("size", C.c_int64), ("weight_decay", C.c_float)]
+
+
+class AdamW(C.Structure):
+    """mgp_adamw_t"""
+    _fields_ = [
+        ("type", C.c_int), ("bits", C.c_int), ("master_copies", C.c_int), ("count", C.c_int64),
+        ("tensors", C.POINTER(AdamWTensor)), ("beta1", C.c_double), ("beta2", C.c_double),
+        ("eps", C.c_double), ("seed", C.c_uint64), ("exp_avg", C.c_void_p),
+        ("exp_avg_sq", C.c_void_p), ("exp_avg_scale", C.c_void_p),
+        ("exp_avg_sq_scale", C.c_void_p), ("master", C.c_void_p), ("table", C.c_void_p),
+    ]
+
+
+class AdamWStep(C.Structure):
+    """mgp_adamw_step_t"""
+    _fields_ = [
+        ("grads", c_void_pp), ("grad_type", C.c_int), ("form_norm", C.c_int),
+        ("grad_scale", C.c_double), ("max_norm", C.c_double), ("norm", C.c_void_p),
+        ("step", C.c_int64), ("step_device", C.c_void_p), ("rate_device", C.c_void_p),
+        ("rate", C.c_float),
+    ]
+
+
 PROGRESS_CB = C.CFUNCTYPE(None, C.POINTER(Progress), C.c_void_p)
 
 
@@ -300,6 +326,13 @@ _SIGNATURES = {
                                                   C.c_void_p, C.c_void_p, C.c_void_p,
                                                   C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
                                                   C.c_void_p]),
+    "mgp_adamw_layout": (C.c_int, [C.POINTER(AdamW), c_int64_p, c_int64_p]),
+    "mgp_adamw_create": (C.c_int, [C.POINTER(AdamW), C.c_void_p, C.c_int64, c_void_pp]),
+    "mgp_adamw_destroy": (C.c_int, [C.c_void_p]),
+    "mgp_adamw_workspace": (C.c_int, [C.c_void_p, C.POINTER(AdamWStep), c_int64_p]),
+    "mgp_adamw_step_device": (C.c_int, [C.c_void_p, C.POINTER(AdamWStep), C.c_void_p, C.c_int64,
+                                        C.c_void_p]),
+    "mgp_adamw_values_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "mgp_rff_prior_values": (C.c_int, [c_float_p, C.c_int64, C.c_int, c_double_p, c_double_p,
                                        c_double_p, C.c_int, C.c_double, c_double_p, C.c_int,
                                        c_float_p]),
