@@ -741,7 +741,7 @@ MGP_API int mgp_rff_prior_values(const float* X, int64_t n, int d,
  * asynchronously on the caller's HIP stream (NULL: the default stream), take
  * their work buffers from the caller and allocate nothing, so that they can be
  * recorded into a HIP graph; the device of the arrays must be current.  Results
- * share no memory with what a call reads, except that a layer norm's y may be x, its
+ * share no memory with what a call reads, except that a norm's y may be x, its
  * dx dy or x, and a dropout's y x or residual.  Sums and statistics are fp32.  Empty inputs (rows = 0) are valid: sums over them
  * are 0.  No counterpart in the reference. */
 
@@ -820,6 +820,38 @@ MGP_API int mgp_gated_layer_backward_device(const mgp_gated_layer_t* args, const
                                             void* dw_up, void* db_gate, void* db_up,
                                             void* workspace, int64_t workspace_bytes,
                                             void* stream);
+
+/* A group norm with an activation, channels last: x [samples][positions][channels]
+ * (row n positions + l, any row stride), the channels in `groups` of consecutive
+ * ones; y = act((x - mean) * rstd * weight + bias), mean and rstd = 1 / sqrt(var +
+ * eps) over a sample's positions and a group's channels.  activation: as of the gated
+ * layer, or -1 for none.  weight, bias [channels] may be NULL (ones, zeros);
+ * param_type: their type, the element type or float32.  y may be x. */
+typedef struct mgp_group_norm {
+  int type;
+  int param_type;
+  int activation;
+  float eps;
+  int64_t samples;
+  int64_t positions;
+  int64_t channels;
+  int64_t groups;
+  const void* x;
+  int64_t x_stride;
+  const void* weight;
+  const void* bias;
+} mgp_group_norm_t;
+MGP_API int mgp_group_norm_workspace(const mgp_group_norm_t* args, int backward, int64_t* bytes);
+/* stats (may be NULL): [samples][groups][2], mean and rstd, for the backward pass. */
+MGP_API int mgp_group_norm_device(const mgp_group_norm_t* args, void* y, int64_t y_stride,
+                                  float* stats, void* workspace, int64_t workspace_bytes,
+                                  void* stream);
+/* dx (may be dy or x), dweight and dbias [channels] (of param_type); any may be NULL. */
+MGP_API int mgp_group_norm_backward_device(const mgp_group_norm_t* args, const void* dy,
+                                           int64_t dy_stride, const float* stats, void* dx,
+                                           int64_t dx_stride, void* dweight, void* dbias,
+                                           void* workspace, int64_t workspace_bytes,
+                                           void* stream);
 
 /* AdamW over many tensors at once (decoupled weight decay):
  *   g = grad * grad_scale * min(1, max_norm / norm), norm = |all grads * grad_scale|

@@ -69,6 +69,16 @@ class GatedLayer(C.Structure):
     ]
 
 
+class GroupNorm(C.Structure):
+    """mgp_group_norm_t"""
+    _fields_ = [
+        ("type", C.c_int), ("param_type", C.c_int), ("activation", C.c_int), ("eps", C.c_float),
+        ("samples", C.c_int64), ("positions", C.c_int64), ("channels", C.c_int64),
+        ("groups", C.c_int64), ("x", C.c_void_p), ("x_stride", C.c_int64),
+        ("weight", C.c_void_p), ("bias", C.c_void_p),
+    ]
+
+
 class AdamWTensor(C.Structure):
     """mgp_adamw_tensor_t"""
     _fields_ = [("param", C.c_void_p), ("size", C.c_int64), ("weight_decay", C.c_float)]
@@ -326,6 +336,12 @@ _SIGNATURES = {
                                                   C.c_void_p, C.c_void_p, C.c_void_p,
                                                   C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
                                                   C.c_void_p]),
+    "mgp_group_norm_workspace": (C.c_int, [C.POINTER(GroupNorm), C.c_int, c_int64_p]),
+    "mgp_group_norm_device": (C.c_int, [C.POINTER(GroupNorm), C.c_void_p, C.c_int64, C.c_void_p,
+                                        C.c_void_p, C.c_int64, C.c_void_p]),
+    "mgp_group_norm_backward_device": (C.c_int, [C.POINTER(GroupNorm), C.c_void_p, C.c_int64,
+                                                 C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p,
+                                                 C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
     "mgp_adamw_layout": (C.c_int, [C.POINTER(AdamW), c_int64_p, c_int64_p]),
     "mgp_adamw_create": (C.c_int, [C.POINTER(AdamW), C.c_void_p, C.c_int64, c_void_pp]),
     "mgp_adamw_destroy": (C.c_int, [C.c_void_p]),

@@ -85,4 +85,17 @@ void dispatch_act(int act, F&& f) {
   }
 }
 
+// The same within a kernel, for an activation that is the same for all threads.
+template <class F>
+__device__ __forceinline__ void dispatch_act_device(int act, F&& f) {
+  if (act == ACT_SILU)
+    f(std::integral_constant<int, ACT_SILU>{});
+  else if (act == ACT_GELU)
+    f(std::integral_constant<int, ACT_GELU>{});
+  else if (act == ACT_SIGMOID)
+    f(std::integral_constant<int, ACT_SIGMOID>{});
+  else
+    f(std::integral_constant<int, ACT_RELU>{});
+}
+
 }  // namespace mgp

@@ -112,6 +112,39 @@ GatedArgs gated_args(const mgp_gated_layer_t* a) {
           a->b_up};
 }
 
+GroupArgs group_args(const mgp_group_norm_t* a) {
+  MGP_REQUIRE(a != nullptr, "null arguments");
+  MGP_REQUIRE(valid_elem(a->type), "unknown element type");
+  MGP_REQUIRE(a->activation == -1 || valid_activation(a->activation), "unknown activation");
+  MGP_REQUIRE(a->samples >= 0 && a->samples < kMaxRows && a->positions >= 0 &&
+                  a->positions < kMaxRows && a->samples * a->positions < kMaxRows,
+              "samples, positions and their product must be in [0, 2^31)");
+  MGP_REQUIRE(a->channels >= 1 && a->channels <= kMaxWidth, "channels must be in [1, 2^24]");
+  MGP_REQUIRE(a->groups >= 1 && a->channels % a->groups == 0,
+              "the channels must be a multiple of the groups");
+  MGP_REQUIRE(a->param_type == a->type || a->param_type == ELEM_F32,
+              "weight and bias must be of the element type or float32");
+  MGP_REQUIRE(std::isfinite(a->eps) && a->eps >= 0.0f, "eps must be finite and >= 0");
+  check_rows("x", a->x, a->x_stride, a->samples * a->positions, a->channels);
+  return {a->type,          a->activation,   a->x,      a->x_stride, a->samples, a->positions,
+          (int)a->channels, (int)a->groups, a->weight, a->bias,     a->param_type == ELEM_F32,
+          a->eps};
+}
+
+Span row_span(const char* name, const GroupArgs& a, const void* p, int64_t stride) {
+  return span(name, p, a.samples * a.positions, a.channels, stride, elem_bytes(a.type));
+}
+Span param_span(const char* name, const GroupArgs& a, const void* p) {
+  return span(name, p, 1, a.channels, a.channels, a.f32_params ? 4 : elem_bytes(a.type));
+}
+void check_pairs(const float* stats) {
+  MGP_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 7) == 0, "the statistics must be 8-byte aligned");
+}
+Span stats_span(const GroupArgs& a, const void* p) {
+  const int64_t n = 2 * a.samples * a.groups;
+  return span("stats", p, a.positions ? 1 : 0, n, n, sizeof(float));
+}
+
 }  // namespace
 
 extern "C" {
@@ -230,6 +263,66 @@ int mgp_gated_layer_backward_device(const mgp_gated_layer_t* args, const void* d
     }
     gated_backward(a, dh, dh_stride, {dx, dw_gate, dw_up, db_gate, db_up}, workspace,
                    static_cast<hipStream_t>(stream));
+  });
+}
+
+int mgp_group_norm_workspace(const mgp_group_norm_t* args, int backward, int64_t* bytes) {
+  return guarded([&] {
+    MGP_REQUIRE(bytes != nullptr, "null result");
+    *bytes = (int64_t)group_norm_bytes(group_args(args), backward != 0);
+  });
+}
+
+int mgp_group_norm_device(const mgp_group_norm_t* args, void* y, int64_t y_stride, float* stats,
+                          void* workspace, int64_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    const GroupArgs a = group_args(args);
+    check_rows("y", y, y_stride, a.samples * a.positions, a.channels);
+    const Span out = row_span("y", a, y, y_stride), moments = stats_span(a, stats);
+    const Span of_x = row_span("x", a, a.x, a.x_stride);
+    check_pairs(stats);
+    check_apart(out, of_x, true);
+    check_apart(moments, of_x, false);
+    check_apart(moments, out, false);
+    for (const Span& q : {param_span("weight", a, a.weight), param_span("bias", a, a.bias)}) {
+      check_apart(out, q, false);
+      check_apart(moments, q, false);
+    }
+    check_workspace(workspace, workspace_bytes, group_norm_bytes(a, false));
+    group_norm(a, y, y_stride, stats, workspace, static_cast<hipStream_t>(stream));
+  });
+}
+
+int mgp_group_norm_backward_device(const mgp_group_norm_t* args, const void* dy,
+                                   int64_t dy_stride, const float* stats, void* dx,
+                                   int64_t dx_stride, void* dweight, void* dbias,
+                                   void* workspace, int64_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    const GroupArgs a = group_args(args);
+    const int64_t rows = a.samples * a.positions;
+    check_rows("dy", dy, dy_stride, rows, a.channels);
+    MGP_REQUIRE(rows == 0 || stats != nullptr, "null statistics");
+    check_pairs(stats);
+    if (dx) check_rows("dx", dx, dx_stride, rows, a.channels);
+    const Span of_dy = row_span("dy", a, dy, dy_stride), of_x = row_span("x", a, a.x, a.x_stride);
+    const Span of_dx = row_span("dx", a, dx, dx_stride);
+    const Span of_dw = param_span("dweight", a, dweight), of_db = param_span("dbias", a, dbias);
+    check_apart(of_dx, of_dy, true);
+    check_apart(of_dx, of_x, true);
+    for (const Span& out : {of_dx, of_dw, of_db}) {
+      if (out.name != of_dx.name) {
+        check_apart(out, of_dy, false);
+        check_apart(out, of_x, false);
+        check_apart(out, of_dx, false);
+      }
+      check_apart(out, param_span("weight", a, a.weight), false);
+      check_apart(out, param_span("bias", a, a.bias), false);
+      check_apart(out, stats_span(a, stats), false);
+    }
+    check_apart(of_dw, of_db, false);
+    check_workspace(workspace, workspace_bytes, group_norm_bytes(a, true));
+    group_norm_backward(a, dy, dy_stride, stats, dx, dx_stride, dweight, dbias, workspace,
+                        static_cast<hipStream_t>(stream));
   });
 }
 

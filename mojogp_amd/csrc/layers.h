@@ -53,6 +53,29 @@ void layer_norm_backward(const NormArgs& a, const void* dy, int64_t dy_stride, c
                          void* dx, int64_t dx_stride, void* dweight, void* dbias, void* ws,
                          hipStream_t st);
 
+// y = act((x - mean) rstd w + b), mean and rstd over a sample's positions and the
+// channels of a group; x's row of sample n and position l is n positions + l.
+// stats[samples][groups][2] = mean, rstd (or null).
+struct GroupArgs {
+  int type;
+  int activation;  // or -1: none
+  const void* x;
+  int64_t x_stride;
+  int64_t samples, positions;
+  int channels, groups;
+  const void* weight;  // [channels] or null (ones), of the element type or float32
+  const void* bias;    // [channels] or null (zeros), as weight
+  bool f32_params;
+  float eps;
+};
+size_t group_norm_bytes(const GroupArgs& a, bool backward);
+void group_norm(const GroupArgs& a, void* y, int64_t y_stride, float* stats, void* ws,
+                hipStream_t st);
+// dx, dweight and dbias may be null; of x's and the parameters' types.
+void group_norm_backward(const GroupArgs& a, const void* dy, int64_t dy_stride, const float* stats,
+                         void* dx, int64_t dx_stride, void* dweight, void* dbias, void* ws,
+                         hipStream_t st);
+
 // y = residual + x keep / (1 - rate), keep from draw offset + (row width + col).
 struct DropoutArgs {
   int type;

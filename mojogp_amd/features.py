@@ -227,6 +227,88 @@ def layer_norm_backward(dy, x, weight, saved, *, bias=True):
     return dx, dweight, dbias
 
 
+# ---------------------------------------------------------------- group norm
+
+def _activation(activation):
+    if activation is None:
+        return -1
+    act = ACTIVATIONS.get(activation) if isinstance(activation, str) else None
+    if act is None:
+        raise ValueError(f"unknown activation {activation!r}; one of {sorted(ACTIVATIONS)} or None")
+    return act
+
+
+def _group_args(x, groups, weight, bias, eps, activation):
+    dtype, code, index, stream = _first(x, "x")
+    act = _activation(activation)
+    if x.dim() < 2:
+        raise ValueError(f"x must have shape (samples, ..., channels), got {tuple(x.shape)}")
+    px, rows, width, stride = _rows(x, "x", dtype, index)
+    samples = x.shape[0]
+    positions = 1
+    for size in x.shape[1:-1]:
+        positions *= size
+    if not isinstance(groups, int) or groups < 1 or width % groups:
+        raise ValueError(f"groups must divide the {width} channels, got {groups!r}")
+    given = weight if weight is not None else bias
+    ptype, pcode = dtype, code
+    if given is not None and given.dtype is not dtype:
+        ptype, pcode = given.dtype, _types.get(given.dtype)
+        if pcode != 0:
+            raise TypeError(f"weight and bias must have x's element type or be float32, got "
+                            f"{ptype}, which does not fit {dtype}")
+    pw = _vector(weight, "weight", width, ptype, index)
+    pb = _vector(bias, "bias", width, ptype, index)
+    return (_lib.GroupNorm(code, pcode, act, eps, samples, positions, width, groups, px, stride,
+                           pw, pb), dtype, index, stream)
+
+
+def _group_workspace(a, x, backward):
+    nbytes = C.c_int64(0)
+    _lib.call("mgp_group_norm_workspace", C.byref(a), backward, C.byref(nbytes))
+    return _workspace(x, nbytes.value), nbytes.value
+
+
+def group_norm(x, groups, weight=None, bias=None, eps=1e-5, *, activation=None, save=False,
+               out=None):
+    """Group norm with an activation, channels last: ``act((x - mean) / sqrt(var + eps) *
+    weight + bias)``.
+
+    x [samples, ..., channels] (positions between the two, if any); mean and variance
+    of each sample are those of all its positions and of ``channels / groups``
+    consecutive channels.  weight and bias ([channels], of x's type or float32) may be
+    None; activation: None or one of ``gated_layer``'s.  ``out`` may be x, but share no
+    memory with it otherwise.  With ``save=True`` returns ``(y, saved)``, ``saved`` being
+    what the backward pass takes (mean and reciprocal deviation of every sample's
+    groups, float32)."""
+    a, dtype, index, stream = _group_args(x, groups, weight, bias, eps, activation)
+    y, py, stride = _result(out, "out", x, x.shape, dtype, index)
+    stats = x.new_empty((a.samples, groups, 2), dtype=_torch().float32) if save else None
+    ws, nbytes = _group_workspace(a, x, 0)
+    _lib.call("mgp_group_norm_device", C.byref(a), py, stride, _address(stats), _address(ws),
+              nbytes, stream)
+    return (y, stats) if save else y
+
+
+def group_norm_backward(dy, x, groups, weight, bias, saved, *, activation=None):
+    """Gradients ``(dx, dweight, dbias)`` of ``group_norm(x, groups, weight, bias)`` with
+    the same activation; None for what is None.  What goes into the activation is
+    formed again from x: nothing but ``saved`` is kept between the passes."""
+    a, dtype, index, stream = _group_args(x, groups, weight, bias, 0.0, activation)
+    pdy, _, _, dy_stride = _rows(dy, "dy", dtype, index, x.shape)
+    if saved is None or saved.shape != (a.samples, groups, 2) or _types.get(saved.dtype) != 0 \
+            or not saved.is_contiguous() or saved.get_device() != index:
+        raise ValueError("saved must be what group_norm(..., save=True) returned for this x")
+    dx = x.new_empty(x.shape)
+    dweight = None if weight is None else weight.new_empty((a.channels,))
+    dbias = None if bias is None else bias.new_empty((a.channels,))
+    ws, nbytes = _group_workspace(a, x, 1)
+    _lib.call("mgp_group_norm_backward_device", C.byref(a), pdy, dy_stride, saved.data_ptr(),
+              dx.data_ptr(), a.channels, _address(dweight), _address(dbias), _address(ws), nbytes,
+              stream)
+    return dx, dweight, dbias
+
+
 # ---------------------------------------------------------------- dropout
 
 def _dropout(x, name, rate, seed, offset, residual, out):

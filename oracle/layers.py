@@ -40,6 +40,35 @@ def activate(act, g):
     return g * s, s * (1.0 + g * (1.0 - s))
 
 
+def _groups(x, groups):
+    """x [samples, positions, channels] with the channels as (group, channel)."""
+    return x.reshape(x.shape[0], -1, groups, x.shape[-1] // groups)
+
+
+def group_norm(x, groups, w=None, b=None, act=None, eps=1e-5):
+    x = np.asarray(x, np.float64)
+    xc = _groups(x, groups)
+    xc = xc - xc.mean(axis=(1, 3), keepdims=True)
+    xh = (xc / np.sqrt((xc * xc).mean(axis=(1, 3), keepdims=True) + eps)).reshape(x.shape)
+    z = xh * (1.0 if w is None else w) + (0.0 if b is None else b)
+    return z if act is None else activate(act, z)[0]
+
+
+def group_norm_backward(dy, x, groups, w=None, b=None, act=None, eps=1e-5):
+    x, dy = np.asarray(x, np.float64), np.asarray(dy, np.float64)
+    xc = _groups(x, groups)
+    xc = xc - xc.mean(axis=(1, 3), keepdims=True)
+    rstd = 1.0 / np.sqrt((xc * xc).mean(axis=(1, 3), keepdims=True) + eps)
+    xh = (xc * rstd).reshape(x.shape)
+    one = 1.0 if w is None else w
+    dz = dy if act is None else dy * activate(act, xh * one + (0.0 if b is None else b))[1]
+    g, h = _groups(dz * one, groups), _groups(xh, groups)
+    dx = rstd * (g - g.mean(axis=(1, 3), keepdims=True)
+                 - h * (g * h).mean(axis=(1, 3), keepdims=True))
+    axes = tuple(range(x.ndim - 1))
+    return dx.reshape(x.shape), (dz * xh).sum(axis=axes), dz.sum(axis=axes)
+
+
 def gated_layer(x, wg, wu, bg=None, bu=None, act="silu"):
     g = x @ wg.T + (0.0 if bg is None else bg)
     u = x @ wu.T + (0.0 if bu is None else bu)
