@@ -853,6 +853,39 @@ MGP_API int mgp_group_norm_backward_device(const mgp_group_norm_t* args, const v
                                            void* workspace, int64_t workspace_bytes,
                                            void* stream);
 
+/* Rows of x [rows][width] as 8-bit integers: codes[r][c] = rint(x * by), ties to even,
+ * by = 127 / largest |x| of the row, scales[r] = largest / 127 (both quotients rounded to
+ * fp32).  Rows of codes are 16-byte aligned, codes_stride bytes apart; the columns from
+ * width to the next multiple of 16 become 0.  Rows whose largest value is below 2^-120
+ * are zeros with scale 0; rows that are not finite have scale NaN. width <= 131072. */
+MGP_API int mgp_int8_quantize_device(int type, const void* x, int64_t x_stride, int64_t rows,
+                                     int64_t width, void* codes, int64_t codes_stride,
+                                     float* scales, void* stream);
+/* A layer whose weights are such rows (the bytes up to the next multiple of 16 of
+ * width, zeros, are read): y = act(s s_gate sum(q w_gate) + b_gate), where q and s are
+ * x's rows as above and the sum is exact; with w_up (not NULL) times (s s_up sum(q w_up)
+ * + b_up).  x, biases [hidden] (may be NULL) and y are of one element type.  activation:
+ * as of the gated layer, or -1 for none where w_up is NULL. */
+typedef struct mgp_int8_layer {
+  int type;
+  int activation;
+  int64_t rows;
+  int64_t width;
+  int64_t hidden;
+  const void* x;
+  int64_t x_stride;
+  const void* w_gate;
+  const void* w_up;
+  int64_t w_stride;
+  const float* s_gate;
+  const float* s_up;
+  const void* b_gate;
+  const void* b_up;
+} mgp_int8_layer_t;
+MGP_API int mgp_int8_layer_workspace(const mgp_int8_layer_t* args, int64_t* bytes);
+MGP_API int mgp_int8_layer_device(const mgp_int8_layer_t* args, void* y, int64_t y_stride,
+                                  void* workspace, int64_t workspace_bytes, void* stream);
+
 /* AdamW over many tensors at once (decoupled weight decay):
  *   g = grad * grad_scale * min(1, max_norm / norm), norm = |all grads * grad_scale|
  *   m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g^2

@@ -79,6 +79,17 @@ class GroupNorm(C.Structure):
     ]
 
 
+class Int8Layer(C.Structure):
+    """mgp_int8_layer_t"""
+    _fields_ = [
+        ("type", C.c_int), ("activation", C.c_int), ("rows", C.c_int64), ("width", C.c_int64),
+        ("hidden", C.c_int64), ("x", C.c_void_p), ("x_stride", C.c_int64),
+        ("w_gate", C.c_void_p), ("w_up", C.c_void_p), ("w_stride", C.c_int64),
+        ("s_gate", C.c_void_p), ("s_up", C.c_void_p), ("b_gate", C.c_void_p),
+        ("b_up", C.c_void_p),
+    ]
+
+
 class AdamWTensor(C.Structure):
     """mgp_adamw_tensor_t"""
     _fields_ = [("param", C.c_void_p), ("size", C.c_int64), ("weight_decay", C.c_float)]
@@ -342,6 +353,11 @@ _SIGNATURES = {
     "mgp_group_norm_backward_device": (C.c_int, [C.POINTER(GroupNorm), C.c_void_p, C.c_int64,
                                                  C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p,
                                                  C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
+    "mgp_int8_quantize_device": (C.c_int, [C.c_int, C.c_void_p, C.c_int64, C.c_int64, C.c_int64,
+                                           C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
+    "mgp_int8_layer_workspace": (C.c_int, [C.POINTER(Int8Layer), c_int64_p]),
+    "mgp_int8_layer_device": (C.c_int, [C.POINTER(Int8Layer), C.c_void_p, C.c_int64, C.c_void_p,
+                                        C.c_int64, C.c_void_p]),
     "mgp_adamw_layout": (C.c_int, [C.POINTER(AdamW), c_int64_p, c_int64_p]),
     "mgp_adamw_create": (C.c_int, [C.POINTER(AdamW), C.c_void_p, C.c_int64, c_void_pp]),
     "mgp_adamw_destroy": (C.c_int, [C.c_void_p]),

@@ -137,6 +137,43 @@ Span row_span(const char* name, const GroupArgs& a, const void* p, int64_t strid
 Span param_span(const char* name, const GroupArgs& a, const void* p) {
   return span(name, p, 1, a.channels, a.channels, a.f32_params ? 4 : elem_bytes(a.type));
 }
+void check_codes(const char* name, const void* p, int64_t stride, int64_t rows, int64_t width) {
+  if (rows == 0) return;
+  MGP_REQUIRE(p != nullptr, std::string("null device array ") + name);
+  MGP_REQUIRE(aligned16(p) && stride % 16 == 0 && stride >= round_up(width, 16) &&
+                  stride < ((int64_t)1 << 23),
+              std::string("rows of ") + name +
+                  " must be 16-byte aligned, below 8 MB and hold the width rounded up to 16");
+}
+
+Int8Args int8_args(const mgp_int8_layer_t* a) {
+  MGP_REQUIRE(a != nullptr, "null arguments");
+  check_shape(a->type, a->rows, a->width);
+  MGP_REQUIRE(a->width <= kInt8Width, "8-bit rows have at most 131072 columns");
+  MGP_REQUIRE(a->hidden >= 1 && a->hidden <= kMaxWidth, "hidden must be in [1, 2^24]");
+  const bool gated = a->w_up != nullptr;
+  MGP_REQUIRE(valid_activation(a->activation) || (a->activation == -1 && !gated),
+              "unknown activation");
+  check_rows("x", a->x, a->x_stride, a->rows, a->width);
+  check_codes("w_gate", a->w_gate, a->w_stride, a->hidden, a->width);
+  MGP_REQUIRE(a->s_gate != nullptr && (a->s_up != nullptr) == gated, "null scales");
+  if (gated) check_codes("w_up", a->w_up, a->w_stride, a->hidden, a->width);
+  return {a->type,
+          a->activation,
+          a->rows,
+          a->width,
+          a->hidden,
+          a->x,
+          a->x_stride,
+          static_cast<const int8_t*>(a->w_gate),
+          static_cast<const int8_t*>(a->w_up),
+          a->w_stride,
+          a->s_gate,
+          a->s_up,
+          a->b_gate,
+          gated ? a->b_up : nullptr};
+}
+
 void check_pairs(const float* stats) {
   MGP_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 7) == 0, "the statistics must be 8-byte aligned");
 }
@@ -323,6 +360,55 @@ int mgp_group_norm_backward_device(const mgp_group_norm_t* args, const void* dy,
     check_workspace(workspace, workspace_bytes, group_norm_bytes(a, true));
     group_norm_backward(a, dy, dy_stride, stats, dx, dx_stride, dweight, dbias, workspace,
                         static_cast<hipStream_t>(stream));
+  });
+}
+
+int mgp_int8_quantize_device(int type, const void* x, int64_t x_stride, int64_t rows,
+                             int64_t width, void* codes, int64_t codes_stride, float* scales,
+                             void* stream) {
+  return guarded([&] {
+    check_shape(type, rows, width);
+    MGP_REQUIRE(width <= kInt8Width, "8-bit rows have at most 131072 columns");
+    check_rows("x", x, x_stride, rows, width);
+    check_codes("codes", codes, codes_stride, rows, width);
+    MGP_REQUIRE(rows == 0 || scales != nullptr, "null scales");
+    const Span of_x = span("x", x, rows, width, x_stride, elem_bytes(type));
+    const Span of_codes = span("codes", codes, rows, round_up(width, 16), codes_stride, 1);
+    const Span of_scales = span("scales", scales, 1, rows, rows, sizeof(float));
+    check_apart(of_codes, of_x, false);
+    check_apart(of_scales, of_x, false);
+    check_apart(of_codes, of_scales, false);
+    int8_quantize(type, x, x_stride, rows, width, static_cast<int8_t*>(codes), codes_stride,
+                  scales, static_cast<hipStream_t>(stream));
+  });
+}
+
+int mgp_int8_layer_workspace(const mgp_int8_layer_t* args, int64_t* bytes) {
+  return guarded([&] {
+    MGP_REQUIRE(bytes != nullptr, "null result");
+    *bytes = (int64_t)int8_bytes(int8_args(args));
+  });
+}
+
+int mgp_int8_layer_device(const mgp_int8_layer_t* args, void* y, int64_t y_stride,
+                          void* workspace, int64_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    const Int8Args a = int8_args(args);
+    check_rows("y", y, y_stride, a.rows, a.hidden);
+    if (a.rows == 0) return;
+    const size_t e = elem_bytes(a.type);
+    const int64_t pad = round_up(a.width, 16);
+    const Span out = span("y", y, a.rows, a.hidden, y_stride, e);
+    for (const Span& in : {span("x", a.x, a.rows, a.width, a.x_stride, e),
+                           span("w_gate", a.w_gate, a.hidden, pad, a.w_stride, 1),
+                           span("w_up", a.w_up, a.hidden, pad, a.w_stride, 1),
+                           span("s_gate", a.s_gate, 1, a.hidden, a.hidden, sizeof(float)),
+                           span("s_up", a.s_up, 1, a.hidden, a.hidden, sizeof(float)),
+                           span("b_gate", a.b_gate, 1, a.hidden, a.hidden, e),
+                           span("b_up", a.b_up, 1, a.hidden, a.hidden, e)})
+      check_apart(out, in, false);
+    check_workspace(workspace, workspace_bytes, int8_bytes(a));
+    int8_layer(a, y, y_stride, workspace, static_cast<hipStream_t>(stream));
   });
 }
 

@@ -110,4 +110,25 @@ struct GatedGrads {  // contiguous, any may be null
 void gated_backward(const GatedArgs& a, const void* dh, int64_t dh_stride, const GatedGrads& g,
                     void* ws, hipStream_t st);
 
+// Rows in 8-bit integers: codes[rows][codes_stride] (zeros from width up to the next
+// multiple of 16) and a scale for each.
+void int8_quantize(int type, const void* x, int64_t x_stride, int64_t rows, int64_t width,
+                   int8_t* codes, int64_t codes_stride, float* scales, hipStream_t st);
+
+// A layer whose weights are such rows; w_up null: act(x Wg^T + bg), otherwise times
+// x Wu^T + bu.
+struct Int8Args {
+  int type, activation;  // of x, biases and the result; -1: none
+  int64_t rows, width, hidden;
+  const void* x;
+  int64_t x_stride;
+  const int8_t *w_gate, *w_up;
+  int64_t w_stride;
+  const float *s_gate, *s_up;
+  const void *b_gate, *b_up;  // [hidden] or null
+};
+constexpr int64_t kInt8Width = 131072;  // 127^2 of so many are below 2^31
+size_t int8_bytes(const Int8Args& a);
+void int8_layer(const Int8Args& a, void* y, int64_t y_stride, void* ws, hipStream_t st);
+
 }  // namespace mgp

@@ -401,3 +401,88 @@ def gated_layer_backward(dh, x, w_gate, w_up, b_gate=None, b_up=None, *, activat
     _lib.call("mgp_gated_layer_backward_device", C.byref(a), pdh, dh_stride,
               *(_address(t) for t in g), _address(ws), nbytes, stream)
     return g
+
+
+# ---------------------------------------------------------------- layers in 8-bit integers
+
+class Int8Weights(NamedTuple):
+    """What int8_weights returns: codes (int8, [rows, width rounded up to 16], zeros
+    behind width), a float32 scale for each row, and the width."""
+    codes: object
+    scale: object
+    width: int
+
+
+def int8_weights(w):
+    """Weights [hidden, width] as 8-bit integers with a scale for each row, for
+    ``int8_layer`` and ``int8_gated_layer``: half the bytes of 16-bit ones.
+
+    The codes are -127 .. 127, the row times 127 over its largest value, rounded to
+    even.  A row that is not finite gets the scale NaN.  At most 131072 columns."""
+    dtype, code, index, stream = _first(w, "w")
+    pw, rows, width, stride = _rows(w, "w", dtype, index)
+    if w.dim() != 2:
+        raise ValueError(f"w must have shape (hidden, width), got {tuple(w.shape)}")
+    torch = _torch()
+    padded = -(-width // 16) * 16
+    codes = w.new_empty((rows, padded), dtype=torch.int8)
+    scale = w.new_empty((rows,), dtype=torch.float32)
+    _lib.call("mgp_int8_quantize_device", code, pw, stride, rows, width, codes.data_ptr(), padded,
+              scale.data_ptr(), stream)
+    return Int8Weights(codes, scale, width)
+
+
+def _int8_side(w, name, width, index, hidden=None):
+    """(codes' address, scales' address, rows, row stride)"""
+    if not isinstance(w, Int8Weights):
+        raise TypeError(f"{name} must be what int8_weights returned, got {type(w).__name__}")
+    torch = _torch()
+    _check(w.codes, f"{name}.codes", torch.int8, index)
+    _check(w.scale, f"{name}.scale", torch.float32, index)
+    padded = -(-width // 16) * 16
+    if w.width != width or w.codes.dim() != 2 or w.codes.shape[1] != padded \
+            or not w.codes.is_contiguous():
+        raise ValueError(f"{name} must be weights of {width} columns, got {w.width} in codes of "
+                         f"shape {tuple(w.codes.shape)}")
+    rows = w.codes.shape[0]
+    if rows == 0 or (hidden is not None and rows != hidden):
+        raise ValueError(f"{name} must have {hidden or 'at least one'} rows, got {rows}")
+    return w.codes.data_ptr(), _vector(w.scale, f"{name}.scale", rows, torch.float32, index), rows
+
+
+def _int8(x, gate, up, b_gate, b_up, act, names, out):
+    dtype, code, index, stream = _first(x, "x")
+    px, rows, width, stride = _rows(x, "x", dtype, index)
+    wg, sg, hidden = _int8_side(gate, names[0], width, index)
+    wu = su = None
+    if up is not None:
+        wu, su, _ = _int8_side(up, names[1], width, index, hidden)
+    bg = _vector(b_gate, names[2], hidden, dtype, index)
+    bu = _vector(b_up, names[3], hidden, dtype, index)
+    a = _lib.Int8Layer(code, act, rows, width, hidden, px, stride, wg, wu, gate.codes.shape[1], sg,
+                       su, bg, bu)
+    y, py, y_stride = _result(out, "out", x, (*x.shape[:-1], hidden), dtype, index)
+    nbytes = C.c_int64(0)
+    _lib.call("mgp_int8_layer_workspace", C.byref(a), C.byref(nbytes))
+    ws = _workspace(x, nbytes.value)
+    _lib.call("mgp_int8_layer_device", C.byref(a), py, y_stride, _address(ws), nbytes.value, stream)
+    return y
+
+
+def int8_layer(x, weights, bias=None, *, activation=None, out=None):
+    """``act(x w^T + bias)`` with weights from ``int8_weights`` and each row of x rounded
+    to 8 bits in the same way, the sums being exact.
+
+    x [..., width] and bias [hidden] (or None) of one element type, which the result
+    [..., hidden] has too; activation: None or one of ``gated_layer``'s.  Rows that
+    are not finite give NaN.  ``out`` shares no memory with the inputs."""
+    return _int8(x, weights, None, bias, None, _activation(activation),
+                 ("weights", "", "bias", ""), out)
+
+
+def int8_gated_layer(x, w_gate, w_up, b_gate=None, b_up=None, *, activation="silu", out=None):
+    """``gated_layer`` with weights from ``int8_weights``, and x as in ``int8_layer``."""
+    act = _activation(activation)
+    if act < 0:
+        raise ValueError(f"unknown activation None; one of {sorted(ACTIVATIONS)}")
+    return _int8(x, w_gate, w_up, b_gate, b_up, act, ("w_gate", "w_up", "b_gate", "b_up"), out)

@@ -83,6 +83,35 @@ def gated_layer_backward(dh, x, wg, wu, bg=None, bu=None, act="silu"):
     return dg @ wg + du @ wu, dg.T @ x, du.T @ x, dg.sum(axis=0), du.sum(axis=0)
 
 
+def int8_rows(x):
+    """(codes, scales) of rows: 127 over the largest value, both quotients rounded to
+    float32 and the products to whole numbers, ties to even."""
+    x = np.asarray(x, np.float64)
+    most = np.abs(x).max(axis=1)
+    some = most >= 2.0 ** -120
+    by = np.where(some, 127 / np.where(some, most, 1), 0).astype(np.float32).astype(np.float64)
+    scale = np.where(some, most / 127, 0).astype(np.float32).astype(np.float64)
+    return np.rint(x * by[:, None]).astype(np.int64), scale
+
+
+def int8_layer(x, wg, bg=None, wu=None, bu=None, act=None):
+    """(result, the size of its sums before they meet anything that cancels)"""
+    q, s = int8_rows(x)
+
+    def project(w, b):
+        c, sw = int8_rows(w)
+        p = (q @ c.T) * s[:, None] * sw
+        return p + (0.0 if b is None else b), np.abs(p)
+
+    y, size = project(wg, bg)
+    if act is not None:
+        y = activate(act, y)[0]
+    if wu is not None:
+        u, _ = project(wu, bu)
+        y = y * u
+    return y, size
+
+
 def philox(counter, key):
     """The four words of Philox4x32-10 (Salmon et al. 2011) of a 128-bit counter
     and a 64-bit key, in Python integers."""
