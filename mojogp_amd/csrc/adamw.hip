@@ -32,7 +32,7 @@ namespace mgp {
 namespace {
 
 constexpr int kGrads = 400;  // gradients a launch: 3200 of 4096 bytes of arguments
-constexpr int kNormBlocks = 256, kNormThreads = 1024;
+constexpr int kNormBlocks = 2048;
 
 struct Grads {
   const void* at[kGrads];
@@ -79,35 +79,43 @@ __device__ __forceinline__ void store4(T* p, int64_t left, const float* v) {
 
 // ---------------------------------------------------------------- norm of the gradients
 
-// part[block]: the sum of squares of a block's chunks, in 64 bits
+// part[block]: the sum of squares of a block's chunks, in 64 bits.  Four chunks a round,
+// their loads all out before the first is used.
 template <class G>
-__global__ __launch_bounds__(kNormThreads) void k_adamw_norm(Grads grads,
-                                                             const AdamEntry* __restrict__ entries,
-                                                             const AdamChunk* __restrict__ chunks,
-                                                             uint32_t first, uint32_t count,
-                                                             uint32_t tensor0,
-                                                             double* __restrict__ part) {
-  __shared__ double red[kNormThreads / 64];
+__global__ __launch_bounds__(256) void k_adamw_norm(Grads grads,
+                                                    const AdamEntry* __restrict__ entries,
+                                                    const AdamChunk* __restrict__ chunks,
+                                                    uint32_t first, uint32_t count,
+                                                    uint32_t tensor0, double* __restrict__ part) {
+  constexpr int U = 4, P = (int)(kAdamChunk / 1024);
+  __shared__ double red[4];
   double s = 0.0;
-  // two chunks of 2048 a round
-  for (uint32_t c = blockIdx.x * 2 + (threadIdx.x >> 9); c < count; c += gridDim.x * 2) {
-    const uint32_t at = __builtin_amdgcn_readfirstlane(first + c);
-    const uint32_t t = __builtin_amdgcn_readfirstlane(chunks[at].tensor);
-    const G* g = static_cast<const G*>(grads.at[t - tensor0]);
-    if (g == nullptr) continue;
-    const int64_t i = (int64_t)chunks[at].chunk * kAdamChunk + 4 * (threadIdx.x & 511);
-    const Four<G> a = load4(g + i, entries[t].size - i);
+  for (uint32_t c = blockIdx.x * U; c < count; c += gridDim.x * U) {
+    Four<G> a[U][P];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) s = fma((double)(float)a.v[k], (double)(float)a.v[k], s);
+    for (int u = 0; u < U; ++u) {
+      const AdamChunk ck = chunks[first + min(c + u, count - 1)];
+      const G* g = static_cast<const G*>(grads.at[ck.tensor - tensor0]);
+      const int64_t i = (int64_t)ck.chunk * kAdamChunk + 4 * threadIdx.x;
+      const int64_t size = g && c + u < count ? entries[ck.tensor].size : 0;
+#pragma unroll
+      for (int p = 0; p < P; ++p) a[u][p] = load4(g + i + p * 1024, size - i - p * 1024);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const double x = (double)(float)a[u][p].v[k];
+          s = fma(x, x, s);
+        }
   }
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x != 0) return;
-#pragma unroll
-  for (int w = 1; w < kNormThreads / 64; ++w) s += red[w];
-  part[blockIdx.x] = s;
+  if (threadIdx.x == 0) part[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 struct ScalarArgs {
@@ -116,30 +124,32 @@ struct ScalarArgs {
   double grad_scale, max_norm;
   float* norm_out;
   double beta1, beta2;
-  int64_t step;
   const int64_t* step_device;
-  float rate;
   const float* rate_device;
+  Scalars host;
   Scalars* out;
 };
 
 __global__ __launch_bounds__(256) void k_adamw_scalars(ScalarArgs a) {
   __shared__ double red[4];
   double s = 0.0;
+#pragma unroll 8
   for (int i = threadIdx.x; i < a.parts; i += 256) s += a.part[i];
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x != 0) return;
-  Scalars r;
+  Scalars r = a.host;
   const double norm = sqrt(red[0] + red[1] + red[2] + red[3]) * fabs(a.grad_scale);
   r.factor = a.grad_scale * (norm > a.max_norm ? a.max_norm / norm : 1.0);
   r.skip = !(norm < HUGE_VAL);
-  const double t = (double)(a.step_device ? *a.step_device : a.step);
-  r.c1 = (float)(1.0 / (1.0 - pow(a.beta1, t)));
-  r.c2 = (float)(1.0 / (1.0 - pow(a.beta2, t)));
-  r.rate = a.rate_device ? *a.rate_device : a.rate;
+  if (a.step_device) {
+    const double t = (double)*a.step_device;
+    r.c1 = (float)(1.0 / (1.0 - pow(a.beta1, t)));
+    r.c2 = (float)(1.0 / (1.0 - pow(a.beta2, t)));
+  }
+  if (a.rate_device) r.rate = *a.rate_device;
   *a.out = r;
   if (a.norm_out) *a.norm_out = (float)norm;
 }
@@ -150,22 +160,31 @@ __global__ __launch_bounds__(256) void k_adamw_scalars(ScalarArgs a) {
 // (the field of 2^LOWEST is 1), evenly spaced below; rounded up where the cut-off
 // part and (draw + 1/2) / 2^16 of a code's step pass the step.  In a double's high word
 // a step is 2^17; below 2^LOWEST the value is brought into that binade first.
+// twice: 2 draw.
 template <int LOWEST>
-__device__ __forceinline__ int code_of(double x, uint32_t draw, int most) {
+__device__ __forceinline__ int code_of(double x, uint32_t twice, int most) {
   constexpr double kLow = LOWEST == -6 ? 0x1p-6 : 0x1p-30;
   static_assert(LOWEST == -6 || LOWEST == -30, "");
+  constexpr uint32_t kField = (uint32_t)(LOWEST + 1022) << 20;
   const bool low = x < kLow;
-  const double y = low ? x + kLow : x;
-  const uint32_t high = (uint32_t)(__double_as_longlong(y) >> 32);
-  const int code = (int)((high + 2 * draw + 1) >> 17) - ((LOWEST + 1022) << 3) - (low ? 8 : 0);
-  return min(code, most);
+  const uint32_t high = (uint32_t)(__double_as_longlong(low ? x + kLow : x) >> 32);
+  return min((int)((high + (twice + (low ? 1u - kField - (8u << 17) : 1u - kField))) >> 17), most);
 }
 
-// Largest of 64 lanes, of the bits of |value|: NaN is above infinity.
+// Largest of 64 lanes, of the bits of |value| (NaN is above infinity): within rows of
+// 16 lanes, then across them, to lane 63.
 __device__ __forceinline__ uint32_t wave_largest(uint32_t u) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) u = max(u, (uint32_t)__shfl_xor((int)u, o));
-  return u;
+  auto other = [](uint32_t v, auto control, auto rows) __attribute__((always_inline)) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, control.value, rows.value, 0xf, false);
+  };
+  using std::integral_constant;
+  u = max(u, other(u, integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{}));
+  u = max(u, other(u, integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{}));
+  u = max(u, other(u, integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{}));
+  u = max(u, other(u, integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{}));
+  u = max(u, other(u, integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{}));
+  u = max(u, other(u, integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{}));
+  return (uint32_t)__builtin_amdgcn_readlane((int)u, 63);
 }
 
 // The scale of a block and the factor of its values, from the largest of them.
@@ -218,21 +237,26 @@ struct StepArgs {
   const Scalars* device;  // or null: host's
 };
 
-template <class P, class G, bool EIGHT, bool MASTER>
-__global__ __launch_bounds__(256) void k_adamw(Grads grads, StepArgs a) {
-  constexpr int U = (int)(kAdamChunk / 1024);
-  const AdamChunk ck = a.chunks[a.first + blockIdx.x];
-  const AdamEntry e = a.entries[ck.tensor];
-  const G* __restrict__ g = static_cast<const G*>(grads.at[ck.tensor - a.tensor0]);
-  if (g == nullptr) return;
-  const Scalars s = a.device ? *a.device : a.host;
-  if (s.skip) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  // a wave's blocks of 256 lie side by side
-  const int64_t i0 = (int64_t)ck.chunk * kAdamChunk + wave * 256 + 4 * lane;
-  P* __restrict__ param = static_cast<P*>(e.param);
-  float* __restrict__ master = a.master + e.first;
+// What a workgroup works on: the arrays of its chunk of a tensor.
+template <class P, class G>
+struct ChunkAt {
+  const G* g;
+  P* param;
+  float *master, *m, *v;      // 32-bit states
+  uint8_t *mc, *vc;           // 8-bit ones
+  float *ms, *vs;
+  int64_t first;              // of the chunk's values in the states
+  int left;                   // values of the tensor from the chunk's first on, up to a chunk
+  float keep;                 // 1 - rate decay
+};
 
+// FULL: none of the chunk's values is past the tensor's end.
+template <class P, class G, bool EIGHT, bool MASTER, bool FULL>
+__device__ __forceinline__ void step_chunk(const ChunkAt<P, G>& c, const StepArgs& a,
+                                           const Scalars& s, uint64_t t) {
+  constexpr int U = (int)(kAdamChunk / 1024);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Four<G> gr[U];
   Four<P> pr[U];
   Four<float> wr[U], mr[U], vr[U];
@@ -240,42 +264,46 @@ __global__ __launch_bounds__(256) void k_adamw(Grads grads, StepArgs a) {
   float ms[U], vs[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int64_t i = i0 + u * 1024, left = e.size - i;
-    gr[u] = load4(g + i, left);
+    const int i0 = u * 1024 + wave * 256, i = i0 + 4 * lane;
+    const int left = FULL ? 4 : c.left - i;
+    gr[u] = load4(c.g + i, left);
     if constexpr (MASTER)
-      wr[u] = load4(master + i, left);
+      wr[u] = load4(c.master + i, left);
     else
-      pr[u] = load4(param + i, left);
+      pr[u] = load4(c.param + i, left);
     if constexpr (EIGHT) {
       // the padding of a tensor's last block is there to be read and written
-      const int64_t b = (e.first + i) >> 8;
-      const bool in = (i & ~(int64_t)255) < e.size;
-      mc[u] = in ? *reinterpret_cast<const uint32_t*>(static_cast<uint8_t*>(a.exp_avg) + e.first + i) : 0u;
-      vc[u] = in ? *reinterpret_cast<const uint32_t*>(static_cast<uint8_t*>(a.exp_avg_sq) + e.first + i) : 0u;
-      ms[u] = in ? a.exp_avg_scale[b] : 0.0f;
-      vs[u] = in ? a.exp_avg_sq_scale[b] : 0.0f;
+      const bool in = FULL || i0 < c.left;
+      mc[u] = in ? *reinterpret_cast<const uint32_t*>(c.mc + i) : 0u;
+      vc[u] = in ? *reinterpret_cast<const uint32_t*>(c.vc + i) : 0u;
+      ms[u] = in ? c.ms[i0 >> 8] : 0.0f;
+      vs[u] = in ? c.vs[i0 >> 8] : 0.0f;
     } else {
-      mr[u] = load4(static_cast<const float*>(a.exp_avg) + e.first + i, left);
-      vr[u] = load4(static_cast<const float*>(a.exp_avg_sq) + e.first + i, left);
+      mr[u] = load4(c.m + i, left);
+      vr[u] = load4(c.v + i, left);
     }
   }
-  const float keep = 1.0f - s.rate * e.decay;
-  uint64_t t = 0;
-  if constexpr (EIGHT) t = (uint64_t)(a.step_device ? *a.step_device : a.step);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int64_t i = i0 + u * 1024, left = e.size - i;
-    if ((i & ~(int64_t)255) >= e.size) continue;  // (of the whole wave)
+    const int i0 = u * 1024 + wave * 256, i = i0 + 4 * lane;
+    const int left = FULL ? 4 : c.left - i;
+    if (!FULL && i0 >= c.left) continue;
     float m[4], v[4];
     if constexpr (EIGHT) {
       double md[4], vd[4];
       uint32_t mu = 0, vu = 0;
+      double gd[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) gd[k] = (double)(float)gr[u].v[k];
+      if (s.factor != 1.0) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) gd[k] *= s.factor;
+      }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const double gd = (double)(float)gr[u].v[k] * s.factor;
-        md[k] = mean_of(a.b1, (double)value_m(mc[u], k) * (double)ms[u], 1.0 - a.b1, gd);
-        vd[k] = mean_of(a.b2, (double)value_v(vc[u], k) * (double)vs[u], 1.0 - a.b2, gd * gd);
-        if (k >= left) md[k] = vd[k] = 0.0;
+        md[k] = mean_of(a.b1, (double)value_m(mc[u], k) * (double)ms[u], 1.0 - a.b1, gd[k]);
+        vd[k] = mean_of(a.b2, (double)value_v(vc[u], k) * (double)vs[u], 1.0 - a.b2, gd[k] * gd[k]);
+        if (!FULL && k >= left) md[k] = vd[k] = 0.0;
         m[k] = (float)md[k];
         v[k] = (float)vd[k];
         mu = max(mu, __float_as_uint(m[k]) & 0x7fffffffu);
@@ -283,21 +311,23 @@ __global__ __launch_bounds__(256) void k_adamw(Grads grads, StepArgs a) {
       }
       const Scale sm = scale_of(wave_largest(mu), kTopM, 1.0f / kTopM);
       const Scale sv = scale_of(wave_largest(vu), kTopV, 1.0f / kTopV);
-      const Draws dr = philox((uint64_t)(e.first + i) >> 2, a.seed, t);
+      const Draws dr = philox((uint64_t)(c.first + i) >> 2, a.seed, t);
       uint32_t cm = 0, cv = 0;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int x = code_of<-6>(fabs(md[k]) * (double)sm.by, dr.w[k] & 0xffffu, 126);
-        int y = code_of<-30>(vd[k] * (double)sv.by, dr.w[k] >> 16, 255);
-        if (vd[k] > 0.0 && sv.by > 0.0f) y = max(y, 1);
-        cm |= (uint32_t)(x | (md[k] < 0.0 ? 128 : 0)) << (8 * k);
-        cv |= (uint32_t)y << (8 * k);
+        const int x = code_of<-6>(fabs(md[k]) * (double)sm.by, (dr.w[k] & 0xffffu) << 1, 126);
+        const uint32_t sign = (uint32_t)(__double_as_longlong(md[k]) >> 56) & 128u;
+        const double y = vd[k] * (double)sv.by;
+        // (the high word of a value that is not 0 is not)
+        const int some = (int)min((uint32_t)(__double_as_longlong(y) >> 32), 1u);
+        cm |= ((uint32_t)x | sign) << (8 * k);
+        cv |= (uint32_t)max(code_of<-30>(y, dr.w[k] >> 16 << 1, 255), some) << (8 * k);
       }
-      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.exp_avg) + e.first + i) = cm;
-      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.exp_avg_sq) + e.first + i) = cv;
+      *reinterpret_cast<uint32_t*>(c.mc + i) = cm;
+      *reinterpret_cast<uint32_t*>(c.vc + i) = cv;
       if (lane == 0) {
-        a.exp_avg_scale[(e.first + i) >> 8] = sm.scale;
-        a.exp_avg_sq_scale[(e.first + i) >> 8] = sv.scale;
+        c.ms[i0 >> 8] = sm.scale;
+        c.vs[i0 >> 8] = sv.scale;
       }
     } else {
       const float b1 = (float)a.b1, b2 = (float)a.b2;
@@ -308,8 +338,8 @@ __global__ __launch_bounds__(256) void k_adamw(Grads grads, StepArgs a) {
         m[k] = fmaf(b1, mr[u].v[k], r1 * x);
         v[k] = fmaf(b2, vr[u].v[k], r2 * (x * x));
       }
-      store4(static_cast<float*>(a.exp_avg) + e.first + i, left, m);
-      store4(static_cast<float*>(a.exp_avg_sq) + e.first + i, left, v);
+      store4(c.m + i, left, m);
+      store4(c.v + i, left, v);
     }
     float p[4];
 #pragma unroll
@@ -318,11 +348,47 @@ __global__ __launch_bounds__(256) void k_adamw(Grads grads, StepArgs a) {
       const float root = __builtin_amdgcn_sqrtf(v[k] * s.c2) + a.eps;
       const float update = m[k] * s.c1 * __builtin_amdgcn_rcpf(root);
       const float w = MASTER ? wr[u].v[k] : (float)pr[u].v[k];
-      p[k] = fmaf(w, keep, -s.rate * update);
+      p[k] = fmaf(w, c.keep, -s.rate * update);
+      // a value in fp32: rounded to float16 together with the sum, a parameter would not
+      // always be what its master copy rounds to
+      asm("" : "+v"(p[k]));
     }
-    if constexpr (MASTER) store4(master + i, left, p);
-    store4(param + i, left, p);
+    if constexpr (MASTER) store4(c.master + i, left, p);
+    store4(c.param + i, left, p);
   }
+}
+
+template <class P, class G, bool EIGHT, bool MASTER>
+__global__ __launch_bounds__(256) void k_adamw(Grads grads, StepArgs a) {
+  const AdamChunk ck = a.chunks[a.first + blockIdx.x];
+  const AdamEntry e = a.entries[ck.tensor];
+  const G* g = static_cast<const G*>(grads.at[ck.tensor - a.tensor0]);
+  if (g == nullptr) return;
+  const Scalars s = a.device ? *a.device : a.host;
+  if (s.skip) return;
+  const int64_t at = (int64_t)ck.chunk * kAdamChunk, first = e.first + at;
+  uint64_t t = 0;
+  ChunkAt<P, G> c;
+  c.g = g + at;
+  c.param = static_cast<P*>(e.param) + at;
+  if constexpr (MASTER) c.master = a.master + first;
+  if constexpr (EIGHT) {
+    c.mc = static_cast<uint8_t*>(a.exp_avg) + first;
+    c.vc = static_cast<uint8_t*>(a.exp_avg_sq) + first;
+    c.ms = a.exp_avg_scale + (first >> 8);
+    c.vs = a.exp_avg_sq_scale + (first >> 8);
+    t = (uint64_t)(a.step_device ? *a.step_device : a.step);
+  } else {
+    c.m = static_cast<float*>(a.exp_avg) + first;
+    c.v = static_cast<float*>(a.exp_avg_sq) + first;
+  }
+  c.first = first;
+  c.left = (int)min(e.size - at, kAdamChunk);
+  c.keep = 1.0f - s.rate * e.decay;
+  if (c.left == (int)kAdamChunk)
+    step_chunk<P, G, EIGHT, MASTER, true>(c, a, s, t);
+  else
+    step_chunk<P, G, EIGHT, MASTER, false>(c, a, s, t);
 }
 
 // Values of 8-bit states, four a thread.
@@ -412,6 +478,8 @@ void adamw_step(const AdamPlan& p, const AdamStep& s, void* ws, hipStream_t st) 
   const AdamEntry* entries = static_cast<const AdamEntry*>(p.table);
   const AdamChunk* chunks = reinterpret_cast<const AdamChunk*>(entries + p.tensors.size());
   const bool wide = s.grad_type == ELEM_F32;
+  const Scalars host{s.grad_scale, (float)(1.0 / (1.0 - std::pow(p.beta1, (double)s.step))),
+                     (float)(1.0 / (1.0 - std::pow(p.beta2, (double)s.step))), s.rate, 0};
   Scalars* scalars = nullptr;
   if (on_device(s)) {
     scalars = static_cast<Scalars*>(ws);
@@ -420,7 +488,7 @@ void adamw_step(const AdamPlan& p, const AdamStep& s, void* ws, hipStream_t st) 
       dispatch_elem(s.grad_type, [&](auto tag) {
         int64_t at = 0;
         for_groups(p, s, [&](uint32_t t0, const Grads& g, uint32_t c0, uint32_t count) {
-          k_adamw_norm<decltype(tag)><<<kNormBlocks, kNormThreads, 0, st>>>(
+          k_adamw_norm<decltype(tag)><<<kNormBlocks, 256, 0, st>>>(
               g, entries, chunks, c0, count, t0, part + at);
           at += kNormBlocks;
         });
@@ -428,7 +496,7 @@ void adamw_step(const AdamPlan& p, const AdamStep& s, void* ws, hipStream_t st) 
     }
     k_adamw_scalars<<<1, 256, 0, st>>>({part, s.norm ? (int)(groups(p) * kNormBlocks) : 0,
                                         s.grad_scale, s.max_norm, s.norm_out, p.beta1, p.beta2,
-                                        s.step, s.step_device, s.rate, s.rate_device, scalars});
+                                        s.step_device, s.rate_device, host, scalars});
   }
   StepArgs a{entries,
              chunks,
@@ -445,8 +513,7 @@ void adamw_step(const AdamPlan& p, const AdamStep& s, void* ws, hipStream_t st) 
              p.seed,
              s.step,
              s.step_device,
-             {s.grad_scale, (float)(1.0 / (1.0 - std::pow(p.beta1, (double)s.step))),
-              (float)(1.0 / (1.0 - std::pow(p.beta2, (double)s.step))), s.rate, 0},
+             host,
              scalars};
   dispatch_elem(p.type, [&](auto tag) {
     using P = decltype(tag);

@@ -18,78 +18,83 @@
 #include <type_traits>
 
 #include "activation.h"
+#include "product.h"
 
 namespace mgp {
 
 namespace {
 
-template <class T>
-struct Raw {  // one vector as it lies in memory
-  T v[Vec16<T>::N];
+// How a kernel reads: elements of type T, V channels a thread (16 bytes of them, or
+// one where a row has fewer).
+template <class E, int V_>
+struct Kind {
+  using T = E;
+  static constexpr int V = V_;
 };
 
-// Vectors go at any alignment; of a row's last one `left` elements exist.
-template <class T>
-__device__ __forceinline__ Raw<T> load_raw(const T* p, int left) {
-  constexpr int V = Vec16<T>::N;
-  Raw<T> a;
-  if (left >= V) {
-    __builtin_memcpy(&a, p, sizeof(a));
-  } else {
-#pragma unroll
-    for (int k = 0; k < V; ++k) a.v[k] = k < left ? p[k] : (T)0.0f;
-  }
+template <class K>
+struct Raw {  // one vector as it lies in memory
+  typename K::T v[K::V];
+};
+
+// Vectors go at any alignment.
+template <class K>
+__device__ __forceinline__ Raw<K> load_raw(const typename K::T* p) {
+  Raw<K> a;
+  __builtin_memcpy(&a, p, sizeof(a));
   return a;
 }
 
-template <class T>
-__device__ __forceinline__ void store_raw(T* p, int left, const float* v) {
-  constexpr int V = Vec16<T>::N;
-  Raw<T> a;
+// The elements of a vector from the `from`th on.
+template <class K>
+__device__ __forceinline__ void store_raw(typename K::T* p, int from, const float* v) {
+  Raw<K> a;
 #pragma unroll
-  for (int k = 0; k < V; ++k) a.v[k] = (T)v[k];
-  if (left >= V) {
+  for (int k = 0; k < K::V; ++k) a.v[k] = (typename K::T)v[k];
+  if (from == 0) {
     __builtin_memcpy(p, &a, sizeof(a));
   } else {
 #pragma unroll
-    for (int k = 0; k < V; ++k)
-      if (k < left) p[k] = a.v[k];
+    for (int k = 0; k < K::V; ++k)
+      if (k >= from) p[k] = a.v[k];
   }
 }
 
 // V parameters from channel c on, or the default
-template <class T>
-__device__ __forceinline__ void load_params(const void* p, int64_t c, int left, bool f32,
-                                            float none, float* v) {
+template <class K>
+__device__ __forceinline__ void load_params(const void* p, int c, bool f32, float none, float* v) {
+  if (p == nullptr) {
 #pragma unroll
-  for (int k = 0; k < Vec16<T>::N; ++k)
-    v[k] = p == nullptr || k >= left ? none
-           : f32                     ? static_cast<const float*>(p)[c + k]
-                                     : (float)static_cast<const T*>(p)[c + k];
+    for (int k = 0; k < K::V; ++k) v[k] = none;
+  } else if (f32) {
+    load_run<K::V>(static_cast<const float*>(p) + c, K::V, v);
+  } else {
+    load_run<K::V>(static_cast<const typename K::T*>(p) + c, K::V, v);
+  }
 }
 
 // z -> act(z); and with its derivative.
-template <class T>
+template <class K>
 __device__ __forceinline__ void act_values(int act, float* z) {
-  constexpr int V = Vec16<T>::N;
+  constexpr int V = K::V;
   auto go = [&](auto which) __attribute__((always_inline)) {
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       float a, slope;
-      activate<which.value, sizeof(T) == 2>(z[k], a, slope);
+      activate<which.value, sizeof(typename K::T) == 2>(z[k], a, slope);
       z[k] = a;
     }
   };
   if (act >= 0) dispatch_act_device(act, go);
 }
-template <class T>
+template <class K>
 __device__ __forceinline__ void act_slopes(int act, const float* z, float* slopes) {
-  constexpr int V = Vec16<T>::N;
+  constexpr int V = K::V;
   auto go = [&](auto which) __attribute__((always_inline)) {
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       float a;
-      activate<which.value, sizeof(T) == 2>(z[k], a, slopes[k]);
+      activate<which.value, sizeof(typename K::T) == 2>(z[k], a, slopes[k]);
     }
   };
   if (act >= 0) {
@@ -110,11 +115,12 @@ struct GroupKernel {
   float2* part;    // partial results of channels
   float2* coef;    // [samples][groups]: the two group sums over m
   float inv_m;     // 1 / m
+  bool apart;      // the result shares no memory with what is read
   // whole samples: vectors of a row, rows at a time, samples at a time, threads a
   // group (its sums)
   int cv, rows, at_a_time, lanes;
   int64_t batches;
-  // stretches: rows of one, how many a sample, column blocks of 256 vectors
+  // stretches: rows of one, how many a sample, column blocks of cv vectors
   int64_t stretch;
   int stretches, blocks;
 };
@@ -126,22 +132,35 @@ struct GroupKernel {
 constexpr int kMostThreads = 512;
 enum Join : int { CHANNELS = 0, VECTORS = 1, LANES = 2, THREAD = 3 };
 // Statistics that a vector's channels have: one, or each its own.
-template <class T, int JOIN>
-constexpr int kStats = JOIN == CHANNELS || JOIN == THREAD ? Vec16<T>::N : 1;
+template <class K, int JOIN>
+constexpr int kStats = JOIN == CHANNELS || JOIN == THREAD ? K::V : 1;
+
+// The channels of a thread: vector j of those from `base` on.  The last one of a row
+// ends with it, and shares its first `dup` channels with the one before, so that rows of
+// any width are read as vectors.  A result in the place of what is read is stored by
+// one thread (from): the shared channels may be read when the other has written
+// them, and are not used.
+template <class K>
+struct Columns {
+  int col, dup, from;
+  __device__ __forceinline__ Columns(const GroupKernel& s, int base, int j) {
+    const int first = base + j * K::V;
+    dup = max(first + K::V - s.a.channels, 0);
+    col = first - dup;
+    from = s.apart ? 0 : dup;
+  }
+};
 
 // What a thread is in such a workgroup.
-template <class T, int R, int JOIN>
-struct Place {
-  static constexpr int V = Vec16<T>::N;
-  int slot, col, left, sample, row;  // sample: among those at a time; row: its first
-  int slots;                         // rows at a time that are taken, of one sample
+template <class K>
+struct Place : Columns<K> {
+  int slot, sample, row;  // sample: among those at a time; row: its first
+  int slots;              // rows at a time that are taken, of one sample
   bool active;
-  __device__ __forceinline__ explicit Place(const GroupKernel& s) {
+  __device__ __forceinline__ explicit Place(const GroupKernel& s)
+      : Columns<K>(s, 0, (int)threadIdx.x - (int)threadIdx.x / s.cv * s.cv) {
     slot = threadIdx.x / s.cv;
-    col = (threadIdx.x - slot * s.cv) * V;
-    left = s.a.channels - col;
-    const int positions = (int)min(s.a.positions, (int64_t)1 << 30);
-    slots = min(s.rows, positions);
+    slots = min(s.rows, (int)min(s.a.positions, (int64_t)1 << 30));
     sample = slot / slots;
     row = slot - sample * slots;
     active = sample < s.at_a_time;
@@ -165,11 +184,11 @@ __device__ __forceinline__ void block_sums(float* v, int size) {
 
 // Where the entries of a pair (sample at a time, group) lie in LDS: runs of `run` from
 // `at` on, one for each of the sample's slots, `width` apart.
-template <class T, int JOIN>
+template <class K, int JOIN>
 struct Entries {
   int run, width;
   __device__ __forceinline__ explicit Entries(const GroupKernel& s) {
-    constexpr int V = Vec16<T>::N;
+    constexpr int V = K::V;
     const int size = s.a.channels / s.a.groups;
     run = JOIN == VECTORS ? size / V : size;
     width = JOIN == VECTORS ? s.cv : s.cv * V;
@@ -181,31 +200,48 @@ __device__ __forceinline__ float lane_sum(float v, int lanes) {
   return v;
 }
 
-template <class T, int R, int JOIN>
+template <class K, int R, int JOIN>
 __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
-  constexpr int V = Vec16<T>::N;
+  using T = typename K::T;
+  constexpr int V = K::V;
   extern __shared__ float2 lds[];
-  const Place<T, R, JOIN> at(s);
+  const Place<K> at(s);
   const int size = s.a.channels / s.a.groups;
   const int64_t L = s.a.positions;
   float w[V], b[V];
-  load_params<T>(s.a.weight, at.col, at.left, s.a.f32_params, 1.0f, w);
-  load_params<T>(s.a.bias, at.col, at.left, s.a.f32_params, 0.0f, b);
-  for (int64_t batch = blockIdx.x; batch < s.batches; batch += gridDim.x) {
-    const int64_t n = batch * s.at_a_time + at.sample;
-    const bool in = at.active && n < s.a.samples;
+  load_params<K>(s.a.weight, at.col, s.a.f32_params, 1.0f, w);
+  load_params<K>(s.a.bias, at.col, s.a.f32_params, 0.0f, b);
+  auto load = [&](int64_t n, Raw<K> (&x)[R]) __attribute__((always_inline)) {
     const T* px = static_cast<const T*>(s.a.x) + (n * L + at.row) * s.a.x_stride + at.col;
-    Raw<T> x[R];
     int count = 0;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const bool has = in && at.row + r * at.slots < L;
-      x[r] = load_raw(px + (int64_t)r * at.slots * s.a.x_stride, has ? at.left : 0);
+      const bool has = at.active && n < s.a.samples && at.row + r * at.slots < L;
+      if (has) x[r] = load_raw<K>(px + (int64_t)r * at.slots * s.a.x_stride);
       count += has;
     }
-    constexpr int MV = kStats<T, JOIN>;
+    return count;
+  };
+  // single rows: the next ones are loaded ahead
+  Raw<K> ahead[R];
+  int count_ahead = 0;
+  if constexpr (R == 1) count_ahead = load((int64_t)blockIdx.x * s.at_a_time + at.sample, ahead);
+  for (int64_t batch = blockIdx.x; batch < s.batches; batch += gridDim.x) {
+    const int64_t n = batch * s.at_a_time + at.sample;
+    const bool in = at.active && n < s.a.samples;
+    Raw<K> x[R];
+    int count;
+    if constexpr (R == 1) {
+      x[0] = ahead[0];
+      count = count_ahead;
+      count_ahead = load(n + (int64_t)gridDim.x * s.at_a_time, ahead);
+    } else {
+      count = load(n, x);
+    }
+    constexpr int MV = kStats<K, JOIN>;
     float mean[MV], rstd[MV];
     if constexpr (JOIN == THREAD || JOIN == LANES) {
+      if (!in) x[0] = Raw<K>{};
       // of V sums those of a thread's groups
       auto join = [&](const float (&v)[V], float (&sum)[MV]) __attribute__((always_inline)) {
         if constexpr (JOIN == THREAD) {
@@ -243,11 +279,11 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
       if (s.stats && in && (JOIN == THREAD || at.col % size == 0)) {
 #pragma unroll
         for (int k = 0; k < MV; ++k)
-          if (k % size == 0 && k < at.left)
+          if (k % size == 0 && k >= at.dup)
             s.stats[n * s.a.groups + (at.col + k) / size] = {mean[k], rstd[k]};
       }
     } else {
-      const Entries<T, JOIN> e(s);
+      const Entries<K, JOIN> e(s);
       float2* group = lds + (blockDim.x / s.cv) * e.width;  // a pair's mean and rstd
       if (JOIN == VECTORS) {
         const float base = (float)x[0].v[0];
@@ -284,7 +320,7 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
             const float d = r < count ? (float)x[r].v[k] - m : 0.0f;
             q = fmaf(d, d, q);
           }
-          lds[at.slot * e.width + at.col + k] = {m, q};
+          if (k >= at.dup) lds[at.slot * e.width + at.col + k] = {m, q};
         }
       }
       __syncthreads();
@@ -342,8 +378,8 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
 #pragma unroll
           for (int k = 0; k < V; ++k)
             z[k] = fmaf(((float)x[r].v[k] - mean[k % MV]) * rstd[k % MV], w[k], b[k]);
-          act_values<T>(s.a.activation, z);
-          store_raw(py + (int64_t)r * at.slots * s.ldo, at.left, z);
+          act_values<K>(s.a.activation, z);
+          store_raw<K>(py + (int64_t)r * at.slots * s.ldo, at.from, z);
         }
       }
     }
@@ -351,18 +387,18 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
 }
 
 // dz of one vector, and what z it had: xhat.
-template <class T, int MV>
-__device__ __forceinline__ void vector_dz(const GroupArgs& a, const Raw<T>& x, const Raw<T>& dy,
+template <class K, int MV>
+__device__ __forceinline__ void vector_dz(const GroupArgs& a, const Raw<K>& x, const Raw<K>& dy,
                                           const float (&mean)[MV], const float (&rstd)[MV],
                                           const float* w, const float* b, float* xhat, float* dz) {
-  constexpr int V = Vec16<T>::N;
+  constexpr int V = K::V;
   float z[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) {
     xhat[k] = ((float)x.v[k] - mean[k % MV]) * rstd[k % MV];
     z[k] = fmaf(xhat[k], w[k], b[k]);
   }
-  act_slopes<T>(a.activation, z, dz);
+  act_slopes<K>(a.activation, z, dz);
 #pragma unroll
   for (int k = 0; k < V; ++k) dz[k] *= (float)dy.v[k];
 }
@@ -382,41 +418,63 @@ __device__ __forceinline__ void load_stats(const GroupArgs& a, const float2* sta
 }
 
 // part[block][channels]: sums of dz and dz xhat over the block's samples.
-template <class T, int R, int JOIN>
+template <class K, int R, int JOIN>
 __global__ __launch_bounds__(kMostThreads) void k_group_bwd(GroupKernel s) {
-  constexpr int V = Vec16<T>::N;
+  using T = typename K::T;
+  constexpr int V = K::V;
   extern __shared__ float2 lds[];
-  const Place<T, R, JOIN> at(s);
+  const Place<K> at(s);
   const int size = s.a.channels / s.a.groups;
   const int64_t L = s.a.positions;
   float w[V], b[V], sum_a[V], sum_b[V];
-  load_params<T>(s.a.weight, at.col, at.left, s.a.f32_params, 1.0f, w);
-  load_params<T>(s.a.bias, at.col, at.left, s.a.f32_params, 0.0f, b);
+  load_params<K>(s.a.weight, at.col, s.a.f32_params, 1.0f, w);
+  load_params<K>(s.a.bias, at.col, s.a.f32_params, 0.0f, b);
 #pragma unroll
   for (int k = 0; k < V; ++k) sum_a[k] = sum_b[k] = 0.0f;
-  for (int64_t batch = blockIdx.x; batch < s.batches; batch += gridDim.x) {
-    const int64_t n = batch * s.at_a_time + at.sample;
-    const bool in = at.active && n < s.a.samples;
+  constexpr int MV = kStats<K, JOIN>;
+  struct Rows {
+    Raw<K> x[R], dy[R];
+    float mean[MV], rstd[MV];
+    int count;
+  };
+  auto load = [&](int64_t n, Rows& v) __attribute__((always_inline)) {
     const int64_t row0 = n * L + at.row;
     const T* px = static_cast<const T*>(s.a.x) + row0 * s.a.x_stride + at.col;
     const T* pd = static_cast<const T*>(s.dy) + row0 * s.ldy + at.col;
-    Raw<T> x[R], dy[R];
-    int count = 0;
+    const bool in = at.active && n < s.a.samples;
+    v.count = 0;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const bool has = in && at.row + r * at.slots < L;
-      x[r] = load_raw(px + (int64_t)r * at.slots * s.a.x_stride, has ? at.left : 0);
-      dy[r] = load_raw(pd + (int64_t)r * at.slots * s.ldy, has ? at.left : 0);
-      count += has;
+      if (has) {
+        v.x[r] = load_raw<K>(px + (int64_t)r * at.slots * s.a.x_stride);
+        v.dy[r] = load_raw<K>(pd + (int64_t)r * at.slots * s.ldy);
+      }
+      v.count += has;
     }
-    constexpr int MV = kStats<T, JOIN>;
-    float mean[MV], rstd[MV], t1[MV], t2[MV];  // t1, t2: the sample's group sums
     if (in) {
-      load_stats(s.a, s.stats, n, at.col, mean, rstd);
+      load_stats(s.a, s.stats, n, at.col, v.mean, v.rstd);
     } else {
 #pragma unroll
-      for (int k = 0; k < MV; ++k) mean[k] = rstd[k] = 0.0f;
+      for (int k = 0; k < MV; ++k) v.mean[k] = v.rstd[k] = 0.0f;
     }
+  };
+  Rows ahead;  // single rows: the next ones are loaded ahead
+  if constexpr (R == 1) load((int64_t)blockIdx.x * s.at_a_time + at.sample, ahead);
+  for (int64_t batch = blockIdx.x; batch < s.batches; batch += gridDim.x) {
+    const int64_t n = batch * s.at_a_time + at.sample;
+    const bool in = at.active && n < s.a.samples;
+    Rows now;
+    if constexpr (R == 1) {
+      now = ahead;
+      load(n + (int64_t)gridDim.x * s.at_a_time, ahead);
+    } else {
+      load(n, now);
+    }
+    const auto &x = now.x, &dy = now.dy;
+    const auto &mean = now.mean, &rstd = now.rstd;
+    const int count = now.count;
+    float t1[MV], t2[MV];  // the sample's group sums
     {
       float a1[V], a2[V];
 #pragma unroll
@@ -425,10 +483,9 @@ __global__ __launch_bounds__(kMostThreads) void k_group_bwd(GroupKernel s) {
       for (int r = 0; r < R; ++r) {
         if (r < count) {
           float xhat[V], dz[V];
-          vector_dz(s.a, x[r], dy[r], mean, rstd, w, b, xhat, dz);
+          vector_dz<K>(s.a, x[r], dy[r], mean, rstd, w, b, xhat, dz);
 #pragma unroll
           for (int k = 0; k < V; ++k) {
-            if (k >= at.left) dz[k] = 0.0f;
             a1[k] += dz[k];
             a2[k] = fmaf(dz[k], xhat[k], a2[k]);
           }
@@ -452,12 +509,13 @@ __global__ __launch_bounds__(kMostThreads) void k_group_bwd(GroupKernel s) {
       t1[0] = lane_sum(t1[0], s.lanes);
       t2[0] = lane_sum(t2[0], s.lanes);
     } else {
-      const Entries<T, JOIN> e(s);
+      const Entries<K, JOIN> e(s);
       float2* group = lds + (blockDim.x / s.cv) * e.width;
       if (at.active) {
 #pragma unroll
         for (int k = 0; k < MV; ++k)
-          lds[at.slot * e.width + (JOIN == VECTORS ? at.col / V : at.col + k)] = {t1[k], t2[k]};
+          if (JOIN == VECTORS || k >= at.dup)
+            lds[at.slot * e.width + (JOIN == VECTORS ? at.col / V : at.col + k)] = {t1[k], t2[k]};
       }
       __syncthreads();
       const int pairs = s.at_a_time * s.a.groups;
@@ -493,17 +551,17 @@ __global__ __launch_bounds__(kMostThreads) void k_group_bwd(GroupKernel s) {
       }
     }
     if (in) {
-      T* po = static_cast<T*>(s.out) + row0 * s.ldo + at.col;
+      T* po = static_cast<T*>(s.out) + (n * L + at.row) * s.ldo + at.col;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         if (r < count) {
           float xhat[V], dz[V];
-          vector_dz(s.a, x[r], dy[r], mean, rstd, w, b, xhat, dz);
+          vector_dz<K>(s.a, x[r], dy[r], mean, rstd, w, b, xhat, dz);
 #pragma unroll
           for (int k = 0; k < V; ++k)
             dz[k] = rstd[k % MV] *
                     fmaf(w[k], dz[k], -s.inv_m * fmaf(xhat[k], t2[k % MV], t1[k % MV]));
-          store_raw(po + (int64_t)r * at.slots * s.ldo, at.left, dz);
+          store_raw<K>(po + (int64_t)r * at.slots * s.ldo, at.from, dz);
         }
       }
     }
@@ -514,7 +572,8 @@ __global__ __launch_bounds__(kMostThreads) void k_group_bwd(GroupKernel s) {
   const int width = s.cv * V, taken = at.slots * s.at_a_time;
   if (at.active) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) lds[at.slot * width + at.col + k] = {sum_a[k], sum_b[k]};
+    for (int k = 0; k < V; ++k)
+      if (k >= at.dup) lds[at.slot * width + at.col + k] = {sum_a[k], sum_b[k]};
   }
   __syncthreads();
   for (int c = threadIdx.x; c < s.a.channels; c += blockDim.x) {
@@ -532,26 +591,24 @@ __global__ __launch_bounds__(kMostThreads) void k_group_bwd(GroupKernel s) {
 
 constexpr int kPartThreads = 256;
 
-// A stretch of rows of one sample, in one block of columns.
-template <class T>
-struct Piece {
-  static constexpr int V = Vec16<T>::N;
-  int64_t n, row0, rows;  // first row within the sample
-  int64_t chunk;
-  int col, cv, slots, slot, left, base;  // vectors of the block, rows at a time; base: its first channel
+// A stretch of rows of a sample, in one block of columns.
+template <class K>
+struct Piece : Columns<K> {
+  int chunk, slots, slot, base, cv;  // rows at a time; base, cv: first channel, vectors of the block
+  int64_t row0, rows;                // first row within the sample
   bool active;
-  __device__ __forceinline__ Piece(const GroupKernel& s, int64_t item) {
-    const int64_t block = item % s.blocks, at = item / s.blocks;
-    chunk = at % s.stretches;
-    n = at / s.stretches;
+  static __device__ __forceinline__ int vectors(const GroupKernel& s, int block) {
+    return min(s.cv, (s.a.channels + K::V - 1) / K::V - block * s.cv);
+  }
+  __device__ __forceinline__ Piece(const GroupKernel& s, int block)
+      : Columns<K>(s, block * s.cv * K::V, (int)threadIdx.x % vectors(s, block)) {
+    chunk = blockIdx.x / s.blocks;
     row0 = chunk * s.stretch;
     rows = min(s.stretch, s.a.positions - row0);
-    base = (int)block * kPartThreads * V;
-    cv = min(kPartThreads, (s.a.channels - base + V - 1) / V);
+    base = block * s.cv * K::V;
+    cv = vectors(s, block);
     slots = kPartThreads / cv;
     slot = threadIdx.x / cv;
-    col = base + (threadIdx.x - slot * cv) * V;
-    left = s.a.channels - col;
     active = slot < slots;
   }
   __device__ __forceinline__ int64_t count_of(int slot_) const {  // its rows
@@ -559,92 +616,123 @@ struct Piece {
   }
 };
 
+// U rows of a thread at a time, the next ones loaded ahead.  Rows past the last are
+// read as the last.
+template <class K, int U, bool BACK>
+struct Stream {
+  using T = typename K::T;
+  const T *px, *pd;
+  int64_t sx, sd, last;
+  Raw<K> x[U], dy[BACK ? U : 1];
+  __device__ __forceinline__ void load(int64_t i) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t r = min(i + u, last);
+      x[u] = load_raw<K>(px + r * sx);
+      if constexpr (BACK) dy[u] = load_raw<K>(pd + r * sd);
+    }
+  }
+  // of the `count` > 0 rows of sample n
+  __device__ __forceinline__ Stream(const GroupKernel& s, const Piece<K>& at, int64_t n,
+                                    int64_t count)
+      : sx((int64_t)at.slots * s.a.x_stride), sd((int64_t)at.slots * s.ldy), last(count - 1) {
+    const int64_t row = n * s.a.positions + at.row0 + at.slot;
+    px = static_cast<const T*>(s.a.x) + row * s.a.x_stride + at.col;
+    pd = BACK ? static_cast<const T*>(s.dy) + row * s.ldy + at.col : nullptr;
+    load(0);
+  }
+};
+
 // part[sample][stretch][channels]: mean and centred squares of a channel; BACK: its
 // sums of dz and dz xhat.
-template <class T, bool BACK, int MV>
-__global__ __launch_bounds__(kPartThreads) void k_group_part(GroupKernel s, int64_t items) {
-  constexpr int V = Vec16<T>::N, U = 4;
+template <class K, bool BACK, int MV>
+__global__ __launch_bounds__(kPartThreads) void k_group_part(GroupKernel s) {
+  constexpr int V = K::V, U = BACK ? 2 : 4;
   __shared__ float2 lds[kPartThreads * V];
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const Piece<T> at(s, item);
-    const int64_t row = at.n * s.a.positions + at.row0 + at.slot;
-    const T* px = static_cast<const T*>(s.a.x) + row * s.a.x_stride + at.col;
-    const int64_t sx = (int64_t)at.slots * s.a.x_stride;
-    const int64_t count = at.active ? at.count_of(at.slot) : 0;
+  const Piece<K> at(s, blockIdx.x % s.blocks);
+  const int64_t count = at.active ? at.count_of(at.slot) : 0;
+  float w[V], b[V];
+  if constexpr (BACK) {
+    load_params<K>(s.a.weight, at.col, s.a.f32_params, 1.0f, w);
+    load_params<K>(s.a.bias, at.col, s.a.f32_params, 0.0f, b);
+  }
+  for (int64_t n = blockIdx.y; n < s.a.samples; n += gridDim.y) {
     float m[V], q[V];  // or the two sums
 #pragma unroll
     for (int k = 0; k < V; ++k) m[k] = q[k] = 0.0f;
-    if constexpr (!BACK) {
-      int64_t done = 0;
-      const Raw<T> base = load_raw(px, count ? at.left : 0);  // means are formed from here
-      for (; done + U <= count; done += U) {
-        Raw<T> x[U];
+    if (count > 0) {
+      Stream<K, U, BACK> rows(s, at, n, count);
+      if constexpr (!BACK) {
+        const Raw<K> base = rows.x[0];  // means are formed from here
+        int64_t done = 0;
+        for (; done + U <= count; done += U) {
+          Raw<K> x[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) x[u] = load_raw(px + (done + u) * sx, at.left);
-        const float n1 = (float)done, share = (float)U / (float)(done + U);
+          for (int u = 0; u < U; ++u) x[u] = rows.x[u];
+          rows.load(done + U);
+          const float n1 = (float)done, share = (float)U / (float)(done + U);
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-          float v[U];
+          for (int k = 0; k < V; ++k) {
+            float v[U];
 #pragma unroll
-          for (int u = 0; u < U; ++u) v[u] = (float)x[u].v[k] - (float)base.v[k];
-          const float mean = ((v[0] + v[1]) + (v[2] + v[3])) * 0.25f;
-          float sq = 0.0f;
+            for (int u = 0; u < U; ++u) v[u] = (float)x[u].v[k] - (float)base.v[k];
+            const float mean = ((v[0] + v[1]) + (v[2] + v[3])) * 0.25f;
+            float sq = 0.0f;
 #pragma unroll
-          for (int u = 0; u < U; ++u) sq = fmaf(v[u] - mean, v[u] - mean, sq);
-          const float d = mean - m[k];
-          m[k] = fmaf(d, share, m[k]);
-          q[k] += fmaf(d * d, n1 * share, sq);
+            for (int u = 0; u < U; ++u) sq = fmaf(v[u] - mean, v[u] - mean, sq);
+            const float d = mean - m[k];
+            m[k] = fmaf(d, share, m[k]);
+            q[k] += fmaf(d * d, n1 * share, sq);
+          }
         }
-      }
-      for (; done < count; ++done) {
-        const Raw<T> x = load_raw(px + done * sx, at.left);
-        const float n1 = (float)done, share = 1.0f / (float)(done + 1);
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const float d = ((float)x.v[k] - (float)base.v[k]) - m[k];
-          m[k] = fmaf(d, share, m[k]);
-          q[k] = fmaf(d * d, n1 * share, q[k]);
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < V; ++k) m[k] += (float)base.v[k];
-    } else if (at.active) {
-      const T* pd = static_cast<const T*>(s.dy) + row * s.ldy + at.col;
-      const int64_t sd = (int64_t)at.slots * s.ldy;
-      float w[V], b[V], mean[MV], rstd[MV];
-      load_params<T>(s.a.weight, at.col, at.left, s.a.f32_params, 1.0f, w);
-      load_params<T>(s.a.bias, at.col, at.left, s.a.f32_params, 0.0f, b);
-      load_stats(s.a, s.stats, at.n, at.col, mean, rstd);
-      auto add = [&](const Raw<T>& x, const Raw<T>& dy) __attribute__((always_inline)) {
-        float xhat[V], dz[V];
-        vector_dz(s.a, x, dy, mean, rstd, w, b, xhat, dz);
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          m[k] += dz[k];
-          q[k] = fmaf(dz[k], xhat[k], q[k]);
-        }
-      };
-      int64_t done = 0;
-      for (; done + U <= count; done += U) {
-        Raw<T> x[U], dy[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          x[u] = load_raw(px + (done + u) * sx, at.left);
-          dy[u] = load_raw(pd + (done + u) * sd, at.left);
+          if (done + u < count) {
+            const float n1 = (float)(done + u), share = 1.0f / (n1 + 1.0f);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+              const float d = ((float)rows.x[u].v[k] - (float)base.v[k]) - m[k];
+              m[k] = fmaf(d, share, m[k]);
+              q[k] = fmaf(d * d, n1 * share, q[k]);
+            }
+          }
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) add(x[u], dy[u]);
+        for (int k = 0; k < V; ++k) m[k] += (float)base.v[k];
+      } else {
+        float mean[MV], rstd[MV];
+        load_stats(s.a, s.stats, n, at.col, mean, rstd);
+        auto add = [&](const Raw<K>& x, const Raw<K>& dy) __attribute__((always_inline)) {
+          float xhat[V], dz[V];
+          vector_dz<K>(s.a, x, dy, mean, rstd, w, b, xhat, dz);
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            m[k] += dz[k];
+            q[k] = fmaf(dz[k], xhat[k], q[k]);
+          }
+        };
+        for (int64_t done = 0; done < count; done += U) {
+          Raw<K> x[U], dy[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            x[u] = rows.x[u];
+            dy[u] = rows.dy[u];
+          }
+          rows.load(done + U);
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (done + u < count) add(x[u], dy[u]);
+        }
       }
-      for (; done < count; ++done)
-        add(load_raw(px + done * sx, at.left), load_raw(pd + done * sd, at.left));
     }
     const int width = at.cv * V;
     if (at.active) {
 #pragma unroll
-      for (int k = 0; k < V; ++k) lds[at.slot * width + at.col - at.base + k] = {m[k], q[k]};
+      for (int k = 0; k < V; ++k)
+        if (k >= at.dup) lds[at.slot * width + at.col - at.base + k] = {m[k], q[k]};
     }
     __syncthreads();
-    float2* to = s.part + (at.n * s.stretches + at.chunk) * s.a.channels + at.base;
+    float2* to = s.part + (n * s.stretches + at.chunk) * s.a.channels + at.base;
     const int used = (int)min((int64_t)at.slots, at.rows);
     for (int c = threadIdx.x; c < min(width, s.a.channels - at.base); c += kPartThreads) {
       float2 t = lds[c];
@@ -675,124 +763,135 @@ __global__ __launch_bounds__(kPartThreads) void k_group_part(GroupKernel s, int6
   }
 }
 
-// A wave a group: its mean and rstd, or (BACK) the two sums over m.
+__device__ __forceinline__ float block_sum(float v, float* red) {
+  v = lane_sum(v, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// A workgroup a group: its mean and rstd, or (BACK) the two sums over m.  The first
+// 2048 partial results stay in registers between the two sweeps.
 template <class T, bool BACK>
 __global__ __launch_bounds__(256) void k_group_merge(GroupKernel s) {
-  const int lane = threadIdx.x & 63;
+  constexpr int KEPT = 8;
+  __shared__ float red[4];
   const int size = s.a.channels / s.a.groups;
-  const int64_t pairs = s.a.samples * s.a.groups, all = (int64_t)s.stretches * size;
-  for (int64_t p = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); p < pairs;
-       p += (int64_t)gridDim.x * 4) {
+  const int64_t pairs = s.a.samples * s.a.groups;
+  const int64_t all = (int64_t)s.stretches * size;
+  for (int64_t p = blockIdx.x; p < pairs; p += gridDim.x) {
     const int64_t n = p / s.a.groups;
     const int g = (int)(p - n * s.a.groups);
     const float2* from = s.part + n * s.stretches * s.a.channels + (int64_t)g * size;
+    struct Entry {
+      float2 v;
+      float by;  // its rows, or its channel's weight
+    };
+    auto entry = [&](int64_t i) __attribute__((always_inline)) {
+      Entry e{{0.0f, 0.0f}, 0.0f};
+      if (i < all) {
+        const int chunk = (int)(i / size), d = (int)(i - (int64_t)chunk * size), c = g * size + d;
+        e.v = from[(int64_t)chunk * s.a.channels + d];
+        if constexpr (BACK)
+          e.by = s.a.weight == nullptr ? 1.0f
+                 : s.a.f32_params      ? static_cast<const float*>(s.a.weight)[c]
+                                       : (float)static_cast<const T*>(s.a.weight)[c];
+        else
+          e.by = (float)min(s.stretch, s.a.positions - chunk * s.stretch);
+      }
+      return e;
+    };
+    Entry kept[KEPT];
+#pragma unroll
+    for (int k = 0; k < KEPT; ++k) kept[k] = entry(threadIdx.x + 256 * k);
     auto sweep = [&](auto f) __attribute__((always_inline)) {
       float t = 0.0f;
-      for (int64_t i = lane; i < all; i += 64) {
-        const int64_t chunk = i / size;
-        const int d = (int)(i - chunk * size);
-        t += f(from[chunk * s.a.channels + d],
-               (float)min(s.stretch, s.a.positions - chunk * s.stretch), g * size + d);
-      }
-      return lane_sum(t, 64);
+#pragma unroll
+      for (int k = 0; k < KEPT; ++k) t += f(kept[k]);
+      for (int64_t i = threadIdx.x + 256 * KEPT; i < all; i += 256) t += f(entry(i));
+      return block_sum(t, red);
     };
     if constexpr (!BACK) {
       const float base = from[0].x;
-      const float m =
-          fmaf(sweep([&](float2 v, float c, int) { return (v.x - base) * c; }), s.inv_m, base);
-      const float var = sweep([&](float2 v, float c, int) {
-                          return fmaf(c * (v.x - m), v.x - m, v.y);
+      const float m = fmaf(sweep([&](const Entry& e) { return (e.v.x - base) * e.by; }), s.inv_m,
+                           base);
+      const float var = sweep([&](const Entry& e) {
+                          return fmaf(e.by * (e.v.x - m), e.v.x - m, e.v.y);
                         }) * s.inv_m;
-      if (lane == 0) s.stats[p] = {m, 1.0f / sqrtf(var + s.a.eps)};
+      if (threadIdx.x == 0) s.stats[p] = {m, 1.0f / sqrtf(var + s.a.eps)};
     } else {
-      auto weight = [&](int c) __attribute__((always_inline)) {
-        return s.a.weight == nullptr ? 1.0f
-               : s.a.f32_params      ? static_cast<const float*>(s.a.weight)[c]
-                                     : (float)static_cast<const T*>(s.a.weight)[c];
-      };
-      const float t1 = sweep([&](float2 v, float, int c) { return v.x * weight(c); });
-      const float t2 = sweep([&](float2 v, float, int c) { return v.y * weight(c); });
-      if (lane == 0) s.coef[p] = {t1 * s.inv_m, t2 * s.inv_m};
+      const float t1 = sweep([](const Entry& e) { return e.v.x * e.by; });
+      const float t2 = sweep([](const Entry& e) { return e.v.y * e.by; });
+      if (threadIdx.x == 0) s.coef[p] = {t1 * s.inv_m, t2 * s.inv_m};
     }
   }
 }
 
 // y, or (BACK) dx, of a stretch.
-template <class T, bool BACK, int MV>
-__global__ __launch_bounds__(kPartThreads) void k_group_apply(GroupKernel s, int64_t items) {
-  constexpr int V = Vec16<T>::N, U = BACK ? 2 : 4;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const Piece<T> at(s, item);
-    if (!at.active) continue;
-    const int64_t row = at.n * s.a.positions + at.row0 + at.slot, count = at.count_of(at.slot);
-    const T* px = static_cast<const T*>(s.a.x) + row * s.a.x_stride + at.col;
-    T* po = static_cast<T*>(s.out) + row * s.ldo + at.col;
-    const int64_t sx = (int64_t)at.slots * s.a.x_stride, so = (int64_t)at.slots * s.ldo;
-    float w[V], b[V], mean[MV], rstd[MV];
-    load_params<T>(s.a.weight, at.col, at.left, s.a.f32_params, 1.0f, w);
-    load_params<T>(s.a.bias, at.col, at.left, s.a.f32_params, 0.0f, b);
-    load_stats(s.a, s.stats, at.n, at.col, mean, rstd);
-    if constexpr (!BACK) {
-      auto put = [&](const Raw<T>& x, int64_t i) __attribute__((always_inline)) {
+template <class K, bool BACK, int MV>
+__global__ __launch_bounds__(kPartThreads) void k_group_apply(GroupKernel s) {
+  using T = typename K::T;
+  constexpr int V = K::V, U = BACK ? 2 : 4;
+  const Piece<K> at(s, blockIdx.x % s.blocks);
+  const int64_t count = at.active ? at.count_of(at.slot) : 0;
+  if (count == 0) return;
+  const int64_t so = (int64_t)at.slots * s.ldo;
+  float w[V], b[V];
+  load_params<K>(s.a.weight, at.col, s.a.f32_params, 1.0f, w);
+  load_params<K>(s.a.bias, at.col, s.a.f32_params, 0.0f, b);
+  for (int64_t n = blockIdx.y; n < s.a.samples; n += gridDim.y) {
+    Stream<K, U, BACK> rows(s, at, n, count);
+    T* po = static_cast<T*>(s.out) + (n * s.a.positions + at.row0 + at.slot) * s.ldo + at.col;
+    float mean[MV], rstd[MV], c1[MV], c2[MV];
+    load_stats(s.a, s.stats, n, at.col, mean, rstd);
+    if constexpr (BACK) load_stats(s.a, s.coef, n, at.col, c1, c2);
+    for (int64_t i = 0; i < count; i += U) {
+      Raw<K> x[U], dy[BACK ? U : 1];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        x[u] = rows.x[u];
+        if constexpr (BACK) dy[u] = rows.dy[u];
+      }
+      rows.load(i + U);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i + u >= count) continue;
         float z[V];
+        if constexpr (BACK) {
+          float xhat[V];
+          vector_dz<K>(s.a, x[u], dy[u], mean, rstd, w, b, xhat, z);
 #pragma unroll
-        for (int k = 0; k < V; ++k)
-          z[k] = fmaf(((float)x.v[k] - mean[k % MV]) * rstd[k % MV], w[k], b[k]);
-        act_values<T>(s.a.activation, z);
-        store_raw(po + i * so, at.left, z);
-      };
-      int64_t i = 0;
-      for (; i + U <= count; i += U) {
-        Raw<T> x[U];
+          for (int k = 0; k < V; ++k)
+            z[k] = rstd[k % MV] * fmaf(w[k], z[k], -fmaf(xhat[k], c2[k % MV], c1[k % MV]));
+        } else {
 #pragma unroll
-        for (int u = 0; u < U; ++u) x[u] = load_raw(px + (i + u) * sx, at.left);
-#pragma unroll
-        for (int u = 0; u < U; ++u) put(x[u], i + u);
-      }
-      for (; i < count; ++i) put(load_raw(px + i * sx, at.left), i);
-    } else {
-      const T* pd = static_cast<const T*>(s.dy) + row * s.ldy + at.col;
-      const int64_t sd = (int64_t)at.slots * s.ldy;
-      float c1[MV], c2[MV];
-      load_stats(s.a, s.coef, at.n, at.col, c1, c2);
-      auto put = [&](const Raw<T>& x, const Raw<T>& dy, int64_t i) __attribute__((always_inline)) {
-        float xhat[V], dz[V];
-        vector_dz(s.a, x, dy, mean, rstd, w, b, xhat, dz);
-#pragma unroll
-        for (int k = 0; k < V; ++k)
-          dz[k] = rstd[k % MV] * fmaf(w[k], dz[k], -fmaf(xhat[k], c2[k % MV], c1[k % MV]));
-        store_raw(po + i * so, at.left, dz);
-      };
-      int64_t i = 0;
-      for (; i + U <= count; i += U) {
-        Raw<T> x[U], dy[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          x[u] = load_raw(px + (i + u) * sx, at.left);
-          dy[u] = load_raw(pd + (i + u) * sd, at.left);
+          for (int k = 0; k < V; ++k)
+            z[k] = fmaf(((float)x[u].v[k] - mean[k % MV]) * rstd[k % MV], w[k], b[k]);
+          act_values<K>(s.a.activation, z);
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) put(x[u], dy[u], i + u);
+        store_raw<K>(po + (i + u) * so, at.from, z);
       }
-      for (; i < count; ++i)
-        put(load_raw(px + i * sx, at.left), load_raw(pd + i * sd, at.left), i);
     }
   }
 }
 
-// dweight, dbias: sums of the partial results in a fixed order, 16 channels a
-// workgroup.
+// dweight, dbias: sums of the partial results in a fixed order, kParamChannels channels
+// (64 bytes of partial results) a workgroup.
+constexpr int kParamChannels = 8;
 template <class P>
 __global__ __launch_bounds__(1024) void k_group_params(const float2* __restrict__ part,
                                                        int64_t parts, int channels,
                                                        P* __restrict__ dweight,
                                                        P* __restrict__ dbias) {
-  __shared__ float2 red[64][16];
-  const int c = threadIdx.x & 15, line = threadIdx.x >> 4, channel = blockIdx.x * 16 + c;
+  __shared__ float2 red[1024 / kParamChannels][kParamChannels];
+  constexpr int LINES = 1024 / kParamChannels;
+  const int c = threadIdx.x % kParamChannels, line = threadIdx.x / kParamChannels;
+  const int channel = blockIdx.x * kParamChannels + c;
   float2 t = {0.0f, 0.0f};
   if (channel < channels) {
-#pragma unroll 4
-    for (int64_t p = line; p < parts; p += 64) {
+#pragma unroll 8
+    for (int64_t p = line; p < parts; p += LINES) {
       const float2 v = part[p * channels + channel];
       t.x += v.x;
       t.y += v.y;
@@ -800,7 +899,7 @@ __global__ __launch_bounds__(1024) void k_group_params(const float2* __restrict_
   }
   red[line][c] = t;
   __syncthreads();
-  for (int o = 32; o >= 1; o >>= 1) {
+  for (int o = LINES / 2; o >= 1; o >>= 1) {
     if (line < o) {
       red[line][c].x += red[line + o][c].x;
       red[line][c].y += red[line + o][c].y;
@@ -815,12 +914,19 @@ __global__ __launch_bounds__(1024) void k_group_params(const float2* __restrict_
 // ---------------------------------------------------------------- host side
 
 constexpr int64_t kBackBlocks = 1024;  // partial results of whole samples, at most
+constexpr int64_t kStretches = 1024;    // workgroups of samples in stretches
 
-struct Cut {
+struct GroupCut {
   bool whole;  // samples in a workgroup's registers
   int join = CHANNELS, r = 1, threads = 256;
   size_t lds = 0;
 };
+
+// Channels of a thread: 16 bytes, or one in rows that have fewer.
+inline int lane_channels(const GroupArgs& a) {
+  const int v = a.type == ELEM_F32 ? 4 : 8;
+  return a.channels < v ? 1 : v;
+}
 
 inline int pow2_at_most(int64_t v) {
   int p = 1;
@@ -829,21 +935,23 @@ inline int pow2_at_most(int64_t v) {
 }
 
 // Fills in how the call is cut.
-Cut cut_of(GroupKernel& s, bool back) {
+GroupCut cut_of(GroupKernel& s, bool back) {
   const GroupArgs& a = s.a;
-  const int V = a.type == ELEM_F32 ? 4 : 8;
+  const int V = lane_channels(a);
   const int size = a.channels / a.groups, most = back ? 8 : 16;
   const int64_t cv = ceil_div((int64_t)a.channels, (int64_t)V), L = a.positions;
   s.inv_m = (float)(1.0 / ((double)L * size));
-  Cut c{};
+  GroupCut c{};
   int threads = 256;
   while (threads < kMostThreads && (cv > threads || ceil_div(L, (int64_t)(threads / cv)) > 4)) threads *= 2;
   c.whole = cv <= threads && ceil_div(L, (int64_t)(threads / cv)) <= most;
   if (!c.whole) {
     s.blocks = (int)ceil_div(cv, (int64_t)kPartThreads);
-    // about eight workgroups a CU, each thread at least eight rows
-    const int64_t slots = std::max<int64_t>(1, kPartThreads / cv);
-    const int64_t want = ceil_div((int64_t)2048, a.samples * s.blocks);
+    s.cv = (int)ceil_div(cv, (int64_t)s.blocks);
+    s.blocks = (int)ceil_div(cv, (int64_t)s.cv);
+    // about four workgroups a CU, each thread at least eight rows
+    const int64_t slots = std::max<int64_t>(1, kPartThreads / s.cv);
+    const int64_t want = ceil_div((int64_t)kStretches, a.samples * s.blocks);
     s.stretches = (int)std::max<int64_t>(1, std::min(want, L / (8 * slots)));
     s.stretch = ceil_div(L, (int64_t)s.stretches);
     s.stretches = (int)ceil_div(L, s.stretch);
@@ -880,41 +988,52 @@ inline unsigned back_blocks(const GroupKernel& s) {
   return (unsigned)std::min<int64_t>(s.batches, kBackBlocks);
 }
 
-template <class T, bool BACK, class F>
-void dispatch_whole(const Cut& c, F&& f) {
+// Runs f with a kernel's rows a thread and join.
+template <class K, bool BACK, class F>
+void dispatch_whole(const GroupCut& c, F&& f) {
+  using std::integral_constant;
   auto with = [&](auto r) {
-    if (c.join == CHANNELS)
-      f(r, std::integral_constant<int, CHANNELS>{});
-    else
-      f(r, std::integral_constant<int, VECTORS>{});
+    if constexpr (K::V > 1) {  // (of one channel a thread, channels are vectors)
+      if (c.join == CHANNELS) return f(r, integral_constant<int, CHANNELS>{});
+    }
+    f(r, integral_constant<int, VECTORS>{});
   };
-  if (c.join == THREAD) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, THREAD>{});
-  if (c.join == LANES) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, LANES>{});
-  if (c.r == 1)
-    with(std::integral_constant<int, 1>{});
-  else if (c.r == 4)
-    with(std::integral_constant<int, 4>{});
-  else
-    with(std::integral_constant<int, BACK ? 8 : 16>{});
+  if constexpr (K::V > 1) {
+    if (c.join == THREAD) return f(integral_constant<int, 1>{}, integral_constant<int, THREAD>{});
+  }
+  if (c.join == LANES) return f(integral_constant<int, 1>{}, integral_constant<int, LANES>{});
+  if (c.r == 1) return with(integral_constant<int, 1>{});
+  if (c.r == 4) return with(integral_constant<int, 4>{});
+  with(integral_constant<int, BACK ? 8 : 16>{});
 }
 
-template <class T, bool BACK>
+// Runs f with the call's Kind.
+template <class F>
+void dispatch_kind(const GroupArgs& a, F&& f) {
+  dispatch_elem(a.type, [&](auto tag) {
+    using T = decltype(tag);
+    if (lane_channels(a) == 1)
+      f(Kind<T, 1>{});
+    else
+      f(Kind<T, Vec16<T>::N>{});
+  });
+}
+
+template <class K, bool BACK>
 void launch_stretches(GroupKernel& s, hipStream_t st) {
-  const int64_t items = s.a.samples * s.stretches * s.blocks;
-  const unsigned grid = (unsigned)std::min<int64_t>(items, 1 << 16);
-  const unsigned waves =
-      (unsigned)std::min<int64_t>(ceil_div(s.a.samples * s.a.groups, (int64_t)4), 1 << 14);
+  const unsigned gx = (unsigned)(s.stretches * s.blocks);
+  const dim3 grid(gx, (unsigned)std::min<int64_t>(s.a.samples, std::max(1, (1 << 15) / (int)gx)));
+  const unsigned pairs = (unsigned)std::min<int64_t>(s.a.samples * s.a.groups, 1 << 16);
   auto go = [&](auto mv) {
-    k_group_part<T, BACK, mv.value><<<grid, kPartThreads, 0, st>>>(s, items);
+    k_group_part<K, BACK, mv.value><<<grid, kPartThreads, 0, st>>>(s);
     if (BACK && s.out == nullptr) return;
-    k_group_merge<T, BACK><<<waves, 256, 0, st>>>(s);
-    k_group_apply<T, BACK, mv.value><<<grid, kPartThreads, 0, st>>>(s, items);
+    k_group_merge<typename K::T, BACK><<<pairs, 256, 0, st>>>(s);
+    k_group_apply<K, BACK, mv.value><<<grid, kPartThreads, 0, st>>>(s);
   };
-  constexpr int V = Vec16<T>::N;
-  if (s.a.channels / s.a.groups % V == 0)  // a vector's channels are of one group
+  if (s.a.channels / s.a.groups % K::V == 0)  // a vector's channels are of one group
     go(std::integral_constant<int, 1>{});
   else
-    go(std::integral_constant<int, V>{});
+    go(std::integral_constant<int, K::V>{});
 }
 
 inline size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -928,7 +1047,7 @@ size_t group_norm_bytes(const GroupArgs& a, bool back) {
   if (a.samples * a.positions == 0) return 0;
   GroupKernel s{};
   s.a = a;
-  const Cut c = cut_of(s, back);
+  const GroupCut c = cut_of(s, back);
   const size_t row = (size_t)a.channels * sizeof(float2);
   if (c.whole) return back ? aligned(back_blocks(s) * row) : 0;
   return aligned((size_t)(a.samples * s.stretches) * row) + pairs_bytes(a);
@@ -942,20 +1061,21 @@ void group_norm(const GroupArgs& a, void* y, int64_t y_stride, float* stats, voi
   s.out = y;
   s.ldo = y_stride;
   s.stats = reinterpret_cast<float2*>(stats);
-  const Cut c = cut_of(s, false);
-  dispatch_elem(a.type, [&](auto tag) {
-    using T = decltype(tag);
+  s.apart = y != a.x;
+  const GroupCut c = cut_of(s, false);
+  dispatch_kind(a, [&](auto kind) {
+    using K = decltype(kind);
     if (!c.whole) {
       s.part = static_cast<float2*>(ws);
       if (!stats)
         s.stats = s.part + aligned((size_t)(a.samples * s.stretches) * a.channels * sizeof(float2)) /
                                sizeof(float2);
-      launch_stretches<T, false>(s, st);
+      launch_stretches<K, false>(s, st);
       return;
     }
-    const unsigned grid = (unsigned)std::min<int64_t>(s.batches, 1 << 16);
-    dispatch_whole<T, false>(c, [&](auto r, auto join) {
-      k_group_fwd<T, r.value, join.value><<<grid, c.threads, c.lds, st>>>(s);
+    const unsigned grid = (unsigned)std::min<int64_t>(s.batches, 2048);
+    dispatch_whole<K, false>(c, [&](auto r, auto join) {
+      k_group_fwd<K, r.value, join.value><<<grid, c.threads, c.lds, st>>>(s);
     });
   });
   MGP_HIP_CHECK(hipGetLastError());
@@ -971,28 +1091,29 @@ void group_norm_backward(const GroupArgs& a, const void* dy, int64_t dy_stride, 
   s.out = dx;
   s.ldo = dx_stride;
   s.stats = reinterpret_cast<float2*>(const_cast<float*>(stats));
+  s.apart = dx != a.x && dx != dy;
   const bool params = dweight || dbias;
   int64_t parts = 0;
   if (a.samples * a.positions > 0) {
-    const Cut c = cut_of(s, true);
-    dispatch_elem(a.type, [&](auto tag) {
-      using T = decltype(tag);
+    const GroupCut c = cut_of(s, true);
+    dispatch_kind(a, [&](auto kind) {
+      using K = decltype(kind);
       s.part = static_cast<float2*>(ws);
       if (!c.whole) {
         parts = a.samples * s.stretches;
         s.coef = s.part + aligned((size_t)parts * a.channels * sizeof(float2)) / sizeof(float2);
-        launch_stretches<T, true>(s, st);
+        launch_stretches<K, true>(s, st);
         return;
       }
       parts = back_blocks(s);
       if (!params) s.part = nullptr;
-      dispatch_whole<T, true>(c, [&](auto r, auto join) {
-        k_group_bwd<T, r.value, join.value><<<(unsigned)parts, c.threads, c.lds, st>>>(s);
+      dispatch_whole<K, true>(c, [&](auto r, auto join) {
+        k_group_bwd<K, r.value, join.value><<<(unsigned)parts, c.threads, c.lds, st>>>(s);
       });
     });
   }
   if (params) {
-    const unsigned grid = (unsigned)ceil_div((int64_t)a.channels, (int64_t)16);
+    const unsigned grid = (unsigned)ceil_div((int64_t)a.channels, (int64_t)kParamChannels);
     const float2* part = static_cast<const float2*>(ws);
     dispatch_elem(a.f32_params ? ELEM_F32 : a.type, [&](auto tag) {
       using P = decltype(tag);
