@@ -121,8 +121,8 @@ struct GroupKernel {
   int cv, rows, at_a_time, lanes;
   int64_t batches;
   // stretches: rows of one, how many a sample, column blocks of cv vectors
-  int64_t stretch;
-  int stretches, blocks;
+  int stretch, short_stretch;  // of partial results, and of the results
+  int stretches, shorts, blocks;
 };
 
 // How a sample's group sums come together in a workgroup that holds whole samples:
@@ -408,18 +408,24 @@ template <int MV>
 __device__ __forceinline__ void load_stats(const GroupArgs& a, const float2* stats, int64_t n,
                                            int col, float (&mean)[MV], float (&rstd)[MV]) {
   const int size = a.channels / a.groups;
+  int g = col / size, in = col - g * size;
+  const float2* row = stats + n * a.groups;
 #pragma unroll
   for (int k = 0; k < MV; ++k) {
-    const int c = min(col + k, a.channels - 1);
-    const float2 r = stats[n * a.groups + c / size];
+    const float2 r = row[g];
     mean[k] = r.x;
     rstd[k] = r.y;
+    if (++in == size && k + 1 < MV) {
+      in = 0;
+      ++g;
+    }
   }
 }
 
 // part[block][channels]: sums of dz and dz xhat over the block's samples.
 template <class K, int R, int JOIN>
-__global__ __launch_bounds__(kMostThreads) void k_group_bwd(GroupKernel s) {
+__global__ __launch_bounds__(kMostThreads)
+    __attribute__((amdgpu_waves_per_eu(R == 1 && kStats<K, JOIN> == 1 ? 4 : 2))) void k_group_bwd(GroupKernel s) {
   using T = typename K::T;
   constexpr int V = K::V;
   extern __shared__ float2 lds[];
@@ -475,6 +481,7 @@ __global__ __launch_bounds__(kMostThreads) void k_group_bwd(GroupKernel s) {
     const auto &mean = now.mean, &rstd = now.rstd;
     const int count = now.count;
     float t1[MV], t2[MV];  // the sample's group sums
+    float xhat[V], dz[V];  // single rows keep them
     {
       float a1[V], a2[V];
 #pragma unroll
@@ -482,7 +489,6 @@ __global__ __launch_bounds__(kMostThreads) void k_group_bwd(GroupKernel s) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         if (r < count) {
-          float xhat[V], dz[V];
           vector_dz<K>(s.a, x[r], dy[r], mean, rstd, w, b, xhat, dz);
 #pragma unroll
           for (int k = 0; k < V; ++k) {
@@ -555,8 +561,7 @@ __global__ __launch_bounds__(kMostThreads) void k_group_bwd(GroupKernel s) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         if (r < count) {
-          float xhat[V], dz[V];
-          vector_dz<K>(s.a, x[r], dy[r], mean, rstd, w, b, xhat, dz);
+          if constexpr (R > 1) vector_dz<K>(s.a, x[r], dy[r], mean, rstd, w, b, xhat, dz);
 #pragma unroll
           for (int k = 0; k < V; ++k)
             dz[k] = rstd[k % MV] *
@@ -592,26 +597,27 @@ __global__ __launch_bounds__(kMostThreads) void k_group_bwd(GroupKernel s) {
 constexpr int kPartThreads = 256;
 
 // A stretch of rows of a sample, in one block of columns.
-template <class K>
+template <class K, bool APPLY>
 struct Piece : Columns<K> {
   int chunk, slots, slot, base, cv;  // rows at a time; base, cv: first channel, vectors of the block
-  int64_t row0, rows;                // first row within the sample
+  int row0, rows;                    // first row within the sample
   bool active;
   static __device__ __forceinline__ int vectors(const GroupKernel& s, int block) {
     return min(s.cv, (s.a.channels + K::V - 1) / K::V - block * s.cv);
   }
   __device__ __forceinline__ Piece(const GroupKernel& s, int block)
       : Columns<K>(s, block * s.cv * K::V, (int)threadIdx.x % vectors(s, block)) {
-    chunk = blockIdx.x / s.blocks;
-    row0 = chunk * s.stretch;
-    rows = min(s.stretch, s.a.positions - row0);
+    chunk = s.blocks == 1 ? (int)blockIdx.x : (int)(blockIdx.x / s.blocks);
+    const int stretch = APPLY ? s.short_stretch : s.stretch;
+    row0 = chunk * stretch;
+    rows = min(stretch, (int)s.a.positions - row0);
     base = block * s.cv * K::V;
     cv = vectors(s, block);
     slots = kPartThreads / cv;
     slot = threadIdx.x / cv;
     active = slot < slots;
   }
-  __device__ __forceinline__ int64_t count_of(int slot_) const {  // its rows
+  __device__ __forceinline__ int count_of(int slot_) const {  // its rows
     return rows > slot_ ? (rows - slot_ + slots - 1) / slots : 0;
   }
 };
@@ -622,9 +628,10 @@ template <class K, int U, bool BACK>
 struct Stream {
   using T = typename K::T;
   const T *px, *pd;
-  int64_t sx, sd, last;
+  int64_t sx, sd;
+  int last;
   Raw<K> x[U], dy[BACK ? U : 1];
-  __device__ __forceinline__ void load(int64_t i) {
+  __device__ __forceinline__ void load(int i) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t r = min(i + u, last);
@@ -633,8 +640,8 @@ struct Stream {
     }
   }
   // of the `count` > 0 rows of sample n
-  __device__ __forceinline__ Stream(const GroupKernel& s, const Piece<K>& at, int64_t n,
-                                    int64_t count)
+  template <class P>
+  __device__ __forceinline__ Stream(const GroupKernel& s, const P& at, int64_t n, int count)
       : sx((int64_t)at.slots * s.a.x_stride), sd((int64_t)at.slots * s.ldy), last(count - 1) {
     const int64_t row = n * s.a.positions + at.row0 + at.slot;
     px = static_cast<const T*>(s.a.x) + row * s.a.x_stride + at.col;
@@ -649,8 +656,8 @@ template <class K, bool BACK, int MV>
 __global__ __launch_bounds__(kPartThreads) void k_group_part(GroupKernel s) {
   constexpr int V = K::V, U = BACK ? 2 : 4;
   __shared__ float2 lds[kPartThreads * V];
-  const Piece<K> at(s, blockIdx.x % s.blocks);
-  const int64_t count = at.active ? at.count_of(at.slot) : 0;
+  const Piece<K, false> at(s, s.blocks == 1 ? 0 : (int)(blockIdx.x % s.blocks));
+  const int count = at.active ? at.count_of(at.slot) : 0;
   float w[V], b[V];
   if constexpr (BACK) {
     load_params<K>(s.a.weight, at.col, s.a.f32_params, 1.0f, w);
@@ -664,7 +671,7 @@ __global__ __launch_bounds__(kPartThreads) void k_group_part(GroupKernel s) {
       Stream<K, U, BACK> rows(s, at, n, count);
       if constexpr (!BACK) {
         const Raw<K> base = rows.x[0];  // means are formed from here
-        int64_t done = 0;
+        int done = 0;
         for (; done + U <= count; done += U) {
           Raw<K> x[U];
 #pragma unroll
@@ -711,7 +718,7 @@ __global__ __launch_bounds__(kPartThreads) void k_group_part(GroupKernel s) {
             q[k] = fmaf(dz[k], xhat[k], q[k]);
           }
         };
-        for (int64_t done = 0; done < count; done += U) {
+        for (int done = 0; done < count; done += U) {
           Raw<K> x[U], dy[U];
 #pragma unroll
           for (int u = 0; u < U; ++u) {
@@ -733,7 +740,7 @@ __global__ __launch_bounds__(kPartThreads) void k_group_part(GroupKernel s) {
     }
     __syncthreads();
     float2* to = s.part + (n * s.stretches + at.chunk) * s.a.channels + at.base;
-    const int used = (int)min((int64_t)at.slots, at.rows);
+    const int used = min(at.slots, at.rows);
     for (int c = threadIdx.x; c < min(width, s.a.channels - at.base); c += kPartThreads) {
       float2 t = lds[c];
       if constexpr (BACK) {
@@ -745,7 +752,7 @@ __global__ __launch_bounds__(kPartThreads) void k_group_part(GroupKernel s) {
       } else {
         // rows of the first `more` slots: one more than of the others
         const float few = (float)(at.rows / at.slots);
-        const int more = (int)(at.rows - at.rows / at.slots * at.slots);
+        const int more = at.rows - at.rows / at.slots * at.slots;
         float sum = 0.0f;
         for (int k = 1; k < used; ++k)
           sum = fmaf(lds[k * width + c].x - t.x, few + (k < more ? 1.0f : 0.0f), sum);
@@ -798,7 +805,7 @@ __global__ __launch_bounds__(256) void k_group_merge(GroupKernel s) {
                  : s.a.f32_params      ? static_cast<const float*>(s.a.weight)[c]
                                        : (float)static_cast<const T*>(s.a.weight)[c];
         else
-          e.by = (float)min(s.stretch, s.a.positions - chunk * s.stretch);
+          e.by = (float)min(s.stretch, (int)s.a.positions - chunk * s.stretch);
       }
       return e;
     };
@@ -833,8 +840,8 @@ template <class K, bool BACK, int MV>
 __global__ __launch_bounds__(kPartThreads) void k_group_apply(GroupKernel s) {
   using T = typename K::T;
   constexpr int V = K::V, U = BACK ? 2 : 4;
-  const Piece<K> at(s, blockIdx.x % s.blocks);
-  const int64_t count = at.active ? at.count_of(at.slot) : 0;
+  const Piece<K, true> at(s, s.blocks == 1 ? 0 : (int)(blockIdx.x % s.blocks));
+  const int count = at.active ? at.count_of(at.slot) : 0;
   if (count == 0) return;
   const int64_t so = (int64_t)at.slots * s.ldo;
   float w[V], b[V];
@@ -846,7 +853,7 @@ __global__ __launch_bounds__(kPartThreads) void k_group_apply(GroupKernel s) {
     float mean[MV], rstd[MV], c1[MV], c2[MV];
     load_stats(s.a, s.stats, n, at.col, mean, rstd);
     if constexpr (BACK) load_stats(s.a, s.coef, n, at.col, c1, c2);
-    for (int64_t i = 0; i < count; i += U) {
+    for (int i = 0; i < count; i += U) {
       Raw<K> x[U], dy[BACK ? U : 1];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -953,8 +960,12 @@ GroupCut cut_of(GroupKernel& s, bool back) {
     const int64_t slots = std::max<int64_t>(1, kPartThreads / s.cv);
     const int64_t want = ceil_div((int64_t)kStretches, a.samples * s.blocks);
     s.stretches = (int)std::max<int64_t>(1, std::min(want, L / (8 * slots)));
-    s.stretch = ceil_div(L, (int64_t)s.stretches);
-    s.stretches = (int)ceil_div(L, s.stretch);
+    s.stretch = (int)ceil_div(L, (int64_t)s.stretches);
+    s.stretches = (int)ceil_div(L, (int64_t)s.stretch);
+    // the results', which leave no partial ones behind: more of them, of two rows a thread
+    const int64_t more = std::max<int64_t>(1, std::min(2 * want, L / (4 * slots)));
+    s.short_stretch = (int)ceil_div(L, more);
+    s.shorts = (int)ceil_div(L, (int64_t)s.short_stretch);
     return c;
   }
   s.cv = (int)cv;
@@ -1021,14 +1032,16 @@ void dispatch_kind(const GroupArgs& a, F&& f) {
 
 template <class K, bool BACK>
 void launch_stretches(GroupKernel& s, hipStream_t st) {
-  const unsigned gx = (unsigned)(s.stretches * s.blocks);
-  const dim3 grid(gx, (unsigned)std::min<int64_t>(s.a.samples, std::max(1, (1 << 15) / (int)gx)));
+  auto grid = [&](int stretches) {
+    const int x = stretches * s.blocks;
+    return dim3((unsigned)x, (unsigned)std::min<int64_t>(s.a.samples, std::max(1, (1 << 15) / x)));
+  };
   const unsigned pairs = (unsigned)std::min<int64_t>(s.a.samples * s.a.groups, 1 << 16);
   auto go = [&](auto mv) {
-    k_group_part<K, BACK, mv.value><<<grid, kPartThreads, 0, st>>>(s);
+    k_group_part<K, BACK, mv.value><<<grid(s.stretches), kPartThreads, 0, st>>>(s);
     if (BACK && s.out == nullptr) return;
     k_group_merge<typename K::T, BACK><<<pairs, 256, 0, st>>>(s);
-    k_group_apply<K, BACK, mv.value><<<grid, kPartThreads, 0, st>>>(s);
+    k_group_apply<K, BACK, mv.value><<<grid(s.shorts), kPartThreads, 0, st>>>(s);
   };
   if (s.a.channels / s.a.groups % K::V == 0)  // a vector's channels are of one group
     go(std::integral_constant<int, 1>{});
