@@ -156,6 +156,7 @@ template <class K>
 struct Place : Columns<K> {
   int slot, sample, row;  // sample: among those at a time; row: its first
   int slots;              // rows at a time that are taken, of one sample
+  int rows;               // its rows of a sample
   bool active;
   __device__ __forceinline__ explicit Place(const GroupKernel& s)
       : Columns<K>(s, 0, (int)threadIdx.x - (int)threadIdx.x / s.cv * s.cv) {
@@ -164,8 +165,23 @@ struct Place : Columns<K> {
     sample = slot / slots;
     row = slot - sample * slots;
     active = sample < s.at_a_time;
+    rows = ((int)min(s.a.positions, (int64_t)1 << 30) - row + slots - 1) / slots;
+  }
+  // Elements from the batch's first row to the thread's; how many rows it has in one.
+  __device__ __forceinline__ int64_t offset(const GroupKernel& s, int64_t stride) const {
+    return (sample * s.a.positions + row) * stride + this->col;
+  }
+  __device__ __forceinline__ int count(const GroupKernel& s, int64_t batch) const {
+    const int live = (int)min((int64_t)s.at_a_time, s.a.samples - batch * s.at_a_time);
+    return active && sample < live ? rows : 0;
   }
 };
+
+// Elements from the first row to a batch's.
+__device__ __forceinline__ int64_t batch_offset(const GroupKernel& s, int64_t batch,
+                                                int64_t stride) {
+  return batch * s.at_a_time * s.a.positions * stride;
+}
 
 // Sums of a thread's values over blocks of `size` (a power of two up to V).
 template <int V>
@@ -211,33 +227,18 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
   float w[V], b[V];
   load_params<K>(s.a.weight, at.col, s.a.f32_params, 1.0f, w);
   load_params<K>(s.a.bias, at.col, s.a.f32_params, 0.0f, b);
-  auto load = [&](int64_t n, Raw<K> (&x)[R]) __attribute__((always_inline)) {
-    const T* px = static_cast<const T*>(s.a.x) + (n * L + at.row) * s.a.x_stride + at.col;
-    int count = 0;
+  const int64_t off = at.offset(s, s.a.x_stride), off_y = at.offset(s, s.ldo);
+  auto load = [&](int64_t batch, Raw<K> (&x)[R]) __attribute__((always_inline)) {
+    const T* px = static_cast<const T*>(s.a.x) + batch_offset(s, batch, s.a.x_stride) + off;
+    const int count = at.count(s, batch);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const bool has = at.active && n < s.a.samples && at.row + r * at.slots < L;
-      if (has) x[r] = load_raw<K>(px + (int64_t)r * at.slots * s.a.x_stride);
-      count += has;
-    }
+    for (int r = 0; r < R; ++r)
+      if (r < count) x[r] = load_raw<K>(px + (int64_t)r * at.slots * s.a.x_stride);
     return count;
   };
-  // single rows: the next ones are loaded ahead
-  Raw<K> ahead[R];
-  int count_ahead = 0;
-  if constexpr (R == 1) count_ahead = load((int64_t)blockIdx.x * s.at_a_time + at.sample, ahead);
-  for (int64_t batch = blockIdx.x; batch < s.batches; batch += gridDim.x) {
+  auto one = [&](int64_t batch, Raw<K> (&x)[R], int count) __attribute__((always_inline)) {
     const int64_t n = batch * s.at_a_time + at.sample;
-    const bool in = at.active && n < s.a.samples;
-    Raw<K> x[R];
-    int count;
-    if constexpr (R == 1) {
-      x[0] = ahead[0];
-      count = count_ahead;
-      count_ahead = load(n + (int64_t)gridDim.x * s.at_a_time, ahead);
-    } else {
-      count = load(n, x);
-    }
+    const bool in = count > 0;
     constexpr int MV = kStats<K, JOIN>;
     float mean[MV], rstd[MV];
     if constexpr (JOIN == THREAD || JOIN == LANES) {
@@ -261,7 +262,8 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
         for (int k = 0; k < V; ++k)
           base[k] = (float)(size == 1 ? x[0].v[k] : size == 2 ? x[0].v[k & ~1] : x[0].v[k & ~3]);
       } else {
-        base[0] = __shfl((float)x[0].v[0], (threadIdx.x & 63) & ~(s.lanes - 1));
+        base[0] = (float)x[0].v[0];
+        if (s.lanes > 1) base[0] = __shfl(base[0], (threadIdx.x & 63) & ~(s.lanes - 1));
       }
 #pragma unroll
       for (int k = 0; k < V; ++k) v[k] = (float)x[0].v[k] - base[k % MV];
@@ -362,15 +364,14 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
       if (at.active) {
 #pragma unroll
         for (int k = 0; k < MV; ++k) {
-          const int c = min(at.col + k, s.a.channels - 1);
-          const float2 r = group[at.sample * s.a.groups + c / size];
+          const float2 r = group[at.sample * s.a.groups + (at.col + k) / size];
           mean[k] = r.x;
           rstd[k] = r.y;
         }
       }
     }
     if (in) {
-      T* py = static_cast<T*>(s.out) + (n * L + at.row) * s.ldo + at.col;
+      T* py = static_cast<T*>(s.out) + batch_offset(s, batch, s.ldo) + off_y;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         if (r < count) {
@@ -382,6 +383,32 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
           store_raw<K>(py + (int64_t)r * at.slots * s.ldo, at.from, z);
         }
       }
+    }
+  };
+  if constexpr (R == 1) {  // single rows: U batches at a time, the next ones loaded ahead
+    constexpr int U = JOIN == LANES ? 2 : 1;
+    const int64_t step = gridDim.x;
+    Raw<K> ahead[U][R];
+    int counts[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) counts[u] = load(blockIdx.x + u * step, ahead[u]);
+    for (int64_t batch = blockIdx.x; batch < s.batches; batch += U * step) {
+      Raw<K> x[U][R];
+      int count[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        x[u][0] = ahead[u][0];
+        count[u] = counts[u];
+        counts[u] = load(batch + (U + u) * step, ahead[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) one(batch + u * step, x[u], count[u]);
+    }
+  } else {
+    for (int64_t batch = blockIdx.x; batch < s.batches; batch += gridDim.x) {
+      Raw<K> x[R];
+      const int count = load(batch, x);
+      one(batch, x, count);
     }
   }
 }
@@ -403,13 +430,11 @@ __device__ __forceinline__ void vector_dz(const GroupArgs& a, const Raw<K>& x, c
   for (int k = 0; k < V; ++k) dz[k] *= (float)dy.v[k];
 }
 
-// mean and rstd of a vector's channels
+// mean and rstd of a vector's channels, the first of which is the `in`th of group g;
+// row: those of the sample
 template <int MV>
-__device__ __forceinline__ void load_stats(const GroupArgs& a, const float2* stats, int64_t n,
-                                           int col, float (&mean)[MV], float (&rstd)[MV]) {
-  const int size = a.channels / a.groups;
-  int g = col / size, in = col - g * size;
-  const float2* row = stats + n * a.groups;
+__device__ __forceinline__ void load_stats(int size, const float2* row, int g, int in,
+                                           float (&mean)[MV], float (&rstd)[MV]) {
 #pragma unroll
   for (int k = 0; k < MV; ++k) {
     const float2 r = row[g];
@@ -443,46 +468,55 @@ __global__ __launch_bounds__(kMostThreads)
     float mean[MV], rstd[MV];
     int count;
   };
-  auto load = [&](int64_t n, Rows& v) __attribute__((always_inline)) {
-    const int64_t row0 = n * L + at.row;
-    const T* px = static_cast<const T*>(s.a.x) + row0 * s.a.x_stride + at.col;
-    const T* pd = static_cast<const T*>(s.dy) + row0 * s.ldy + at.col;
-    const bool in = at.active && n < s.a.samples;
-    v.count = 0;
+  const int64_t off_x = at.offset(s, s.a.x_stride), off_d = at.offset(s, s.ldy),
+                off_o = at.offset(s, s.ldo);
+  const int group = at.col / size, within = at.col - group * size;
+  auto load = [&](int64_t batch, Rows& v) __attribute__((always_inline)) {
+    const T* px = static_cast<const T*>(s.a.x) + batch_offset(s, batch, s.a.x_stride) + off_x;
+    const T* pd = static_cast<const T*>(s.dy) + batch_offset(s, batch, s.ldy) + off_d;
+    v.count = at.count(s, batch);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const bool has = in && at.row + r * at.slots < L;
-      if (has) {
+      if (r < v.count) {
         v.x[r] = load_raw<K>(px + (int64_t)r * at.slots * s.a.x_stride);
         v.dy[r] = load_raw<K>(pd + (int64_t)r * at.slots * s.ldy);
       }
-      v.count += has;
     }
-    if (in) {
-      load_stats(s.a, s.stats, n, at.col, v.mean, v.rstd);
-    } else {
-#pragma unroll
-      for (int k = 0; k < MV; ++k) v.mean[k] = v.rstd[k] = 0.0f;
-    }
+    if (v.count > 0)
+      load_stats(size, s.stats + (batch * s.at_a_time + at.sample) * s.a.groups, group, within,
+                 v.mean, v.rstd);
   };
   Rows ahead;  // single rows: the next ones are loaded ahead
-  if constexpr (R == 1) load((int64_t)blockIdx.x * s.at_a_time + at.sample, ahead);
+  if constexpr (R == 1) load(blockIdx.x, ahead);
   for (int64_t batch = blockIdx.x; batch < s.batches; batch += gridDim.x) {
-    const int64_t n = batch * s.at_a_time + at.sample;
-    const bool in = at.active && n < s.a.samples;
     Rows now;
     if constexpr (R == 1) {
       now = ahead;
-      load(n + (int64_t)gridDim.x * s.at_a_time, ahead);
+      load(batch + gridDim.x, ahead);
     } else {
-      load(n, now);
+      load(batch, now);
     }
     const auto &x = now.x, &dy = now.dy;
     const auto &mean = now.mean, &rstd = now.rstd;
     const int count = now.count;
-    float t1[MV], t2[MV];  // the sample's group sums
-    float xhat[V], dz[V];  // single rows keep them
-    {
+    const bool in = count > 0;
+    float t1[MV], t2[MV];   // the sample's group sums
+    float xhat[V], dz[V];   // single rows keep them, dz times the weight
+#pragma unroll
+    for (int k = 0; k < MV; ++k) t1[k] = t2[k] = 0.0f;
+    if constexpr (R == 1) {
+      if (in) {
+        vector_dz<K>(s.a, x[0], dy[0], mean, rstd, w, b, xhat, dz);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          sum_a[k] += dz[k];
+          sum_b[k] = fmaf(dz[k], xhat[k], sum_b[k]);
+          dz[k] *= w[k];
+          t1[k % MV] += dz[k];
+          t2[k % MV] = fmaf(dz[k], xhat[k], t2[k % MV]);
+        }
+      }
+    } else {
       float a1[V], a2[V];
 #pragma unroll
       for (int k = 0; k < V; ++k) a1[k] = a2[k] = 0.0f;
@@ -497,8 +531,6 @@ __global__ __launch_bounds__(kMostThreads)
           }
         }
       }
-#pragma unroll
-      for (int k = 0; k < MV; ++k) t1[k] = t2[k] = 0.0f;
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         sum_a[k] += a1[k];
@@ -516,7 +548,7 @@ __global__ __launch_bounds__(kMostThreads)
       t2[0] = lane_sum(t2[0], s.lanes);
     } else {
       const Entries<K, JOIN> e(s);
-      float2* group = lds + (blockDim.x / s.cv) * e.width;
+      float2* sums = lds + (blockDim.x / s.cv) * e.width;
       if (at.active) {
 #pragma unroll
         for (int k = 0; k < MV; ++k)
@@ -543,29 +575,34 @@ __global__ __launch_bounds__(kMostThreads)
         }
         t.x = lane_sum(t.x, s.lanes);
         t.y = lane_sum(t.y, s.lanes);
-        if (p < pairs && lane == 0) group[p] = t;
+        if (p < pairs && lane == 0) sums[p] = t;
       }
       __syncthreads();
       if (at.active) {
 #pragma unroll
         for (int k = 0; k < MV; ++k) {
-          const int c = min(at.col + k, s.a.channels - 1);
-          const float2 r = group[at.sample * s.a.groups + c / size];
+          const float2 r = sums[at.sample * s.a.groups + (at.col + k) / size];
           t1[k] = r.x;
           t2[k] = r.y;
         }
       }
     }
     if (in) {
-      T* po = static_cast<T*>(s.out) + (n * L + at.row) * s.ldo + at.col;
+      T* po = static_cast<T*>(s.out) + batch_offset(s, batch, s.ldo) + off_o;
+#pragma unroll
+      for (int k = 0; k < MV; ++k) {
+        t1[k] *= s.inv_m * rstd[k];
+        t2[k] *= s.inv_m * rstd[k];
+      }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         if (r < count) {
           if constexpr (R > 1) vector_dz<K>(s.a, x[r], dy[r], mean, rstd, w, b, xhat, dz);
 #pragma unroll
-          for (int k = 0; k < V; ++k)
-            dz[k] = rstd[k % MV] *
-                    fmaf(w[k], dz[k], -s.inv_m * fmaf(xhat[k], t2[k % MV], t1[k % MV]));
+          for (int k = 0; k < V; ++k) {
+            const float g = R > 1 ? dz[k] * w[k] : dz[k];
+            dz[k] = fmaf(g, rstd[k % MV], -fmaf(xhat[k], t2[k % MV], t1[k % MV]));
+          }
           store_raw<K>(po + (int64_t)r * at.slots * s.ldo, at.from, dz);
         }
       }
@@ -708,7 +745,8 @@ __global__ __launch_bounds__(kPartThreads) void k_group_part(GroupKernel s) {
         for (int k = 0; k < V; ++k) m[k] += (float)base.v[k];
       } else {
         float mean[MV], rstd[MV];
-        load_stats(s.a, s.stats, n, at.col, mean, rstd);
+        const int size = s.a.channels / s.a.groups, g = at.col / size;
+        load_stats(size, s.stats + n * s.a.groups, g, at.col - g * size, mean, rstd);
         auto add = [&](const Raw<K>& x, const Raw<K>& dy) __attribute__((always_inline)) {
           float xhat[V], dz[V];
           vector_dz<K>(s.a, x, dy, mean, rstd, w, b, xhat, dz);
@@ -844,6 +882,7 @@ __global__ __launch_bounds__(kPartThreads) void k_group_apply(GroupKernel s) {
   const int count = at.active ? at.count_of(at.slot) : 0;
   if (count == 0) return;
   const int64_t so = (int64_t)at.slots * s.ldo;
+  const int size = s.a.channels / s.a.groups, g = at.col / size;
   float w[V], b[V];
   load_params<K>(s.a.weight, at.col, s.a.f32_params, 1.0f, w);
   load_params<K>(s.a.bias, at.col, s.a.f32_params, 0.0f, b);
@@ -851,8 +890,18 @@ __global__ __launch_bounds__(kPartThreads) void k_group_apply(GroupKernel s) {
     Stream<K, U, BACK> rows(s, at, n, count);
     T* po = static_cast<T*>(s.out) + (n * s.a.positions + at.row0 + at.slot) * s.ldo + at.col;
     float mean[MV], rstd[MV], c1[MV], c2[MV];
-    load_stats(s.a, s.stats, n, at.col, mean, rstd);
-    if constexpr (BACK) load_stats(s.a, s.coef, n, at.col, c1, c2);
+    load_stats(size, s.stats + n * s.a.groups, g, at.col - g * size, mean, rstd);
+    float wr[V];
+    if constexpr (BACK) {
+      load_stats(size, s.coef + n * s.a.groups, g, at.col - g * size, c1, c2);
+#pragma unroll
+      for (int k = 0; k < MV; ++k) {
+        c1[k] *= rstd[k];
+        c2[k] *= rstd[k];
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) wr[k] = w[k] * rstd[k % MV];
+    }
     for (int i = 0; i < count; i += U) {
       Raw<K> x[U], dy[BACK ? U : 1];
 #pragma unroll
@@ -870,7 +919,7 @@ __global__ __launch_bounds__(kPartThreads) void k_group_apply(GroupKernel s) {
           vector_dz<K>(s.a, x[u], dy[u], mean, rstd, w, b, xhat, z);
 #pragma unroll
           for (int k = 0; k < V; ++k)
-            z[k] = rstd[k % MV] * fmaf(w[k], z[k], -fmaf(xhat[k], c2[k % MV], c1[k % MV]));
+            z[k] = fmaf(wr[k], z[k], -fmaf(xhat[k], c2[k % MV], c1[k % MV]));
         } else {
 #pragma unroll
           for (int k = 0; k < V; ++k)
