@@ -9,8 +9,8 @@
 // 2^23, the product x by is rounded once to a whole number, ties to even, which the
 // low byte then holds.
 //
-// Matrix-core bound at twice the 16-bit rate: the tiled product of product.h with
-// 128 columns a stage; rows are quantised by one pass of their own before it.  Few
+// Matrix-core bound, at up to twice the 16-bit rate; rows are quantised by one pass
+// of their own before the product.  Few
 // rows (k_int8_few) are bound by reading the weights once, at half the bytes of
 // 16-bit ones, and by latency: up to 16 rows each workgroup quantises what it needs
 // itself, in the one launch.
@@ -19,10 +19,14 @@
 
 #include "activation.h"
 #include "product.h"
+#include "sym_common.h"
 
 namespace mgp {
 
 namespace {
+
+typedef int i4 __attribute__((ext_vector_type(4)));
+typedef int i16 __attribute__((ext_vector_type(16)));
 
 constexpr float kCodeMost = 127.0f;
 
@@ -184,42 +188,309 @@ __device__ __forceinline__ void zeros(float* v) {
   for (int k = 0; k < N; ++k) v[k] = 0.0f;
 }
 
-template <class T, bool GATED>
-struct EndEpi {
-  static constexpr bool FORWARD = true;
-  EndArgs a;
-  template <class TL>
-  __device__ __forceinline__ void run(i4 (&acc)[TL::TM][TL::TN], int64_t m0, int64_t n0,
-                                      int64_t) const {
-    constexpr int N = TL::RUN;
-    const int lane = threadIdx.x & 63;
-    const int64_t f = n0 + N * (lane >> 4), left = a.hidden - f;
-    if (left <= 0) return;
-    float sg[N], bg[N], su[GATED ? N : 1], bu[GATED ? N : 1];
-    load_run<N>(a.sg + f, left, sg);
-    zeros<N>(bg);
-    if (a.bg) load_run<N>(static_cast<const T*>(a.bg) + f, left, bg);
-    if constexpr (GATED) {
-      load_run<N>(a.su + f, left, su);
-      zeros<N>(bu);
-      if (a.bu) load_run<N>(static_cast<const T*>(a.bu) + f, left, bu);
-    }
-#pragma unroll
-    for (int m = 0; m < TL::TM; ++m) {
-      const int64_t r = m0 + m * 16 + (lane & 15);
-      if (r >= a.rows) continue;
-      int g[N], u[N];
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        g[k] = acc[m][k / 4][k % 4];
-        u[k] = GATED ? acc[m][TL::T1 % TL::TN + k / 4][k % 4] : 0;
-      }
-      float o[N];
-      finish<T, N, GATED>(g, u, a.sx[r], sg, su, bg, bu, a.act, o);
-      store_run<N>(static_cast<T*>(a.y) + r * a.ldy + f, left, o);
-    }
+// ---------------------------------------------------------------- tiles
+
+// Tile of 32 TN WN columns (weight rows) by 32 TM WM rows, one wave 32 TN by 32 TM of it
+// in 32 x 32 x 32 matrix instructions.  Both operands go through LDS by direct loads, SB
+// columns a stage, two buffers; 16-byte chunk c of row r at c ^ (r / (256 / SB) %
+// CHUNKS).  The weight rows are dealt to LDS so that a lane's results are 16 consecutive
+// columns of 32 (of each projection: gated, half of a wave's rows are up's).
+template <int TM_, int TN_, int WM_, int WN_, int SB_, bool GATED_>
+struct ByteTile {
+  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, SB = SB_;
+  static constexpr bool GATED = GATED_;
+  static constexpr int W = WM * WN, THREADS = 64 * W;
+  static constexpr int BQ = 32 * TM * WM, BP = 32 * TN * WN;
+  static constexpr int T1 = GATED ? TN / 2 : TN;
+  static constexpr int CP = GATED ? BP / 2 : BP;  // output columns of a tile
+  static constexpr int LDS = (BP + BQ) * SB, CHUNKS = SB / 16;
+  static constexpr int ROWS = 1024 / SB;                        // of LDS, a load
+  static constexpr int IP = BP / ROWS / W, IQ = BQ / ROWS / W;  // loads a stage
+  static constexpr int FRAGS = TM + TN, STEPS = SB / 32;
+  // the loads' rows of one projection: a wave's own, or every second load's
+  static constexpr bool BY_WAVE = W * ROWS == 64;
+  static_assert(TN == 2 && (BY_WAVE || W * ROWS == 32) && (STEPS == 2 || STEPS == 4), "");
+  static __device__ __forceinline__ int chunk(int r, int c) {
+    return (c ^ (r / (256 / SB))) & (CHUNKS - 1);
   }
 };
+
+struct ByteShape {
+  const int8_t *wg, *wu, *x;
+  int ldw, ldx;
+  int64_t hidden, rows;
+  int K;
+  uint32_t tiles_p, tiles_q;
+};
+
+// What a wave loads of a stage: 64 lanes x 16 bytes an instruction.
+template <class TL>
+struct ByteLoader {
+  int vp, vq;         // byte offset of a lane from an instruction's first row
+  int kpos;           // its column within the stage
+  int soff[TL::IP + TL::IQ];
+  bool exists[TL::IP + TL::IQ];
+  const char *bp[2], *bq;
+  int left;           // columns still to load
+
+  __device__ __forceinline__ void init(const ByteShape& s, uint32_t tp, uint32_t tq) {
+    const int lane = threadIdx.x & 63, lr = lane / TL::CHUNKS;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = TL::chunk(wave * TL::ROWS + lr, lane & (TL::CHUNKS - 1));
+    const int64_t n0 = (int64_t)tp * TL::CP, m0 = (int64_t)tq * TL::BQ;
+    kpos = c * 16;
+    const int prow = lr / 4 % 2 * 16 + lr / 8 * 4 + lr % 4;
+    vp = prow * s.ldw + kpos;
+    vq = lr * s.ldx + kpos;
+    bp[0] = reinterpret_cast<const char*>(s.wg) + n0 * s.ldw;
+    bp[1] = TL::GATED ? reinterpret_cast<const char*>(s.wu) + n0 * s.ldw : bp[0];
+    if (TL::GATED && TL::BY_WAVE && wave >= TL::W / 2) bp[0] = bp[1];
+    bq = reinterpret_cast<const char*>(s.x) + m0 * s.ldx;
+#pragma unroll
+    for (int i = 0; i < TL::IP; ++i) {
+      const int first = (i * TL::W + wave) * TL::ROWS, in = first % (32 * TL::TN);
+      const int r = first / (32 * TL::TN) * 32 * TL::T1 + in / 32 % TL::T1 * 32 + in % 32 / 8 * 4;
+      soff[i] = r * s.ldw;
+      exists[i] = n0 + r + prow < s.hidden;
+    }
+#pragma unroll
+    for (int i = 0; i < TL::IQ; ++i) {
+      const int r = (i * TL::W + wave) * TL::ROWS;
+      soff[TL::IP + i] = r * s.ldx;
+      exists[TL::IP + i] = m0 + r + lr < s.rows;
+    }
+    left = s.K;
+  }
+
+  // Loads the next stage into buf.
+  __device__ __forceinline__ void load(char* __restrict__ buf) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool in = kpos < left;
+#pragma unroll
+    for (int i = 0; i < TL::IP; ++i)
+      load_lds(bp[TL::GATED && !TL::BY_WAVE ? i % 2 : 0], in && exists[i] ? vp : kOutOfRange, soff[i],
+               buf + (i * TL::W + wave) * 1024);
+#pragma unroll
+    for (int i = 0; i < TL::IQ; ++i)
+      load_lds(bq, in && exists[TL::IP + i] ? vq : kOutOfRange, soff[TL::IP + i],
+               buf + TL::BP * TL::SB + (i * TL::W + wave) * 1024);
+    left -= TL::SB;
+    bp[0] += TL::SB;
+    bp[1] += TL::SB;
+    bq += TL::SB;
+  }
+};
+
+// The fragments of 32 columns: those of the wave's weight rows, then of its rows of x.
+template <class TL>
+struct ByteFrags {
+  Frag f[TL::FRAGS];
+  __device__ __forceinline__ void read(const char* __restrict__ buf, int step, int wm, int wn) {
+    const int lane = threadIdx.x & 63, i = lane & 31;
+    const int at = i * TL::SB + TL::chunk(i, step * 2 + (lane >> 5)) * 16;
+#pragma unroll
+    for (int t = 0; t < TL::TN; ++t)
+      f[t].v = *reinterpret_cast<const f4*>(buf + (wn * TL::TN + t) * 32 * TL::SB + at);
+#pragma unroll
+    for (int t = 0; t < TL::TM; ++t)
+      f[TL::TN + t].v = *reinterpret_cast<const f4*>(buf + (TL::BP + (wm * TL::TM + t) * 32) * TL::SB + at);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  __device__ __forceinline__ void multiply(i16 (&acc)[TL::TM][TL::TN]) const {
+#pragma unroll
+    for (int m = 0; m < TL::TM; ++m)
+#pragma unroll
+      for (int n = 0; n < TL::TN; ++n)
+        acc[m][n] = __builtin_amdgcn_mfma_i32_32x32x32_i8(
+            __builtin_bit_cast(i4, f[n].v), __builtin_bit_cast(i4, f[TL::TN + m].v), acc[m][n], 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+};
+
+// The barrier of a stage: a wave's own loads into LDS and its reads from it have
+// ended, then every wave's.  The waits stand here as the compiler's are not to be
+// relied on (it adds one for such loads where it takes buffers to alias).  A counter
+// of loads counts stores too: behind a tile's end, whose stores were issued after
+// these loads had ended, only the reads are waited for (drained), and the stores have
+// until the next barrier.
+__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void arrive(bool drained) {
+  if (!drained) loads_done();
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// One stage of the running sum.  even holds the fragments of its first 32 columns.  The
+// barrier stands before the last products: behind it, under them, go the loads of
+// the stage after the next, into the buffer that every wave has read by then, and
+// the reads of the next stage's first fragments.
+template <class TL, class Load>
+__device__ __forceinline__ void byte_stage(const char* __restrict__ cur,
+                                           const char* __restrict__ nxt, bool real, bool more,
+                                           bool next_real, bool drained, int wm, int wn, ByteFrags<TL>& even,
+                                           i16 (&acc)[TL::TM][TL::TN], Load&& load) {
+  ByteFrags<TL> odd;
+  if (real) {
+    odd.read(cur, 1, wm, wn);
+    even.multiply(acc);
+    if constexpr (TL::STEPS == 4) {
+      even.read(cur, 2, wm, wn);
+      odd.multiply(acc);
+      odd.read(cur, 3, wm, wn);
+      even.multiply(acc);
+    }
+  }
+  if (more) {
+    arrive(drained);
+    if (next_real) even.read(nxt, 0, wm, wn);
+    load();
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  if (real) odd.multiply(acc);
+}
+
+// The results of a wave: acc[m][n][e] of lane l is row 32 m + l % 32 and, of matrix
+// n / T1, column 32 (n % T1) + 16 (l / 32) + e.  A row's 32 columns meet in LDS (out,
+// the wave's own), so that they are written together: stored from where they are,
+// in halves of 16 bytes a row, they took longer than the products.
+template <class T, class TL>
+__device__ __forceinline__ void byte_end(const EndArgs& a, const i16 (&acc)[TL::TM][TL::TN],
+                                         int64_t m0, int64_t n0, char* out) {
+  constexpr int N = 8, ROW = 32 * sizeof(T), CHUNKS = ROW / 16, V = 16 / sizeof(T);
+  const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
+  float sx[TL::TM];
+#pragma unroll
+  for (int m = 0; m < TL::TM; ++m) sx[m] = a.sx[min(m0 + i + 32 * m, a.rows - 1)];
+#pragma unroll
+  for (int t = 0; t < TL::T1; ++t) {
+    const int64_t f = n0 + 32 * t;
+    if (f >= a.hidden) {
+      if (t == 0) loads_done();
+      break;
+    }
+    T o[TL::TM][16];
+#pragma unroll
+    for (int q = 0; q < 16; q += N) {
+      const int64_t c = f + 16 * h + q, left = a.hidden - c;
+      float sg[N], bg[N], su[N], bu[N];
+      zeros<N>(sg);
+      zeros<N>(bg);
+      zeros<N>(su);
+      zeros<N>(bu);
+      if (left > 0) {
+        load_run<N>(a.sg + c, left, sg);
+        if (a.bg) load_run<N>(static_cast<const T*>(a.bg) + c, left, bg);
+        if constexpr (TL::GATED) {
+          load_run<N>(a.su + c, left, su);
+          if (a.bu) load_run<N>(static_cast<const T*>(a.bu) + c, left, bu);
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < TL::TM; ++m) {
+        int g[N], u[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          g[k] = acc[m][t][q + k];
+          u[k] = acc[m][TL::TN - 1][q + k];
+        }
+        float v[N];
+        finish<T, N, TL::GATED>(g, u, sx[m], sg, su, bg, bu, a.act, v);
+#pragma unroll
+        for (int k = 0; k < N; ++k) o[m][q + k] = (T)v[k];
+      }
+    }
+    if (t == 0) loads_done();  // before the first store
+#pragma unroll
+    for (int m = 0; m < TL::TM; ++m) {
+      // 16-byte chunk c of row r at c ^ (r / (256 / ROW) % CHUNKS): off each other's banks
+      auto at = [&](int r, int c) __attribute__((always_inline)) {
+        return reinterpret_cast<f4*>(out + r * ROW + ((c ^ (r / (256 / ROW))) % CHUNKS) * 16);
+      };
+#pragma unroll
+      for (int c = 0; c < CHUNKS / 2; ++c) {
+        f4 x;
+        __builtin_memcpy(&x, &o[m][c * V], 16);
+        *at(i, h * (CHUNKS / 2) + c) = x;
+      }
+      wave_lds_sync();
+      const int64_t c0 = f + lane % CHUNKS * V, left = a.hidden - c0;
+#pragma unroll
+      for (int r = lane / CHUNKS; r < 32; r += 64 / CHUNKS) {
+        const f4 x = *at(r, lane % CHUNKS);
+        const int64_t row = m0 + 32 * m + r;
+        T* to = static_cast<T*>(a.y) + row * a.ldy + c0;
+        if (row < a.rows && left > 0) {
+          if (left >= V) {
+            __builtin_memcpy(to, &x, 16);
+          } else {
+            T e[V];
+            __builtin_memcpy(e, &x, 16);
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+              if (k < left) to[k] = e[k];
+          }
+        }
+      }
+      wave_lds_sync();
+    }
+  }
+}
+
+// Workgroups go on to further tiles of their XCD; the loads of the next tile's first
+// stages are out before the end of the one before.  An odd number of stages is
+// made even by an empty one, so that each has its buffer at compile time.
+template <class T, class TL>
+__global__ __launch_bounds__(TL::THREADS)
+    __attribute__((amdgpu_waves_per_eu(2, 2))) void k_int8_tiles(ByteShape s, EndArgs a) {
+  __shared__ __align__(1024) char b0[TL::LDS];
+  __shared__ __align__(1024) char b1[TL::LDS];
+  __shared__ __align__(1024) char out[TL::W][32 * 32 * sizeof(T)];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave % TL::WM, wn = wave / TL::WM;
+  const uint32_t tiles = s.tiles_p * s.tiles_q;
+  const int stages = (s.K + TL::SB - 1) / TL::SB, pairs = (stages + 1) / 2;
+
+  uint32_t tp, tq;
+  tile_of(blockIdx.x, s.tiles_p, s.tiles_q, tp, tq);
+  ByteLoader<TL> ld;
+  ld.init(s, tp, tq);
+  ld.load(b0);
+  if (stages > 1) ld.load(b1);
+  arrive(false);
+  ByteFrags<TL> even;
+  even.read(b0, 0, wm, wn);
+  for (uint32_t id = blockIdx.x;;) {
+    const bool drained = id != blockIdx.x;  // the end of a tile has waited for the loads
+    const int64_t n0 = (int64_t)tp * TL::CP + wn * 32 * TL::T1;
+    const int64_t m0 = (int64_t)tq * TL::BQ + wm * 32 * TL::TM;
+    id += gridDim.x;
+    const bool next = id < tiles;
+    i16 acc[TL::TM][TL::TN];
+#pragma unroll
+    for (int m = 0; m < TL::TM; ++m)
+#pragma unroll
+      for (int n = 0; n < TL::TN; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[m][n][e] = 0;
+    for (int p = 0; p < pairs; ++p) {
+      const bool last = p + 1 == pairs, both = 2 * p + 1 < stages;
+      byte_stage<TL>(b0, b1, true, both || next, both, drained && p == 0, wm, wn, even, acc, [&] {
+        if (!last) {
+          ld.load(b0);
+        } else if (next) {
+          tile_of(id, s.tiles_p, s.tiles_q, tp, tq);
+          ld.init(s, tp, tq);
+          ld.load(b0);
+        }
+      });
+      byte_stage<TL>(b1, b0, both, !last || next, !last, false, wm, wn, even, acc, [&] {
+        if (2 * p + 3 < stages || (last && next && stages > 1)) ld.load(b1);
+      });
+    }
+    byte_end<T, TL>(a, acc, m0, n0, out[wave]);
+    if (!next) return;
+    even.read(b0, 0, wm, wn);
+  }
+}
 
 // ---------------------------------------------------------------- few rows
 
@@ -230,6 +501,11 @@ struct FewArgs {
   const int8_t *wg, *wu;
   int64_t ldw, width;
 };
+
+__device__ __forceinline__ i4 mma_i8(const Frag& a, const Frag& b, i4 c) {
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i4, a.v),
+                                               __builtin_bit_cast(i4, b.v), c, 0, 0, 0);
+}
 
 // A workgroup takes 16 columns (of both projections) for 16 MT rows; its 8 waves share
 // the reduction and read their fragments from memory.  FUSED: the rows are elements; the
@@ -367,19 +643,33 @@ void launch_layer(const Int8Args& a, const EndArgs& end, const int8_t* codes, hi
     if (a.rows <= 32) return go(std::integral_constant<int, 2>{}, std::false_type{});
     return go(std::integral_constant<int, 4>{}, std::false_type{});
   }
-  GemmShape s{};
-  s.p = {reinterpret_cast<const char*>(a.w_gate), reinterpret_cast<const char*>(a.w_up), a.w_stride,
-         a.hidden};
-  s.q = {reinterpret_cast<const char*>(codes), nullptr, ldx, a.rows};
-  s.K = s.k_split = ldx;
-  const EndEpi<T, GATED> epi{end};
-  const bool big = cut_product((GATED ? 2 : 1) * a.hidden, a.rows, ceil_div(ldx, (int64_t)128), 1,
-                               true, 1, 0.0)
-                       .big;
-  if (big)
-    launch_tiles<BigTile<int8_t, false, GATED, 1>>(s, 1, epi, st);
+  auto tiles = [&](auto tile, int64_t at_once) {
+    using TL = decltype(tile);
+    const ByteShape s{a.w_gate,
+                      a.w_up,
+                      codes,
+                      (int)a.w_stride,
+                      (int)ldx,
+                      a.hidden,
+                      a.rows,
+                      (int)ldx,
+                      (uint32_t)ceil_div(a.hidden, (int64_t)TL::CP),
+                      (uint32_t)ceil_div(a.rows, (int64_t)TL::BQ)};
+    const int64_t all = (int64_t)s.tiles_p * s.tiles_q;
+    k_int8_tiles<T, TL><<<(unsigned)std::min(all, at_once), TL::THREADS, 0, st>>>(s, end);
+  };
+  // 256 x 256 by 8 waves where cut_product finds rounds of them the shorter (its stages
+  // are of as many bytes and instructions here); below 256 tiles of 128 x 128, half that
+  // many rows a tile, which leave no CU idle.  Device time, 64 x 128 / 128 x 128 / 256 x
+  // 256: 500 x 1024 -> 4096 10.9 / 13.3 us, 1500 x 256 -> 1024 7.2 / 9.1, 1500 x 1024 ->
+  // 4096 21.5 / 18.5, 4000 x 1024 -> 2 x 4096 47 (big) / 56.7
+  const int64_t cols = (GATED ? 2 : 1) * a.hidden;
+  if (cut_product(cols, a.rows, ceil_div(ldx, (int64_t)128), 1, true, 1, 0.0).big)
+    tiles(ByteTile<4, 2, 2, 4, 128, GATED>{}, 256);
+  else if (ceil_div(cols, (int64_t)128) * ceil_div(a.rows, (int64_t)128) > 256)
+    tiles(ByteTile<2, 2, 2, 2, 128, GATED>{}, 512);
   else
-    launch_tiles<SmallTile<int8_t, false, GATED, 1>>(s, 1, epi, st);
+    tiles(ByteTile<1, 2, 2, 2, 128, GATED>{}, 512);
 }
 
 }  // namespace

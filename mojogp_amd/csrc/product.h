@@ -51,21 +51,9 @@ struct Frag {
   f4 v;
 };
 
-// The sums of a product: fp32, of 8-bit integers 32-bit ones.
-typedef int i4 __attribute__((ext_vector_type(4)));
 template <class T>
-using AccOf = typename std::conditional<sizeof(T) == 1, i4, f4>::type;
-
-__device__ __forceinline__ i4 mma_i8(const Frag& a, const Frag& b, i4 c) {
-  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i4, a.v),
-                                               __builtin_bit_cast(i4, b.v), c, 0, 0, 0);
-}
-
-template <class T>
-__device__ __forceinline__ AccOf<T> mma(const Frag& a, const Frag& b, AccOf<T> c) {
-  if constexpr (sizeof(T) == 1) {
-    return mma_i8(a, b, c);
-  } else if constexpr (sizeof(T) == 4) {
+__device__ __forceinline__ f4 mma(const Frag& a, const Frag& b, f4 c) {
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[k], b.v[k], c, 0, 0, 0);
     return c;
@@ -145,7 +133,6 @@ constexpr uint32_t part_steps(bool of_p) {
 template <class T, int TM_, int TN_, int WM_, int WN_, bool TR_, bool DUAL_, int PARTS_>
 struct Tile {
   using Elem = T;
-  using Acc = AccOf<T>;
   static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_;
   static constexpr bool TR = TR_, DUAL = DUAL_;
   static constexpr int PARTS = PARTS_;  // products a sum is made of (PartOrder)
@@ -153,7 +140,7 @@ struct Tile {
   static constexpr int BQ = 16 * TM * WM, BP = 16 * TN * WN;
   static constexpr int T1 = DUAL ? TN / 2 : TN;  // 16-row tiles of one matrix a wave
   static constexpr int RUN = 4 * T1;
-  static constexpr int E = sizeof(T);  // 2, or 1 (NT alone)
+  static constexpr int E = sizeof(T);  // 2
   static constexpr int SB = 128;                   // reduction bytes of a row a stage
   static constexpr int KS = SB / E;                // reduction elements a stage
   static constexpr int LDS = (BP + BQ) * SB;  // one buffer
@@ -318,7 +305,7 @@ __device__ __forceinline__ Frag read_frag(const char* __restrict__ buf, int row,
 template <class TL>
 __device__ __forceinline__ void stage(Loader<TL>& ld, const char* __restrict__ cur,
                                       char* __restrict__ nxt, bool more, int wm, int wn,
-                                      typename TL::Acc (&acc)[TL::TM][TL::TN]) {
+                                      f4 (&acc)[TL::TM][TL::TN]) {
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks) {
     Frag p[TL::TN], q[TL::TM];
@@ -400,11 +387,11 @@ __global__ __launch_bounds__(TL::THREADS) void k_gemm(GemmShape s, EPI epi) {
     const int64_t m0 = (int64_t)tq * TL::BQ + wm * TL::TM * 16, part = (int64_t)tq * TL::WM + wm;
     const bool next = STAYS && id + gridDim.x < tiles;
     id += gridDim.x;
-    typename TL::Acc acc[TL::TM][TL::TN];
+    f4 acc[TL::TM][TL::TN];
 #pragma unroll
     for (int m = 0; m < TL::TM; ++m)
 #pragma unroll
-      for (int n = 0; n < TL::TN; ++n) acc[m][n] = typename TL::Acc{0, 0, 0, 0};
+      for (int n = 0; n < TL::TN; ++n) acc[m][n] = f4{0.f, 0.f, 0.f, 0.f};
     const auto to_next = [&] {
       tile_of(id, (uint32_t)s.tiles_p, (uint32_t)s.tiles_q, tp, tq);
       ld.init(s, (int64_t)tp * CP, (int64_t)tq * TL::BQ, k0, K);

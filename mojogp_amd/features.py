@@ -436,18 +436,16 @@ def _int8_side(w, name, width, index, hidden=None):
     """(codes' address, scales' address, rows, row stride)"""
     if not isinstance(w, Int8Weights):
         raise TypeError(f"{name} must be what int8_weights returned, got {type(w).__name__}")
-    torch = _torch()
-    _check(w.codes, f"{name}.codes", torch.int8, index)
-    _check(w.scale, f"{name}.scale", torch.float32, index)
-    padded = -(-width // 16) * 16
-    if w.width != width or w.codes.dim() != 2 or w.codes.shape[1] != padded \
-            or not w.codes.is_contiguous():
-        raise ValueError(f"{name} must be weights of {width} columns, got {w.width} in codes of "
-                         f"shape {tuple(w.codes.shape)}")
-    rows = w.codes.shape[0]
+    codes, scale, columns = w
+    _check(codes, f"{name}.codes", _torch().int8, index)
+    shape = codes.shape
+    rows = shape[0] if len(shape) == 2 else 0
+    if columns != width or shape != (rows, -(-width // 16) * 16) or not codes.is_contiguous():
+        raise ValueError(f"{name} must be weights of {width} columns, got {columns} in codes of "
+                         f"shape {tuple(shape)}")
     if rows == 0 or (hidden is not None and rows != hidden):
         raise ValueError(f"{name} must have {hidden or 'at least one'} rows, got {rows}")
-    return w.codes.data_ptr(), _vector(w.scale, f"{name}.scale", rows, torch.float32, index), rows
+    return codes.data_ptr(), _vector(scale, f"{name}.scale", rows, _torch().float32, index), rows
 
 
 def _int8(x, gate, up, b_gate, b_up, act, names, out):

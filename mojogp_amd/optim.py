@@ -17,6 +17,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 import numbers
+import operator
 
 import numpy as np
 
@@ -24,6 +25,7 @@ from . import _lib
 from .features import _no_graph, _stream, _torch, _types
 
 _FLOAT_MOST = float(np.finfo(np.float32).max)
+_required, _shape_of, _dtype_of = map(operator.attrgetter, ("requires_grad", "shape", "dtype"))
 
 
 class AdamW:
@@ -129,7 +131,13 @@ class AdamW:
 
     def _addresses_of(self, grads, dtype):
         """Gradients' addresses, each checked."""
-        out, index = [], self._index
+        tensor = _torch().Tensor
+        if set(map(type, grads)) == {tensor} and set(map(tensor.get_device, grads)) == {self._index} \
+                and all(map(tensor.is_contiguous, grads)) \
+                and set(map(_dtype_of, grads)) == {dtype} and not any(map(_required, grads)) \
+                and list(map(_shape_of, grads)) == self._shapes:
+            return list(map(tensor.data_ptr, grads))
+        out, index = [], self._index  # one by one: None among them, or one to be named
         for i, (g, shape) in enumerate(zip(grads, self._shapes)):
             if g is None:
                 out.append(None)
@@ -168,9 +176,8 @@ class AdamW:
             raise ValueError(f"the parameters are on device {self._index}, the current device "
                              f"is {current}")
         if torch.is_grad_enabled():
-            for i, p in enumerate(self.params):
-                if p.requires_grad:
-                    _no_graph(f"params[{i}]")
+            if any(map(_required, self.params)):
+                _no_graph(f"params[{list(map(_required, self.params)).index(True)}]")
         if [p.data_ptr() for p in self.params] != self._addresses:
             raise ValueError("the parameters' memory is no longer where it was when the optimizer "
                              "was made")

@@ -100,7 +100,7 @@ def int8_layer(x, wg, bg=None, wu=None, bu=None, act=None):
 
     def project(w, b):
         c, sw = int8_rows(w)
-        p = (q @ c.T) * s[:, None] * sw
+        p = (q.astype(np.float64) @ c.T.astype(np.float64)) * s[:, None] * sw  # (sums exact)
         return p + (0.0 if b is None else b), np.abs(p)
 
     y, size = project(wg, bg)
