@@ -116,18 +116,49 @@ struct GroupKernel {
   float2* coef;    // [samples][groups]: the two group sums over m
   float inv_m;     // 1 / m
   bool apart;      // the result shares no memory with what is read
-  // whole samples: vectors of a row, rows at a time, samples at a time, threads a
+  // in registers: vectors of a row, rows at a time, samples at a time, threads a
   // group (its sums)
   int cv, rows, at_a_time, lanes;
   int64_t batches;
+  // blocks of groups a sample is dealt out in, one a workgroup; in the kernels a.groups
+  // and a.channels are a block's, and these a sample's
+  int group_blocks, all_groups, all_channels;
   // stretches: rows of one, how many a sample, column blocks of cv vectors
   int stretch, short_stretch;  // of partial results, and of the results
   int stretches, shorts, blocks;
 };
 
+// What a workgroup that holds samples, or groups of one, takes: batches of samples from
+// `first` on, `step` apart, or (groups) the one sample `first`.  Neighbouring groups,
+// which share lines of memory, go to workgroups of one XCD.
+struct Share {
+  int64_t first, step;
+};
+template <class T>
+__device__ __forceinline__ Share share_of(GroupKernel& s) {
+  if (s.group_blocks == 1) return {blockIdx.x, gridDim.x};
+  const uint32_t total = gridDim.x, xcd = blockIdx.x & 7, per = total >> 3, rest = total & 7;
+  const uint32_t unit = xcd * per + min(xcd, rest) + (blockIdx.x >> 3);
+  const uint32_t n = unit / (uint32_t)s.group_blocks, block = unit - n * s.group_blocks;
+  const int col = (int)block * s.a.channels;
+  const auto on = [&](const void* p, bool f32) {
+    return p == nullptr ? p
+           : f32        ? static_cast<const void*>(static_cast<const float*>(p) + col)
+                        : static_cast<const void*>(static_cast<const T*>(p) + col);
+  };
+  s.a.x = on(s.a.x, false);
+  s.dy = on(s.dy, false);
+  s.out = const_cast<void*>(on(s.out, false));
+  s.a.weight = on(s.a.weight, s.a.f32_params);
+  s.a.bias = on(s.a.bias, s.a.f32_params);
+  if (s.stats) s.stats += block * s.a.groups;
+  if (s.part) s.part += (int64_t)n * s.all_channels + col;
+  return {n, s.batches};
+}
+
 // How a sample's group sums come together in a workgroup that holds whole samples:
 // through LDS from an entry for each channel or each vector (whose channels are all of
-// one group), or, of single positions, by lane exchanges (groups of vectors) or within
+// one group; of its `dup` first ones the vector before has them), or, of single positions, by lane exchanges (groups of vectors) or within
 // a thread (several groups a vector).
 constexpr int kMostThreads = 512;
 enum Join : int { CHANNELS = 0, VECTORS = 1, LANES = 2, THREAD = 3 };
@@ -142,8 +173,8 @@ constexpr int kStats = JOIN == CHANNELS || JOIN == THREAD ? K::V : 1;
 // them, and are not used.
 template <class K>
 struct Columns {
-  int col, dup, from;
-  __device__ __forceinline__ Columns(const GroupKernel& s, int base, int j) {
+  int vector, col, dup, from;
+  __device__ __forceinline__ Columns(const GroupKernel& s, int base, int j) : vector(j) {
     const int first = base + j * K::V;
     dup = max(first + K::V - s.a.channels, 0);
     col = first - dup;
@@ -206,7 +237,7 @@ struct Entries {
   __device__ __forceinline__ explicit Entries(const GroupKernel& s) {
     constexpr int V = K::V;
     const int size = s.a.channels / s.a.groups;
-    run = JOIN == VECTORS ? size / V : size;
+    run = JOIN == VECTORS ? (size + V - 1) / V : size;
     width = JOIN == VECTORS ? s.cv : s.cv * V;
   }
 };
@@ -221,6 +252,7 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
   using T = typename K::T;
   constexpr int V = K::V;
   extern __shared__ float2 lds[];
+  const Share mine = share_of<T>(s);
   const Place<K> at(s);
   const int size = s.a.channels / s.a.groups;
   const int64_t L = s.a.positions;
@@ -282,33 +314,33 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
 #pragma unroll
         for (int k = 0; k < MV; ++k)
           if (k % size == 0 && k >= at.dup)
-            s.stats[n * s.a.groups + (at.col + k) / size] = {mean[k], rstd[k]};
+            s.stats[n * s.all_groups + (at.col + k) / size] = {mean[k], rstd[k]};
       }
     } else {
       const Entries<K, JOIN> e(s);
       float2* group = lds + (blockDim.x / s.cv) * e.width;  // a pair's mean and rstd
       if (JOIN == VECTORS) {
-        const float base = (float)x[0].v[0];
+        const float base = (float)x[0].v[V - 1];
         float m = 0.0f, q = 0.0f;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           if (r < count) {
 #pragma unroll
-            for (int k = 0; k < V; ++k) m += (float)x[r].v[k] - base;
+            for (int k = 0; k < V; ++k) m += k >= at.dup ? (float)x[r].v[k] - base : 0.0f;
           }
         }
-        m = base + (count ? m / (float)(count * V) : 0.0f);
+        m = base + (count ? m / (float)(count * (V - at.dup)) : 0.0f);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           if (r < count) {
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-              const float d = (float)x[r].v[k] - m;
+              const float d = k >= at.dup ? (float)x[r].v[k] - m : 0.0f;
               q = fmaf(d, d, q);
             }
           }
         }
-        if (at.active) lds[at.slot * e.width + at.col / V] = {m, q};
+        if (at.active) lds[at.slot * e.width + at.vector] = {m, q};
       } else if (at.active) {
 #pragma unroll
         for (int k = 0; k < V; ++k) {
@@ -329,7 +361,7 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
       const int pairs = s.at_a_time * s.a.groups;
       const int lane = threadIdx.x & (s.lanes - 1);
       const int teams = blockDim.x / s.lanes;
-      const int all = at.slots * e.run;
+      const int all = at.slots * e.run, shared = JOIN == VECTORS ? e.run * V - size : 0;
       for (int p0 = 0; p0 < pairs; p0 += teams) {
         const int p = p0 + threadIdx.x / s.lanes;
         const bool has = p < pairs;
@@ -340,9 +372,9 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
           if (has) {
             for (int i = lane; i < all; i += s.lanes) {
               const int slot = i / e.run;
-              const int c = ((int)L - slot + at.slots - 1) / at.slots;
-              t += f(from[slot * e.width + i - slot * e.run],
-                     (float)c * (JOIN == VECTORS ? V : 1));
+              const int c = ((int)L - slot + at.slots - 1) / at.slots, in = i - slot * e.run;
+              const int each = JOIN == VECTORS ? V - (in == e.run - 1 ? shared : 0) : 1;
+              t += f(from[slot * e.width + in], (float)(c * each));
             }
           }
           return lane_sum(t, s.lanes);
@@ -357,7 +389,7 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
           const float2 r = {m, 1.0f / sqrtf(var + s.a.eps)};
           group[p] = r;
           const int64_t to = batch * s.at_a_time + q;
-          if (s.stats && to < s.a.samples) s.stats[to * s.a.groups + g] = r;
+          if (s.stats && to < s.a.samples) s.stats[to * s.all_groups + g] = r;
         }
       }
       __syncthreads();
@@ -387,12 +419,12 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
   };
   if constexpr (R == 1) {  // single rows: U batches at a time, the next ones loaded ahead
     constexpr int U = JOIN == LANES ? 2 : 1;
-    const int64_t step = gridDim.x;
+    const int64_t step = mine.step;
     Raw<K> ahead[U][R];
     int counts[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) counts[u] = load(blockIdx.x + u * step, ahead[u]);
-    for (int64_t batch = blockIdx.x; batch < s.batches; batch += U * step) {
+    for (int u = 0; u < U; ++u) counts[u] = load(mine.first + u * step, ahead[u]);
+    for (int64_t batch = mine.first; batch < s.batches; batch += U * step) {
       Raw<K> x[U][R];
       int count[U];
 #pragma unroll
@@ -405,7 +437,7 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
       for (int u = 0; u < U; ++u) one(batch + u * step, x[u], count[u]);
     }
   } else {
-    for (int64_t batch = blockIdx.x; batch < s.batches; batch += gridDim.x) {
+    for (int64_t batch = mine.first; batch < s.batches; batch += mine.step) {
       Raw<K> x[R];
       const int count = load(batch, x);
       one(batch, x, count);
@@ -454,9 +486,9 @@ __global__ __launch_bounds__(kMostThreads)
   using T = typename K::T;
   constexpr int V = K::V;
   extern __shared__ float2 lds[];
+  const Share mine = share_of<T>(s);
   const Place<K> at(s);
   const int size = s.a.channels / s.a.groups;
-  const int64_t L = s.a.positions;
   float w[V], b[V], sum_a[V], sum_b[V];
   load_params<K>(s.a.weight, at.col, s.a.f32_params, 1.0f, w);
   load_params<K>(s.a.bias, at.col, s.a.f32_params, 0.0f, b);
@@ -483,16 +515,16 @@ __global__ __launch_bounds__(kMostThreads)
       }
     }
     if (v.count > 0)
-      load_stats(size, s.stats + (batch * s.at_a_time + at.sample) * s.a.groups, group, within,
+      load_stats(size, s.stats + (batch * s.at_a_time + at.sample) * s.all_groups, group, within,
                  v.mean, v.rstd);
   };
   Rows ahead;  // single rows: the next ones are loaded ahead
-  if constexpr (R == 1) load(blockIdx.x, ahead);
-  for (int64_t batch = blockIdx.x; batch < s.batches; batch += gridDim.x) {
+  if constexpr (R == 1) load(mine.first, ahead);
+  for (int64_t batch = mine.first; batch < s.batches; batch += mine.step) {
     Rows now;
     if constexpr (R == 1) {
       now = ahead;
-      load(batch + gridDim.x, ahead);
+      load(batch + mine.step, ahead);
     } else {
       load(batch, now);
     }
@@ -512,8 +544,9 @@ __global__ __launch_bounds__(kMostThreads)
           sum_a[k] += dz[k];
           sum_b[k] = fmaf(dz[k], xhat[k], sum_b[k]);
           dz[k] *= w[k];
-          t1[k % MV] += dz[k];
-          t2[k % MV] = fmaf(dz[k], xhat[k], t2[k % MV]);
+          const float g = JOIN != VECTORS || k >= at.dup ? dz[k] : 0.0f;
+          t1[k % MV] += g;
+          t2[k % MV] = fmaf(g, xhat[k], t2[k % MV]);
         }
       }
     } else {
@@ -535,8 +568,9 @@ __global__ __launch_bounds__(kMostThreads)
       for (int k = 0; k < V; ++k) {
         sum_a[k] += a1[k];
         sum_b[k] += a2[k];
-        t1[k % MV] = fmaf(a1[k], w[k], t1[k % MV]);
-        t2[k % MV] = fmaf(a2[k], w[k], t2[k % MV]);
+        const float g = JOIN != VECTORS || k >= at.dup ? w[k] : 0.0f;
+        t1[k % MV] = fmaf(a1[k], g, t1[k % MV]);
+        t2[k % MV] = fmaf(a2[k], g, t2[k % MV]);
       }
     }
     if (s.out == nullptr) continue;
@@ -553,7 +587,7 @@ __global__ __launch_bounds__(kMostThreads)
 #pragma unroll
         for (int k = 0; k < MV; ++k)
           if (JOIN == VECTORS || k >= at.dup)
-            lds[at.slot * e.width + (JOIN == VECTORS ? at.col / V : at.col + k)] = {t1[k], t2[k]};
+            lds[at.slot * e.width + (JOIN == VECTORS ? at.vector : at.col + k)] = {t1[k], t2[k]};
       }
       __syncthreads();
       const int pairs = s.at_a_time * s.a.groups;
@@ -625,7 +659,7 @@ __global__ __launch_bounds__(kMostThreads)
       t.x += v.x;
       t.y += v.y;
     }
-    s.part[(int64_t)blockIdx.x * s.a.channels + c] = t;
+    s.part[(s.group_blocks == 1 ? (int64_t)blockIdx.x * s.all_channels : 0) + c] = t;
   }
 }
 
@@ -969,6 +1003,7 @@ __global__ __launch_bounds__(1024) void k_group_params(const float2* __restrict_
 
 // ---------------------------------------------------------------- host side
 
+constexpr int kForwardRows = 16, kBackRows = 8;  // of a thread, in registers
 constexpr int64_t kBackBlocks = 1024;  // partial results of whole samples, at most
 constexpr int64_t kStretches = 1024;    // workgroups of samples in stretches
 
@@ -990,18 +1025,48 @@ inline int pow2_at_most(int64_t v) {
   return p;
 }
 
+// Threads of a workgroup that holds `cv` vectors of `positions` rows, or 0.
+inline int threads_of(int64_t cv, int64_t positions, int most) {
+  int threads = 256;
+  while (threads < kMostThreads && (cv > threads || ceil_div(positions, threads / cv) > 4))
+    threads *= 2;
+  return cv <= threads && ceil_div(positions, threads / cv) <= most ? threads : 0;
+}
+
+// Groups a workgroup takes of a sample (a divisor of them), 0: none fit.  All of a
+// small sample's; otherwise as many as leave every CU a workgroup, in rows of 512 bytes
+// at least: narrower ones read memory in parts of lines (32 x 4096 x 512 bf16, forward,
+// by single groups of 32 bytes a row 147 us, in stretches of whole rows 97; 2417 x 1 x
+// 3776 fp32, 7.5 KB a row 55 us, in stretches 268).
+inline int groups_of(const GroupArgs& a, int V, int size, int most) {
+  const int64_t row = size * (int64_t)elem_bytes(a.type);
+  const bool small = a.positions * a.groups * row <= 32768;
+  int best = 0;
+  for (int gb = a.groups; gb >= 1; --gb) {
+    if (a.groups % gb != 0) continue;
+    if (!threads_of(ceil_div((int64_t)gb * size, (int64_t)V), a.positions, most)) continue;
+    // (a block's rows hold a vector, its workgroups are a launch's)
+    if (gb < a.groups && (gb * size < V || a.samples * (a.groups / gb) >= (1 << 24))) break;
+    if (gb < a.groups && gb * row < 512) break;
+    best = gb;
+    if (small || a.samples * (a.groups / gb) >= 256) break;
+  }
+  return best;
+}
+
 // Fills in how the call is cut.
 GroupCut cut_of(GroupKernel& s, bool back) {
-  const GroupArgs& a = s.a;
-  const int V = lane_channels(a);
-  const int size = a.channels / a.groups, most = back ? 8 : 16;
-  const int64_t cv = ceil_div((int64_t)a.channels, (int64_t)V), L = a.positions;
+  const int64_t L = s.a.positions;
+  const int V = lane_channels(s.a), size = s.a.channels / s.a.groups;
   s.inv_m = (float)(1.0 / ((double)L * size));
+  s.all_groups = s.a.groups;
+  s.all_channels = s.a.channels;
   GroupCut c{};
-  int threads = 256;
-  while (threads < kMostThreads && (cv > threads || ceil_div(L, (int64_t)(threads / cv)) > 4)) threads *= 2;
-  c.whole = cv <= threads && ceil_div(L, (int64_t)(threads / cv)) <= most;
+  const int most = back ? kBackRows : kForwardRows, gb = groups_of(s.a, V, size, most);
+  c.whole = gb > 0;
   if (!c.whole) {
+    const GroupArgs& a = s.a;
+    const int64_t cv = ceil_div((int64_t)a.channels, (int64_t)V);
     s.blocks = (int)ceil_div(cv, (int64_t)kPartThreads);
     s.cv = (int)ceil_div(cv, (int64_t)s.blocks);
     s.blocks = (int)ceil_div(cv, (int64_t)s.cv);
@@ -1011,19 +1076,25 @@ GroupCut cut_of(GroupKernel& s, bool back) {
     s.stretches = (int)std::max<int64_t>(1, std::min(want, L / (8 * slots)));
     s.stretch = (int)ceil_div(L, (int64_t)s.stretches);
     s.stretches = (int)ceil_div(L, (int64_t)s.stretch);
-    // the results', which leave no partial ones behind: more of them, of two rows a thread
+    // the results', which leave no partial ones behind: more of them, of four rows a thread
     const int64_t more = std::max<int64_t>(1, std::min(2 * want, L / (4 * slots)));
     s.short_stretch = (int)ceil_div(L, more);
     s.shorts = (int)ceil_div(L, (int64_t)s.short_stretch);
     return c;
   }
+  s.group_blocks = s.a.groups / gb;
+  s.a.groups = gb;
+  s.a.channels = gb * size;
+  const GroupArgs& a = s.a;
+  const int64_t cv = ceil_div((int64_t)a.channels, (int64_t)V);
+  const int threads = threads_of(cv, L, most);
   s.cv = (int)cv;
   s.rows = threads / s.cv;
   c.threads = threads;
-  s.at_a_time = (int)std::max<int64_t>(1, s.rows / L);
+  s.at_a_time = s.group_blocks > 1 ? 1 : (int)std::max<int64_t>(1, s.rows / L);
   s.batches = ceil_div(a.samples, (int64_t)s.at_a_time);
   const int64_t r = ceil_div(L, (int64_t)s.rows);
-  c.r = r <= 1 ? 1 : r <= 4 ? 4 : most;
+  c.r = r <= 1 ? 1 : r <= 4 ? 4 : r <= 8 ? 8 : 16;
   const bool pow2 = (size & (size - 1)) == 0;
   if (L == 1 && pow2 && size < V) {
     c.join = THREAD;
@@ -1032,9 +1103,9 @@ GroupCut cut_of(GroupKernel& s, bool back) {
     c.join = LANES;
     s.lanes = size / V;
   } else {
-    c.join = size % V == 0 ? VECTORS : CHANNELS;
+    c.join = size % V == 0 || gb == 1 ? VECTORS : CHANNELS;
     const int64_t slots = std::min<int64_t>(s.rows, L);
-    const int64_t entries = slots * (c.join == VECTORS ? size / V : size);
+    const int64_t entries = slots * (c.join == VECTORS ? ceil_div(size, V) : size);
     const int64_t pairs = (int64_t)s.at_a_time * a.groups;
     s.lanes = std::min({64, pow2_at_most(2 * entries - 1),
                         pow2_at_most(std::max<int64_t>(1, threads / pairs))});
@@ -1044,8 +1115,13 @@ GroupCut cut_of(GroupKernel& s, bool back) {
   return c;
 }
 
-inline unsigned back_blocks(const GroupKernel& s) {
-  return (unsigned)std::min<int64_t>(s.batches, kBackBlocks);
+// Workgroups, and rows of partial results that they leave (BACK).
+inline unsigned workgroups(const GroupKernel& s, bool back) {
+  if (s.group_blocks > 1) return (unsigned)(s.a.samples * s.group_blocks);
+  return (unsigned)std::min<int64_t>(s.batches, back ? kBackBlocks : 2048);
+}
+inline int64_t back_parts(const GroupKernel& s) {
+  return s.group_blocks > 1 ? s.a.samples : workgroups(s, true);
 }
 
 // Runs f with a kernel's rows a thread and join.
@@ -1064,7 +1140,8 @@ void dispatch_whole(const GroupCut& c, F&& f) {
   if (c.join == LANES) return f(integral_constant<int, 1>{}, integral_constant<int, LANES>{});
   if (c.r == 1) return with(integral_constant<int, 1>{});
   if (c.r == 4) return with(integral_constant<int, 4>{});
-  with(integral_constant<int, BACK ? 8 : 16>{});
+  if (c.r == 8) return with(integral_constant<int, 8>{});
+  if constexpr (!BACK) with(integral_constant<int, 16>{});
 }
 
 // Runs f with the call's Kind.
@@ -1111,7 +1188,7 @@ size_t group_norm_bytes(const GroupArgs& a, bool back) {
   s.a = a;
   const GroupCut c = cut_of(s, back);
   const size_t row = (size_t)a.channels * sizeof(float2);
-  if (c.whole) return back ? aligned(back_blocks(s) * row) : 0;
+  if (c.whole) return back ? aligned((size_t)back_parts(s) * row) : 0;
   return aligned((size_t)(a.samples * s.stretches) * row) + pairs_bytes(a);
 }
 
@@ -1135,9 +1212,8 @@ void group_norm(const GroupArgs& a, void* y, int64_t y_stride, float* stats, voi
       launch_stretches<K, false>(s, st);
       return;
     }
-    const unsigned grid = (unsigned)std::min<int64_t>(s.batches, 2048);
     dispatch_whole<K, false>(c, [&](auto r, auto join) {
-      k_group_fwd<K, r.value, join.value><<<grid, c.threads, c.lds, st>>>(s);
+      k_group_fwd<K, r.value, join.value><<<workgroups(s, false), c.threads, c.lds, st>>>(s);
     });
   });
   MGP_HIP_CHECK(hipGetLastError());
@@ -1167,10 +1243,10 @@ void group_norm_backward(const GroupArgs& a, const void* dy, int64_t dy_stride, 
         launch_stretches<K, true>(s, st);
         return;
       }
-      parts = back_blocks(s);
+      parts = back_parts(s);
       if (!params) s.part = nullptr;
       dispatch_whole<K, true>(c, [&](auto r, auto join) {
-        k_group_bwd<K, r.value, join.value><<<(unsigned)parts, c.threads, c.lds, st>>>(s);
+        k_group_bwd<K, r.value, join.value><<<workgroups(s, true), c.threads, c.lds, st>>>(s);
       });
     });
   }
