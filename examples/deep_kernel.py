@@ -1,6 +1,6 @@
 """A deep kernel: gated layers, layer norms and dropout in front of a Gaussian process.
 
-    python -m examples.deep_kernel [--points 4000] [--steps 80] [--type bf16]
+    python -m examples.deep_kernel [--points 4000] [--steps 80] [--type bf16] [--bits 8] [--int8]
 
 The features z = f(x), normalised so that they cannot run away from each other,
 are the points of an RBF kernel; layers, kernel parameters and noise are trained
@@ -11,8 +11,10 @@ on the GP's marginal likelihood:
 With alpha = K^-1 y, probes Z (Z Z^T / T = I on average) and U = K^-1 Z its
 gradient with respect to the points is the input gradient of K for the weight
 columns [-alpha / 2 | U / (2 T)] and [alpha | Z]; it goes back through the
-layers by their own backward passes.  torch holds the arrays and does the
-vector work of the conjugate gradients and of Adam.
+layers by their own backward passes, and one AdamW step over all of them, with float32
+copies of 16-bit weights and states in 32 or 8 bits, follows.  The trained layers
+serve test points in their own type or in 8-bit integers.  torch holds the arrays and
+does the vector work of the conjugate gradients.
 """
 
 import argparse
@@ -21,7 +23,7 @@ import ctypes as C
 import numpy as np
 import torch
 
-from mojogp_amd import _lib, features
+from mojogp_amd import _lib, features, optim
 from mojogp_amd._provider import NativeProvider
 
 TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
@@ -62,6 +64,22 @@ class Features:
         f = features.gated_layer(y1, *self.last, activation="gelu")
         z, s2 = features.layer_norm(f, eps=EPS, save=True)
         return z, (x, h0, y0, s0, h1, y1, s1, f, s2, offset, rate)
+
+    def int8(self):
+        """z of x with every layer's weights in 8-bit integers: a function, for serving."""
+        def weights(layer):
+            return [*map(features.int8_weights, layer[:2]), *layer[2:]]
+
+        first, second, last = map(weights, (self.first, self.second, self.last))
+
+        def serve(x):
+            h0 = features.int8_gated_layer(x, *first)
+            h1 = features.int8_gated_layer(features.layer_norm(h0, *self.norm1), *second) + h0
+            f = features.int8_gated_layer(features.layer_norm(h1, *self.norm2), *last,
+                                          activation="gelu")
+            return features.layer_norm(f, eps=EPS)
+
+        return serve
 
     def backward(self, dz, tape):
         """Gradients in the order of parameters()."""
@@ -117,11 +135,13 @@ def likelihood_gradients(provider, y, probes, tol=1e-3):
 
 
 class Adam:
+    """Of the kernel's parameters, which are on the host."""
+
     def __init__(self, rate):
         self.rate, self.step, self.state = rate, 0, {}
 
     def update(self, params, grads):
-        """New values of float32 arrays (numpy or torch)."""
+        """New values of arrays."""
         self.step += 1
         out = []
         for i, (p, g) in enumerate(zip(params, grads)):
@@ -134,18 +154,18 @@ class Adam:
 
 
 def train(x, y, *, width=64, outputs=4, steps=80, kind="bf16", probes=10, rate=0.01, seed=0,
-          report=print):
+          bits=32, report=print):
     """Trains on x [n, inputs], y [n] (numpy); returns the model, its kernel
     parameters, noise and the history of y^T K^-1 y / n."""
     dtype = TYPES[kind]
     gen = torch.Generator(device="cuda")
     gen.manual_seed(seed)
     model = Features(x.shape[1], width, outputs, dtype, gen)
-    master = [p.float() for p in model.parameters()]  # Adam's copies
+    layers_adam = optim.AdamW(model.parameters(), bits=bits, master=kind != "f32", seed=seed)
     xs = torch.from_numpy(x).to("cuda", dtype)
     ys = torch.from_numpy(y).cuda()
     raw = [np.log(np.array([1.0] * outputs + [1.0, 0.1]))]  # lengthscales, outputscale, noise
-    layers_adam, kernel_adam = Adam(rate), Adam(3.0 * rate)
+    kernel_adam = Adam(3.0 * rate)
     history = []
     for step in range(steps):
         z, tape = model.forward(xs, offset=step * len(x) * width)
@@ -159,20 +179,19 @@ def train(x, y, *, width=64, outputs=4, steps=80, kind="bf16", probes=10, rate=0
             provider.close()
         history.append(fit / len(x))
         grads = model.backward((dz / len(x)).to(dtype), tape)
-        master = layers_adam.update(master, [g.float() for g in grads])
-        for p, m in zip(model.parameters(), master):
-            p.copy_(m)
+        layers_adam.step(grads, rate, step + 1)
         raw = kernel_adam.update(raw, [dtheta / len(x) * theta])
         if report and (step % 10 == 0 or step == steps - 1):
             report(f"step {step:4d}  y K^-1 y / n {history[-1]:.4f}  noise {theta[-1]:.4f}")
     return model, theta, history
 
 
-def predict(model, theta, x, y, xs):
-    """Predictive mean at xs (dropout off)."""
+def predict(model, theta, x, y, xs, int8=False):
+    """Predictive mean at xs (dropout off; int8: by the layers in 8-bit integers, for
+    both sides of the kernel)."""
     dtype = model.first[0].dtype
-    z, zs = (model.forward(torch.from_numpy(a).to("cuda", dtype), rate=0.0)[0].float()
-             for a in (x, xs))
+    serve = model.int8() if int8 else lambda a: model.forward(a, rate=0.0)[0]
+    z, zs = (serve(torch.from_numpy(a).to("cuda", dtype)).float() for a in (x, xs))
     provider = NativeProvider("rbf", True, z.cpu().numpy(), theta[:-1], float(theta[-1]))
     try:
         alpha = solve(provider, torch.from_numpy(y).cuda()[None])
@@ -196,11 +215,13 @@ def main():
     parser.add_argument("--points", type=int, default=4000)
     parser.add_argument("--steps", type=int, default=80)
     parser.add_argument("--type", choices=sorted(TYPES), default="bf16")
+    parser.add_argument("--bits", type=int, choices=(8, 32), default=32, help="AdamW's states")
+    parser.add_argument("--int8", action="store_true", help="serve in 8-bit integers")
     args = parser.parse_args()
     x, y = data(args.points + 1000)
     n = args.points
-    model, theta, _ = train(x[:n], y[:n], steps=args.steps, kind=args.type)
-    mean = predict(model, theta, x[:n], y[:n], x[n:])
+    model, theta, _ = train(x[:n], y[:n], steps=args.steps, kind=args.type, bits=args.bits)
+    mean = predict(model, theta, x[:n], y[:n], x[n:], args.int8)
     print(f"test RMSE {np.sqrt(np.mean((mean - y[n:]) ** 2)):.4f} of a spread of {y[n:].std():.4f}")
 
 
