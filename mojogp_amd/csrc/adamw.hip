@@ -44,7 +44,7 @@ struct Scalars {
   double factor;   // of the gradients
   float c1, c2;    // 1 / (1 - b1^t), 1 / (1 - b2^t)
   float rate;
-  int skip;        // the norm is not finite: nothing is changed
+  int skip;        // the norm is not finite, or step or rate is none: nothing is changed
 };
 
 // Four elements at any alignment, of which `left` exist; zeros past them.
@@ -143,13 +143,18 @@ __global__ __launch_bounds__(256) void k_adamw_scalars(ScalarArgs a) {
   Scalars r = a.host;
   const double norm = sqrt(red[0] + red[1] + red[2] + red[3]) * fabs(a.grad_scale);
   r.factor = a.grad_scale * (norm > a.max_norm ? a.max_norm / norm : 1.0);
-  r.skip = !(norm < HUGE_VAL);
+  r.skip = !((float)norm < HUGE_VALF);
   if (a.step_device) {
-    const double t = (double)*a.step_device;
+    const int64_t step = *a.step_device;
+    const double t = (double)step;
+    r.skip |= step < 1;
     r.c1 = (float)(1.0 / (1.0 - pow(a.beta1, t)));
     r.c2 = (float)(1.0 / (1.0 - pow(a.beta2, t)));
   }
-  if (a.rate_device) r.rate = *a.rate_device;
+  if (a.rate_device) {
+    r.rate = *a.rate_device;
+    r.skip |= !(r.rate >= 0.0f && r.rate < HUGE_VALF);
+  }
   *a.out = r;
   if (a.norm_out) *a.norm_out = (float)norm;
 }

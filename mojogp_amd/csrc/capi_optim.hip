@@ -192,8 +192,25 @@ int mgp_adamw_step_device(void* plan, const mgp_adamw_step_t* args, void* worksp
       const Span* w = q ? shared(*h, q, bytes) : nullptr;
       MGP_REQUIRE(w == nullptr, std::string(name) + " shares memory with " + w->name);
     };
-    for (size_t i = 0; i < p.tensors.size(); ++i)
-      apart("a gradient", s.grads[i], (size_t)p.tensors[i].size * elem);
+    // what a step writes besides the plan's memory
+    const Span results[2] = {{static_cast<const char*>(workspace),
+                              static_cast<const char*>(workspace) + need, "the workspace"},
+                             {reinterpret_cast<const char*>(s.norm_out),
+                              reinterpret_cast<const char*>(s.norm_out) + sizeof(float), "norm"}};
+    auto outside = [&](const char* name, const void* q, size_t bytes, int from, int to) {
+      const char *b = static_cast<const char*>(q), *e = b + bytes;
+      for (int k = from; k < to; ++k)
+        MGP_REQUIRE(!q || !results[k].begin || e <= results[k].begin || results[k].end <= b,
+                    std::string(name) + " shares memory with " + results[k].name);
+    };
+    for (size_t i = 0; i < p.tensors.size(); ++i) {
+      const size_t bytes = (size_t)p.tensors[i].size * elem;
+      apart("a gradient", s.grads[i], bytes);
+      if (bytes) outside("a gradient", s.grads[i], bytes, 0, 2);
+    }
+    outside("norm", s.norm_out, sizeof(float), 0, 1);
+    outside("step", s.step_device, sizeof(int64_t), 0, 2);
+    outside("rate", s.rate_device, sizeof(float), 0, 2);
     apart("norm", s.norm_out, sizeof(float));
     apart("step", s.step_device, sizeof(int64_t));
     apart("rate", s.rate_device, sizeof(float));
@@ -212,6 +229,9 @@ int mgp_adamw_values_device(void* plan, float* exp_avg, float* exp_avg_sq, void*
       const Span* w = shared(*h, q, bytes);
       MGP_REQUIRE(w == nullptr, std::string("a result shares memory with ") + w->name);
     }
+    MGP_REQUIRE(bytes == 0 || exp_avg + h->plan.values <= exp_avg_sq ||
+                    exp_avg_sq + h->plan.values <= exp_avg,
+                "the results share memory");
     adamw_values(h->plan, exp_avg, exp_avg_sq, static_cast<hipStream_t>(stream));
   });
 }

@@ -1042,7 +1042,8 @@ inline int groups_of(const GroupArgs& a, int V, int size, int most) {
   const int64_t row = size * (int64_t)elem_bytes(a.type);
   const bool small = a.positions * a.groups * row <= 32768;
   int best = 0;
-  for (int gb = a.groups; gb >= 1; --gb) {
+  // (more than the threads' vectors hold never fit)
+  for (int gb = std::min(a.groups, std::max(1, kMostThreads * V / size)); gb >= 1; --gb) {
     if (a.groups % gb != 0) continue;
     if (!threads_of(ceil_div((int64_t)gb * size, (int64_t)V), a.positions, most)) continue;
     // (a block's rows hold a vector, its workgroups are a launch's)

@@ -252,8 +252,9 @@ def _group_args(x, groups, weight, bias, eps, activation):
         raise ValueError(f"groups must divide the {width} channels, got {groups!r}")
     given = weight if weight is not None else bias
     ptype, pcode = dtype, code
-    if given is not None and given.dtype is not dtype:
-        ptype, pcode = given.dtype, _types.get(given.dtype)
+    if given is not None and getattr(given, "dtype", None) is not dtype:
+        ptype = getattr(given, "dtype", type(given).__name__)
+        pcode = _types.get(ptype)
         if pcode != 0:
             raise TypeError(f"weight and bias must have x's element type or be float32, got "
                             f"{ptype}, which does not fit {dtype}")
@@ -296,7 +297,7 @@ def group_norm_backward(dy, x, groups, weight, bias, saved, *, activation=None):
     formed again from x: nothing but ``saved`` is kept between the passes."""
     a, dtype, index, stream = _group_args(x, groups, weight, bias, 0.0, activation)
     pdy, _, _, dy_stride = _rows(dy, "dy", dtype, index, x.shape)
-    if saved is None or saved.shape != (a.samples, groups, 2) or _types.get(saved.dtype) != 0 \
+    if getattr(saved, "shape", None) != (a.samples, groups, 2) or _types.get(saved.dtype) != 0 \
             or not saved.is_contiguous() or saved.get_device() != index:
         raise ValueError("saved must be what group_norm(..., save=True) returned for this x")
     dx = x.new_empty(x.shape)

@@ -41,7 +41,9 @@ class AdamW:
     ``bits=8`` holds the running means as 8-bit floats with a float32 scale for each
     256 values of a parameter (2.03 bytes a value instead of 8), rounded up or down by
     draws that are functions of ``seed``, the step and the value's place alone.  The
-    update itself is formed before the rounding.
+    update itself is formed before the rounding.  A gradient that is not finite, or whose
+    square is not in float32, makes NaN of the states of its scale's 256 values, where
+    ``step`` forms no norm that catches it.
 
     exp_avg, exp_avg_sq (float32, or codes with exp_avg_scale and exp_avg_sq_scale) and
     master are flat arrays in which each parameter's values start at the next multiple
@@ -163,7 +165,9 @@ class AdamW:
         type, or all float32), None for those that are left as they are.
 
         rate and step (1 at the first step) are numbers, or device tensors of one
-        element (float32, int64), which a recorded graph reads at every replay.
+        element (float32, int64), which a recorded graph reads at every replay (the
+        optimizer has to live as long as the graph); where such a step is below 1, or such a
+        rate negative or not finite, everything is left as it is.
         The gradients are multiplied by ``grad_scale`` and, where ``max_norm`` is
         given, by max_norm over their common norm if that is larger.  With max_norm or
         ``norm=True`` the norm comes back (float32, on the device), and a norm that is

@@ -172,6 +172,26 @@ def test_a_norm_that_is_not_finite_changes_nothing(bits, bad):
         assert torch.equal(t, kept[k])
 
 
+@pytest.mark.parametrize("step, rate", [(0, 0.1), (-3, 0.1), (1, float("nan")), (1, float("inf")),
+                                        (1, -0.1)])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_device_numbers_that_are_refused_on_the_host_change_nothing(bits, step, rate):
+    p = torch.ones(300, device="cuda")
+    opt = optim.AdamW([p], bits=bits)
+    g = torch.ones_like(p)
+    opt.step([g], torch.full((), rate, device="cuda"), torch.full((), step, device="cuda"))
+    assert torch.equal(p, torch.ones_like(p))
+    assert all(not t.any() for t in opt.state().values())
+
+
+def test_a_norm_past_float32_changes_nothing():
+    """Of finite gradients: 2^126 times the root of 300."""
+    p = torch.ones(300, device="cuda")
+    opt = optim.AdamW([p])
+    norm = opt.step([torch.full_like(p, 2.0 ** 126)], 0.1, 1, max_norm=1.0)
+    assert torch.isinf(norm) and torch.equal(p, torch.ones_like(p)) and not opt.exp_avg.any()
+
+
 def test_large_and_small_gradients_norm():
     """Squares beyond and below fp32."""
     p = torch.zeros(1000, device="cuda")

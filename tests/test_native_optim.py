@@ -109,6 +109,36 @@ def test_steps_are_refused():
         _lib.call("mgp_adamw_destroy", plan)
 
 
+def test_what_a_step_writes_shares_no_memory():
+    """The workspace and the norm with the gradients, the step, the rate and each other."""
+    plan, _ = _create(_args([100, 50]))
+    ws = 7 << 32
+    try:
+        for grads, kw, what in (
+                ([None, ws - 196], {}, "a gradient shares memory with the workspace"),
+                ([None, BASE - 400], {"norm": BASE - 204}, "a gradient shares memory with norm"),
+                ([None, None], {"norm": ws + 8}, "norm shares memory with the workspace"),
+                ([None, None], {"norm": BASE - 64, "step_device": BASE - 64},
+                 "step shares memory with norm"),
+                ([None, None], {"rate_device": ws + 252}, "rate shares memory with the workspace")):
+            s = _lib.AdamWStep(grads=(C.c_void_p * 2)(*grads), grad_type=F32, grad_scale=1.0,
+                               form_norm=1, max_norm=1.0, step=1, rate=1e-3)
+            for k, v in kw.items():
+                setattr(s, k, v)
+            nbytes = C.c_int64(0)
+            _lib.call("mgp_adamw_workspace", plan, C.byref(s), C.byref(nbytes))
+            with pytest.raises(_lib.NativeCallError, match=what):
+                _lib.call("mgp_adamw_step_device", plan, C.byref(s), ws, nbytes.value, None)
+    finally:
+        _lib.call("mgp_adamw_destroy", plan)
+    plan, _ = _create(_args([100], bits=8))
+    try:
+        with pytest.raises(_lib.NativeCallError, match="the results share memory"):
+            _lib.call("mgp_adamw_values_device", plan, 8 << 32, (8 << 32) + 1020, None)
+    finally:
+        _lib.call("mgp_adamw_destroy", plan)
+
+
 def test_python_entry_refuses_what_is_on_the_host():
     with pytest.raises(ValueError, match="device tensors"):
         optim.AdamW([torch.zeros(4)])
