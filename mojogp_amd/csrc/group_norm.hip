@@ -117,8 +117,8 @@ struct GroupKernel {
   float inv_m;     // 1 / m
   bool apart;      // the result shares no memory with what is read
   // in registers: vectors of a row, rows at a time, samples at a time, threads a
-  // group (its sums)
-  int cv, rows, at_a_time, lanes;
+  // group (its sums), and of them on the entries of one row
+  int cv, rows, at_a_time, lanes, run_lanes;
   int64_t batches;
   // blocks of groups a sample is dealt out in, one a workgroup; in the kernels a.groups
   // and a.channels are a block's, and these a sample's
@@ -157,14 +157,14 @@ __device__ __forceinline__ Share share_of(GroupKernel& s) {
 }
 
 // How a sample's group sums come together in a workgroup that holds whole samples:
-// through LDS from an entry for each channel or each vector (whose channels are all of
-// one group; of its `dup` first ones the vector before has them), or, of single positions, by lane exchanges (groups of vectors) or within
-// a thread (several groups a vector).
+// through LDS from an entry for each vector (whose channels are all of one group) or for
+// each group that has channels of it, or, of single positions, by lane exchanges
+// (groups of vectors) or within a thread (several groups a vector).
 constexpr int kMostThreads = 512;
-enum Join : int { CHANNELS = 0, VECTORS = 1, LANES = 2, THREAD = 3 };
+enum Join : int { SEGMENTS = 0, VECTORS = 1, LANES = 2, THREAD = 3 };
 // Statistics that a vector's channels have: one, or each its own.
 template <class K, int JOIN>
-constexpr int kStats = JOIN == CHANNELS || JOIN == THREAD ? K::V : 1;
+constexpr int kStats = JOIN == SEGMENTS || JOIN == THREAD ? K::V : 1;
 
 // The channels of a thread: vector j of those from `base` on.  The last one of a row
 // ends with it, and shares its first `dup` channels with the one before, so that rows of
@@ -229,18 +229,91 @@ __device__ __forceinline__ void block_sums(float* v, int size) {
   }
 }
 
-// Where the entries of a pair (sample at a time, group) lie in LDS: runs of `run` from
-// `at` on, one for each of the sample's slots, `width` apart.
+// Groups that V consecutive channels belong to, at most; vectors that hold channels of a
+// group.
+__host__ __device__ constexpr int most_groups(int V, int size) {
+  return (V + size - 2) / size + 1 < V ? (V + size - 2) / size + 1 : V;
+}
+__host__ __device__ constexpr int vectors_of(int join, int V, int size) {
+  return join == VECTORS ? (size + V - 1) / V : (size + V - 2) / V + 1;
+}
+
+// The entries in LDS: `each` for a vector of a slot (of the groups from that of the
+// vector's own first channel on), `plane` apart, so that neighbouring threads write
+// neighbouring ones.  (Planes are 64 bytes off each other's banks: neighbouring groups
+// are read together.)
+__host__ __device__ constexpr int plane_of(int threads) { return (threads + 31) / 32 * 32 + 8; }
 template <class K, int JOIN>
 struct Entries {
-  int run, width;
-  __device__ __forceinline__ explicit Entries(const GroupKernel& s) {
+  int size, run, plane, all;
+  int few, more;  // rows of a slot: one more than few in the first `more` slots
+  __device__ __forceinline__ Entries(const GroupKernel& s, int size_, int slots) : size(size_) {
+    run = vectors_of(JOIN, K::V, size);
+    plane = plane_of(s.rows * s.cv);
+    all = plane * (JOIN == VECTORS ? 1 : most_groups(K::V, size));
+    few = (int)s.a.positions / slots;
+    more = (int)s.a.positions - few * slots;
+  }
+  // the first entry of group g in a slot
+  __device__ __forceinline__ int first_of(int g) const {
+    const int j0 = g * size / K::V;
+    return j0 + (JOIN == VECTORS ? 0 : (g - j0 * K::V / size) * plane);
+  }
+  // f(entry, its rows, its channels) of group g for a sample whose first slot is `first`,
+  // dealt out among the pair's lanes.
+  template <class F>
+  __device__ __forceinline__ void each_of(const GroupKernel& s, const float2* first, int slots,
+                                          int lane, int g, F&& f) const {
     constexpr int V = K::V;
-    const int size = s.a.channels / s.a.groups;
-    run = JOIN == VECTORS ? (size + V - 1) / V : size;
-    width = JOIN == VECTORS ? s.cv : s.cv * V;
+    const int c0 = g * size, j0 = c0 / V, at0 = first_of(g);
+    const int in0 = lane & (s.run_lanes - 1), rows = s.lanes / s.run_lanes;
+    for (int slot = lane / s.run_lanes; slot < slots; slot += rows) {
+      const int c = few + (slot < more);
+      for (int in = in0; in < run; in += s.run_lanes) {
+        const int v0 = (j0 + in) * V, n = min(v0 + V, c0 + size) - max(v0, c0);
+        if (n > 0) f(first[slot * s.cv + (in == 0 ? at0 : j0 + in)], c, n);
+      }
+    }
   }
 };
+
+// Runs add(k, n) for each of a vector's own channels, n being how many of its group
+// went before in the vector, and end(t) behind the last one of each group.
+template <int V, class A, class E>
+__device__ __forceinline__ void segments(int size, int within, int dup, A&& add, E&& end) {
+  int n = 0, t = 0;
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    const bool last = ++within == size;
+    if (k >= dup) {
+      add(k, n);
+      ++n;
+      if (last || k == V - 1) {
+        end(t);
+        ++t;
+        n = 0;
+      }
+    }
+    if (last) within = 0;
+  }
+}
+
+// mean and rstd of a vector's channels, the first of which is the `in`th of group g;
+// row: those of the sample
+template <int MV>
+__device__ __forceinline__ void load_stats(int size, const float2* row, int g, int in,
+                                           float (&mean)[MV], float (&rstd)[MV]) {
+#pragma unroll
+  for (int k = 0; k < MV; ++k) {
+    const float2 r = row[g];
+    mean[k] = r.x;
+    rstd[k] = r.y;
+    if (++in == size && k + 1 < MV) {
+      in = 0;
+      ++g;
+    }
+  }
+}
 
 __device__ __forceinline__ float lane_sum(float v, int lanes) {
   for (int o = lanes >> 1; o >= 1; o >>= 1) v += __shfl_xor(v, o);
@@ -255,10 +328,11 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
   const Share mine = share_of<T>(s);
   const Place<K> at(s);
   const int size = s.a.channels / s.a.groups;
-  const int64_t L = s.a.positions;
   float w[V], b[V];
   load_params<K>(s.a.weight, at.col, s.a.f32_params, 1.0f, w);
   load_params<K>(s.a.bias, at.col, s.a.f32_params, 0.0f, b);
+  const Entries<K, JOIN> e(s, size, at.slots);
+  const int first_group = at.col / size, within = at.col - first_group * size;
   const int64_t off = at.offset(s, s.a.x_stride), off_y = at.offset(s, s.ldo);
   auto load = [&](int64_t batch, Raw<K> (&x)[R]) __attribute__((always_inline)) {
     const T* px = static_cast<const T*>(s.a.x) + batch_offset(s, batch, s.a.x_stride) + off;
@@ -317,8 +391,7 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
             s.stats[n * s.all_groups + (at.col + k) / size] = {mean[k], rstd[k]};
       }
     } else {
-      const Entries<K, JOIN> e(s);
-      float2* group = lds + (blockDim.x / s.cv) * e.width;  // a pair's mean and rstd
+      float2* group = lds + e.all;  // a pair's mean and rstd
       if (JOIN == VECTORS) {
         const float base = (float)x[0].v[V - 1];
         float m = 0.0f, q = 0.0f;
@@ -340,46 +413,51 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
             }
           }
         }
-        if (at.active) lds[at.slot * e.width + at.vector] = {m, q};
+        if (at.active) lds[threadIdx.x] = {m, q};
       } else if (at.active) {
+        const float share = count ? 1.0f / (float)count : 0.0f;
+        float mean_of = 0.0f, sq_of = 0.0f;  // of a group's channels so far
+        segments<V>(
+            size, within, at.dup,
+            [&](int k, int n) __attribute__((always_inline)) {
+              const float base = (float)x[0].v[k];
+              float m = 0.0f, q = 0.0f;
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const float base = (float)x[0].v[k];
-          float m = 0.0f, q = 0.0f;
+              for (int r = 0; r < R; ++r) m += r < count ? (float)x[r].v[k] - base : 0.0f;
+              m = fmaf(m, share, base);
 #pragma unroll
-          for (int r = 0; r < R; ++r) m += r < count ? (float)x[r].v[k] - base : 0.0f;
-          m = base + (count ? m / (float)count : 0.0f);
-#pragma unroll
-          for (int r = 0; r < R; ++r) {
-            const float d = r < count ? (float)x[r].v[k] - m : 0.0f;
-            q = fmaf(d, d, q);
-          }
-          if (k >= at.dup) lds[at.slot * e.width + at.col + k] = {m, q};
-        }
+              for (int r = 0; r < R; ++r) {
+                const float d = r < count ? (float)x[r].v[k] - m : 0.0f;
+                q = fmaf(d, d, q);
+              }
+              const float part = __builtin_amdgcn_rcpf((float)(n + 1));
+              const float d = n ? m - mean_of : 0.0f;
+              mean_of = n ? fmaf(d, part, mean_of) : m;
+              sq_of = fmaf(d * d, (float)(n * count) * part, n ? sq_of + q : q);
+            },
+            [&](int t) __attribute__((always_inline)) {
+              lds[t * e.plane + threadIdx.x] = {mean_of, sq_of};
+            });
       }
       __syncthreads();
       const int pairs = s.at_a_time * s.a.groups;
       const int lane = threadIdx.x & (s.lanes - 1);
       const int teams = blockDim.x / s.lanes;
-      const int all = at.slots * e.run, shared = JOIN == VECTORS ? e.run * V - size : 0;
       for (int p0 = 0; p0 < pairs; p0 += teams) {
         const int p = p0 + threadIdx.x / s.lanes;
         const bool has = p < pairs;
         const int q = p / s.a.groups, g = p - q * s.a.groups;
-        const float2* from = lds + q * at.slots * e.width + g * e.run;
+        const float2* from = lds + q * at.slots * s.cv;
         auto sweep = [&](auto f) __attribute__((always_inline)) {
           float t = 0.0f;
-          if (has) {
-            for (int i = lane; i < all; i += s.lanes) {
-              const int slot = i / e.run;
-              const int c = ((int)L - slot + at.slots - 1) / at.slots, in = i - slot * e.run;
-              const int each = JOIN == VECTORS ? V - (in == e.run - 1 ? shared : 0) : 1;
-              t += f(from[slot * e.width + in], (float)(c * each));
-            }
-          }
+          if (has)
+            e.each_of(s, from, at.slots, lane, g,
+                      [&](float2 v, int c, int n) __attribute__((always_inline)) {
+                        t += f(v, (float)(c * n));
+                      });
           return lane_sum(t, s.lanes);
         };
-        const float base = has ? from[0].x : 0.0f;
+        const float base = has ? from[e.first_of(g)].x : 0.0f;
         const float m =
             fmaf(sweep([&](float2 v, float c) { return (v.x - base) * c; }), s.inv_m, base);
         const float var = sweep([&](float2 v, float c) {
@@ -393,14 +471,8 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
         }
       }
       __syncthreads();
-      if (at.active) {
-#pragma unroll
-        for (int k = 0; k < MV; ++k) {
-          const float2 r = group[at.sample * s.a.groups + (at.col + k) / size];
-          mean[k] = r.x;
-          rstd[k] = r.y;
-        }
-      }
+      if (at.active)
+        load_stats(size, group + at.sample * s.a.groups, first_group, within, mean, rstd);
     }
     if (in) {
       T* py = static_cast<T*>(s.out) + batch_offset(s, batch, s.ldo) + off_y;
@@ -462,23 +534,6 @@ __device__ __forceinline__ void vector_dz(const GroupArgs& a, const Raw<K>& x, c
   for (int k = 0; k < V; ++k) dz[k] *= (float)dy.v[k];
 }
 
-// mean and rstd of a vector's channels, the first of which is the `in`th of group g;
-// row: those of the sample
-template <int MV>
-__device__ __forceinline__ void load_stats(int size, const float2* row, int g, int in,
-                                           float (&mean)[MV], float (&rstd)[MV]) {
-#pragma unroll
-  for (int k = 0; k < MV; ++k) {
-    const float2 r = row[g];
-    mean[k] = r.x;
-    rstd[k] = r.y;
-    if (++in == size && k + 1 < MV) {
-      in = 0;
-      ++g;
-    }
-  }
-}
-
 // part[block][channels]: sums of dz and dz xhat over the block's samples.
 template <class K, int R, int JOIN>
 __global__ __launch_bounds__(kMostThreads)
@@ -503,6 +558,7 @@ __global__ __launch_bounds__(kMostThreads)
   const int64_t off_x = at.offset(s, s.a.x_stride), off_d = at.offset(s, s.ldy),
                 off_o = at.offset(s, s.ldo);
   const int group = at.col / size, within = at.col - group * size;
+  const Entries<K, JOIN> e(s, size, at.slots);
   auto load = [&](int64_t batch, Rows& v) __attribute__((always_inline)) {
     const T* px = static_cast<const T*>(s.a.x) + batch_offset(s, batch, s.a.x_stride) + off_x;
     const T* pd = static_cast<const T*>(s.dy) + batch_offset(s, batch, s.ldy) + off_d;
@@ -581,45 +637,41 @@ __global__ __launch_bounds__(kMostThreads)
       t1[0] = lane_sum(t1[0], s.lanes);
       t2[0] = lane_sum(t2[0], s.lanes);
     } else {
-      const Entries<K, JOIN> e(s);
-      float2* sums = lds + (blockDim.x / s.cv) * e.width;
+      float2* sums = lds + e.all;
       if (at.active) {
-#pragma unroll
-        for (int k = 0; k < MV; ++k)
-          if (JOIN == VECTORS || k >= at.dup)
-            lds[at.slot * e.width + (JOIN == VECTORS ? at.vector : at.col + k)] = {t1[k], t2[k]};
+        if constexpr (JOIN == VECTORS) {
+          lds[threadIdx.x] = {t1[0], t2[0]};
+        } else {
+          float2 sum = {0.0f, 0.0f};
+          segments<V>(
+              size, within, at.dup,
+              [&](int k, int n) __attribute__((always_inline)) {
+                sum.x = n ? sum.x + t1[k] : t1[k];
+                sum.y = n ? sum.y + t2[k] : t2[k];
+              },
+              [&](int t) __attribute__((always_inline)) { lds[t * e.plane + threadIdx.x] = sum; });
+        }
       }
       __syncthreads();
       const int pairs = s.at_a_time * s.a.groups;
       const int lane = threadIdx.x & (s.lanes - 1);
       const int teams = blockDim.x / s.lanes;
-      const int all = at.slots * e.run;
       for (int p0 = 0; p0 < pairs; p0 += teams) {
         const int p = p0 + threadIdx.x / s.lanes;
         const int q = p / s.a.groups, g = p - q * s.a.groups;
-        const float2* from = lds + q * at.slots * e.width + g * e.run;
         float2 t = {0.0f, 0.0f};
-        if (p < pairs) {
-          for (int i = lane; i < all; i += s.lanes) {
-            const int slot = i / e.run;
-            const float2 v = from[slot * e.width + i - slot * e.run];
-            t.x += v.x;
-            t.y += v.y;
-          }
-        }
+        if (p < pairs)
+          e.each_of(s, lds + q * at.slots * s.cv, at.slots, lane, g,
+                    [&](float2 v, int, int) __attribute__((always_inline)) {
+                      t.x += v.x;
+                      t.y += v.y;
+                    });
         t.x = lane_sum(t.x, s.lanes);
         t.y = lane_sum(t.y, s.lanes);
         if (p < pairs && lane == 0) sums[p] = t;
       }
       __syncthreads();
-      if (at.active) {
-#pragma unroll
-        for (int k = 0; k < MV; ++k) {
-          const float2 r = sums[at.sample * s.a.groups + (at.col + k) / size];
-          t1[k] = r.x;
-          t2[k] = r.y;
-        }
-      }
+      if (at.active) load_stats(size, sums + at.sample * s.a.groups, group, within, t1, t2);
     }
     if (in) {
       T* po = static_cast<T*>(s.out) + batch_offset(s, batch, s.ldo) + off_o;
@@ -641,7 +693,7 @@ __global__ __launch_bounds__(kMostThreads)
         }
       }
     }
-    if constexpr (JOIN == CHANNELS || JOIN == VECTORS) __syncthreads();
+    if constexpr (JOIN == SEGMENTS || JOIN == VECTORS) __syncthreads();
   }
   if (s.part == nullptr) return;
   // the slots' sums of each channel
@@ -1009,7 +1061,7 @@ constexpr int64_t kStretches = 1024;    // workgroups of samples in stretches
 
 struct GroupCut {
   bool whole;  // samples in a workgroup's registers
-  int join = CHANNELS, r = 1, threads = 256;
+  int join = SEGMENTS, r = 1, threads = 256;
   size_t lds = 0;
 };
 
@@ -1104,13 +1156,22 @@ GroupCut cut_of(GroupKernel& s, bool back) {
     c.join = LANES;
     s.lanes = size / V;
   } else {
-    c.join = size % V == 0 || gb == 1 ? VECTORS : CHANNELS;
-    const int64_t slots = std::min<int64_t>(s.rows, L);
-    const int64_t entries = slots * (c.join == VECTORS ? ceil_div(size, V) : size);
+    c.join = size % V == 0 || gb == 1 ? VECTORS : SEGMENTS;
+    const int slots = (int)std::min<int64_t>(s.rows, L), run = vectors_of(c.join, V, size);
     const int64_t pairs = (int64_t)s.at_a_time * a.groups;
-    s.lanes = std::min({64, pow2_at_most(2 * entries - 1),
+    s.lanes = std::min({64, pow2_at_most(2 * (int64_t)slots * run - 1),
                         pow2_at_most(std::max<int64_t>(1, threads / pairs))});
-    c.lds = ((size_t)s.rows * s.cv * (c.join == VECTORS ? 1 : V) + (size_t)pairs) * sizeof(float2);
+    // the fewest rounds over a pair's entries
+    int fewest = 0;
+    for (int on = s.lanes; on >= 1; on /= 2) {
+      const int rounds = ceil_div(slots, s.lanes / on) * ceil_div(run, on);
+      if (fewest == 0 || rounds < fewest) {
+        fewest = rounds;
+        s.run_lanes = on;
+      }
+    }
+    const int each = c.join == VECTORS ? 1 : most_groups(V, size);
+    c.lds = ((size_t)plane_of(s.rows * s.cv) * each + (size_t)pairs) * sizeof(float2);
   }
   if (back) c.lds = std::max(c.lds, (size_t)s.rows * s.cv * V * sizeof(float2));
   return c;
@@ -1131,7 +1192,7 @@ void dispatch_whole(const GroupCut& c, F&& f) {
   using std::integral_constant;
   auto with = [&](auto r) {
     if constexpr (K::V > 1) {  // (of one channel a thread, channels are vectors)
-      if (c.join == CHANNELS) return f(r, integral_constant<int, CHANNELS>{});
+      if (c.join == SEGMENTS) return f(r, integral_constant<int, SEGMENTS>{});
     }
     f(r, integral_constant<int, VECTORS>{});
   };
