@@ -259,20 +259,21 @@ struct Entries {
     const int j0 = g * size / K::V;
     return j0 + (JOIN == VECTORS ? 0 : (g - j0 * K::V / size) * plane);
   }
-  // f(entry, its rows, its channels) of group g for a sample whose first slot is `first`,
+  // f(entry, its values) of group g for a sample whose first slot is `first`,
   // dealt out among the pair's lanes.
   template <class F>
   __device__ __forceinline__ void each_of(const GroupKernel& s, const float2* first, int slots,
                                           int lane, int g, F&& f) const {
     constexpr int V = K::V;
     const int c0 = g * size, j0 = c0 / V, at0 = first_of(g);
-    const int in0 = lane & (s.run_lanes - 1), rows = s.lanes / s.run_lanes;
-    for (int slot = lane / s.run_lanes; slot < slots; slot += rows) {
-      const int c = few + (slot < more);
-      for (int in = in0; in < run; in += s.run_lanes) {
-        const int v0 = (j0 + in) * V, n = min(v0 + V, c0 + size) - max(v0, c0);
-        if (n > 0) f(first[slot * s.cv + (in == 0 ? at0 : j0 + in)], c, n);
-      }
+    const int rows = s.lanes / s.run_lanes, slot0 = lane / s.run_lanes;
+    for (int in = lane & (s.run_lanes - 1); in < run; in += s.run_lanes) {
+      const int v0 = (j0 + in) * V, n = min(v0 + V, c0 + size) - max(v0, c0);
+      if (n <= 0) break;
+      const float2* from = first + (in == 0 ? at0 : j0 + in) + slot0 * s.cv;
+      const float less = (float)(few * n), greater = (float)((few + 1) * n);
+      for (int slot = slot0; slot < slots; slot += rows, from += rows * s.cv)
+        f(*from, slot < more ? greater : less);
     }
   }
 };
@@ -422,13 +423,17 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
             [&](int k, int n) __attribute__((always_inline)) {
               const float base = (float)x[0].v[k];
               float m = 0.0f, q = 0.0f;
+              if constexpr (R == 1) {
+                m = base;
+              } else {
 #pragma unroll
-              for (int r = 0; r < R; ++r) m += r < count ? (float)x[r].v[k] - base : 0.0f;
-              m = fmaf(m, share, base);
+                for (int r = 0; r < R; ++r) m += r < count ? (float)x[r].v[k] - base : 0.0f;
+                m = fmaf(m, share, base);
 #pragma unroll
-              for (int r = 0; r < R; ++r) {
-                const float d = r < count ? (float)x[r].v[k] - m : 0.0f;
-                q = fmaf(d, d, q);
+                for (int r = 0; r < R; ++r) {
+                  const float d = r < count ? (float)x[r].v[k] - m : 0.0f;
+                  q = fmaf(d, d, q);
+                }
               }
               const float part = __builtin_amdgcn_rcpf((float)(n + 1));
               const float d = n ? m - mean_of : 0.0f;
@@ -448,23 +453,33 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
         const bool has = p < pairs;
         const int q = p / s.a.groups, g = p - q * s.a.groups;
         const float2* from = lds + q * at.slots * s.cv;
-        auto sweep = [&](auto f) __attribute__((always_inline)) {
-          float t = 0.0f;
-          if (has)
-            e.each_of(s, from, at.slots, lane, g,
-                      [&](float2 v, int c, int n) __attribute__((always_inline)) {
-                        t += f(v, (float)(c * n));
-                      });
-          return lane_sum(t, s.lanes);
-        };
-        const float base = has ? from[e.first_of(g)].x : 0.0f;
-        const float m =
-            fmaf(sweep([&](float2 v, float c) { return (v.x - base) * c; }), s.inv_m, base);
-        const float var = sweep([&](float2 v, float c) {
-                            return fmaf(c * (v.x - m), v.x - m, v.y);
-                          }) * s.inv_m;
+        // a lane's entries from the mean of its first one, then the lanes'
+        float base = 0.0f, sum = 0.0f, sq = 0.0f, n = 0.0f;
+        if (has)
+          e.each_of(s, from, at.slots, lane, g, [&](float2 v, float c) __attribute__((always_inline)) {
+            base = n == 0.0f ? v.x : base;
+            const float d = v.x - base;
+            sum = fmaf(c, d, sum);
+            sq += fmaf(c * d, d, v.y);
+            n += c;
+          });
+        float m = 0.0f;
+        if (n > 0.0f) {
+          const float d = sum * __builtin_amdgcn_rcpf(n);
+          m = base + d;
+          sq = fmaf(-sum, d, sq);
+        }
+        for (int o = s.lanes >> 1; o >= 1; o >>= 1) {
+          const float n2 = __shfl_xor(n, o), m2 = __shfl_xor(m, o), sq2 = __shfl_xor(sq, o);
+          if (n == 0.0f) m = m2;
+          const float d = n2 == 0.0f ? 0.0f : m2 - m, part = n2 * __builtin_amdgcn_rcpf(n + n2);
+          if (n2 > 0.0f) m = fmaf(d, part, m);
+          sq += fmaf(d * d, n * (n2 > 0.0f ? part : 0.0f), sq2);
+          n += n2;
+        }
         if (has && lane == 0) {
-          const float2 r = {m, 1.0f / sqrtf(var + s.a.eps)};
+          // (below 0 by rounding; NaN stays)
+          const float2 r = {m, 1.0f / sqrtf(fmaf(sq < 0.0f ? 0.0f : sq, s.inv_m, s.a.eps))};
           group[p] = r;
           const int64_t to = batch * s.at_a_time + q;
           if (s.stats && to < s.a.samples) s.stats[to * s.all_groups + g] = r;
@@ -662,7 +677,7 @@ __global__ __launch_bounds__(kMostThreads)
         float2 t = {0.0f, 0.0f};
         if (p < pairs)
           e.each_of(s, lds + q * at.slots * s.cv, at.slots, lane, g,
-                    [&](float2 v, int, int) __attribute__((always_inline)) {
+                    [&](float2 v, float) __attribute__((always_inline)) {
                       t.x += v.x;
                       t.y += v.y;
                     });
