@@ -116,9 +116,9 @@ struct GroupKernel {
   float2* coef;    // [samples][groups]: the two group sums over m
   float inv_m;     // 1 / m
   bool apart;      // the result shares no memory with what is read
-  // in registers: vectors of a row, rows at a time, samples at a time, threads a
-  // group (its sums), and of them on the entries of one row
-  int cv, rows, at_a_time, lanes, run_lanes;
+  // in registers: vectors of a row, rows of a sample at a time, samples at a time, threads
+  // a group (its sums), and of them on the entries of one row
+  int cv, slots, at_a_time, lanes, run_lanes;
   int64_t batches;
   // blocks of groups a sample is dealt out in, one a workgroup; in the kernels a.groups
   // and a.channels are a block's, and these a sample's
@@ -192,7 +192,7 @@ struct Place : Columns<K> {
   __device__ __forceinline__ explicit Place(const GroupKernel& s)
       : Columns<K>(s, 0, (int)threadIdx.x - (int)threadIdx.x / s.cv * s.cv) {
     slot = threadIdx.x / s.cv;
-    slots = min(s.rows, (int)min(s.a.positions, (int64_t)1 << 30));
+    slots = s.slots;
     sample = slot / slots;
     row = slot - sample * slots;
     active = sample < s.at_a_time;
@@ -249,7 +249,7 @@ struct Entries {
   int few, more;  // rows of a slot: one more than few in the first `more` slots
   __device__ __forceinline__ Entries(const GroupKernel& s, int size_, int slots) : size(size_) {
     run = vectors_of(JOIN, K::V, size);
-    plane = plane_of(s.rows * s.cv);
+    plane = plane_of(slots * s.at_a_time * s.cv);
     all = plane * (JOIN == VECTORS ? 1 : most_groups(K::V, size));
     few = (int)s.a.positions / slots;
     more = (int)s.a.positions - few * slots;
@@ -396,24 +396,31 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
       if (JOIN == VECTORS) {
         const float base = (float)x[0].v[V - 1];
         float m = 0.0f, q = 0.0f;
+        auto moments = [&](auto odd) __attribute__((always_inline)) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          if (r < count) {
+          for (int r = 0; r < R; ++r) {
+            if (r < count) {
 #pragma unroll
-            for (int k = 0; k < V; ++k) m += k >= at.dup ? (float)x[r].v[k] - base : 0.0f;
-          }
-        }
-        m = base + (count ? m / (float)(count * (V - at.dup)) : 0.0f);
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          if (r < count) {
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-              const float d = k >= at.dup ? (float)x[r].v[k] - m : 0.0f;
-              q = fmaf(d, d, q);
+              for (int k = 0; k < V; ++k)
+                m += !odd.value || k >= at.dup ? (float)x[r].v[k] - base : 0.0f;
             }
           }
-        }
+          m = base + (count ? m / (float)(count * (V - at.dup)) : 0.0f);
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            if (r < count) {
+#pragma unroll
+              for (int k = 0; k < V; ++k) {
+                const float d = !odd.value || k >= at.dup ? (float)x[r].v[k] - m : 0.0f;
+                q = fmaf(d, d, q);
+              }
+            }
+          }
+        };
+        if (s.a.channels % V == 0)  // no vector shares channels
+          moments(std::false_type{});
+        else
+          moments(std::true_type{});
         if (at.active) lds[threadIdx.x] = {m, q};
       } else if (at.active) {
         const float share = count ? 1.0f / (float)count : 0.0f;
@@ -491,13 +498,15 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
     }
     if (in) {
       T* py = static_cast<T*>(s.out) + batch_offset(s, batch, s.ldo) + off_y;
+      float wr[V];
+#pragma unroll
+      for (int k = 0; k < V; ++k) wr[k] = w[k] * rstd[k % MV];
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         if (r < count) {
           float z[V];
 #pragma unroll
-          for (int k = 0; k < V; ++k)
-            z[k] = fmaf(((float)x[r].v[k] - mean[k % MV]) * rstd[k % MV], w[k], b[k]);
+          for (int k = 0; k < V; ++k) z[k] = fmaf((float)x[r].v[k] - mean[k % MV], wr[k], b[k]);
           act_values<K>(s.a.activation, z);
           store_raw<K>(py + (int64_t)r * at.slots * s.ldo, at.from, z);
         }
@@ -1157,12 +1166,14 @@ GroupCut cut_of(GroupKernel& s, bool back) {
   const int64_t cv = ceil_div((int64_t)a.channels, (int64_t)V);
   const int threads = threads_of(cv, L, most);
   s.cv = (int)cv;
-  s.rows = threads / s.cv;
-  c.threads = threads;
-  s.at_a_time = s.group_blocks > 1 ? 1 : (int)std::max<int64_t>(1, s.rows / L);
+  // as many rows a thread in every slot, and no waves without rows
+  const int64_t r = ceil_div(L, (int64_t)(threads / s.cv));
+  s.slots = (int)ceil_div(L, r);
+  s.at_a_time = s.group_blocks > 1 ? 1 : threads / s.cv / s.slots;
   s.batches = ceil_div(a.samples, (int64_t)s.at_a_time);
-  const int64_t r = ceil_div(L, (int64_t)s.rows);
-  c.r = r <= 1 ? 1 : r <= 4 ? 4 : r <= 8 ? 8 : 16;
+  const int slots = s.slots, taken = slots * s.at_a_time;
+  c.threads = (int)round_up(taken * s.cv, 64);
+  c.r = r <= 1 ? 1 : r <= 2 ? 2 : r <= 4 ? 4 : r <= 8 ? 8 : 16;
   const bool pow2 = (size & (size - 1)) == 0;
   if (L == 1 && pow2 && size < V) {
     c.join = THREAD;
@@ -1172,10 +1183,10 @@ GroupCut cut_of(GroupKernel& s, bool back) {
     s.lanes = size / V;
   } else {
     c.join = size % V == 0 || gb == 1 ? VECTORS : SEGMENTS;
-    const int slots = (int)std::min<int64_t>(s.rows, L), run = vectors_of(c.join, V, size);
+    const int run = vectors_of(c.join, V, size);
     const int64_t pairs = (int64_t)s.at_a_time * a.groups;
     s.lanes = std::min({64, pow2_at_most(2 * (int64_t)slots * run - 1),
-                        pow2_at_most(std::max<int64_t>(1, threads / pairs))});
+                        pow2_at_most(std::max<int64_t>(1, c.threads / pairs))});
     // the fewest rounds over a pair's entries
     int fewest = 0;
     for (int on = s.lanes; on >= 1; on /= 2) {
@@ -1186,9 +1197,9 @@ GroupCut cut_of(GroupKernel& s, bool back) {
       }
     }
     const int each = c.join == VECTORS ? 1 : most_groups(V, size);
-    c.lds = ((size_t)plane_of(s.rows * s.cv) * each + (size_t)pairs) * sizeof(float2);
+    c.lds = ((size_t)plane_of(taken * s.cv) * each + (size_t)pairs) * sizeof(float2);
   }
-  if (back) c.lds = std::max(c.lds, (size_t)s.rows * s.cv * V * sizeof(float2));
+  if (back) c.lds = std::max(c.lds, (size_t)taken * s.cv * V * sizeof(float2));
   return c;
 }
 
@@ -1216,6 +1227,7 @@ void dispatch_whole(const GroupCut& c, F&& f) {
   }
   if (c.join == LANES) return f(integral_constant<int, 1>{}, integral_constant<int, LANES>{});
   if (c.r == 1) return with(integral_constant<int, 1>{});
+  if (c.r == 2) return with(integral_constant<int, 2>{});
   if (c.r == 4) return with(integral_constant<int, 4>{});
   if (c.r == 8) return with(integral_constant<int, 8>{});
   if constexpr (!BACK) with(integral_constant<int, 16>{});
