@@ -14,6 +14,7 @@ asynchronously on the current stream and can be recorded into a graph.
 
 from __future__ import annotations
 
+import array
 import ctypes as C
 import math
 import numbers
@@ -142,7 +143,7 @@ class AdamW:
         out, index = [], self._index  # one by one: None among them, or one to be named
         for i, (g, shape) in enumerate(zip(grads, self._shapes)):
             if g is None:
-                out.append(None)
+                out.append(0)
                 continue
             if getattr(g, "dtype", None) is not dtype or g.shape != shape or g.requires_grad \
                     or not g.is_contiguous() or g.get_device() != index:
@@ -182,7 +183,7 @@ class AdamW:
         if torch.is_grad_enabled():
             if any(map(_required, self.params)):
                 _no_graph(f"params[{list(map(_required, self.params)).index(True)}]")
-        if [p.data_ptr() for p in self.params] != self._addresses:
+        if list(map(torch.Tensor.data_ptr, self.params)) != self._addresses:
             raise ValueError("the parameters' memory is no longer where it was when the optimizer "
                              "was made")
         grads = list(grads)
@@ -192,9 +193,9 @@ class AdamW:
         if dtype is not self._dtype and dtype is not torch.float32:
             raise TypeError(f"gradients must be of the parameters' type ({self._dtype}) or "
                             f"float32, got {dtype}")
-        pointers = (C.c_void_p * len(grads))(*self._addresses_of(grads, dtype))
-        s = _lib.AdamWStep(grads=pointers, grad_type=_types[dtype], grad_scale=grad_scale,
-                           max_norm=math.inf)
+        pointers = array.array("Q", self._addresses_of(grads, dtype))
+        s = _lib.AdamWStep(grads=C.cast(pointers.buffer_info()[0], _lib.c_void_pp),
+                           grad_type=_types[dtype], grad_scale=grad_scale, max_norm=math.inf)
         if isinstance(step, numbers.Integral) and not isinstance(step, bool):
             if not 1 <= step < 1 << 53:
                 raise ValueError(f"step must be at least 1, got {step}")
