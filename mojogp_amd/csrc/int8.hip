@@ -10,10 +10,11 @@
 // low byte then holds.
 //
 // Matrix-core bound, at up to twice the 16-bit rate; rows are quantised by one pass
-// of their own before the product.  Few
-// rows (k_int8_few) are bound by reading the weights once, at half the bytes of
+// of their own before the product.  65536 x 1024 -> 2 x 4096 bf16: codes 40 us, product 670
+// (1640 TOPS; of it matrix instructions alone 403, waiting for loads 120, a tile's end 150).
+// Few rows (k_int8_few) are bound by reading the weights once, at half the bytes of
 // 16-bit ones, and by latency: up to 16 rows each workgroup quantises what it needs
-// itself, in the one launch.
+// itself, in the one launch (1 x 512 -> 2 x 2048 bf16 4.7 us).
 #include <algorithm>
 #include <type_traits>
 
@@ -619,8 +620,15 @@ void launch_quantize(const T* x, int64_t ldx, int64_t rows, int64_t width, int8_
 
 enum Way : int { FUSED_ROWS, FEW_ROWS, TILES };
 
+// Up to 16 rows in the one launch where it costs each round of 256 workgroups less to
+// quantise them than a second launch takes: 1 x 512 -> 2 x 2048 bf16 4.0 us (with codes
+// of their own 6.0), 16 x 512 5.7 (6.4), but 16 x 1024 8.5 (6.7), 16 x 4096 27.6 (11.8), 4 x
+// 2048 8.7 (7.6), 1 x 2048 6.9 (7.2), 1 x 4096 13.6 (10.3); to 2 x 16384, 1 x 512 7.6 (8.8),
+// 16 x 256 9.0 (8.1).  More rows by few up to 512 workgroups: 128 x 1024 -> 4096 10.1 us
+// (tiles 11.3), 192 x 1024 -> 4096 12.6 (11.5), 500 x 64 -> 512 6.1 (7.9).
 inline Way way_of(const Int8Args& a) {
-  if (a.rows <= 16) return FUSED_ROWS;
+  if (a.rows <= 16 && (a.rows + 4) * a.width * ceil_div(a.hidden, (int64_t)4096) <= 12288)
+    return FUSED_ROWS;
   return ceil_div(a.rows, (int64_t)64) * ceil_div(a.hidden, (int64_t)16) <= 512 ? FEW_ROWS : TILES;
 }
 

@@ -202,3 +202,24 @@ def test_refusals():
             (lambda: features.int8_layer(x.clone().requires_grad_(), w), ValueError, "gradient")):
         with pytest.raises(err, match=what):
             call()
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("rows, width, hidden", [(1, 2453, 17), (1, 2470, 17), (4, 1500, 4097),
+                                                 (16, 614, 40), (16, 615, 40), (7, 4001, 33),
+                                                 (5, 700, 9001), (16, 130, 8200)])
+def test_few_wide_rows(kind, rows, width, hidden):
+    """Up to 16 rows in one launch, with codes of their own before it, and in tiles."""
+    rng = np.random.default_rng(width)
+    x = _dev(rng.normal(size=(rows, width)), kind, 1)
+    wg, wu = (_dev(rng.normal(size=(hidden, width)) / np.sqrt(width), kind) for _ in range(2))
+    b = _dev(0.3 * rng.normal(size=hidden), kind)
+    qg, qu = features.int8_weights(wg), features.int8_weights(wu)
+    for up, act in ((None, None), (qu, "silu")):
+        if up is None:
+            y = features.int8_layer(x, qg, b)
+            want, _ = ol.int8_layer(_host(x), _host(wg), _host(b))
+        else:
+            y = features.int8_gated_layer(x, qg, up, b, activation=act)
+            want, _ = ol.int8_layer(_host(x), _host(wg), _host(b), _host(wu), None, act)
+        assert np.linalg.norm(_host(y) - want) <= (UNIT[kind] + F32) * np.linalg.norm(want)
