@@ -2,8 +2,8 @@
 
 Python + NumPy host surface over hand-written HIP kernels reached through the
 C-ABI library libmojogp_amd.so (ctypes).  Nothing here imports torch;
-mojogp_amd.features (layers that learn a GP's inputs) works on the torch device
-tensors that its caller brings.
+mojogp_amd.features (layers that learn a GP's inputs) and mojogp_amd.optim (the step
+that trains them) work on the torch device tensors that their caller brings.
 
     from mojogp_amd import SingleOutputGP, MultiOutputGP, MultiOutputLMCGP, RBF, Matern52
 """

@@ -14,6 +14,12 @@
 // Larger samples go in stretches of rows (k_group_part, k_group_merge,
 // k_group_apply), which read them twice.  Statistics are fp32 means and centred
 // squares, merged by counts: a level far above the spread costs no digits.
+//
+// Measured: 250000 x 1 x 256 bf16 by 8 channels, silu, forward 72 us, backward 96 (4.4 and 4.6
+// TB/s with the statistics); 32 x 4096 x 512 bf16 in stretches, forward 38 + 53 us,
+// backward 52 + 76 (3.6 to 7 TB/s, the second reads partly from the last-level cache).
+// Samples in registers wait on VALU too: 3000 x 64 x 512 bf16 by 16 channels, forward 111 us
+// (3.5 TB/s), backward 255.
 #include <algorithm>
 #include <type_traits>
 

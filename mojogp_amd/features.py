@@ -5,7 +5,9 @@
     z = dropout(y, 0.1, seed, offset=step * y.numel())
 
 and their gradients (``gated_layer_backward``, ``layer_norm_backward``,
-``dropout_backward``).  The gradient that enters at the top is
+``dropout_backward``); ``group_norm`` with its activation for features that have
+positions, and ``group_norm_backward``; for serving what was trained, layers whose
+weights are 8-bit integers (``int8_weights``, ``int8_layer``, ``int8_gated_layer``).  The gradient that enters at the top is
 ``NativeProvider.input_gradient_device``: that of the marginal likelihood with
 respect to the kernel's points.
 
