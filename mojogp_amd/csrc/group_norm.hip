@@ -246,9 +246,11 @@ __host__ __device__ constexpr int vectors_of(int join, int V, int size) {
 
 // The entries in LDS: `each` for a vector of a slot (of the groups from that of the
 // vector's own first channel on), `plane` apart, so that neighbouring threads write
-// neighbouring ones.  (Planes are 64 bytes off each other's banks: neighbouring groups
-// are read together.)
-__host__ __device__ constexpr int plane_of(int threads) { return (threads + 31) / 32 * 32 + 8; }
+// neighbouring ones.  (Planes are 64 bytes off each other's banks, as neighbouring groups
+// are read together, but for the widest, which fill 64 KB with the groups' results.)
+__host__ __device__ constexpr int plane_of(int threads) {
+  return (threads + 31) / 32 * 32 + (threads <= 256 ? 8 : 0);
+}
 template <class K, int JOIN>
 struct Entries {
   int size, run, plane, all;

@@ -97,6 +97,22 @@ def test_group_norm(kind, n, l, c, groups, pad):
 
 
 @pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("n, l, c, groups, pad", [
+    # a group a channel, to the most that a workgroup holds
+    (300, 5, 4096, 4096, 0), (260, 2, 4090, 4090, 0), (70, 12, 100, 100, 0), (50, 28, 14, 14, 0),
+    # groups that cut vectors, in slots of one row and of several
+    (400, 34, 60, 5, 0), (20, 60, 300, 25, 0), (9, 100, 96, 8, 3), (30, 11, 54, 18, 1),
+    (33, 8, 1001, 7, 0),
+])
+def test_groups_that_cut_vectors(kind, n, l, c, groups, pad):
+    rng = np.random.default_rng(n + l + c)
+    x = rng.normal(size=(n, l, c)) * rng.uniform(0.5, 2, (n, 1, 1)) + rng.normal(size=(n, 1, c))
+    x = _dev(x, kind, pad, min(pad, 1))
+    w, b = _dev(1 + 0.2 * rng.normal(size=c), kind), _dev(0.3 * rng.normal(size=c), kind)
+    _check(x, _dev(rng.normal(size=(n, l, c)), kind, pad), groups, w, b, ACTS[(n + c) % 4], kind)
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("shape", [(40, 1, 64), (6, 30, 48), (2, 2500, 24)])
 def test_activations(kind, act, shape):
