@@ -283,13 +283,6 @@ def _rounded(x, draw, lowest, most):
     return torch.where(x < 2.0 ** lowest, small, normal).clamp_max(most)
 
 
-def _scale(x, top):
-    """The scale of each block, largest / top, and the factor into its units, both
-    in 32 bits from the largest value in 32 bits."""
-    most = x.amax(1, keepdim=True).float()
-    return most * (1.0 / top), torch.where(most > 0, top / most.double(), 0.0).float().double()
-
-
 def _decoded(s, key):
     """The values of 8-bit states, in 64 bits."""
     code = s[key].view(-1, BLOCK)
@@ -331,12 +324,13 @@ def _adamw_plain(s, case):
         out["exp_avg_sq"] = s["exp_avg_sq"].copy_(v.view(-1))
         return out
     word = _words(s["seed"], s["step"], m.numel()).view(-1, BLOCK)
-    ms, by = _scale(m.abs(), 448.0)
-    code = _rounded(m.abs() * by, word & 0xFFFF, -6, 126)
-    s["exp_avg"].copy_(torch.where(m < 0, code + 128, code).view(-1))
-    vs, by = _scale(v, 1.875)
-    code = _rounded(v * by, word >> 16, -30, 255)
-    s["exp_avg_sq"].copy_(torch.where(v * by > 0, code.clamp_min(1), 0).view(-1))
+    ms = (m.abs().amax(1, keepdim=True) / 448).float()
+    vs = (v.amax(1, keepdim=True) / 1.875).float()
+    code = _rounded(torch.where(ms > 0, m.abs() / ms.double(), 0.0), word & 0xFFFF, -6, 126)
+    code = torch.where(m < 0, code + 128, code)
+    s["exp_avg"].copy_(code.view(-1))
+    code = _rounded(torch.where(vs > 0, v / vs.double(), 0.0), word >> 16, -30, 255)
+    s["exp_avg_sq"].copy_(torch.where((v > 0) & (vs > 0), code.clamp_min(1), 0).view(-1))
     s["exp_avg_scale"].copy_(ms.view(-1))
     s["exp_avg_sq_scale"].copy_(vs.view(-1))
     out["exp_avg"] = _decoded(s, "exp_avg").float().view(-1)
@@ -481,18 +475,12 @@ def _exact_codes(x, share, lowest, top):
     return torch.clamp(torch.floor(x / step + share) * step, max=top)
 
 
-def _exact_scale(x, top):
-    most = torch.linalg.vector_norm(x, ord=math.inf, dim=1, keepdim=True).float().double()
-    share = torch.tensor(1.0 / top, dtype=torch.float32).item()
-    by = torch.nan_to_num(top / most, posinf=0.0).float().double()
-    return (most * share).float().double(), by
-
-
 def _exact_states(s, m, v):
     um, uv = (u.view(-1, BLOCK) for u in _exact_uniform(s["seed"], s["step"], m.numel()))
-    (ms, bm), (vs, bv) = (_exact_scale(t.abs(), top) for t, top in ((m, 448.0), (v, 1.875)))
-    x = _exact_codes(m.abs() * bm, um, -6, 448.0)
-    y = _exact_codes(v * bv, uv, -30, 1.875)
+    ms = (m.abs().amax(1, keepdim=True) / 448).float().double()
+    vs = (v.amax(1, keepdim=True) / 1.875).float().double()
+    x = _exact_codes(torch.nan_to_num(m.abs() / ms), um, -6, 448.0)
+    y = _exact_codes(torch.nan_to_num(v / vs), uv, -30, 1.875)
     y = torch.where(v > 0, y.clamp_min(2.0 ** -33), 0.0)
     return torch.sign(m) * x * ms, y * vs
 
