@@ -896,14 +896,16 @@ MGP_API int mgp_int8_layer_device(const mgp_int8_layer_t* args, void* y, int64_t
  * each tensor's from a multiple of 256 on; what lies behind a tensor's last value
  * stays unread.
  * 32-bit states: exp_avg, exp_avg_sq are float.  8-bit states: bytes, with one float
- * scale for 256 values.  exp_avg: an OCP e4m3 value times its scale (largest |m| *
- * (1/448)).  exp_avg_sq: exponent e (5 bits) and mantissa f (3 bits), (1 + f/8)
- * 2^(e-31) or, for e = 0, f/8 2^-30, times its scale (largest v * (1/1.875)).  Value i
+ * scale for 256 values.  exp_avg: an OCP e4m3 value times its scale (largest |m| /
+ * 448).  exp_avg_sq: exponent e (5 bits) and mantissa f (3 bits), (1 + f/8)
+ * 2^(e-31) or, for e = 0, f/8 2^-30, times its scale (largest v / 1.875).  Means and
+ * quotients are formed in 64 bits; a scale is rounded once, to fp32, and a value's code
+ * is that of the value over that scale.  Value i
  * is rounded by word i % 4 of the Philox4x32-10 block of counter (i / 4, t) and key
- * seed, its low half for m, its high half for v: in units of a code's step, the value
+ * seed, its low half for m, its high half for v: in units of a code's step, the quotient
  * plus (half + 1/2) / 2^16 is cut off.  A v above 0 has code 1 at least.  Blocks
- * whose largest value is below 2^-120 become 0; an infinity or NaN makes NaN of its
- * block's state. */
+ * whose largest value is below 2^-120 become 0; an infinity or NaN, or a scale that is
+ * not in fp32, makes NaN of its block's state. */
 typedef struct mgp_adamw_tensor {
   void* param;
   int64_t size;

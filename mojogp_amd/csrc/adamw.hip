@@ -196,26 +196,58 @@ __device__ __forceinline__ uint32_t wave_largest(uint32_t u) {
   return (uint32_t)__builtin_amdgcn_readlane((int)u, 63);
 }
 
-// The scale of a block and the factor of its values, from the largest of them.
-// Blocks that end below 2^-120 (whose factor would pass fp32) are held as zeros.
-struct Scale {
-  float scale, by;
-};
-__device__ __forceinline__ Scale scale_of(uint32_t largest, float top, float inv_top) {
-  const float a = __uint_as_float(largest);
-  const bool none = largest < 0x03800000u;  // 2^-120
-  return {none ? 0.0f : a * inv_top, none ? 0.0f : top / a};
+// A block's scale is the fp32 rounding of the 64-bit quotient largest / top, and a code is
+// decided by the 64-bit quotient of a value and that scale.  A 32-bit factor in the place
+// of either quotient makes another last place of half the scales and moves a code in two
+// million by a step.
+
+// largest / top in fp32, of the largest of a lane's values: the lanes' largest is the
+// block's, as roundings keep the order.  The quotient in 64 bits is that of a division (by
+// 7 or 15 times a power of two no quotient lies near enough to a tie for the correction
+// to miss it).  Blocks that end below 2^-120 are held as zeros.
+__device__ __forceinline__ float scale_from(double largest, double top) {
+  const double inv = 1.0 / top;
+  double q = largest * inv;
+  q = fma(fma(-q, top, largest), inv, q);
+  return largest < 0x1p-120 ? 0.0f : (float)q;
 }
 
-// b x + r y, every operation rounded: a scale is the fp32 rounding of the largest of
-// these, and sums of 8-bit gradients and means come to lie on its ties, where a
-// fused addition would make another scale of some than the formula does.
+// A block's scale from its lanes'; one that is not in fp32 is NaN.
+__device__ __forceinline__ float wave_scale(float lane_scale) {
+  const uint32_t u = wave_largest(__float_as_uint(lane_scale) & 0x7fffffffu);
+  return __uint_as_float(u < 0x7f800000u ? u : 0x7fc00000u);
+}
+
+// x / scale in 64 bits; inv is the reciprocal to within a few last places.  (No quotient of
+// 53 by 24 bits lies within 2^-24 of a last place from a tie.)
+__device__ __forceinline__ double over(double x, double scale, double inv) {
+  const double q = x * inv;
+  return fma(fma(-q, scale, x), inv, q);
+}
+
+// 1 / x by the approximation of v_rcp_f64, squared away twice.
+__device__ __forceinline__ double reciprocal(double x) {
+  double r = __builtin_amdgcn_rcp(x);
+  r = fma(fma(-x, r, 1.0), r, r);
+  return fma(fma(-x, r, 1.0), r, r);
+}
+
+__device__ __forceinline__ double lane_value(double x, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// b x + r y, every operation rounded: sums of 8-bit gradients and means come to lie on
+// the ties of their scales' roundings, where a fused addition would make another scale of
+// some than the formula does.
 __device__ __forceinline__ double mean_of(double b, double x, double r, double y) {
 #pragma clang fp contract(off)
   return b * x + r * y;
 }
 
-constexpr float kTopM = 448.0f, kTopV = 1.875f;
+constexpr double kTopM = 448.0, kTopV = 1.875;
 
 __device__ __forceinline__ float value_m(uint32_t codes, int k) {
   return k == 0   ? __builtin_amdgcn_cvt_f32_fp8(codes, 0)
@@ -300,7 +332,6 @@ __device__ __forceinline__ void step_chunk(const ChunkAt<P, G>& c, const StepArg
     float m[4], v[4];
     if constexpr (EIGHT) {
       double md[4], vd[4];
-      uint32_t mu = 0, vu = 0;
       double gd[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) gd[k] = (double)(float)gr[u].v[k];
@@ -315,28 +346,34 @@ __device__ __forceinline__ void step_chunk(const ChunkAt<P, G>& c, const StepArg
         if (!FULL && k >= left) md[k] = vd[k] = 0.0;
         m[k] = (float)md[k];
         v[k] = (float)vd[k];
-        mu = max(mu, __float_as_uint(m[k]) & 0x7fffffffu);
-        vu = max(vu, __float_as_uint(v[k]) & 0x7fffffffu);
       }
-      const Scale sm = scale_of(wave_largest(mu), kTopM, 1.0f / kTopM);
-      const Scale sv = scale_of(wave_largest(vu), kTopV, 1.0f / kTopV);
+      // the largest; and what is not finite, which a maximum may pass over, by a sum
+      const double lm = fmax(fmax(fabs(md[0]), fabs(md[1])), fmax(fabs(md[2]), fabs(md[3])));
+      const double lv = fmax(fmax(vd[0], vd[1]), fmax(vd[2], vd[3]));
+      const double am = (md[0] + md[1]) + (md[2] + md[3]), av = (vd[0] + vd[1]) + (vd[2] + vd[3]);
+      const float qm = scale_from(fma(am, 0.0, lm), kTopM), qv = scale_from(fma(av, 0.0, lv), kTopV);
+      const float sm = wave_scale(qm), sv = wave_scale(qv);
+      // both reciprocals at once, m's by the first 32 lanes; of a block of zeros, what is
+      // left over a scale of one is below every draw's border
+      const float sm1 = sm > 0.0f ? sm : 1.0f, sv1 = sv > 0.0f ? sv : 1.0f;
+      const double inv = reciprocal((double)(lane < 32 ? sm1 : sv1));
+      const double im = lane_value(inv, 0), iv = lane_value(inv, 63);
+      const int least = sv > 0.0f ? 1 : 0;  // of a v above zero
       const Draws dr = philox((uint64_t)(c.first + i) >> 2, a.seed, t);
       uint32_t cm = 0, cv = 0;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int x = code_of<-6>(fabs(md[k]) * (double)sm.by, (dr.w[k] & 0xffffu) << 1, 126);
+        const int x = code_of<-6>(over(fabs(md[k]), (double)sm1, im), (dr.w[k] & 0xffffu) << 1, 126);
         const uint32_t sign = (uint32_t)(__double_as_longlong(md[k]) >> 56) & 128u;
-        const double y = vd[k] * (double)sv.by;
-        // (the high word of a value that is not 0 is not)
-        const int some = (int)min((uint32_t)(__double_as_longlong(y) >> 32), 1u);
+        const int y = code_of<-30>(over(vd[k], (double)sv1, iv), dr.w[k] >> 16 << 1, 255);
         cm |= ((uint32_t)x | sign) << (8 * k);
-        cv |= (uint32_t)max(code_of<-30>(y, dr.w[k] >> 16 << 1, 255), some) << (8 * k);
+        cv |= (uint32_t)max(y, vd[k] > 0.0 ? least : 0) << (8 * k);
       }
       *reinterpret_cast<uint32_t*>(c.mc + i) = cm;
       *reinterpret_cast<uint32_t*>(c.vc + i) = cv;
       if (lane == 0) {
-        c.ms[i0 >> 8] = sm.scale;
-        c.vs[i0 >> 8] = sv.scale;
+        c.ms[i0 >> 8] = sm;
+        c.vs[i0 >> 8] = sv;
       }
     } else {
       const float b1 = (float)a.b1, b2 = (float)a.b2;

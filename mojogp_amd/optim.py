@@ -42,9 +42,10 @@ class AdamW:
     ``bits=8`` holds the running means as 8-bit floats with a float32 scale for each
     256 values of a parameter (2.03 bytes a value instead of 8), rounded up or down by
     draws that are functions of ``seed``, the step and the value's place alone.  The
-    update itself is formed before the rounding.  A gradient that is not finite, or whose
-    square is not in float32, makes NaN of the states of its scale's 256 values, where
-    ``step`` forms no norm that catches it.
+    update itself is formed before the rounding.  A gradient that is not finite makes
+    NaN of the states of its scale's 256 values, and one whose square passes float32 (by
+    about a thousandfold at the default betas) of their second means, where ``step``
+    forms no norm that catches it.
 
     exp_avg, exp_avg_sq (float32, or codes with exp_avg_scale and exp_avg_sq_scale) and
     master are flat arrays in which each parameter's values start at the next multiple

@@ -5,8 +5,6 @@ from __future__ import annotations
 
 import numpy as np
 
-from .layers import philox
-
 BLOCK = 256
 TOP_M, TOP_V = 448.0, 1.875
 
@@ -33,20 +31,30 @@ def decode(codes, scale, signed):
 
 def words(seed, step, count):
     """A 32-bit word for each value: word i % 4 of the block with counter (i / 4, step)."""
-    out = [philox(b | (step << 64), seed) for b in range((count + 3) // 4)]
-    return np.array(out, np.int64).ravel()[:count]
+    low = np.uint64(0xFFFFFFFF)
+    half = np.uint64(32)
+    block = np.arange((count + 3) // 4, dtype=np.uint64)
+    c = [block & low, block >> half, np.full_like(block, step & 0xFFFFFFFF),
+         np.full_like(block, step >> 32)]
+    k = [seed & 0xFFFFFFFF, seed >> 32]
+    for _ in range(10):
+        p0, p1 = c[0] * np.uint64(0xD2511F53), c[2] * np.uint64(0xCD9E8D57)
+        c = [(p1 >> half) ^ c[1] ^ np.uint64(k[0]), p1 & low,
+             (p0 >> half) ^ c[3] ^ np.uint64(k[1]), p0 & low]
+        k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+    return np.stack(c, axis=1).astype(np.int64).ravel()[:count]
 
 
 def encode(x, draws, signed):
-    """(codes, scales) of values in blocks: a value goes to the neighbour above with the
+    """(codes, scales) of values in blocks.  A block's scale is its largest value over the
+    format's, rounded once; a value over the scale goes to the neighbour above with the
     probability of its way there."""
     x = np.asarray(x, np.float64).reshape(-1, BLOCK)
     values, top = (TABLE_M, TOP_M) if signed else (TABLE_V, TOP_V)
-    most = np.abs(x).max(axis=1).astype(np.float32)
-    some = most >= np.float32(2.0 ** -120)
-    scale = np.where(some, most * np.float32(1.0 / top), np.float32(0))
-    by = np.where(some, (top / np.where(some, most, 1).astype(np.float64)), 0).astype(np.float32)
-    a = np.abs(x) * by.astype(np.float64)[:, None]
+    most = np.abs(x).max(axis=1)
+    scale = np.where(most >= 2.0 ** -120, most / top, 0.0).astype(np.float32)
+    some = scale > 0
+    a = np.where(some[:, None], np.abs(x) / np.where(some, scale, 1).astype(np.float64)[:, None], 0.0)
     below = np.clip(np.searchsorted(values, a, side="right") - 1, 0, len(values) - 1)
     above = np.minimum(below + 1, len(values) - 1)
     gap = np.where(above > below, values[above] - values[below], 1.0)
@@ -55,7 +63,7 @@ def encode(x, draws, signed):
     if signed:
         code = code | np.where(x < 0, 128, 0)
     else:
-        code = np.where(a > 0, np.maximum(code, 1), code)
+        code = np.where((x > 0) & some[:, None], np.maximum(code, 1), code)
     return code.ravel(), scale
 
 
