@@ -940,8 +940,9 @@ MGP_API int mgp_adamw_destroy(void* plan);
  * float32 (grad_type); tensors whose entry is NULL are left as they are.  form_norm:
  * the norm is formed and written to norm (may be NULL), gradients are scaled down to
  * max_norm (infinity: they are not), and nothing is changed where it is not finite in
- * float; nor is it where step_device holds less than 1, or rate_device a rate that is
- * negative or not finite. */
+ * float; without it max_norm and norm are not used.  Nor is anything changed where
+ * step_device holds less than 1, or rate_device a rate that is negative or not
+ * finite. */
 typedef struct mgp_adamw_step {
   const void* const* grads;
   int grad_type;

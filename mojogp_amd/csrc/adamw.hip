@@ -124,7 +124,7 @@ __global__ __launch_bounds__(256) void k_adamw_norm(Grads grads,
 
 struct ScalarArgs {
   const double* part;
-  int parts;  // 0: no norm
+  int parts;  // 0: no norm, and its fields are not read
   double grad_scale, max_norm;
   float* norm_out;
   double beta1, beta2;
@@ -145,9 +145,12 @@ __global__ __launch_bounds__(256) void k_adamw_scalars(ScalarArgs a) {
   __syncthreads();
   if (threadIdx.x != 0) return;
   Scalars r = a.host;
-  const double norm = sqrt(red[0] + red[1] + red[2] + red[3]) * fabs(a.grad_scale);
-  r.factor = a.grad_scale * (norm > a.max_norm ? a.max_norm / norm : 1.0);
-  r.skip = !((float)norm < HUGE_VALF);
+  if (a.parts > 0) {
+    const double norm = sqrt(red[0] + red[1] + red[2] + red[3]) * fabs(a.grad_scale);
+    r.factor = a.grad_scale * (norm > a.max_norm ? a.max_norm / norm : 1.0);
+    r.skip = !((float)norm < HUGE_VALF);
+    if (a.norm_out) *a.norm_out = (float)norm;
+  }
   if (a.step_device) {
     const int64_t step = *a.step_device;
     const double t = (double)step;
@@ -160,7 +163,6 @@ __global__ __launch_bounds__(256) void k_adamw_scalars(ScalarArgs a) {
     r.skip |= !(r.rate >= 0.0f && r.rate < HUGE_VALF);
   }
   *a.out = r;
-  if (a.norm_out) *a.norm_out = (float)norm;
 }
 
 // ---------------------------------------------------------------- 8-bit states
