@@ -173,7 +173,10 @@ class AdamW:
         The gradients are multiplied by ``grad_scale`` and, where ``max_norm`` is
         given, by max_norm over their common norm if that is larger.  With max_norm or
         ``norm=True`` the norm comes back (float32, on the device), and a norm that is
-        not finite leaves everything unchanged."""
+        not finite leaves everything unchanged.
+
+        To torch's autograd a step changes its parameters in place: a graph that saved one
+        refuses its backward pass afterwards.  (Replays of a recorded graph go unnoticed.)"""
         torch = _torch()
         if self._plan is None:
             raise ValueError("the optimizer is closed")
@@ -222,6 +225,8 @@ class AdamW:
             ws = self.exp_avg.new_empty(nbytes, dtype=torch.uint8)
         _lib.call("mgp_adamw_step_device", self._plan, C.byref(s),
                   None if ws is None else ws.data_ptr(), nbytes, _stream(torch, current))
+        changed = self.params if all(pointers) else [p for p, at in zip(self.params, pointers) if at]
+        torch.autograd.graph.increment_version(changed)
         return result
 
     def values(self):

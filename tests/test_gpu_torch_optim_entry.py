@@ -39,3 +39,30 @@ def test_without_a_norm_its_fields_are_not_used(bits, max_norm, device):
     assert torch.equal(params[1], params[0]) and float(norm) == 7.0
     for k, t in want.state().items():
         assert torch.equal(got.state()[k], t)
+
+
+@pytest.mark.parametrize("steps_on", ["numbers", "device"])
+def test_autograd_sees_that_parameters_change(steps_on):
+    """A graph of torch's that saved a parameter refuses its backward pass after a step;
+    parameters without a gradient are not changed."""
+    w = torch.ones(5, device="cuda", requires_grad=True)
+    other = torch.ones(5, device="cuda", requires_grad=True)
+    with torch.no_grad():
+        opt = optim.AdamW([w, other])
+    loss, kept = (w * w).sum(), (other * other).sum()
+    versions = w._version, other._version
+    rate, step = 0.1, 1
+    if steps_on == "device":
+        rate = torch.full((), 0.1, device="cuda")
+        step = torch.ones((), device="cuda", dtype=torch.int64)
+    with torch.no_grad():
+        opt.step([torch.ones(5, device="cuda"), None], rate, step)
+    assert w._version > versions[0] and other._version == versions[1]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    kept.backward()
+    assert torch.equal(other.grad, torch.full((5,), 2.0, device="cuda"))
+    with torch.inference_mode():  # tensors without versions
+        p = torch.ones(5, device="cuda")
+        optim.AdamW([p]).step([torch.ones(5, device="cuda")], 0.1, 1)
+    assert not torch.equal(p, torch.ones(5, device="cuda"))
