@@ -224,6 +224,7 @@ class NativeProvider:
         features._rows(Rf, "Rf", dtype, index, shape)
         if not Lf.is_contiguous() or not Rf.is_contiguous():
             raise ValueError("Lf and Rf must be contiguous")
+        given = out
         if out is None:
             out = Lf.new_empty((self.n, self.d))
         else:
@@ -232,6 +233,7 @@ class NativeProvider:
                 raise ValueError("out must be contiguous")
         _lib.call("mgp_input_gradient_device", self.handle, Lf.data_ptr(), Rf.data_ptr(),
                   shape[0] if len(shape) == 2 else 1, out.data_ptr(), stream)
+        features._written(given)
         return out
 
     def gradient_matvec(self, V) -> np.ndarray:

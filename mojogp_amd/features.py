@@ -18,7 +18,8 @@ imported here and computes nothing, it provides the arrays, the memory of the
 results and the current stream, on which every call runs asynchronously.  The
 calls are explicit forward and backward passes and take no part in autograd: an
 array that requires a gradient is refused unless torch.no_grad() says that none is
-recorded.
+recorded.  A result that the caller gives (``out``) counts as changed in place: a graph of
+torch's that saved it refuses its backward pass.
 """
 
 from __future__ import annotations
@@ -165,6 +166,12 @@ def _result(a, name, like, shape, dtype, index):
     return a, address, stride
 
 
+def _written(a):
+    """To torch's autograd a result that the caller gave has changed in place."""
+    if a is not None:
+        _torch().autograd.graph.increment_version(a)
+
+
 def _workspace(like, nbytes):
     return like.new_empty((nbytes,), dtype=_torch().uint8) if nbytes else None
 
@@ -202,6 +209,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, save=False, out=None):
     y, py, stride = _result(out, "out", x, x.shape, dtype, index)
     stats = x.new_empty((a.rows, 2), dtype=_torch().float32) if save else None
     _lib.call("mgp_layer_norm_device", C.byref(a), py, stride, _address(stats), stream)
+    _written(out)
     return (y, stats) if save else y
 
 
@@ -290,6 +298,7 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, *, activation=None, 
     ws, nbytes = _group_workspace(a, x, 0)
     _lib.call("mgp_group_norm_device", C.byref(a), py, stride, _address(stats), _address(ws),
               nbytes, stream)
+    _written(out)
     return (y, stats) if save else y
 
 
@@ -325,6 +334,7 @@ def _dropout(x, name, rate, seed, offset, residual, out):
     y, py, y_stride = _result(out, "out", x, x.shape, dtype, index)
     _lib.call("mgp_dropout_device", code, px, stride, rows, width, rate, seed, offset, pr,
               r_stride, py, y_stride, stream)
+    _written(out)
     return y
 
 
@@ -377,10 +387,11 @@ def gated_layer(x, w_gate, w_up, b_gate=None, b_up=None, *, activation="silu", o
     normal distribution's exact integral), "sigmoid" or "relu".  ``out`` shares no
     memory with the inputs."""
     a, shape, dtype, index, stream = _gated_args(x, w_gate, w_up, b_gate, b_up, activation)
-    out, ph, h_stride = _result(out, "out", x, shape, dtype, index)
+    h, ph, h_stride = _result(out, "out", x, shape, dtype, index)
     ws, nbytes = _gated_workspace(a, x, 0)
     _lib.call("mgp_gated_layer_device", C.byref(a), ph, h_stride, _address(ws), nbytes, stream)
-    return out
+    _written(out)
+    return h
 
 
 def gated_layer_backward(dh, x, w_gate, w_up, b_gate=None, b_up=None, *, activation="silu",
@@ -467,6 +478,7 @@ def _int8(x, gate, up, b_gate, b_up, act, names, out):
     _lib.call("mgp_int8_layer_workspace", C.byref(a), C.byref(nbytes))
     ws = _workspace(x, nbytes.value)
     _lib.call("mgp_int8_layer_device", C.byref(a), py, y_stride, _address(ws), nbytes.value, stream)
+    _written(out)
     return y
 
 
