@@ -126,17 +126,17 @@ struct GroupKernel {
   // a group (its sums), and of them on the entries of one row
   int cv, slots, at_a_time, lanes, run_lanes;
   int64_t batches;
-  // blocks of groups a sample is dealt out in, one a workgroup; in the kernels a.groups
-  // and a.channels are a block's, and these a sample's
+  // blocks of groups a sample is dealt out in; in the kernels a.groups and a.channels are
+  // a block's, and these a sample's
   int group_blocks, all_groups, all_channels;
   // stretches: rows of one, how many a sample, column blocks of cv vectors
   int stretch, short_stretch;  // of partial results, and of the results
   int stretches, shorts, blocks;
 };
 
-// What a workgroup that holds samples, or groups of one, takes: batches of samples from
-// `first` on, `step` apart, or (groups) the one sample `first`.  Neighbouring groups,
-// which share lines of memory, go to workgroups of one XCD.
+// What a workgroup that holds samples, or one block of groups of them, takes: batches of
+// samples from `first` on, `step` apart.  Neighbouring groups, which share lines of
+// memory, go to workgroups of one XCD.
 struct Share {
   int64_t first, step;
 };
@@ -159,7 +159,7 @@ __device__ __forceinline__ Share share_of(GroupKernel& s) {
   s.a.bias = on(s.a.bias, s.a.f32_params);
   if (s.stats) s.stats += block * s.a.groups;
   if (s.part) s.part += (int64_t)n * s.all_channels + col;
-  return {n, s.batches};
+  return {n, total / (uint32_t)s.group_blocks};
 }
 
 // How a sample's group sums come together in a workgroup that holds whole samples:
@@ -1133,9 +1133,7 @@ inline int groups_of(const GroupArgs& a, int V, int size, int most) {
   for (int gb = std::min(a.groups, std::max(1, kMostThreads * V / size)); gb >= 1; --gb) {
     if (a.groups % gb != 0) continue;
     if (!threads_of(ceil_div((int64_t)gb * size, (int64_t)V), a.positions, most)) continue;
-    // (a block's rows hold a vector, its workgroups are a launch's)
-    if (gb < a.groups && (gb * size < V || a.samples * (a.groups / gb) >= (1 << 24))) break;
-    if (gb < a.groups && gb * row < 512) break;
+    if (gb < a.groups && (gb * size < V || gb * row < 512)) break;  // (rows hold a vector)
     best = gb;
     if (small || a.samples * (a.groups / gb) >= 256) break;
   }
@@ -1214,13 +1212,17 @@ GroupCut cut_of(GroupKernel& s, bool back) {
   return c;
 }
 
-// Workgroups, and rows of partial results that they leave (BACK).
-inline unsigned workgroups(const GroupKernel& s, bool back) {
-  if (s.group_blocks > 1) return (unsigned)(s.a.samples * s.group_blocks);
-  return (unsigned)std::min<int64_t>(s.batches, back ? kBackBlocks : 2048);
+// Workgroups that share the samples out among them, for each block of groups: of the
+// backward pass, also the rows of partial results.  (Blocks, forward: as many as samples
+// up to 2^20 workgroups, which start as others end.)
+inline int64_t sharers(const GroupKernel& s, bool back) {
+  const int64_t most = back                   ? kBackBlocks
+                       : s.group_blocks > 1 ? (int64_t)1 << 20
+                                              : 2048;
+  return std::min<int64_t>(s.batches, std::max<int64_t>(1, most / s.group_blocks));
 }
-inline int64_t back_parts(const GroupKernel& s) {
-  return s.group_blocks > 1 ? s.a.samples : workgroups(s, true);
+inline unsigned workgroups(const GroupKernel& s, bool back) {
+  return (unsigned)(sharers(s, back) * s.group_blocks);
 }
 
 // Runs f with a kernel's rows a thread and join.
@@ -1288,7 +1290,7 @@ size_t group_norm_bytes(const GroupArgs& a, bool back) {
   s.a = a;
   const GroupCut c = cut_of(s, back);
   const size_t row = (size_t)a.channels * sizeof(float2);
-  if (c.whole) return back ? aligned((size_t)back_parts(s) * row) : 0;
+  if (c.whole) return back ? aligned((size_t)sharers(s, true) * row) : 0;
   return aligned((size_t)(a.samples * s.stretches) * row) + pairs_bytes(a);
 }
 
@@ -1343,7 +1345,7 @@ void group_norm_backward(const GroupArgs& a, const void* dy, int64_t dy_stride, 
         launch_stretches<K, true>(s, st);
         return;
       }
-      parts = back_parts(s);
+      parts = sharers(s, true);
       if (!params) s.part = nullptr;
       dispatch_whole<K, true>(c, [&](auto r, auto join) {
         k_group_bwd<K, r.value, join.value><<<workgroups(s, true), c.threads, c.lds, st>>>(s);

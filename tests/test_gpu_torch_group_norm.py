@@ -264,3 +264,18 @@ def test_refusals():
         features.group_norm_backward(x[:1], x, 2, None, None, torch.zeros(6, 2, 2, device="cuda"))
     with pytest.raises(ValueError, match="requires a gradient"):
         features.group_norm(x.clone().requires_grad_(), 2)
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("n, l, c, groups, pad", [
+    # groups within lanes, of whole vectors, and that cut vectors
+    (1100, 1, 8192, 64, 0), (1100, 1, 5000, 8, 0), (600, 3, 4400, 4, 1), (300, 5, 8192, 16, 0),
+    (530, 2, 5005, 7, 0),
+])
+def test_many_samples_in_blocks_of_groups(kind, n, l, c, groups, pad):
+    """More samples than workgroups of the backward pass take at a time."""
+    rng = np.random.default_rng(n + l + c)
+    x = rng.normal(size=(n, l, c)) * rng.uniform(0.5, 2, (n, 1, 1)) + rng.normal(size=(n, 1, c))
+    x = _dev(x, kind, pad, min(pad, 1))
+    w, b = _dev(1 + 0.2 * rng.normal(size=c), kind), _dev(0.3 * rng.normal(size=c), kind)
+    _check(x, _dev(rng.normal(size=(n, l, c)), kind, pad), groups, w, b, ACTS[(n + c) % 4], kind)

@@ -78,3 +78,16 @@ def test_results_that_share_memory():
             backward(*args)
     with pytest.raises(_lib.NativeCallError, match="256-byte"):
         backward(None, BASE + 65536, ws=BASE + 16384 + 8)
+
+
+@pytest.mark.parametrize("samples", [1000, 100000, 1 << 22, (1 << 31) - 1])
+@pytest.mark.parametrize("positions, channels, groups, kind", [
+    (1, 256, 32, BF16), (1, 5000, 8, BF16), (1, 3776, 16, F32), (2, 8192, 4, BF16),
+    (4, 16384, 64, F32), (1, 1 << 20, 1 << 10, BF16)])
+def test_partial_sums_of_the_parameters_do_not_grow_with_the_samples(samples, positions, channels,
+                                                                     groups, kind):
+    """Of samples in registers, whole or in blocks of groups: at most 1024 rows."""
+    a = _args(type=kind, param_type=kind, samples=min(samples, ((1 << 31) - 1) // positions),
+              positions=positions, channels=channels, groups=groups, x_stride=channels)
+    assert _bytes(a) == 0
+    assert 0 < _bytes(a, 1) <= 1024 * channels * 8 + 256
