@@ -79,6 +79,19 @@ __device__ __forceinline__ void load_params(const void* p, int c, bool f32, floa
   }
 }
 
+// xhat and z of a vector, by the same operations in every pass: a slope is that of the
+// value that the forward pass activated, at the jump of relu's too.
+template <class K, int MV>
+__device__ __forceinline__ void normalise(const Raw<K>& x, const float (&mean)[MV],
+                                          const float (&rstd)[MV], const float* w, const float* b,
+                                          float* xhat, float* z) {
+#pragma unroll
+  for (int k = 0; k < K::V; ++k) {
+    xhat[k] = ((float)x.v[k] - mean[k % MV]) * rstd[k % MV];
+    z[k] = fmaf(xhat[k], w[k], b[k]);
+  }
+}
+
 // z -> act(z); and with its derivative.
 template <class K>
 __device__ __forceinline__ void act_values(int act, float* z) {
@@ -506,15 +519,11 @@ __global__ __launch_bounds__(kMostThreads) void k_group_fwd(GroupKernel s) {
     }
     if (in) {
       T* py = static_cast<T*>(s.out) + batch_offset(s, batch, s.ldo) + off_y;
-      float wr[V];
-#pragma unroll
-      for (int k = 0; k < V; ++k) wr[k] = w[k] * rstd[k % MV];
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         if (r < count) {
-          float z[V];
-#pragma unroll
-          for (int k = 0; k < V; ++k) z[k] = fmaf((float)x[r].v[k] - mean[k % MV], wr[k], b[k]);
+          float xhat[V], z[V];
+          normalise<K>(x[r], mean, rstd, w, b, xhat, z);
           act_values<K>(s.a.activation, z);
           store_raw<K>(py + (int64_t)r * at.slots * s.ldo, at.from, z);
         }
@@ -556,11 +565,7 @@ __device__ __forceinline__ void vector_dz(const GroupArgs& a, const Raw<K>& x, c
                                           const float* w, const float* b, float* xhat, float* dz) {
   constexpr int V = K::V;
   float z[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    xhat[k] = ((float)x.v[k] - mean[k % MV]) * rstd[k % MV];
-    z[k] = fmaf(xhat[k], w[k], b[k]);
-  }
+  normalise<K>(x, mean, rstd, w, b, xhat, z);
   act_slopes<K>(a.activation, z, dz);
 #pragma unroll
   for (int k = 0; k < V; ++k) dz[k] *= (float)dy.v[k];
@@ -1031,17 +1036,14 @@ __global__ __launch_bounds__(kPartThreads) void k_group_apply(GroupKernel s) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (i + u >= count) continue;
-        float z[V];
+        float xhat[V], z[V];
         if constexpr (BACK) {
-          float xhat[V];
           vector_dz<K>(s.a, x[u], dy[u], mean, rstd, w, b, xhat, z);
 #pragma unroll
           for (int k = 0; k < V; ++k)
             z[k] = fmaf(wr[k], z[k], -fmaf(xhat[k], c2[k % MV], c1[k % MV]));
         } else {
-#pragma unroll
-          for (int k = 0; k < V; ++k)
-            z[k] = fmaf(((float)x[u].v[k] - mean[k % MV]) * rstd[k % MV], w[k], b[k]);
+          normalise<K>(x[u], mean, rstd, w, b, xhat, z);
           act_values<K>(s.a.activation, z);
         }
         store_raw<K>(po + (i + u) * so, at.from, z);

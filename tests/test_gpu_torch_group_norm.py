@@ -279,3 +279,39 @@ def test_many_samples_in_blocks_of_groups(kind, n, l, c, groups, pad):
     x = _dev(x, kind, pad, min(pad, 1))
     w, b = _dev(1 + 0.2 * rng.normal(size=c), kind), _dev(0.3 * rng.normal(size=c), kind)
     _check(x, _dev(rng.normal(size=(n, l, c)), kind, pad), groups, w, b, ACTS[(n + c) % 4], kind)
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("n, l, c, groups", [
+    # single values; groups within a vector, of lanes, of vectors, that cut vectors; in
+    # stretches; in blocks
+    (6000, 1, 16, 16), (6000, 1, 16, 8), (900, 1, 64, 4), (70, 6, 64, 4), (70, 6, 60, 5),
+    (3, 3000, 48, 4), (40, 1, 5000, 8),
+])
+def test_slopes_are_of_the_values_that_were_written(kind, n, l, c, groups):
+    """Values at relu's jump: x is +1 or -1 and the bias what takes weight times the
+    normalised 1 (or a value beside it) to zero within a rounding, so that z is a last bit
+    of either sign.  Where y is above zero the slope is 1, elsewhere 0: with dy = 1 the
+    bias' gradient counts the former."""
+    rng = np.random.default_rng(n + c)
+    x = rng.choice([-1.0, 1.0], (n, l, c))
+    single = l * c // groups == 1
+    if single:
+        x *= 0.0
+    x = _dev(x, kind)
+    w = _dev(rng.uniform(0.5, 2, c), "f32")
+    if kind == "f16":  # z is a multiple of 2^-24 2^2, above float16's half smallest, 2^-25:
+        w = (1024 * w).bfloat16().float()  # xhat's last bit, 2^-24, times w's, 2^2 of 2^9
+    _, saved = features.group_norm(x, groups, save=True)
+    # a sample's own normalised 1, of another one in every channel
+    pick = torch.from_numpy(rng.integers(0, n, c)).cuda()
+    mean, rstd = (saved[pick, torch.arange(c, device="cuda") // (c // groups), k] for k in (0, 1))
+    at = x[pick, 0, torch.arange(c, device="cuda")].float()
+    b = -((at - mean) * rstd) * w
+    y, saved = features.group_norm(x, groups, w, b, activation="relu", save=True)
+    _, _, db = features.group_norm_backward(torch.ones_like(x), x, groups, w, b, saved,
+                                            activation="relu")
+    count = (y > 0).double().sum(dim=(0, 1))
+    # (a single value is its group's mean: z is the bias, 0, wherever it is)
+    assert not count.any() if single else 0 < float(count.sum()) < n * l * c
+    assert torch.equal(db.double(), count)  # whole numbers below 2^24: exact in fp32
