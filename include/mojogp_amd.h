@@ -864,7 +864,8 @@ MGP_API int mgp_int8_quantize_device(int type, const void* x, int64_t x_stride, 
 /* A layer whose weights are such rows (the bytes up to the next multiple of 16 of
  * width, zeros, are read): y = act(s s_gate sum(q w_gate) + b_gate), where q and s are
  * x's rows as above and the sum is exact; with w_up (not NULL) times (s s_up sum(q w_up)
- * + b_up).  x, biases [hidden] (may be NULL) and y are of one element type.  activation:
+ * + b_up).  (sum times s comes first; an infinity where it passes fp32.)  x, biases
+ * [hidden] (may be NULL) and y are of one element type.  activation:
  * as of the gated layer, or -1 for none where w_up is NULL. */
 typedef struct mgp_int8_layer {
   int type;

@@ -9,9 +9,9 @@
 // lie in a table on the device; the gradients, which are new arrays every step, come as
 // a launch's arguments (up to kGrads of them), without a copy to the device.  On 67 million
 // fp32 values the step takes 325 us in 32 bits (5.8 TB/s, part of the gradients from the
-// last-level cache, where the norm has left them), 211 us in 8 bits
-// (5.1 TB/s at 16 bytes), where the instructions for codes and draws just hide behind the
-// memory; the norm 84 us.
+// last-level cache, where the norm has left them), 214 us in 8 bits
+// (5.0 TB/s at 16 bytes), where the instructions for quotients, codes and draws hardly hide
+// behind the memory; the norm 84 us.
 //
 // 8-bit states: 256 values of a tensor share a scale, one wave's four values a lane.
 // m is an OCP e4m3 value times scale (largest |m| / 448), v one of 5 exponent and 3
@@ -221,7 +221,7 @@ __device__ __forceinline__ float wave_scale(float lane_scale) {
 }
 
 // x / scale in 64 bits; inv is the reciprocal to within a few last places.  (No quotient of
-// 53 by 24 bits lies within 2^-24 of a last place from a tie.)
+// 53 by 24 bits lies within 2^-25 of a last place from a tie.)
 __device__ __forceinline__ double over(double x, double scale, double inv) {
   const double q = x * inv;
   return fma(fma(-q, scale, x), inv, q);
